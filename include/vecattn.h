@@ -415,6 +415,103 @@ int va_prefill(int dtype, const void* q, int64_t sqb, int64_t sqh, int64_t sqs,
  * (spattn/threshold/model_tuner.py:53-77). */
 int va_bf16_copy(const float* x, int64_t n, void* out, int32_t* inexact, void* stream);
 
+/*
+ * A key-value cache in pages, and the step of a batch of requests over it.  The
+ * reference keeps one contiguous cache per sequence (its decode call,
+ * spattn/src/models/load_qwen2p5_vl.py:61-66), so these have no counterpart
+ * there.  A cache is num_pages pages of page_size rows for each kv head, with
+ * any strides: row (page, in, h) at page*s?p + in*s?n + h*s?h.  Slot s is row
+ * s % page_size of page s / page_size.  Row i of block_tables (int32, M entries,
+ * row stride stn) lists request i's pages in order.
+ *
+ * va_paged_plan: request i holds kv_lens[i] tokens and adds new_lens[i]
+ * (negative counts as 0).  It takes ceil((kv_lens + new_lens) / page_size) -
+ * ceil(kv_lens / page_size) pages, but none past entry M, from
+ * free_pages[*free_head ..] (free_head NULL: from 0) in the order of the requests,
+ * and they are written behind the pages its table row holds; no other entry of
+ * block_tables is touched.  Outputs: kv_lens_out = kv_lens + new_lens (N);
+ * qo_indptr, the exclusive sum of new_lens (N + 1); for token t < num_tokens its
+ * request_ids, positions and slot_mapping, which are -1, 0 and -1 behind the last
+ * request's tokens; and *pages_taken, the pages asked for.  Where the free pages
+ * do not suffice (*free_head + *pages_taken > num_free) the table entries and
+ * slots without a page are -1, as is the slot of a token past the table's
+ * end or in a page whose entry is negative.  workspace: of
+ * va_paged_plan_workspace_size(N) bytes, 16-byte aligned (0: none).
+ */
+int64_t va_paged_plan_workspace_size(int64_t N);
+int va_paged_plan(const int32_t* kv_lens, const int32_t* new_lens, int64_t N,
+                  int32_t* block_tables, int64_t stn, int64_t M, const int32_t* free_pages,
+                  int64_t num_free, const int32_t* free_head, int64_t page_size,
+                  int64_t num_tokens, int32_t* kv_lens_out, int32_t* qo_indptr,
+                  int64_t* slot_mapping, int64_t* positions, int32_t* request_ids,
+                  int64_t* pages_taken, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Norm of each head's row (weights given: x * rsqrt(mean(x^2) + eps) * w) and
+ * rotation of its first rotary_dim features by position * inv_freq[f], f <
+ * rotary_dim / 2, on the pairs (f, f + rotary_dim/2) or, interleaved, (2f, 2f +
+ * 1); cos and sin are multiplied by `scaling`.  What the reference's patched
+ * forwards do in torch before the attention
+ * (spattn/src/models/load_qwen2p5_vl.py:42-45).  q (B, Hq, S, D) and k (B, Hk,
+ * S, D) to q_out and k_out, any strides with contiguous features.  positions:
+ * (axes, B, S) at axis*spa + b*spb + s; with more than one axis (at most 4)
+ * frequency f takes the axis whose section holds it, `sections` (host memory)
+ * being their lengths, of sum rotary_dim/2.  Weights: D values of q's type or
+ * fp32 (weight_dtype), each NULL for none.  fp32 arithmetic, angles reduced in
+ * fp64, one rounding.  D up to 512.
+ */
+int va_qk_norm_rope(int dtype, const void* q, int64_t sqb, int64_t sqh, int64_t sqs, const void* k,
+                    int64_t skb, int64_t skh, int64_t sks, void* q_out, int64_t sqob,
+                    int64_t sqoh, int64_t sqos, void* k_out, int64_t skob, int64_t skoh,
+                    int64_t skos, int64_t B, int64_t Hq, int64_t Hk, int64_t S, int64_t D,
+                    const int64_t* positions, int64_t spa, int64_t spb, int64_t axes,
+                    const int64_t* sections, const float* inv_freq, int64_t rotary_dim,
+                    const void* q_weight, const void* k_weight, int weight_dtype, float eps,
+                    float scaling, int interleaved, void* stream);
+
+/*
+ * The same for T tokens of a step (rows (t, h), positions (axes, T)) with the
+ * rotated keys and the values going to their slots of the caches.  A token whose
+ * slot is not in [0, num_pages * page_size) writes no key and value (its query
+ * is rotated all the same).  Slots must be distinct.
+ */
+int va_qk_norm_rope_to_cache(
+    int dtype, const void* q, int64_t sqt, int64_t sqh, const void* k, int64_t skt, int64_t skh,
+    const void* v, int64_t svt, int64_t svh, void* q_out, int64_t sqot, int64_t sqoh,
+    void* k_cache, int64_t skcp, int64_t skcn, int64_t skch, void* v_cache, int64_t svcp,
+    int64_t svcn, int64_t svch, int64_t num_pages, int64_t page_size, const int64_t* slot_mapping,
+    int64_t T, int64_t Hq, int64_t Hk, int64_t D, const int64_t* positions, int64_t spa,
+    int64_t axes, const int64_t* sections, const float* inv_freq, int64_t rotary_dim,
+    const void* q_weight, const void* k_weight, int weight_dtype, float eps, float scaling,
+    int interleaved, void* stream);
+
+/* Keys and values of T tokens (rows (t, h)) to their slots, as they are; slots
+ * as in va_qk_norm_rope_to_cache. */
+int va_write_paged_kv(int dtype, const void* k, int64_t skt, int64_t skh, const void* v,
+                      int64_t svt, int64_t svh, void* k_cache, int64_t skcp, int64_t skcn,
+                      int64_t skch, void* v_cache, int64_t svcp, int64_t svcn, int64_t svch,
+                      int64_t num_pages, int64_t page_size, const int64_t* slot_mapping, int64_t T,
+                      int64_t Hk, int64_t D, void* stream);
+
+/*
+ * Decode attention over pages: out[n, h] = softmax(q[n, h] . K^T * softmax_scale)
+ * V over the first kv_lens[n] tokens of request n, GQA as in va_decode_attn; a
+ * request without tokens gives zeros.  Rows become NaN where the request cannot
+ * be read: kv_lens[n] > M * page_size, or an entry of its table row that its
+ * tokens need is not a page in [0, num_pages).  D up to 256.  workspace: of
+ * va_paged_decode_workspace_size() bytes (-1: sizes that are not supported),
+ * 16-byte aligned; calls that may overlap need one each.
+ */
+int64_t va_paged_decode_workspace_size(int dtype, int64_t N, int64_t Hq, int64_t Hk, int64_t D,
+                                       int64_t M, int64_t page_size);
+int va_paged_decode_attn(int dtype, const void* q, int64_t sqn, int64_t sqh, const void* k_cache,
+                         int64_t skp, int64_t skn, int64_t skh, const void* v_cache, int64_t svp,
+                         int64_t svn, int64_t svh, void* out, int64_t son, int64_t soh,
+                         const int32_t* block_tables, int64_t stn, int64_t M,
+                         const int32_t* kv_lens, int64_t N, int64_t Hq, int64_t Hk, int64_t D,
+                         int64_t page_size, int64_t num_pages, float softmax_scale,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

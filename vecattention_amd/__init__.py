@@ -9,6 +9,9 @@ from .dispatch import (DiffusionStepContext, FastPrefillConfig, Full_prefill,
                        customize_prefill_attention, select_cfg_threshold)
 from .tuner import seg_pr_perHead
 from .decode import single_decode_with_kv_cache
+from .rotary import qk_norm_rope
+from .paged import (PagedStep, paged_decode_attention, paged_kv_plan, qk_norm_rope_to_cache,
+                    write_paged_kv)
 
 __all__ = [
     "VecAttention_prefill",
@@ -22,4 +25,10 @@ __all__ = [
     "select_cfg_threshold",
     "seg_pr_perHead",
     "single_decode_with_kv_cache",
+    "qk_norm_rope",
+    "PagedStep",
+    "paged_kv_plan",
+    "write_paged_kv",
+    "qk_norm_rope_to_cache",
+    "paged_decode_attention",
 ]

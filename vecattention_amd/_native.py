@@ -89,6 +89,25 @@ SIGNATURES = {
     "va_prefill": (_int, [_int, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64,
                           _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32,
                           _vp, _i64, _i64, _i64, _int, _i64, _i64, _vp, _i64, _vp]),
+    "va_paged_plan_workspace_size": (_i64, [_i64]),
+    "va_paged_plan": (_int, [_vp, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp,
+                             _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "va_qk_norm_rope": (_int, [_int, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64,
+                               _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                               _vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _int, _f32, _f32,
+                               _int, _vp]),
+    "va_qk_norm_rope_to_cache": (_int, [_int, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64,
+                                        _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64,
+                                        _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _vp,
+                                        _i64, _i64, _vp, _vp, _i64, _vp, _vp, _int, _f32, _f32,
+                                        _int, _vp]),
+    "va_write_paged_kv": (_int, [_int, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
+                                 _i64, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i64,
+                                 _vp]),
+    "va_paged_decode_workspace_size": (_i64, [_int, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "va_paged_decode_attn": (_int, [_int, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64,
+                                    _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
+                                    _i64, _i64, _i64, _i64, _f32, _vp, _i64, _vp]),
 }
 
 

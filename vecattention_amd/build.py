@@ -16,7 +16,8 @@ LIB = os.path.join(HERE, "libvecattn.so")
 SOURCES = ["pool.hip", "select_exact.hip", "select_mfma.hip", "select_tile.hip", "select_max.hip",
            "select_wave.hip", "key_norm.hip",
            "attn_simple.hip", "attn_mfma.hip", "attn_dense.hip", "attn_f32.hip", "decode.hip",
-           "csr.hip", "convert.hip", "api.hip", "noalloc.hip"]
+           "csr.hip", "convert.hip", "paged_plan.hip", "rope.hip", "paged_attn.hip", "paged_api.hip",
+           "api.hip", "noalloc.hip"]
 ARCH = os.environ.get("VA_OFFLOAD_ARCH", "gfx950")
 
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 are generated (they have given
