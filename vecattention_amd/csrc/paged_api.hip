@@ -214,7 +214,7 @@ int64_t va_paged_decode_workspace_size(int dtype, int64_t N, int64_t Hq, int64_t
   a.D = D;
   a.M = M;
   a.page = page_size;
-  return va::plan_paged_attn(dtype, a);
+  return va::paged_attn_workspace(dtype, a);
 }
 
 int va_paged_decode_attn(int dtype, const void* q, int64_t sqn, int64_t sqh, const void* k_cache,

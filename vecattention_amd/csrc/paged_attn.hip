@@ -14,6 +14,7 @@
 // holds `rows` pairs (m, l), and `rows` unnormalised fp32 rows of D.
 #include "common.h"
 #include "lanes.h"
+#include "mfma.h"
 #include "paged_ops.h"
 
 namespace va {
@@ -81,11 +82,11 @@ __device__ inline Place locate(const PagedArgs& a, int64_t (*lds)[2]) {
 // Merges the waves' states of a segment's rows and writes them: to the output
 // (`whole`), or to a partial slot.  sO[wave][row][stride], sm/sl[wave][row].
 template <typename T>
-__device__ inline void finish(const PagedArgs& a, const float* sO, int rstride, int wstride,
+__device__ inline void finish(const PagedArgs& a, int D, const float* sO, int rstride, int wstride,
                               const float* sm, const float* sl, int mstride, int rows, bool whole,
                               int64_t slot, int64_t request, int64_t head, bool empty, bool bad) {
-  for (int i = threadIdx.x; i < rows * int(a.D); i += kPagedThreads) {
-    const int r = i / int(a.D), f = i % int(a.D);
+  for (int i = threadIdx.x; i < rows * D; i += kPagedThreads) {
+    const int r = i / D, f = i % D;
     float m = -__builtin_inff();
 #pragma unroll
     for (int w = 0; w < kPagedWaves; ++w)
@@ -202,7 +203,317 @@ __global__ __launch_bounds__(kPagedThreads) void paged_row_kernel(PagedArgs a) {
       }
     }
     __syncthreads();
-    finish<T>(a, &sO[0][0][0], kRowMaxD, kRowTile * kRowMaxD, &sm[0][0], &sl[0][0], kRowTile,
+    finish<T>(a, int(a.D), &sO[0][0][0], kRowMaxD, kRowTile * kRowMaxD, &sm[0][0], &sl[0][0], kRowTile,
+              rows, count == units, 2 * int64_t(blockIdx.x) + (u > begin), req, hk * a.G + r0,
+              keys == 0, sbad != 0);
+    __syncthreads();
+    u += count;
+    if (u == base + units * a.Hk * a.tiles) {
+      base = u;
+      ++req;
+    }
+  }
+}
+
+// The matrix-core form: head_dim 64 or 128, 16-byte aligned rows.  A wave takes
+// kKeys keys a step and up to 16 query heads of a kv head:
+//   S^T = K Q^T     rows: keys, columns: query heads
+//   O^T += V^T P^T  rows: features, columns: query heads
+// in 16x16 tiles, so that the lane that gets a score (key 4*kg + i of its tile,
+// head c; kg = lane / 16, c = lane % 16) holds that weight where the second
+// product wants it, and every row of K and V goes from memory to the registers
+// of the lane that multiplies it: K's as operand rows, V's with lane c holding
+// features [c*D/16, ..) of its keys, which makes row c of product m feature
+// c*D/16 + m; the pairing of keys is then a byte permutation in registers.  Nothing
+// but the waves' results at a segment's end goes through LDS.
+//
+// 16-bit types round a weight to 8 (11) bits, which would cost as much accuracy
+// as the output's own rounding: it goes in as two parts, high + low, to 2^-16.
+// An infinite value would meet a low part of 0 or below and give NaN, so a
+// wave whose sums hold a NaN repeats its keys with the high part alone.
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+
+template <typename T> struct Mfma16;
+template <> struct Mfma16<bf16_t> {
+  typedef __bf16 e;
+  typedef bf16x8_t vec;
+  __device__ static f32x4_t run(vec a, vec b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <> struct Mfma16<f16_t> {
+  typedef _Float16 e;
+  typedef f16x8_t vec;
+  __device__ static f32x4_t run(vec a, vec b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+
+// Max and sum over the four lanes that hold a column (lanes c, c + 16, ..).
+__device__ inline float column_max(float x) {
+  const uint32_t u = float_to_bits(x);
+  const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return max_halves(__builtin_fmaxf(bits_to_float(p[0]), bits_to_float(p[1])));
+}
+__device__ inline float column_sum(float x) {
+  const uint32_t u = float_to_bits(x);
+  const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return sum_halves(bits_to_float(p[0]) + bits_to_float(p[1]));
+}
+
+constexpr int kTileHeads = 16;
+template <typename T> constexpr int kStepKeys = sizeof(T) == 2 ? 32 : 16;
+template <typename T> constexpr int kTileUnit = kPagedWaves * kStepKeys<T>;
+
+// Places of a step's keys: page id and first key of the page for each tile of
+// 16 keys, which lie in one page when the page size is a multiple of 16.
+template <int kTiles> struct Pages {
+  int32_t id[kTiles];
+  uint32_t first[kTiles];
+};
+
+template <typename T, int D, bool kWholeTiles>
+__global__ __launch_bounds__(kPagedThreads) void paged_tile_kernel(PagedArgs a) {
+  constexpr bool k16 = sizeof(T) == 2;
+  constexpr int kKeys = kStepKeys<T>, kTiles = kKeys / 16, kUnit = kTileUnit<T>;
+  constexpr int kF = D / 16;                       // features of a lane in a row of V
+  constexpr int kKL = k16 ? D / 32 : D / 16;       // 16-byte loads of a lane in a row of K
+  constexpr int kVW = kF * int(sizeof(T)) / 4;     // words of a lane in a row of V
+  constexpr int kStride = D + 4;
+  __shared__ int64_t place[kPagedWaves][2];
+  __shared__ __align__(16) float sO[kPagedWaves][kTileHeads][kStride];
+  __shared__ float sm[kPagedWaves][kTileHeads], sl[kPagedWaves][kTileHeads];
+  __shared__ int sbad;
+  __shared__ int2 srow[kPagedWaves][kKeys];        // (page, row) of a step's keys, any page size
+  const int lane = threadIdx.x % 64;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int kg = lane / 16, c = lane % 16;
+  const Place pl = locate<kUnit>(a, place);
+  const PagedShare share(pl.total, a.groups);
+  const int64_t begin = share.begin(blockIdx.x), end = share.begin(blockIdx.x + 1);
+  const int64_t capacity = a.M * a.page;
+  const uint32_t page = uint32_t(a.page);
+  int64_t req = pl.request, base = pl.start;
+  for (int64_t u = begin; u < end;) {
+    const int32_t keys = paged_keys(a.lens[req], capacity);
+    const int64_t units = paged_units(keys, kUnit);
+    const int64_t seg = (u - base) / units, c0 = (u - base) % units;
+    const int64_t count = end - u < units - c0 ? end - u : units - c0;
+    const int64_t hk = seg / a.tiles, r0 = seg % a.tiles * a.rows;
+    const int rows = int(a.G - r0 < a.rows ? a.G - r0 : a.rows);
+    const int32_t* table = a.table + req * a.table_stride;
+    const T* kbase = static_cast<const T*>(a.k) + hk * a.kh;
+    const T* vbase = static_cast<const T*>(a.v) + hk * a.vh;
+
+    // The queries: column c, features as K's lanes hold them.
+    u32x4_t q[kKL];
+    {
+      const T* qr = static_cast<const T*>(a.q) + req * a.qn + (hk * a.G + r0 + c) * a.qh;
+#pragma unroll
+      for (int s = 0; s < kKL; ++s)
+        q[s] = c < rows ? *reinterpret_cast<const u32x4_t*>(qr + (s * 4 + kg) * (16 / sizeof(T)))
+                        : u32x4_t{0, 0, 0, 0};
+    }
+    bool bad = keys < 0;
+    const uint32_t last = keys > 0 ? uint32_t(keys) - 1 : 0;
+    const uint32_t first = uint32_t(c0) * kUnit + wave * kKeys;
+    int steps = 0;
+    if (keys > 0 && first <= last) {
+      const uint32_t left = (last - first) / kUnit + 1;
+      steps = left < uint32_t(count) ? int(left) : int(count);
+    }
+
+    Pages<kTiles> pg;
+    u32x4_t kr[kTiles][kKL];
+    uint32_t vr[kTiles * 4][kVW];
+    // Page entries of the step at key0; ids that are no pages read page 0.
+    auto look = [&](uint32_t key0) {
+      if constexpr (kWholeTiles) {
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+          const uint32_t k0 = key0 + 16 * t < last ? key0 + 16 * t : last;
+          const uint32_t p = a.by_page.div(k0);
+          int32_t id = table[p];
+          if (id < 0 || id >= a.num_pages) {
+            bad = true;
+            id = 0;
+          }
+          pg.id[t] = id;
+          pg.first[t] = p * page;
+        }
+      } else {
+        if (lane < kKeys) {
+          const uint32_t k0 = key0 + lane < last ? key0 + lane : last;
+          const uint32_t p = a.by_page.div(k0);
+          int32_t id = table[p];
+          if (id < 0 || id >= a.num_pages) {
+            bad = true;
+            id = 0;
+          }
+          srow[wave][lane] = make_int2(id, int(k0 - p * page));
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      }
+    };
+    // Row `r` of tile t of the step at key0: keys past the last read the last one.
+    auto row_of = [&](const T* from, int64_t sp, int64_t sn, uint32_t key0, int t, uint32_t r) {
+      if constexpr (kWholeTiles) {
+        const uint32_t k0 = key0 + 16 * t + r < last ? key0 + 16 * t + r : last;
+        return from + pg.id[t] * sp + (k0 - pg.first[t]) * uint32_t(sn);
+      } else {
+        const int2 at = srow[wave][16 * t + r];
+        return from + at.x * sp + uint32_t(at.y) * uint32_t(sn);
+      }
+    };
+    auto load_k = [&](uint32_t key0) {
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        const T* row = row_of(kbase, a.kp, a.kn, key0, t, c);
+#pragma unroll
+        for (int s = 0; s < kKL; ++s)
+          kr[t][s] = *reinterpret_cast<const u32x4_t*>(row + (s * 4 + kg) * (16 / sizeof(T)));
+      }
+    };
+    auto load_v = [&](uint32_t key0) {
+#pragma unroll
+      for (int j = 0; j < kTiles * 4; ++j) {
+        const T* row = row_of(vbase, a.vp, a.vn, key0, j / 4, 4 * kg + j % 4) + c * kF;
+#pragma unroll
+        for (int w = 0; w < kVW; w += kVW < 4 ? kVW : 4) {
+          if constexpr (kVW >= 4) {
+            const u32x4_t x = *reinterpret_cast<const u32x4_t*>(
+                reinterpret_cast<const uint32_t*>(row) + w);
+            vr[j][w] = x[0], vr[j][w + 1] = x[1], vr[j][w + 2] = x[2], vr[j][w + 3] = x[3];
+          } else {
+            const u32x2_t x = *reinterpret_cast<const u32x2_t*>(row);
+            vr[j][0] = x[0], vr[j][1] = x[1];
+          }
+        }
+      }
+    };
+
+    f32x4_t acc[kF];
+    float m, l;
+    bool high_only = false;
+    for (;;) {
+      m = -__builtin_inff();
+      l = 0.f;
+#pragma unroll
+      for (int f = 0; f < kF; ++f) acc[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      if (steps > 0) {
+        look(first);
+        load_k(first);
+        load_v(first);
+      }
+      for (int i = 0; i < steps; ++i) {
+        const uint32_t key0 = first + uint32_t(i) * kUnit;
+        f32x4_t s[kTiles];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+          s[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int x = 0; x < kKL; ++x) {
+            if constexpr (k16) {
+              typedef typename Mfma16<T>::vec vec;
+              s[t] = Mfma16<T>::run(__builtin_bit_cast(vec, kr[t][x]),
+                                    __builtin_bit_cast(vec, q[x]), s[t]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                    bits_to_float(kr[t][x][e]), bits_to_float(q[x][e]), s[t], 0, 0, 0);
+            }
+          }
+        }
+        if (i + 1 < steps) {
+          look(key0 + kUnit);
+          load_k(key0 + kUnit);
+        }
+        float p[kTiles * 4], top = -__builtin_inff();
+#pragma unroll
+        for (int j = 0; j < kTiles * 4; ++j) {
+          p[j] = s[j / 4][j % 4] * a.scale_log2;
+          if (key0 + 16 * (j / 4) + 4 * kg + j % 4 > last) p[j] = -__builtin_inff();
+          top = __builtin_fmaxf(top, p[j]);  // a NaN score stays out of m and poisons its weight
+        }
+        top = column_max(top);
+        // m trails the maximum by at most 8: weights stay below 2^8.
+        if (__any(top > m + 8.f)) {
+          const float mn = __builtin_fmaxf(m, top);
+          const float f = __builtin_amdgcn_exp2f(m - (mn == -__builtin_inff() ? 0.f : mn));
+          m = mn;
+          l *= f;
+#pragma unroll
+          for (int x = 0; x < kF; ++x) acc[x] *= f;
+        }
+        const float ms = m == -__builtin_inff() ? 0.f : m;
+#pragma unroll
+        for (int j = 0; j < kTiles * 4; ++j) {
+          const bool seen = p[j] != -__builtin_inff();
+          p[j] = __builtin_amdgcn_exp2f(p[j] - ms);
+          l += p[j];
+          // An infinite value of a key whose weight fp16 cannot hold is infinite all the same.
+          if (high_only && seen && p[j] < 0x1p-24f) p[j] = 0x1p-24f;
+        }
+        if constexpr (k16) {
+          typedef typename Mfma16<T>::vec vec;
+          typedef typename Mfma16<T>::e elem;
+          vec hi, lo;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            hi[j] = elem(p[j]);
+            lo[j] = elem(p[j] - float(hi[j]));
+          }
+#pragma unroll
+          for (int x = 0; x < kF; ++x) {
+            // Feature x of the lane's eight keys: halves of words x / 2.
+            const uint32_t sel = x % 2 ? 0x07060302u : 0x05040100u;
+            u32x4_t av;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              av[j] = __builtin_amdgcn_perm(vr[2 * j + 1][x / 2], vr[2 * j][x / 2], sel);
+            acc[x] = Mfma16<T>::run(__builtin_bit_cast(vec, av), hi, acc[x]);
+            if (!high_only) acc[x] = Mfma16<T>::run(__builtin_bit_cast(vec, av), lo, acc[x]);
+          }
+        } else {
+#pragma unroll
+          for (int x = 0; x < kF; ++x)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              acc[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_to_float(vr[j][x]), p[j], acc[x],
+                                                            0, 0, 0);
+        }
+        if (i + 1 < steps) load_v(key0 + kUnit);
+      }
+      if (!k16 || high_only) break;
+      bool nan = false;
+#pragma unroll
+      for (int x = 0; x < kF; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) nan |= acc[x][e] != acc[x][e];
+      if (!__any(nan)) break;
+      high_only = true;
+    }
+    l = column_sum(l);
+
+    if (threadIdx.x == 0) sbad = 0;
+    __syncthreads();
+    if (bad) sbad = 1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int x = 0; x < kF; x += 4)
+        *reinterpret_cast<f32x4_t*>(&sO[wave][c][(4 * kg + e) * kF + x]) =
+            f32x4_t{acc[x][e], acc[x + 1][e], acc[x + 2][e], acc[x + 3][e]};
+    if (kg == 0) {
+      sm[wave][c] = m;
+      sl[wave][c] = l;
+    }
+    __syncthreads();
+    finish<T>(a, D, &sO[0][0][0], kStride, kTileHeads * kStride, &sm[0][0], &sl[0][0], kTileHeads,
               rows, count == units, 2 * int64_t(blockIdx.x) + (u > begin), req, hk * a.G + r0,
               keys == 0, sbad != 0);
     __syncthreads();
@@ -250,25 +561,67 @@ __global__ __launch_bounds__(kPagedThreads) void paged_merge_kernel(PagedArgs a)
 
 static int64_t round256(int64_t x) { return (x + 255) / 256 * 256; }
 
-int64_t plan_paged_attn(int dtype, PagedArgs& a) {
-  (void)dtype;
-  const int64_t unit = kRowUnit, tile = kRowTile;
+// Whether the matrix-core form takes these rows: whole 16-byte pieces, and
+// offsets within a page of 31 bits.
+static bool tile_form(int dtype, const PagedArgs& a) {
+  if (a.D != 64 && a.D != 128) return false;
+  const int64_t es = dtype == kF32 ? 4 : 2, piece = 16 / es;
+  for (const void* p : {a.q, a.k, a.v})
+    if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+  for (int64_t s : {a.qn, a.qh, a.kp, a.kn, a.kh, a.vp, a.vn, a.vh})
+    if (s < 0 || s % piece) return false;
+  for (int64_t s : {a.kn, a.vn})
+    if (s >= (int64_t(1) << 31) / a.page) return false;
+  return true;
+}
+
+// The work for `unit` keys a unit and `tile` heads a tile; its workspace bytes.
+static int64_t plan_form(PagedArgs& a, int64_t unit, int64_t tile, int64_t groups) {
   a.tiles = (a.G + tile - 1) / tile;
   a.rows = (a.G + a.tiles - 1) / a.tiles;
   const int64_t longest = (a.M * a.page + unit - 1) / unit;
   const int64_t most = a.N * a.Hk * a.tiles * (longest > 1 ? longest : 1);  // units, at most
   if (most >= (int64_t(1) << 31)) return -1;
-  a.groups = most < 2048 ? most : 2048;
+  a.groups = most < groups ? most : groups;
   a.by_page = FastDiv(uint32_t(a.page));
   // Pairs and rows of 2 * groups partial slots, and the requests' first units.
   return round256((4 * a.groups * a.rows + 3) / 4 * 16 + 2 * a.groups * a.rows * a.D * 4) +
          round256(8 * (a.N + 1));
 }
+static int64_t plan_tiles(int dtype, PagedArgs& a) {
+  return plan_form(a, dtype == kF32 ? kTileUnit<float> : kTileUnit<bf16_t>, kTileHeads, 512);
+}
+static int64_t plan_rows(PagedArgs& a) { return plan_form(a, kRowUnit, kRowTile, 2048); }
+
+int64_t paged_attn_workspace(int dtype, PagedArgs a) {
+  // Which form runs depends on the tensors' alignment too: enough for either.
+  const int64_t rows = plan_rows(a), tiles = plan_tiles(dtype, a);
+  return rows < 0 || tiles < 0 ? -1 : rows > tiles ? rows : tiles;
+}
+
+template <typename T, int D>
+static void launch_tiles(const PagedArgs& a, hipStream_t stream) {
+  const dim3 grid{unsigned(a.groups)}, block{kPagedThreads};
+  if (a.page % 16 == 0)
+    hipLaunchKernelGGL((paged_tile_kernel<T, D, true>), grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((paged_tile_kernel<T, D, false>), grid, block, 0, stream, a);
+}
 
 template <typename T>
-static hipError_t launch_paged_t(const PagedArgs& a, hipStream_t stream) {
+static hipError_t launch_paged_t(int dtype, PagedArgs& a, void* workspace, hipStream_t stream) {
+  const bool tiles = tile_form(dtype, a);
+  const int64_t need = tiles ? plan_tiles(dtype, a) : plan_rows(a);
+  if (need < 0) return hipErrorInvalidValue;
+  a.part = static_cast<float*>(workspace);
+  a.start = reinterpret_cast<int64_t*>(static_cast<char*>(workspace) + need -
+                                       round256(8 * (a.N + 1)));
   const dim3 grid{unsigned(a.groups)}, block{kPagedThreads};
-  if (a.D <= 64)
+  if (tiles && a.D == 64)
+    launch_tiles<T, 64>(a, stream);
+  else if (tiles)
+    launch_tiles<T, 128>(a, stream);
+  else if (a.D <= 64)
     hipLaunchKernelGGL((paged_row_kernel<T, 1>), grid, block, 0, stream, a);
   else if (a.D <= 128)
     hipLaunchKernelGGL((paged_row_kernel<T, 2>), grid, block, 0, stream, a);
@@ -282,14 +635,9 @@ static hipError_t launch_paged_t(const PagedArgs& a, hipStream_t stream) {
 }
 
 hipError_t launch_paged_attn(int dtype, PagedArgs a, void* workspace, hipStream_t stream) {
-  const int64_t need = plan_paged_attn(dtype, a);
-  if (need < 0) return hipErrorInvalidValue;
-  a.part = static_cast<float*>(workspace);
-  a.start = reinterpret_cast<int64_t*>(static_cast<char*>(workspace) + need -
-                                       round256(8 * (a.N + 1)));
-  if (dtype == kBF16) return launch_paged_t<bf16_t>(a, stream);
-  if (dtype == kF16) return launch_paged_t<f16_t>(a, stream);
-  return launch_paged_t<float>(a, stream);
+  if (dtype == kBF16) return launch_paged_t<bf16_t>(dtype, a, workspace, stream);
+  if (dtype == kF16) return launch_paged_t<f16_t>(dtype, a, workspace, stream);
+  return launch_paged_t<float>(dtype, a, workspace, stream);
 }
 
 }  // namespace va

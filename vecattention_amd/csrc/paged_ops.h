@@ -76,9 +76,9 @@ struct PagedArgs {
   int64_t* start;            // first unit of request i, [N + 1]
   FastDiv by_page;
 };
-// The launch for these sizes (host only): fills tiles, rows and groups of `a`;
-// returns the workspace bytes it needs, -1 where the units do not fit 31 bits.
-int64_t plan_paged_attn(int dtype, PagedArgs& a);
+// Workspace bytes for these sizes (N, Hk, G, D, M, page), -1 where the units do
+// not fit 31 bits.
+int64_t paged_attn_workspace(int dtype, PagedArgs a);
 hipError_t launch_paged_attn(int dtype, PagedArgs a, void* workspace, hipStream_t stream);
 
 }  // namespace va
