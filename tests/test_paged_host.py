@@ -43,14 +43,14 @@ int main() {
     check(0x7fffffffu);
   }
   // every unit has one owner, shares are in order and differ by at most one
-  for (int64_t total : {1, 2, 7, 100, 1023, 4096, 100003})
-    for (int64_t groups : {1, 2, 3, 64, 511, 512, 2048}) {
+  for (uint32_t total : {1, 2, 7, 100, 1023, 4096, 100003})
+    for (uint32_t groups : {1, 2, 3, 64, 511, 512, 2048}) {
       const va::PagedShare s(total, groups);
       if (s.begin(0) != 0 || s.begin(groups) != total) { printf("BAD ends\n"); return 1; }
-      for (int64_t w = 0; w < groups; ++w) {
-        const int64_t n = s.begin(w + 1) - s.begin(w);
+      for (uint32_t w = 0; w < groups; ++w) {
+        const uint32_t n = s.begin(w + 1) - s.begin(w);
         if (n < total / groups || n > total / groups + 1) { printf("BAD share\n"); return 1; }
-        for (int64_t u = s.begin(w); u < s.begin(w + 1); ++u)
+        for (uint32_t u = s.begin(w); u < s.begin(w + 1); ++u)
           if (s.owner(u) != w) { printf("BAD owner\n"); return 1; }
       }
     }

@@ -67,18 +67,17 @@ __host__ __device__ inline int64_t plan_slot(const PlanRow& r, uint32_t pos, uin
 // query heads); its keys are cut into units of `unit` keys, at least one per
 // segment, so that an empty request's rows have a writer.  The units of all
 // segments in order are dealt to `groups` work-groups in contiguous shares whose
-// sizes differ by at most one.
+// sizes differ by at most one.  Fewer than 2^31 units: a 64-bit division
+// costs a wave half a microsecond.
 struct PagedShare {
-  int64_t total, groups;
-  __host__ __device__ PagedShare(int64_t t, int64_t g) : total(t), groups(g) {}
-  __host__ __device__ int64_t begin(int64_t w) const {
-    const int64_t q = total / groups, r = total % groups;
-    return w * q + (w < r ? w : r);
-  }
+  uint32_t groups, each, more;  // the first `more` shares hold one unit more than `each`
+  __host__ __device__ PagedShare(uint32_t total, uint32_t g)
+      : groups(g), each(total / g), more(total - each * g) {}
+  __host__ __device__ uint32_t begin(uint32_t w) const { return w * each + (w < more ? w : more); }
   // Work-group whose share holds unit u.
-  __host__ __device__ int64_t owner(int64_t u) const {
-    const int64_t q = total / groups, r = total % groups, cut = r * (q + 1);
-    return u < cut ? u / (q + 1) : r + (u - cut) / q;  // q > 0 where u >= cut
+  __host__ __device__ uint32_t owner(uint32_t u) const {
+    const uint32_t cut = more * (each + 1);
+    return u < cut ? u / (each + 1) : more + (u - cut) / each;  // each > 0 where u >= cut
   }
 };
 
@@ -87,8 +86,8 @@ struct PagedShare {
 __host__ __device__ inline int32_t paged_keys(int32_t len, int64_t capacity) {
   return len <= 0 ? 0 : int64_t(len) > capacity ? -1 : len;
 }
-__host__ __device__ inline int64_t paged_units(int32_t keys, int unit) {
-  return keys <= 0 ? 1 : (int64_t(keys) + unit - 1) / unit;
+__host__ __device__ inline uint32_t paged_units(int32_t keys, uint32_t unit) {
+  return keys <= 0 ? 1 : (uint32_t(keys) + unit - 1) / unit;
 }
 
 }  // namespace va

@@ -25,58 +25,62 @@ __device__ inline float2* part_ml(const PagedArgs& a, int64_t slot) {
   return reinterpret_cast<float2*>(a.part) + slot * a.rows;
 }
 __device__ inline float* part_row(const PagedArgs& a, int64_t slot, int64_t row) {
-  return a.part + (4 * a.groups * a.rows + 3) / 4 * 4 + (slot * a.rows + row) * a.D;
+  return a.part + 4 * int64_t(a.groups) * a.rows + (slot * a.rows + row) * a.D;
 }
 
-// Where a work-group's share begins.
+// Where a work-group's share begins and ends, and the request of its first unit.
 struct Place {
-  int64_t total, request, start;  // units of all requests; the first request and its first unit
+  uint32_t begin, end;
+  uint32_t base;     // first unit of the request
+  int32_t request, keys;
+};
+struct PlaceLds {
+  uint32_t sum[kPagedWaves], base;
+  int32_t request, keys;
 };
 
 // Sums the units of the requests (every work-group does, N lengths from L2) and
 // finds the request of the share's first unit.  The first work-group leaves
 // the sums for the merge.
 template <int kUnit>
-__device__ inline Place locate(const PagedArgs& a, int64_t (*lds)[2]) {
-  const int64_t capacity = a.M * a.page, per_segment = a.Hk * a.tiles;
-  const int64_t per = (a.N + kPagedThreads - 1) / kPagedThreads;
-  const int64_t lo = threadIdx.x * per < a.N ? threadIdx.x * per : a.N;
-  const int64_t hi = lo + per < a.N ? lo + per : a.N;
-  int64_t mine = 0;
-  for (int64_t i = lo; i < hi; ++i)
-    mine += per_segment * paged_units(paged_keys(a.lens[i], capacity), kUnit);
-  const int lane = threadIdx.x % 64, w = threadIdx.x / 64;
-  int64_t sum = mine;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t u = __shfl_up(sum, d);
-    if (lane >= d) sum += u;
+__device__ inline Place locate(const PagedArgs& a, PlaceLds& lds) {
+  const int64_t capacity = a.M * a.page;
+  const int32_t N = int32_t(a.N), per = (N + kPagedThreads - 1) / kPagedThreads;
+  const int32_t lo = int32_t(threadIdx.x) * per;
+  uint32_t mine = 0;
+  int32_t keys = 0;
+  for (int32_t i = lo; i < lo + per && i < N; ++i) {
+    keys = paged_keys(a.lens[i], capacity);
+    mine += a.per_request * paged_units(keys, kUnit);
   }
-  if (lane == 63) lds[w][0] = sum;
+  const int lane = threadIdx.x % 64, w = threadIdx.x / 64;
+  const uint32_t sum = uint32_t(wave_inclusive_sum(int(mine)));
+  if (lane == 63) lds.sum[w] = sum;
   __syncthreads();
-  int64_t before = 0, total = 0;
+  uint32_t at = sum - mine, total = 0;
 #pragma unroll
   for (int i = 0; i < kPagedWaves; ++i) {
-    if (i < w) before += lds[i][0];
-    total += lds[i][0];
+    if (i < w) at += lds.sum[i];
+    total += lds.sum[i];
   }
-  int64_t at = before + sum - mine;
-  const int64_t begin = PagedShare(total, a.groups).begin(blockIdx.x);
+  const PagedShare share(total, uint32_t(a.groups));
+  const uint32_t begin = share.begin(blockIdx.x);
   const bool first = blockIdx.x == 0;
-  __syncthreads();
   if (first || (begin >= at && begin < at + mine))
-    for (int64_t i = lo; i < hi; ++i) {
-      const int64_t n = per_segment * paged_units(paged_keys(a.lens[i], capacity), kUnit);
+    for (int32_t i = lo; i < lo + per && i < N; ++i) {
+      if (per > 1) keys = paged_keys(a.lens[i], capacity);
+      const uint32_t n = a.per_request * paged_units(keys, kUnit);
       if (first) a.start[i] = at;
       if (begin >= at && begin < at + n) {
-        lds[0][0] = i;
-        lds[0][1] = at;
+        lds.request = i;
+        lds.base = at;
+        lds.keys = keys;
       }
       at += n;
     }
-  if (first && threadIdx.x == 0) a.start[a.N] = total;
+  if (first && threadIdx.x == 0) a.start[N] = total;
   __syncthreads();
-  return Place{total, lds[0][0], lds[0][1]};
+  return Place{begin, share.begin(blockIdx.x + 1), lds.base, lds.request, lds.keys};
 }
 
 // Merges the waves' states of a segment's rows and writes them: to the output
@@ -119,22 +123,22 @@ constexpr int kRowUnit = 128;   // keys of a unit: 32 for each wave
 constexpr int kRowMaxD = 256;
 template <typename T, int NF>
 __global__ __launch_bounds__(kPagedThreads) void paged_row_kernel(PagedArgs a) {
-  __shared__ int64_t place[kPagedWaves][2];
+  __shared__ PlaceLds place;
   __shared__ float sO[kPagedWaves][kRowTile][kRowMaxD], sm[kPagedWaves][kRowTile],
       sl[kPagedWaves][kRowTile];
   __shared__ int sbad;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const Place pl = locate<kRowUnit>(a, place);
-  const PagedShare share(pl.total, a.groups);
-  const int64_t begin = share.begin(blockIdx.x), end = share.begin(blockIdx.x + 1);
+  const uint32_t begin = pl.begin, end = pl.end;
   const int64_t capacity = a.M * a.page;
-  int64_t req = pl.request, base = pl.start;
-  for (int64_t u = begin; u < end;) {
-    const int32_t keys = paged_keys(a.lens[req], capacity);
-    const int64_t units = paged_units(keys, kRowUnit);
-    const int64_t seg = (u - base) / units, c0 = (u - base) % units;
-    const int64_t count = end - u < units - c0 ? end - u : units - c0;
-    const int64_t hk = seg / a.tiles, r0 = seg % a.tiles * a.rows;
+  int64_t req = pl.request;
+  int32_t keys = pl.keys;
+  uint32_t base = pl.base;
+  for (uint32_t u = begin; u < end;) {
+    const uint32_t units = paged_units(keys, kRowUnit);
+    const uint32_t seg = (u - base) / units, c0 = (u - base) - seg * units;
+    const uint32_t count = end - u < units - c0 ? end - u : units - c0;
+    const int32_t hk = int32_t(seg) / a.tiles, r0 = (int32_t(seg) - hk * a.tiles) * a.rows;
     const int rows = int(a.G - r0 < a.rows ? a.G - r0 : a.rows);
     float q[kRowTile][NF], acc[kRowTile][NF], m[kRowTile], l[kRowTile];
 #pragma unroll
@@ -152,7 +156,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_row_kernel(PagedArgs a) {
       }
     }
     bool bad = keys < 0;
-    for (int64_t c = c0; c < c0 + count; ++c) {
+    for (int64_t c = c0; c < int64_t(c0) + count; ++c) {
       const int64_t k0 = c * kRowUnit + wave * 32;
       const int64_t k1 = k0 + 32 < keys ? k0 + 32 : keys;
       for (int64_t key = k0; key < k1; ++key) {
@@ -208,9 +212,9 @@ __global__ __launch_bounds__(kPagedThreads) void paged_row_kernel(PagedArgs a) {
               keys == 0, sbad != 0);
     __syncthreads();
     u += count;
-    if (u == base + units * a.Hk * a.tiles) {
+    if (u < end && u == base + units * a.per_request) {
       base = u;
-      ++req;
+      keys = paged_keys(a.lens[++req], capacity);
     }
   }
 }
@@ -282,7 +286,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_tile_kernel(PagedArgs a) 
   constexpr int kKL = k16 ? D / 32 : D / 16;       // 16-byte loads of a lane in a row of K
   constexpr int kVW = kF * int(sizeof(T)) / 4;     // words of a lane in a row of V
   constexpr int kStride = D + 4;
-  __shared__ int64_t place[kPagedWaves][2];
+  __shared__ PlaceLds place;
   __shared__ __align__(16) float sO[kPagedWaves][kTileHeads][kStride];
   __shared__ float sm[kPagedWaves][kTileHeads], sl[kPagedWaves][kTileHeads];
   __shared__ int sbad;
@@ -291,17 +295,17 @@ __global__ __launch_bounds__(kPagedThreads) void paged_tile_kernel(PagedArgs a) 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int kg = lane / 16, c = lane % 16;
   const Place pl = locate<kUnit>(a, place);
-  const PagedShare share(pl.total, a.groups);
-  const int64_t begin = share.begin(blockIdx.x), end = share.begin(blockIdx.x + 1);
+  const uint32_t begin = pl.begin, end = pl.end;
   const int64_t capacity = a.M * a.page;
   const uint32_t page = uint32_t(a.page);
-  int64_t req = pl.request, base = pl.start;
-  for (int64_t u = begin; u < end;) {
-    const int32_t keys = paged_keys(a.lens[req], capacity);
-    const int64_t units = paged_units(keys, kUnit);
-    const int64_t seg = (u - base) / units, c0 = (u - base) % units;
-    const int64_t count = end - u < units - c0 ? end - u : units - c0;
-    const int64_t hk = seg / a.tiles, r0 = seg % a.tiles * a.rows;
+  int64_t req = pl.request;
+  int32_t keys = pl.keys;
+  uint32_t base = pl.base;
+  for (uint32_t u = begin; u < end;) {
+    const uint32_t units = paged_units(keys, kUnit);
+    const uint32_t seg = (u - base) / units, c0 = (u - base) - seg * units;
+    const uint32_t count = end - u < units - c0 ? end - u : units - c0;
+    const int32_t hk = int32_t(seg) / a.tiles, r0 = (int32_t(seg) - hk * a.tiles) * a.rows;
     const int rows = int(a.G - r0 < a.rows ? a.G - r0 : a.rows);
     const int32_t* table = a.table + req * a.table_stride;
     const T* kbase = static_cast<const T*>(a.k) + hk * a.kh;
@@ -318,11 +322,11 @@ __global__ __launch_bounds__(kPagedThreads) void paged_tile_kernel(PagedArgs a) 
     }
     bool bad = keys < 0;
     const uint32_t last = keys > 0 ? uint32_t(keys) - 1 : 0;
-    const uint32_t first = uint32_t(c0) * kUnit + wave * kKeys;
+    const uint32_t first = c0 * kUnit + wave * kKeys;
     int steps = 0;
     if (keys > 0 && first <= last) {
       const uint32_t left = (last - first) / kUnit + 1;
-      steps = left < uint32_t(count) ? int(left) : int(count);
+      steps = int(left < count ? left : count);
     }
 
     Pages<kTiles> pg;
@@ -518,45 +522,78 @@ __global__ __launch_bounds__(kPagedThreads) void paged_tile_kernel(PagedArgs a) 
               keys == 0, sbad != 0);
     __syncthreads();
     u += count;
-    if (u == base + units * a.Hk * a.tiles) {
+    if (u < end && u == base + units * a.per_request) {
       base = u;
-      ++req;
+      keys = paged_keys(a.lens[++req], capacity);
     }
   }
 }
 
 // Rows of segments that several work-groups share: one work-group of 256
-// threads per (segment, row); the partials go in the work-groups' order.
-template <typename T>
+// threads per (segment, row).  kV features a thread, and as many partials side by
+// side as that leaves threads for, each walked with the loads of U in flight;
+// then their sums, always in the same order.
+template <typename T, int kV>
 __global__ __launch_bounds__(kPagedThreads) void paged_merge_kernel(PagedArgs a) {
-  const int64_t seg = blockIdx.x, r = blockIdx.y, per_request = a.Hk * a.tiles;
-  const int64_t n = seg / per_request, s = seg % per_request;
-  const int64_t hk = s / a.tiles, head = s % a.tiles * a.rows + r;
+  typedef float vec __attribute__((ext_vector_type(kV)));
+  constexpr int U = 4;
+  __shared__ vec sacc[kPagedThreads];
+  __shared__ float smax[kPagedThreads], sden[kPagedThreads];
+  const uint32_t r = blockIdx.y, n = blockIdx.x / a.per_request;
+  const uint32_t s = blockIdx.x - n * a.per_request, hk = s / a.tiles;
+  const uint32_t head = (s - hk * a.tiles) * a.rows + r;
   if (head >= a.G) return;
-  const int64_t base = a.start[n], units = (a.start[n + 1] - base) / per_request;
-  const int64_t u0 = base + s * units, u1 = u0 + units;
+  const uint32_t base = a.start[n], units = (a.start[n + 1] - base) / a.per_request;
+  const uint32_t u0 = base + s * units, u1 = u0 + units;
   const PagedShare share(a.start[a.N], a.groups);
-  const int64_t w0 = share.owner(u0), w1 = share.owner(u1 - 1);
+  const uint32_t w0 = share.owner(u0), w1 = share.owner(u1 - 1);
   if (w0 == w1) return;  // written whole
-  const int64_t first = 2 * w0 + (share.begin(w0) < u0);
-  for (int f = threadIdx.x; f < a.D; f += kPagedThreads) {
-    float m = -__builtin_inff();
-    for (int64_t w = w0; w <= w1; ++w) {
-      const float2 ml = part_ml(a, w == w0 ? first : 2 * w)[r];
-      if (!(ml.y == 0.f)) m = __builtin_fmaxf(m, ml.x);
+  const uint32_t first = 2 * w0 + (share.begin(w0) < u0);
+  const int lanes = int(a.D) / kV, side = kPagedThreads / lanes;
+  const int p = threadIdx.x / lanes, c = threadIdx.x - p * lanes;
+  float m = -__builtin_inff(), l = 0.f;
+  vec acc = vec(0.f);
+  if (p < side)
+    for (uint32_t w = w0 + p; w <= w1; w += side * U) {
+      float2 st[U];
+      vec x[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const uint32_t at = w + i * side;
+        const int64_t slot = at == w0 ? first : 2 * at;
+        st[i] = at <= w1 ? part_ml(a, slot)[r] : make_float2(0.f, 0.f);
+        x[i] = at <= w1 ? reinterpret_cast<const vec*>(part_row(a, slot, r))[c] : vec(0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        if (st[i].y == 0.f) continue;  // no key of any weight
+        const float mn = __builtin_fmaxf(m, st[i].x);
+        const float ms = mn == -__builtin_inff() ? 0.f : mn;
+        const float f = __builtin_amdgcn_exp2f(m - ms), g = __builtin_amdgcn_exp2f(st[i].x - ms);
+        l = l * f + g * st[i].y;
+        acc = acc * f + g * x[i];
+        m = mn;
+      }
     }
-    float l = 0.f, o = 0.f;
-    for (int64_t w = w0; w <= w1; ++w) {
-      const int64_t slot = w == w0 ? first : 2 * w;
-      const float2 ml = part_ml(a, slot)[r];
-      if (ml.y == 0.f) continue;
-      const float c = __builtin_amdgcn_exp2f(ml.x - m);
-      l += c * ml.y;
-      o += c * part_row(a, slot, r)[f];
-    }
-    T* out = static_cast<T*>(a.out) + n * a.on + (hk * a.G + head) * a.oh;
-    out[f] = Round<T>::store(o / l);
+  sacc[threadIdx.x] = acc;
+  smax[threadIdx.x] = m;
+  sden[threadIdx.x] = l;
+  __syncthreads();
+  if (p != 0) return;
+  m = -__builtin_inff();
+  for (int i = 0; i < side; ++i) m = __builtin_fmaxf(m, smax[i * lanes + c]);
+  l = 0.f;
+  acc = vec(0.f);
+  for (int i = 0; i < side; ++i) {
+    const float li = sden[i * lanes + c];
+    if (li == 0.f) continue;
+    const float f = __builtin_amdgcn_exp2f(smax[i * lanes + c] - m);
+    l += f * li;
+    acc += f * sacc[i * lanes + c];
   }
+  T* out = static_cast<T*>(a.out) + n * a.on + (hk * a.G + head) * a.oh + c * kV;
+#pragma unroll
+  for (int i = 0; i < kV; ++i) out[i] = Round<T>::store(acc[i] / l);
 }
 
 static int64_t round256(int64_t x) { return (x + 255) / 256 * 256; }
@@ -577,16 +614,16 @@ static bool tile_form(int dtype, const PagedArgs& a) {
 
 // The work for `unit` keys a unit and `tile` heads a tile; its workspace bytes.
 static int64_t plan_form(PagedArgs& a, int64_t unit, int64_t tile, int64_t groups) {
-  a.tiles = (a.G + tile - 1) / tile;
-  a.rows = (a.G + a.tiles - 1) / a.tiles;
+  a.tiles = int32_t((a.G + tile - 1) / tile);
+  a.rows = int32_t((a.G + a.tiles - 1) / a.tiles);
   const int64_t longest = (a.M * a.page + unit - 1) / unit;
   const int64_t most = a.N * a.Hk * a.tiles * (longest > 1 ? longest : 1);  // units, at most
   if (most >= (int64_t(1) << 31)) return -1;
-  a.groups = most < groups ? most : groups;
+  a.groups = int32_t(most < groups ? most : groups);
+  a.per_request = int32_t(a.Hk * a.tiles);
   a.by_page = FastDiv(uint32_t(a.page));
   // Pairs and rows of 2 * groups partial slots, and the requests' first units.
-  return round256((4 * a.groups * a.rows + 3) / 4 * 16 + 2 * a.groups * a.rows * a.D * 4) +
-         round256(8 * (a.N + 1));
+  return round256(2 * int64_t(a.groups) * a.rows * (8 + 4 * a.D)) + round256(4 * (a.N + 1));
 }
 static int64_t plan_tiles(int dtype, PagedArgs& a) {
   return plan_form(a, dtype == kF32 ? kTileUnit<float> : kTileUnit<bf16_t>, kTileHeads, 512);
@@ -614,8 +651,8 @@ static hipError_t launch_paged_t(int dtype, PagedArgs& a, void* workspace, hipSt
   const int64_t need = tiles ? plan_tiles(dtype, a) : plan_rows(a);
   if (need < 0) return hipErrorInvalidValue;
   a.part = static_cast<float*>(workspace);
-  a.start = reinterpret_cast<int64_t*>(static_cast<char*>(workspace) + need -
-                                       round256(8 * (a.N + 1)));
+  a.start = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + need -
+                                        round256(4 * (a.N + 1)));
   const dim3 grid{unsigned(a.groups)}, block{kPagedThreads};
   if (tiles && a.D == 64)
     launch_tiles<T, 64>(a, stream);
@@ -629,8 +666,11 @@ static hipError_t launch_paged_t(int dtype, PagedArgs& a, void* workspace, hipSt
     hipLaunchKernelGGL((paged_row_kernel<T, 4>), grid, block, 0, stream, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(paged_merge_kernel<T>, dim3(unsigned(a.N * a.Hk * a.tiles), unsigned(a.rows)),
-                     block, 0, stream, a);
+  const dim3 segments{unsigned(a.N * a.per_request), unsigned(a.rows)};
+  if (a.D % 4 == 0)
+    hipLaunchKernelGGL((paged_merge_kernel<T, 4>), segments, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((paged_merge_kernel<T, 1>), segments, block, 0, stream, a);
   return hipGetLastError();
 }
 

@@ -70,10 +70,11 @@ struct PagedArgs {
   int64_t N, Hk, G;          // G query heads per kv head
   int64_t D, page, num_pages;
   float scale_log2;
-  int64_t tiles, rows;       // tiles of at most `rows` query heads per kv head
-  int64_t groups;            // work-groups the units are dealt to
+  int32_t tiles, rows;       // tiles of at most `rows` query heads per kv head
+  int32_t groups;            // work-groups the units are dealt to
+  int32_t per_request;       // segments of a request: Hk * tiles
   float* part;               // partial rows, see paged_attn.hip
-  int64_t* start;            // first unit of request i, [N + 1]
+  uint32_t* start;           // first unit of request i, [N + 1]
   FastDiv by_page;
 };
 // Workspace bytes for these sizes (N, Hk, G, D, M, page), -1 where the units do
