@@ -93,6 +93,22 @@ def test_index_arithmetic(tmp_path):
     assert out.returncode == 0 and out.stdout.strip() == "OK", out.stdout + out.stderr
 
 
+def test_no_matrix_result_is_read_too_soon(tmp_path):
+    from asm_hazards import early_reads
+    from vecattention_amd import build
+    # The checker itself: a branch straight to the read is found, a wait before it is enough.
+    body = ("_Zk:\n v_mfma_f32_16x16x4_f32 a[0:3], v1, v2, a[0:3]\n s_cbranch_vccnz .LBB0_1\n"
+            " s_nop 15\n.LBB0_1:\n{} v_accvgpr_read_b32 v3, a3\n s_endpgm\n")
+    assert len(early_reads(body.format(""))[1]) == 1
+    assert early_reads(body.format(" s_nop 9\n")) == (1, [])
+    out = tmp_path / "paged_attn.s"
+    subprocess.run([build.hipcc(), *build.FLAGS, "--cuda-device-only", "-S",
+                    os.path.join(CSRC, "paged_attn.hip"), "-o", str(out)], check=True,
+                   capture_output=True)
+    count, early = early_reads(out.read_text())
+    assert count > 300 and early == []
+
+
 def test_plain_plan_by_hand():
     table, lens, indptr, slots, pos, req, taken = ref.plan(
         [3, 0, 4], [2, 0, 5], [[8, -1, -1], [-1, -1, -1], [5, -1, -1]], [1, 2, 3], 4, 8)

@@ -9,9 +9,10 @@
 // which a second launch merges in order (no atomics: the same lengths give the
 // same bits).
 //
-// Partial slots: work-group w writes the segment its share begins with (begun
-// before) to slot 2w, and a later one its share ends in to slot 2w + 1.  Slot s
-// holds `rows` pairs (m, l), and `rows` unnormalised fp32 rows of D.
+// Partial slots: work-group w writes the segment its share begins with to slot
+// 2w, and a later one its share ends in to slot 2w + 1.  Slot s holds `rows` pairs
+// (m, l), and `rows` unnormalised fp32 rows of D.  The work-group that a segment
+// begins in leaves the segment's first slot and last work-group for the merge.
 #include "common.h"
 #include "lanes.h"
 #include "mfma.h"
@@ -30,6 +31,7 @@ __device__ inline float* part_row(const PagedArgs& a, int64_t slot, int64_t row)
 
 // Where a work-group's share begins and ends, and the request of its first unit.
 struct Place {
+  PagedShare share;
   uint32_t begin, end;
   uint32_t base;     // first unit of the request
   int32_t request, keys;
@@ -40,8 +42,7 @@ struct PlaceLds {
 };
 
 // Sums the units of the requests (every work-group does, N lengths from L2) and
-// finds the request of the share's first unit.  The first work-group leaves
-// the sums for the merge.
+// finds the request of the share's first unit.
 template <int kUnit>
 __device__ inline Place locate(const PagedArgs& a, PlaceLds& lds) {
   const int64_t capacity = a.M * a.page;
@@ -65,53 +66,64 @@ __device__ inline Place locate(const PagedArgs& a, PlaceLds& lds) {
   }
   const PagedShare share(total, uint32_t(a.groups));
   const uint32_t begin = share.begin(blockIdx.x);
-  const bool first = blockIdx.x == 0;
-  if (first || (begin >= at && begin < at + mine))
+  if (begin >= at && begin < at + mine)
     for (int32_t i = lo; i < lo + per && i < N; ++i) {
       if (per > 1) keys = paged_keys(a.lens[i], capacity);
       const uint32_t n = a.per_request * paged_units(keys, kUnit);
-      if (first) a.start[i] = at;
-      if (begin >= at && begin < at + n) {
+      if (begin < at + n) {
         lds.request = i;
         lds.base = at;
         lds.keys = keys;
+        break;
       }
       at += n;
     }
-  if (first && threadIdx.x == 0) a.start[N] = total;
   __syncthreads();
-  return Place{begin, share.begin(blockIdx.x + 1), lds.base, lds.request, lds.keys};
+  return Place{share, begin, share.begin(blockIdx.x + 1), lds.base, lds.request, lds.keys};
 }
 
 // Merges the waves' states of a segment's rows and writes them: to the output
-// (`whole`), or to a partial slot.  sO[wave][row][stride], sm/sl[wave][row].
-template <typename T>
-__device__ inline void finish(const PagedArgs& a, int D, const float* sO, int rstride, int wstride,
-                              const float* sm, const float* sl, int mstride, int rows, bool whole,
-                              int64_t slot, int64_t request, int64_t head, bool empty, bool bad) {
-  for (int i = threadIdx.x; i < rows * D; i += kPagedThreads) {
-    const int r = i / D, f = i % D;
-    float m = -__builtin_inff();
-#pragma unroll
-    for (int w = 0; w < kPagedWaves; ++w)
-      if (!(sl[w * mstride + r] == 0.f)) m = __builtin_fmaxf(m, sm[w * mstride + r]);
-    float l = 0.f, o = 0.f;
+// (`whole`), or to a partial slot.  sO[wave][row][stride], sm/sl[wave][row];
+// kV features of a row a thread.
+template <typename T, int kV>
+__device__ inline void finish(const PagedArgs& a, int D, const float* sO, int rstride,
+                              int wstride, const float* sm, const float* sl, int mstride, int rows,
+                              bool whole, int64_t slot, int64_t request, int64_t head, bool empty,
+                              bool bad) {
+  typedef float vec __attribute__((ext_vector_type(kV)));
+  const int pieces = D / kV;
+  for (int i = threadIdx.x; i < rows * pieces; i += kPagedThreads) {
+    const int r = i / pieces, f = (i - r * pieces) * kV;
+    float lw[kPagedWaves], mw[kPagedWaves], m = -__builtin_inff();
+    vec ow[kPagedWaves];
 #pragma unroll
     for (int w = 0; w < kPagedWaves; ++w) {
-      const float lw = sl[w * mstride + r];
-      if (lw == 0.f) continue;  // no key seen, or none of any weight
-      const float c = __builtin_amdgcn_exp2f(sm[w * mstride + r] - m);
-      l += c * lw;
-      o += c * sO[w * wstride + r * rstride + f];
+      lw[w] = sl[w * mstride + r];
+      mw[w] = sm[w * mstride + r];
+      ow[w] = *reinterpret_cast<const vec*>(sO + w * wstride + r * rstride + f);
+    }
+#pragma unroll
+    for (int w = 0; w < kPagedWaves; ++w)
+      if (!(lw[w] == 0.f)) m = __builtin_fmaxf(m, mw[w]);
+    float l = 0.f;
+    vec o = vec(0.f);
+#pragma unroll
+    for (int w = 0; w < kPagedWaves; ++w) {
+      const float c = __builtin_amdgcn_exp2f(mw[w] - m);
+      if (lw[w] == 0.f) continue;  // no key seen, or none of any weight
+      l += c * lw[w];
+      o += c * ow[w];
     }
     if (bad) l = __builtin_nanf("");
     if (whole) {
       // No key: 0.  Keys without weight (scores of -infinity alone): 0/0, as the formula has it.
-      T* out = static_cast<T*>(a.out) + request * a.on + (head + r) * a.oh;
-      out[f] = Round<T>::store(empty ? 0.f : o / l);
+      struct alignas(sizeof(T) * kV) Row { T x[kV]; } y;
+#pragma unroll
+      for (int e = 0; e < kV; ++e) y.x[e] = Round<T>::store(empty ? 0.f : o[e] / l);
+      *reinterpret_cast<Row*>(static_cast<T*>(a.out) + request * a.on + (head + r) * a.oh + f) = y;
     } else {
       if (f == 0) part_ml(a, slot)[r] = make_float2(m, l);
-      part_row(a, slot, r)[f] = o;
+      *reinterpret_cast<vec*>(part_row(a, slot, r) + f) = o;
     }
   }
 }
@@ -126,7 +138,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_row_kernel(PagedArgs a) {
   __shared__ PlaceLds place;
   __shared__ float sO[kPagedWaves][kRowTile][kRowMaxD], sm[kPagedWaves][kRowTile],
       sl[kPagedWaves][kRowTile];
-  __shared__ int sbad;
+  __shared__ int sbad[kPagedWaves];
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const Place pl = locate<kRowUnit>(a, place);
   const uint32_t begin = pl.begin, end = pl.end;
@@ -194,9 +206,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_row_kernel(PagedArgs a) {
         }
       }
     }
-    if (threadIdx.x == 0) sbad = 0;
-    __syncthreads();
-    if (bad) sbad = 1;
+    if (u > begin) lds_barrier();  // the segment before has been read
 #pragma unroll
     for (int r = 0; r < kRowTile; ++r) {
 #pragma unroll
@@ -206,11 +216,16 @@ __global__ __launch_bounds__(kPagedThreads) void paged_row_kernel(PagedArgs a) {
         sl[wave][r] = l[r];
       }
     }
-    __syncthreads();
-    finish<T>(a, int(a.D), &sO[0][0][0], kRowMaxD, kRowTile * kRowMaxD, &sm[0][0], &sl[0][0], kRowTile,
+    if (lane == 0) sbad[wave] = bad;
+    lds_barrier();
+    finish<T, 1>(a, int(a.D), &sO[0][0][0], kRowMaxD, kRowTile * kRowMaxD, &sm[0][0], &sl[0][0], kRowTile,
               rows, count == units, 2 * int64_t(blockIdx.x) + (u > begin), req, hk * a.G + r0,
-              keys == 0, sbad != 0);
-    __syncthreads();
+              keys == 0, sbad[0] || sbad[1] || sbad[2] || sbad[3]);
+    if (c0 == 0 && threadIdx.x == 0)
+      a.split[req * a.per_request + seg] =
+          count == units ? make_int2(-1, -1)
+                         : make_int2(2 * int(blockIdx.x) + (u > begin),
+                                     int(pl.share.owner(u + units - 1)));
     u += count;
     if (u < end && u == base + units * a.per_request) {
       base = u;
@@ -267,6 +282,14 @@ __device__ inline float column_sum(float x) {
   return sum_halves(bits_to_float(p[0]) + bits_to_float(p[1]));
 }
 
+// LDS accesses of a wave's lanes before it come before those after it.  The
+// hardware keeps a wave's LDS accesses in order; this keeps the compiler from
+// moving a lane's load ahead of the store of another lane.
+__device__ inline void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 constexpr int kTileHeads = 16;
 template <typename T> constexpr int kStepKeys = sizeof(T) == 2 ? 32 : 16;
 template <typename T> constexpr int kTileUnit = kPagedWaves * kStepKeys<T>;
@@ -278,8 +301,12 @@ template <int kTiles> struct Pages {
   uint32_t first[kTiles];
 };
 
+// Two waves a SIMD: 256 registers each, so that the products' results stay in
+// vector registers.  In accumulation registers the compiler (ROCm 7.2) left out
+// the wait before one of them was read behind a branch, and a quarter of the
+// scores were stale.
 template <typename T, int D, bool kWholeTiles>
-__global__ __launch_bounds__(kPagedThreads) void paged_tile_kernel(PagedArgs a) {
+__global__ __launch_bounds__(kPagedThreads, 2) void paged_tile_kernel(PagedArgs a) {
   constexpr bool k16 = sizeof(T) == 2;
   constexpr int kKeys = kStepKeys<T>, kTiles = kKeys / 16, kUnit = kTileUnit<T>;
   constexpr int kF = D / 16;                       // features of a lane in a row of V
@@ -289,7 +316,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_tile_kernel(PagedArgs a) 
   __shared__ PlaceLds place;
   __shared__ __align__(16) float sO[kPagedWaves][kTileHeads][kStride];
   __shared__ float sm[kPagedWaves][kTileHeads], sl[kPagedWaves][kTileHeads];
-  __shared__ int sbad;
+  __shared__ int sbad[kPagedWaves];
   __shared__ int2 srow[kPagedWaves][kKeys];        // (page, row) of a step's keys, any page size
   const int lane = threadIdx.x % 64;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -348,6 +375,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_tile_kernel(PagedArgs a) 
           pg.first[t] = p * page;
         }
       } else {
+        wave_fence();  // the step before has been read
         if (lane < kKeys) {
           const uint32_t k0 = key0 + lane < last ? key0 + lane : last;
           const uint32_t p = a.by_page.div(k0);
@@ -358,8 +386,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_tile_kernel(PagedArgs a) 
           }
           srow[wave][lane] = make_int2(id, int(k0 - p * page));
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        wave_fence();
       }
     };
     // Row `r` of tile t of the step at key0: keys past the last read the last one.
@@ -503,9 +530,9 @@ __global__ __launch_bounds__(kPagedThreads) void paged_tile_kernel(PagedArgs a) 
     }
     l = column_sum(l);
 
-    if (threadIdx.x == 0) sbad = 0;
-    __syncthreads();
-    if (bad) sbad = 1;
+    if (u > begin) lds_barrier();  // the segment before has been read
+    if (__any(bad)) bad = true;
+    if (lane == 0) sbad[wave] = bad;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -516,11 +543,15 @@ __global__ __launch_bounds__(kPagedThreads) void paged_tile_kernel(PagedArgs a) 
       sm[wave][c] = m;
       sl[wave][c] = l;
     }
-    __syncthreads();
-    finish<T>(a, D, &sO[0][0][0], kStride, kTileHeads * kStride, &sm[0][0], &sl[0][0], kTileHeads,
+    lds_barrier();
+    finish<T, 4>(a, D, &sO[0][0][0], kStride, kTileHeads * kStride, &sm[0][0], &sl[0][0], kTileHeads,
               rows, count == units, 2 * int64_t(blockIdx.x) + (u > begin), req, hk * a.G + r0,
-              keys == 0, sbad != 0);
-    __syncthreads();
+              keys == 0, sbad[0] || sbad[1] || sbad[2] || sbad[3]);
+    if (c0 == 0 && threadIdx.x == 0)
+      a.split[req * a.per_request + seg] =
+          count == units ? make_int2(-1, -1)
+                         : make_int2(2 * int(blockIdx.x) + (u > begin),
+                                     int(pl.share.owner(u + units - 1)));
     u += count;
     if (u < end && u == base + units * a.per_request) {
       base = u;
@@ -530,67 +561,82 @@ __global__ __launch_bounds__(kPagedThreads) void paged_tile_kernel(PagedArgs a) 
 }
 
 // Rows of segments that several work-groups share: one work-group of 256
-// threads per (segment, row).  kV features a thread, and as many partials side by
-// side as that leaves threads for, each walked with the loads of U in flight;
+// threads per (segment, row).  The partials' weights 2^(m - M) go to LDS; kV
+// features a thread, as many partials side by side as that leaves threads for, U
+// of each thread's in flight (the first ones while the weights are computed);
 // then their sums, always in the same order.
+constexpr int kMostGroups = 2048;
 template <typename T, int kV>
 __global__ __launch_bounds__(kPagedThreads) void paged_merge_kernel(PagedArgs a) {
   typedef float vec __attribute__((ext_vector_type(kV)));
   constexpr int U = 4;
+  __shared__ float weight[kMostGroups + 1];
   __shared__ vec sacc[kPagedThreads];
-  __shared__ float smax[kPagedThreads], sden[kPagedThreads];
+  __shared__ float top[kPagedWaves], den[kPagedWaves];
+  const int2 split = a.split[blockIdx.x];
+  if (split.x < 0) return;  // written whole
   const uint32_t r = blockIdx.y, n = blockIdx.x / a.per_request;
   const uint32_t s = blockIdx.x - n * a.per_request, hk = s / a.tiles;
   const uint32_t head = (s - hk * a.tiles) * a.rows + r;
   if (head >= a.G) return;
-  const uint32_t base = a.start[n], units = (a.start[n + 1] - base) / a.per_request;
-  const uint32_t u0 = base + s * units, u1 = u0 + units;
-  const PagedShare share(a.start[a.N], a.groups);
-  const uint32_t w0 = share.owner(u0), w1 = share.owner(u1 - 1);
-  if (w0 == w1) return;  // written whole
-  const uint32_t first = 2 * w0 + (share.begin(w0) < u0);
+  const int w0 = split.x / 2, parts = split.y - w0 + 1;
   const int lanes = int(a.D) / kV, side = kPagedThreads / lanes;
   const int p = threadIdx.x / lanes, c = threadIdx.x - p * lanes;
-  float m = -__builtin_inff(), l = 0.f;
-  vec acc = vec(0.f);
-  if (p < side)
-    for (uint32_t w = w0 + p; w <= w1; w += side * U) {
-      float2 st[U];
-      vec x[U];
+  auto slot = [&](int i) { return int64_t(i == 0 ? split.x : 2 * (w0 + i)); };
+  // Reads past the last partial read it again, with no weight.
+  vec x[U];
+  auto load = [&](int from) {
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const uint32_t at = w + i * side;
-        const int64_t slot = at == w0 ? first : 2 * at;
-        st[i] = at <= w1 ? part_ml(a, slot)[r] : make_float2(0.f, 0.f);
-        x[i] = at <= w1 ? reinterpret_cast<const vec*>(part_row(a, slot, r))[c] : vec(0.f);
-      }
-#pragma unroll
-      for (int i = 0; i < U; ++i) {
-        if (st[i].y == 0.f) continue;  // no key of any weight
-        const float mn = __builtin_fmaxf(m, st[i].x);
-        const float ms = mn == -__builtin_inff() ? 0.f : mn;
-        const float f = __builtin_amdgcn_exp2f(m - ms), g = __builtin_amdgcn_exp2f(st[i].x - ms);
-        l = l * f + g * st[i].y;
-        acc = acc * f + g * x[i];
-        m = mn;
-      }
+    for (int i = 0; i < U; ++i) {
+      const int at = from + p + i * side < parts ? from + p + i * side : parts - 1;
+      x[i] = reinterpret_cast<const vec*>(part_row(a, slot(at), r))[c];
     }
-  sacc[threadIdx.x] = acc;
-  smax[threadIdx.x] = m;
-  sden[threadIdx.x] = l;
-  __syncthreads();
-  if (p != 0) return;
-  m = -__builtin_inff();
-  for (int i = 0; i < side; ++i) m = __builtin_fmaxf(m, smax[i * lanes + c]);
-  l = 0.f;
-  acc = vec(0.f);
-  for (int i = 0; i < side; ++i) {
-    const float li = sden[i * lanes + c];
-    if (li == 0.f) continue;
-    const float f = __builtin_amdgcn_exp2f(smax[i * lanes + c] - m);
-    l += f * li;
-    acc += f * sacc[i * lanes + c];
+  };
+  load(0);
+  float m = -__builtin_inff();
+  for (int i = threadIdx.x; i < parts; i += kPagedThreads) {
+    const float2 ml = part_ml(a, slot(i))[r];
+    if (!(ml.y == 0.f)) m = __builtin_fmaxf(m, ml.x);
   }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) m = __builtin_fmaxf(m, __shfl_xor(m, d));
+  if (threadIdx.x % 64 == 0) top[threadIdx.x / 64] = m;
+  lds_barrier();
+#pragma unroll
+  for (int w = 0; w < kPagedWaves; ++w) m = __builtin_fmaxf(m, top[w]);
+  float l = 0.f;
+  for (int i = threadIdx.x; i < parts; i += kPagedThreads) {
+    const float2 ml = part_ml(a, slot(i))[r];
+    const float f = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - m);  // 0: no key of any weight
+    weight[i] = f;
+    l += f * ml.y;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
+  if (threadIdx.x % 64 == 0) den[threadIdx.x / 64] = l;
+  lds_barrier();
+  vec acc = vec(0.f);
+  for (int from = 0;; from += U * side) {
+    vec y[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) y[i] = x[i];
+    const bool more = from + U * side < parts;
+    if (more) load(from + U * side);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int at = from + p + i * side;
+      const float f = at < parts ? weight[at] : 0.f;
+      if (f != 0.f) acc += f * y[i];
+    }
+    if (!more) break;
+  }
+  sacc[threadIdx.x] = acc;
+  lds_barrier();
+  if (p != 0) return;
+  for (int i = 1; i < side; ++i) acc += sacc[i * lanes + c];
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kPagedWaves; ++w) l += den[w];
   T* out = static_cast<T*>(a.out) + n * a.on + (hk * a.G + head) * a.oh + c * kV;
 #pragma unroll
   for (int i = 0; i < kV; ++i) out[i] = Round<T>::store(acc[i] / l);
@@ -607,6 +653,7 @@ static bool tile_form(int dtype, const PagedArgs& a) {
     if (reinterpret_cast<uintptr_t>(p) % 16) return false;
   for (int64_t s : {a.qn, a.qh, a.kp, a.kn, a.kh, a.vp, a.vn, a.vh})
     if (s < 0 || s % piece) return false;
+  if (reinterpret_cast<uintptr_t>(a.out) % (4 * es) || a.on % 4 || a.oh % 4) return false;
   for (int64_t s : {a.kn, a.vn})
     if (s >= (int64_t(1) << 31) / a.page) return false;
   return true;
@@ -622,13 +669,14 @@ static int64_t plan_form(PagedArgs& a, int64_t unit, int64_t tile, int64_t group
   a.groups = int32_t(most < groups ? most : groups);
   a.per_request = int32_t(a.Hk * a.tiles);
   a.by_page = FastDiv(uint32_t(a.page));
-  // Pairs and rows of 2 * groups partial slots, and the requests' first units.
-  return round256(2 * int64_t(a.groups) * a.rows * (8 + 4 * a.D)) + round256(4 * (a.N + 1));
+  // Pairs and rows of 2 * groups partial slots, and a pair for each segment.
+  return round256(2 * int64_t(a.groups) * a.rows * (8 + 4 * a.D)) +
+         round256(8 * a.N * a.per_request);
 }
 static int64_t plan_tiles(int dtype, PagedArgs& a) {
   return plan_form(a, dtype == kF32 ? kTileUnit<float> : kTileUnit<bf16_t>, kTileHeads, 512);
 }
-static int64_t plan_rows(PagedArgs& a) { return plan_form(a, kRowUnit, kRowTile, 2048); }
+static int64_t plan_rows(PagedArgs& a) { return plan_form(a, kRowUnit, kRowTile, kMostGroups); }
 
 int64_t paged_attn_workspace(int dtype, PagedArgs a) {
   // Which form runs depends on the tensors' alignment too: enough for either.
@@ -651,8 +699,8 @@ static hipError_t launch_paged_t(int dtype, PagedArgs& a, void* workspace, hipSt
   const int64_t need = tiles ? plan_tiles(dtype, a) : plan_rows(a);
   if (need < 0) return hipErrorInvalidValue;
   a.part = static_cast<float*>(workspace);
-  a.start = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + need -
-                                        round256(4 * (a.N + 1)));
+  a.split = reinterpret_cast<int2*>(static_cast<char*>(workspace) + need -
+                                    round256(8 * a.N * a.per_request));
   const dim3 grid{unsigned(a.groups)}, block{kPagedThreads};
   if (tiles && a.D == 64)
     launch_tiles<T, 64>(a, stream);

@@ -74,7 +74,7 @@ struct PagedArgs {
   int32_t groups;            // work-groups the units are dealt to
   int32_t per_request;       // segments of a request: Hk * tiles
   float* part;               // partial rows, see paged_attn.hip
-  uint32_t* start;           // first unit of request i, [N + 1]
+  int2* split;               // per segment: first slot and last work-group, -1 written whole
   FastDiv by_page;
 };
 // Workspace bytes for these sizes (N, Hk, G, D, M, page), -1 where the units do
