@@ -356,36 +356,42 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_tile_kernel(PagedArgs 
       steps = int(left < count ? left : count);
     }
 
-    Pages<kTiles> pg;
+    // Page entries are read a step ahead of the rows they place: `fetch` issues
+    // the reads, `place` puts them to use.  Ids that are no pages read page 0.
+    Pages<kTiles> pg, ahead;
+    int32_t id_ahead = 0;    // any page size: of the lane's key
+    uint32_t in_ahead = 0;
     u32x4_t kr[kTiles][kKL];
     uint32_t vr[kTiles * 4][kVW];
-    // Page entries of the step at key0; ids that are no pages read page 0.
-    auto look = [&](uint32_t key0) {
+    auto fetch = [&](uint32_t key0) {
       if constexpr (kWholeTiles) {
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
-          const uint32_t k0 = key0 + 16 * t < last ? key0 + 16 * t : last;
-          const uint32_t p = a.by_page.div(k0);
-          int32_t id = table[p];
-          if (id < 0 || id >= a.num_pages) {
-            bad = true;
-            id = 0;
-          }
-          pg.id[t] = id;
-          pg.first[t] = p * page;
+          const uint32_t p = a.by_page.div(key0 + 16 * t < last ? key0 + 16 * t : last);
+          ahead.id[t] = table[p];
+          ahead.first[t] = p * page;
         }
       } else {
-        wave_fence();  // the step before has been read
-        if (lane < kKeys) {
-          const uint32_t k0 = key0 + lane < last ? key0 + lane : last;
-          const uint32_t p = a.by_page.div(k0);
-          int32_t id = table[p];
-          if (id < 0 || id >= a.num_pages) {
+        const uint32_t k0 = key0 + lane % kKeys < last ? key0 + lane % kKeys : last;
+        const uint32_t p = a.by_page.div(k0);
+        id_ahead = table[p];
+        in_ahead = k0 - p * page;
+      }
+    };
+    auto place = [&]() {
+      if constexpr (kWholeTiles) {
+        pg = ahead;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+          if (pg.id[t] < 0 || pg.id[t] >= a.num_pages) {
             bad = true;
-            id = 0;
+            pg.id[t] = 0;
           }
-          srow[wave][lane] = make_int2(id, int(k0 - p * page));
-        }
+      } else {
+        const bool page0 = id_ahead < 0 || id_ahead >= a.num_pages;
+        bad |= page0;
+        wave_fence();  // the step before has been read
+        if (lane < kKeys) srow[wave][lane] = make_int2(page0 ? 0 : id_ahead, int(in_ahead));
         wave_fence();
       }
     };
@@ -435,7 +441,9 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_tile_kernel(PagedArgs 
 #pragma unroll
       for (int f = 0; f < kF; ++f) acc[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
       if (steps > 0) {
-        look(first);
+        fetch(first);
+        place();
+        fetch(first + kUnit);
         load_k(first);
         load_v(first);
       }
@@ -460,7 +468,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_tile_kernel(PagedArgs 
           }
         }
         if (i + 1 < steps) {
-          look(key0 + kUnit);
+          place();
+          fetch(key0 + 2 * kUnit);
           load_k(key0 + kUnit);
         }
         float p[kTiles * 4], top = -__builtin_inff();

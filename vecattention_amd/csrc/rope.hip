@@ -192,7 +192,7 @@ __device__ inline void load_weights(const RopeArgs& a, const void* w, int f0, in
 // of a lane are in flight: the first ones before the angles are made, which take
 // as long as they do, and each next one from the moment its place is free.
 template <typename T, int D, int kTokens, bool kCache>
-__global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) void rope_kernel(RopeArgs a) {
   constexpr int kLanes = D / 16, kRows = 256 / kLanes, kHeads = kRows / kTokens;
   constexpr int U = 2;
   static_assert(kHeads >= 1, "a token a row at least");
@@ -380,13 +380,12 @@ static bool whole_pieces(int64_t es, std::initializer_list<const void*> bases,
 
 template <typename T, int D, bool kCache>
 static void launch_rope_pieces(const RopeArgs& a, hipStream_t stream) {
-  // Tokens a work-group: as many as leave 1024 work-groups, up to 8.
+  // Four tokens a work-group where that leaves every CU one, else one: us at 28 +
+  // 4 heads of 128 in bf16, one token / four: 600 tokens 5.0 / 6.3, 1024 6.3 / 7.3,
+  // 2333 13.1 / 11.3, 8192 34.6 / 27.0, 32760 138 / 101 (eight: 13.1, 26.2, 104).
   const int64_t tokens = a.B * a.S;
-  if (tokens >= 8 * 1024)
-    hipLaunchKernelGGL((rope_kernel<T, D, 8, kCache>), dim3(unsigned((tokens + 7) / 8)), dim3(256),
-                       0, stream, a);
-  else if (tokens >= 2 * 1024)
-    hipLaunchKernelGGL((rope_kernel<T, D, 2, kCache>), dim3(unsigned((tokens + 1) / 2)), dim3(256),
+  if (tokens >= 1536)
+    hipLaunchKernelGGL((rope_kernel<T, D, 4, kCache>), dim3(unsigned((tokens + 3) / 4)), dim3(256),
                        0, stream, a);
   else
     hipLaunchKernelGGL((rope_kernel<T, D, 1, kCache>), dim3(unsigned(tokens)), dim3(256), 0,
