@@ -22,7 +22,7 @@ VA_KERNELS_SELECT_WAVE, VA_KERNELS_SELECT_MFMA, VA_KERNELS_SELECT_EXACT = 1, 2, 
 VA_KERNELS_ATTN_MFMA, VA_KERNELS_ATTN_ROW, VA_KERNELS_SPLIT = 16, 32, 64
 VA_KERNELS_ATTN_RING, VA_KERNELS_ATTN_F32 = 128, 256
 
-_DTYPES = {torch.float32: VA_F32, torch.bfloat16: VA_BF16, torch.float16: VA_F16}
+DTYPES = {torch.float32: VA_F32, torch.bfloat16: VA_BF16, torch.float16: VA_F16}
 
 _lock = threading.Lock()
 _lib = None
@@ -157,7 +157,7 @@ def check_flags(fn, flags):
 
 def dtype_code(t):
     try:
-        return _DTYPES[t.dtype]
+        return DTYPES[t.dtype]
     except KeyError:
         raise TypeError(f"unsupported dtype {t.dtype}; expected float32, bfloat16 or float16")
 
@@ -199,7 +199,11 @@ class _Here:
 
 _here = _Here()
 
+# As _raw_stream: torch's lookup without the check that the GPU is initialised
+# (a tensor on it is at hand).
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
 
 def on_device(device):
     """torch.cuda.device(device), without its bookkeeping when there is nothing to switch."""
-    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _here if _current_device() == device.index else torch.cuda.device(device)

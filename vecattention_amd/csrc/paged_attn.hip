@@ -85,14 +85,14 @@ __device__ inline Place locate(const PagedArgs& a, PlaceLds& lds) {
 // Merges the waves' states of a segment's rows and writes them: to the output
 // (`whole`), or to a partial slot.  sO[wave][row][stride], sm/sl[wave][row];
 // kV features of a row a thread.
-template <typename T, int kV>
+template <typename T, int kV, int kThreads = kPagedThreads>
 __device__ inline void finish(const PagedArgs& a, int D, const float* sO, int rstride,
                               int wstride, const float* sm, const float* sl, int mstride, int rows,
                               bool whole, int64_t slot, int64_t request, int64_t head, bool empty,
                               bool bad) {
   typedef float vec __attribute__((ext_vector_type(kV)));
   const int pieces = D / kV;
-  for (int i = threadIdx.x; i < rows * pieces; i += kPagedThreads) {
+  for (int i = threadIdx.x; i < rows * pieces; i += kThreads) {
     const int r = i / pieces, f = (i - r * pieces) * kV;
     float lw[kPagedWaves], mw[kPagedWaves], m = -__builtin_inff();
     vec ow[kPagedWaves];
@@ -292,7 +292,7 @@ __device__ inline void wave_fence() {
 
 constexpr int kTileHeads = 16;
 template <typename T> constexpr int kStepKeys = sizeof(T) == 2 ? 32 : 16;
-template <typename T> constexpr int kTileUnit = kPagedWaves * kStepKeys<T>;
+template <typename T> constexpr int kTileUnit = kPagedWaves * kStepKeys<T>;  // when split
 
 // Places of a step's keys: page id and first key of the page for each tile of
 // 16 keys, which lie in one page when the page size is a multiple of 16.
@@ -305,10 +305,15 @@ template <int kTiles> struct Pages {
 // vector registers.  In accumulation registers the compiler (ROCm 7.2) left out
 // the wait before one of them was read behind a branch, and a quarter of the
 // scores were stale.
-template <typename T, int D, bool kWholeTiles>
-__global__ __launch_bounds__(kPagedThreads, 2) void paged_tile_kernel(PagedArgs a) {
+//
+// kSplit: the units are dealt to the work-groups.  Otherwise a work-group of eight
+// waves takes a whole segment, and there is nothing to merge afterwards.
+template <typename T, int D, bool kWholeTiles, bool kSplit>
+__global__ __launch_bounds__(kSplit ? kPagedThreads : 2 * kPagedThreads, 2) void paged_tile_kernel(
+    PagedArgs a) {
   constexpr bool k16 = sizeof(T) == 2;
-  constexpr int kKeys = kStepKeys<T>, kTiles = kKeys / 16, kUnit = kTileUnit<T>;
+  constexpr int kWaves = kSplit ? kPagedWaves : 2 * kPagedWaves;
+  constexpr int kKeys = kStepKeys<T>, kTiles = kKeys / 16, kUnit = kWaves * kKeys;
   constexpr int kF = D / 16;                       // features of a lane in a row of V
   constexpr int kKL = k16 ? D / 32 : D / 16;       // 16-byte loads of a lane in a row of K
   constexpr int kVW = kF * int(sizeof(T)) / 4;     // words of a lane in a row of V
@@ -316,22 +321,30 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_tile_kernel(PagedArgs 
   __shared__ PlaceLds place;
   __shared__ __align__(16) float sO[kPagedWaves][kTileHeads][kStride];
   __shared__ float sm[kPagedWaves][kTileHeads], sl[kPagedWaves][kTileHeads];
-  __shared__ int sbad[kPagedWaves];
-  __shared__ int2 srow[kPagedWaves][kKeys];        // (page, row) of a step's keys, any page size
+  __shared__ int sbad[kWaves];
+  __shared__ int2 srow[kWaves][kKeys];        // (page, row) of a step's keys, any page size
   const int lane = threadIdx.x % 64;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int kg = lane / 16, c = lane % 16;
-  const Place pl = locate<kUnit>(a, place);
-  const uint32_t begin = pl.begin, end = pl.end;
   const int64_t capacity = a.M * a.page;
   const uint32_t page = uint32_t(a.page);
+  Place pl{PagedShare(1, 1), 0, 0, 0, 0, 0};
+  if constexpr (kSplit) {
+    pl = locate<kUnit>(a, place);
+  } else {
+    pl.request = int32_t(blockIdx.x / uint32_t(a.per_request));
+    pl.keys = paged_keys(a.lens[pl.request], capacity);
+    pl.begin = (blockIdx.x - pl.request * a.per_request) * paged_units(pl.keys, kUnit);
+    pl.end = pl.begin + 1;  // all of the segment's units
+  }
+  const uint32_t begin = pl.begin, end = pl.end;
   int64_t req = pl.request;
   int32_t keys = pl.keys;
   uint32_t base = pl.base;
   for (uint32_t u = begin; u < end;) {
     const uint32_t units = paged_units(keys, kUnit);
     const uint32_t seg = (u - base) / units, c0 = (u - base) - seg * units;
-    const uint32_t count = end - u < units - c0 ? end - u : units - c0;
+    const uint32_t count = kSplit && end - u < units - c0 ? end - u : units - c0;
     const int32_t hk = int32_t(seg) / a.tiles, r0 = (int32_t(seg) - hk * a.tiles) * a.rows;
     const int rows = int(a.G - r0 < a.rows ? a.G - r0 : a.rows);
     const int32_t* table = a.table + req * a.table_stride;
@@ -542,20 +555,55 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_tile_kernel(PagedArgs 
     if (u > begin) lds_barrier();  // the segment before has been read
     if (__any(bad)) bad = true;
     if (lane == 0) sbad[wave] = bad;
+    if constexpr (!kSplit) {
+      // The upper four waves' states join those of the lower four, lane by lane.
+      f32x4_t* upper = reinterpret_cast<f32x4_t*>(&sO[0][0][0]) + (wave % kPagedWaves) * 64 * kF;
+      if (wave >= kPagedWaves) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+        for (int x = 0; x < kF; ++x) upper[x * 64 + lane] = acc[x];
+        if (kg == 0) {
+          sm[wave - kPagedWaves][c] = m;
+          sl[wave - kPagedWaves][c] = l;
+        }
+      }
+      lds_barrier();
+      if (wave < kPagedWaves) {
+        const float mu = sm[wave][c], lu = sl[wave][c];
+        const float mn = lu == 0.f ? m : l == 0.f ? mu : __builtin_fmaxf(m, mu);
+        const float f = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+        const float g = lu == 0.f ? 0.f : __builtin_amdgcn_exp2f(mu - mn);
 #pragma unroll
-      for (int x = 0; x < kF; x += 4)
-        *reinterpret_cast<f32x4_t*>(&sO[wave][c][(4 * kg + e) * kF + x]) =
-            f32x4_t{acc[x][e], acc[x + 1][e], acc[x + 2][e], acc[x + 3][e]};
-    if (kg == 0) {
-      sm[wave][c] = m;
-      sl[wave][c] = l;
+        for (int x = 0; x < kF; ++x) {
+          const f32x4_t up = upper[x * 64 + lane];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            acc[x][e] = (f == 0.f ? 0.f : f * acc[x][e]) + (g == 0.f ? 0.f : g * up[e]);
+        }
+        l = f * l + g * lu;
+        m = mn;
+      }
+      lds_barrier();
+    }
+    if (wave < kPagedWaves) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int x = 0; x < kF; x += 4)
+          *reinterpret_cast<f32x4_t*>(&sO[wave][c][(4 * kg + e) * kF + x]) =
+              f32x4_t{acc[x][e], acc[x + 1][e], acc[x + 2][e], acc[x + 3][e]};
+      if (kg == 0) {
+        sm[wave][c] = m;
+        sl[wave][c] = l;
+      }
     }
     lds_barrier();
-    finish<T, 4>(a, D, &sO[0][0][0], kStride, kTileHeads * kStride, &sm[0][0], &sl[0][0], kTileHeads,
+    bool any_bad = false;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) any_bad |= sbad[w] != 0;
+    finish<T, 4, 64 * kWaves>(a, D, &sO[0][0][0], kStride, kTileHeads * kStride, &sm[0][0], &sl[0][0], kTileHeads,
               rows, count == units, 2 * int64_t(blockIdx.x) + (u > begin), req, hk * a.G + r0,
-              keys == 0, sbad[0] || sbad[1] || sbad[2] || sbad[3]);
+              keys == 0, any_bad);
+    if (!kSplit) break;
     if (c0 == 0 && threadIdx.x == 0)
       a.split[req * a.per_request + seg] =
           count == units ? make_int2(-1, -1)
@@ -693,13 +741,26 @@ int64_t paged_attn_workspace(int dtype, PagedArgs a) {
   return rows < 0 || tiles < 0 ? -1 : rows > tiles ? rows : tiles;
 }
 
-template <typename T, int D>
+// Whether every segment goes to a work-group of its own, from the most keys that
+// the table allows: up to 256 KB of keys and values a segment, up to 512 KB where
+// the segments fill the GPU, and not where they are so many and so short that most
+// waves have no keys.  us, split and merged / whole: 28 + 4 heads of 128 in bf16, 1
+// request: 512 keys 10.7 / 9.7, 1024 10.7 / 14.4; 64 requests: 1024 keys 23.2 /
+// 18.3, 2048 29.9 / 32.8; 16 + 16 heads, 256 requests: 256 keys 98.7 / 119.
+static bool whole_segments(int dtype, const PagedArgs& a) {
+  const int64_t segments = a.N * a.per_request;
+  const int64_t bytes = a.M * a.page * a.D * (dtype == kF32 ? 8 : 4);
+  return segments < 2048 && bytes <= (segments < 256 ? 256 << 10 : 512 << 10);
+}
+
+template <typename T, int D, bool kSplit>
 static void launch_tiles(const PagedArgs& a, hipStream_t stream) {
-  const dim3 grid{unsigned(a.groups)}, block{kPagedThreads};
+  const dim3 grid{unsigned(kSplit ? a.groups : a.N * a.per_request)};
+  const dim3 block{kSplit ? kPagedThreads : 2 * kPagedThreads};
   if (a.page % 16 == 0)
-    hipLaunchKernelGGL((paged_tile_kernel<T, D, true>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((paged_tile_kernel<T, D, true, kSplit>), grid, block, 0, stream, a);
   else
-    hipLaunchKernelGGL((paged_tile_kernel<T, D, false>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((paged_tile_kernel<T, D, false, kSplit>), grid, block, 0, stream, a);
 }
 
 template <typename T>
@@ -711,10 +772,12 @@ static hipError_t launch_paged_t(int dtype, PagedArgs& a, void* workspace, hipSt
   a.split = reinterpret_cast<int2*>(static_cast<char*>(workspace) + need -
                                     round256(8 * a.N * a.per_request));
   const dim3 grid{unsigned(a.groups)}, block{kPagedThreads};
-  if (tiles && a.D == 64)
-    launch_tiles<T, 64>(a, stream);
-  else if (tiles)
-    launch_tiles<T, 128>(a, stream);
+  if (tiles && whole_segments(dtype, a)) {
+    a.D == 64 ? launch_tiles<T, 64, false>(a, stream) : launch_tiles<T, 128, false>(a, stream);
+    return hipGetLastError();
+  }
+  if (tiles)
+    a.D == 64 ? launch_tiles<T, 64, true>(a, stream) : launch_tiles<T, 128, true>(a, stream);
   else if (a.D <= 64)
     hipLaunchKernelGGL((paged_row_kernel<T, 1>), grid, block, 0, stream, a);
   else if (a.D <= 128)

@@ -17,13 +17,15 @@ A cache is (num_pages, page_size, num_kv_heads, head_dim) with kv_layout "NHD",
 contiguous features.  Nothing waits for the GPU or is kept between calls, so the
 calls can be captured into a graph.
 """
+import functools
 import math
+import operator
 from typing import NamedTuple
 
 import torch
 
 from . import _native as nat
-from .rotary import refuse_grad, rotation_args, rows_like, same_device
+from .rotary import refuse_devices, refuse_grad, rotation_args, rows_like
 
 
 class PagedStep(NamedTuple):
@@ -62,78 +64,91 @@ def paged_kv_plan(kv_lens, new_lens, block_tables, free_pages, page_size, num_to
         raise ValueError("free_pages must be a vector")
     if free_head is not None and free_head.numel() != 1:
         raise ValueError("free_head must have one element")
-    for name, t in (("kv_lens", kv_lens), ("new_lens", new_lens), ("block_tables", block_tables),
-                    ("free_pages", free_pages), ("free_head", free_head)):
-        if t is not None and t.dtype != torch.int32:
-            raise TypeError(f"{name} must be int32, not {t.dtype}")
+    if not (kv_lens.dtype == new_lens.dtype == block_tables.dtype == free_pages.dtype
+            == torch.int32) or free_head is not None and free_head.dtype != torch.int32:
+        raise TypeError("lengths, block_tables, free_pages and free_head must be int32")
+    page_size, num_tokens = operator.index(page_size), operator.index(num_tokens)
     if page_size <= 0:
         raise ValueError(f"page_size {page_size}")
     if num_tokens < 0:
         raise ValueError(f"num_tokens {num_tokens}")
     N, M = block_tables.shape
-    if M > 1 and block_tables.stride(1) != 1 or N > 1 and block_tables.stride(0) < M:
+    row, entry = block_tables.stride()
+    if M > 1 and entry != 1 or N > 1 and row < M:
         raise ValueError("block_tables needs contiguous rows of its own")
-    device = block_tables.device
-    if not block_tables.is_cuda:
-        raise RuntimeError("paged_kv_plan runs on the GPU")
-    same_device("paged_kv_plan", device, kv_lens, new_lens, free_pages, free_head)
-    kv_lens, new_lens, free_pages = (t.contiguous() for t in (kv_lens, new_lens, free_pages))
-    out = PagedStep(torch.empty(N, dtype=torch.int32, device=device),
-                    torch.empty(N + 1, dtype=torch.int32, device=device),
-                    torch.empty(num_tokens, dtype=torch.int64, device=device),
-                    torch.empty(num_tokens, dtype=torch.int64, device=device),
-                    torch.empty(num_tokens, dtype=torch.int32, device=device),
-                    torch.empty(1, dtype=torch.int64, device=device))
-    lib = nat.lib()
-    bytes_ = lib.va_paged_plan_workspace_size(N)
-    work = torch.empty(bytes_, dtype=torch.uint8, device=device) if bytes_ else None
+    dev = block_tables.get_device()
+    if not (0 <= dev == kv_lens.get_device() == new_lens.get_device() == free_pages.get_device()
+            and (free_head is None or free_head.get_device() == dev)):
+        refuse_devices("paged_kv_plan", block_tables, kv_lens, new_lens, free_pages, free_head)
+    device, empty = block_tables.device, torch.empty
+    kv_lens, new_lens = kv_lens.contiguous(), new_lens.contiguous()
+    free_pages = free_pages.contiguous()
+    out = PagedStep(empty(N, dtype=torch.int32, device=device),
+                    empty(N + 1, dtype=torch.int32, device=device),
+                    empty(num_tokens, dtype=torch.int64, device=device),
+                    empty(num_tokens, dtype=torch.int64, device=device),
+                    empty(num_tokens, dtype=torch.int32, device=device),
+                    empty(1, dtype=torch.int64, device=device))
+    bytes_ = _plan_workspace(N)
+    work = empty(bytes_, dtype=torch.uint8, device=device) if bytes_ else None
     with nat.on_device(device):
-        rc = lib.va_paged_plan(
-            nat.addr(kv_lens), nat.addr(new_lens), N, nat.addr(block_tables),
-            block_tables.stride(0), M, nat.addr(free_pages), free_pages.shape[0],
-            nat.addr(free_head), page_size, num_tokens, nat.addr(out.kv_lens),
-            nat.addr(out.qo_indptr), nat.addr(out.slot_mapping), nat.addr(out.positions),
-            nat.addr(out.request_ids), nat.addr(out.pages_taken), nat.addr(work), bytes_,
-            nat.stream_addr(device))
+        rc = nat.lib().va_paged_plan(
+            kv_lens.data_ptr(), new_lens.data_ptr(), N, block_tables.data_ptr(), row, M,
+            free_pages.data_ptr(), free_pages.shape[0], nat.addr(free_head), page_size, num_tokens,
+            *[t.data_ptr() for t in out], nat.addr(work), bytes_, nat.stream_addr(device))
     nat.check("va_paged_plan", rc)
     return out
 
 
-def _cache(k_cache, v_cache, kv_layout, Hk, D, dtype):
-    """(num_pages, page_size, page/row/head strides of K, those of V) of a checked cache."""
+# Workspace queries, which depend on their arguments alone.
+@functools.lru_cache(maxsize=1024)
+def _plan_workspace(N):
+    return nat.lib().va_paged_plan_workspace_size(N)
+
+
+@functools.lru_cache(maxsize=1024)
+def _decode_workspace(*sizes):
+    return max(nat.lib().va_paged_decode_workspace_size(*sizes), 16)
+
+
+def _cache(k_cache, v_cache, kv_layout, D, dtype):
+    """(num_pages, page_size, heads, page/row/head strides of K, those of V) of a checked cache."""
     if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
         raise ValueError(f"k_cache {tuple(k_cache.shape)} and v_cache {tuple(v_cache.shape)} must "
                          "be 4-dimensional and alike")
+    kp, k1, k2, kd = k_cache.stride()
+    vp, v1, v2, vd = v_cache.stride()
     if kv_layout == "NHD":
-        row, head = 1, 2
+        pages, page, heads, width = k_cache.shape
+        ks, vs = (kp, k1, k2), (vp, v1, v2)
     elif kv_layout == "HND":
-        row, head = 2, 1
+        pages, heads, page, width = k_cache.shape
+        ks, vs = (kp, k2, k1), (vp, v2, v1)
     else:
         raise KeyError(f"Invalid kv_layout {kv_layout}")
-    if k_cache.shape[head] != Hk or k_cache.shape[3] != D:
-        raise ValueError(f"a {kv_layout} cache of shape {tuple(k_cache.shape)} does not hold "
-                         f"{Hk} heads of {D}")
-    if k_cache.dtype != dtype or v_cache.dtype != dtype:
+    if width != D:
+        raise ValueError(f"a cache of shape {tuple(k_cache.shape)} does not hold rows of {D}")
+    if not k_cache.dtype == v_cache.dtype == dtype:
         raise ValueError("the caches and the rows must share a dtype")
-    if k_cache.shape[0] == 0 or k_cache.shape[row] == 0:
+    if pages == 0 or page == 0:
         raise ValueError("the cache has no pages")
-    ks, vs = k_cache.stride(), v_cache.stride()
-    if (ks[3] != 1 or vs[3] != 1) and D > 1:
+    if (kd != 1 or vd != 1) and D > 1:
         raise ValueError("k_cache and v_cache need contiguous head_dim")
-    return (k_cache.shape[0], k_cache.shape[row], (ks[0], ks[row], ks[head]),
-            (vs[0], vs[row], vs[head]))
+    return pages, page, heads, ks, vs
 
 
 def _tokens(k, v, slot_mapping):
+    """k, v (features contiguous), slots, and k's shape, of a step's checked tokens."""
     if k.dim() != 3 or v.shape != k.shape:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be "
                          "(tokens, num_kv_heads, head_dim)")
     if v.dtype != k.dtype:
         raise ValueError(f"k ({k.dtype}) and v ({v.dtype}) must share a dtype")
-    if tuple(slot_mapping.shape) != (k.shape[0],) or slot_mapping.dtype != torch.int64:
-        raise ValueError(f"slot_mapping must be int64 of ({k.shape[0]},)")
+    T, Hk, D = k.shape
+    if slot_mapping.dtype != torch.int64 or slot_mapping.shape != (T,):
+        raise ValueError(f"slot_mapping must be int64 of ({T},)")
     return (k if k.stride(2) == 1 else k.contiguous(), v if v.stride(2) == 1 else v.contiguous(),
-            slot_mapping.contiguous())
+            slot_mapping.contiguous(), T, Hk, D)
 
 
 def write_paged_kv(k, v, k_cache, v_cache, slot_mapping, kv_layout="NHD"):
@@ -144,21 +159,25 @@ def write_paged_kv(k, v, k_cache, v_cache, slot_mapping, kv_layout="NHD"):
     1)``).  slot_mapping: (T,) int64; a slot outside the cache (-1) takes
     nothing, the others must be distinct.
     """
-    k, v, slot_mapping = _tokens(k, v, slot_mapping)
-    T, Hk, D = k.shape
+    k, v, slot_mapping, T, Hk, D = _tokens(k, v, slot_mapping)
     dtype = nat.dtype_code(k)
-    pages, page, ks, vs = _cache(k_cache, v_cache, kv_layout, Hk, D, k.dtype)
-    if not k.is_cuda:
-        raise RuntimeError("write_paged_kv runs on the GPU")
-    same_device("write_paged_kv", k.device, v, k_cache, v_cache, slot_mapping)
+    pages, page, heads, ks, vs = _cache(k_cache, v_cache, kv_layout, D, k.dtype)
+    if heads != Hk:
+        raise ValueError(f"a cache of {heads} heads for keys of {Hk}")
+    if not (0 <= k.get_device() == v.get_device() == k_cache.get_device() == v_cache.get_device()
+            == slot_mapping.get_device()):
+        refuse_devices("write_paged_kv", k, v, k_cache, v_cache, slot_mapping)
     refuse_grad("write_paged_kv", k, v, k_cache, v_cache)
-    if k.numel() == 0:
+    if T == 0 or Hk == 0 or D == 0:
         return
-    with nat.on_device(k.device):
+    device = k.device
+    kt, kh, _ = k.stride()
+    vt, vh, _ = v.stride()
+    with nat.on_device(device):
         rc = nat.lib().va_write_paged_kv(
-            dtype, nat.addr(k), k.stride(0), k.stride(1), nat.addr(v), v.stride(0), v.stride(1),
-            nat.addr(k_cache), *ks, nat.addr(v_cache), *vs, pages, page, nat.addr(slot_mapping),
-            T, Hk, D, nat.stream_addr(k.device))
+            dtype, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, k_cache.data_ptr(), *ks,
+            v_cache.data_ptr(), *vs, pages, page, slot_mapping.data_ptr(), T, Hk, D,
+            nat.stream_addr(device))
     nat.check("va_write_paged_kv", rc)
 
 
@@ -173,34 +192,45 @@ def qk_norm_rope_to_cache(q, k, v, k_cache, v_cache, slot_mapping, positions, in
     slot_mapping and caches as in ``write_paged_kv``.  Returns the rotated queries
     (T, Hq, D); those of tokens without a slot too.
     """
-    if q.dim() != 3 or q.shape[0] != k.shape[0]:
+    k, v, slot_mapping, T, Hk, D = _tokens(k, v, slot_mapping)
+    if q.dim() != 3 or q.shape[0] != T or q.shape[2] != D:
         raise ValueError(f"q {tuple(q.shape)} must be (tokens, num_qo_heads, head_dim), with k's "
-                         "tokens")
-    k, v, slot_mapping = _tokens(k, v, slot_mapping)
-    T, Hq, D = q.shape
-    Hk = k.shape[1]
+                         "tokens and head_dim")
+    if q.dtype != k.dtype:
+        raise ValueError(f"q ({q.dtype}) and k ({k.dtype}) must share a dtype")
+    Hq = q.shape[1]
     dtype = nat.dtype_code(q)
     positions, spa, axes, sections, rot, wtype = rotation_args(
-        q, k, positions, inv_freq, q_weight, k_weight, mrope_section, (T,))
-    pages, page, ks, vs = _cache(k_cache, v_cache, kv_layout, Hk, D, k.dtype)
-    if not q.is_cuda:
-        raise RuntimeError("qk_norm_rope_to_cache runs on the GPU")
-    same_device("qk_norm_rope_to_cache", q.device, k, v, k_cache, v_cache, slot_mapping, positions,
-                inv_freq, q_weight, k_weight)
+        D, q.dtype, positions, inv_freq, q_weight, k_weight, mrope_section, (T,))
+    pages, page, heads, ks, vs = _cache(k_cache, v_cache, kv_layout, D, k.dtype)
+    if heads != Hk:
+        raise ValueError(f"a cache of {heads} heads for keys of {Hk}")
+    dev = q.get_device()
+    if not (0 <= dev == k.get_device() == v.get_device() == k_cache.get_device()
+            == v_cache.get_device() == slot_mapping.get_device() == positions.get_device()
+            == inv_freq.get_device()
+            and (q_weight is None or q_weight.get_device() == dev)
+            and (k_weight is None or k_weight.get_device() == dev)):
+        refuse_devices("qk_norm_rope_to_cache", q, k, v, k_cache, v_cache, slot_mapping, positions,
+                       inv_freq, q_weight, k_weight)
     refuse_grad("qk_norm_rope_to_cache", q, k, v, k_cache, v_cache, inv_freq, q_weight, k_weight)
     if q.stride(2) != 1:
         q = q.contiguous()
     out = rows_like(q)
     if T == 0 or Hq == 0 or Hk == 0:
         return out
-    with nat.on_device(q.device):
+    device = q.device
+    qt, qh, _ = q.stride()
+    kt, kh, _ = k.stride()
+    vt, vh, _ = v.stride()
+    ot, oh, _ = out.stride()
+    with nat.on_device(device):
         rc = nat.lib().va_qk_norm_rope_to_cache(
-            dtype, nat.addr(q), q.stride(0), q.stride(1), nat.addr(k), k.stride(0), k.stride(1),
-            nat.addr(v), v.stride(0), v.stride(1), nat.addr(out), out.stride(0), out.stride(1),
-            nat.addr(k_cache), *ks, nat.addr(v_cache), *vs, pages, page, nat.addr(slot_mapping),
-            T, Hq, Hk, D, nat.addr(positions), spa, axes, sections, nat.addr(inv_freq), rot,
-            nat.addr(q_weight), nat.addr(k_weight), wtype, eps, attention_scaling,
-            int(interleaved), nat.stream_addr(q.device))
+            dtype, q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
+            out.data_ptr(), ot, oh, k_cache.data_ptr(), *ks, v_cache.data_ptr(), *vs, pages, page,
+            slot_mapping.data_ptr(), T, Hq, Hk, D, positions.data_ptr(), spa, axes, sections,
+            inv_freq.data_ptr(), rot, nat.addr(q_weight), nat.addr(k_weight), wtype,
+            float(eps), float(attention_scaling), 1 if interleaved else 0, nat.stream_addr(device))
     nat.check("va_qk_norm_rope_to_cache", rc)
     return out
 
@@ -222,42 +252,42 @@ def paged_decode_attention(q, k_cache, v_cache, block_tables, kv_lens, kv_layout
     if q.dim() != 3:
         raise ValueError("q must be (requests, num_qo_heads, head_dim)")
     N, Hq, D = q.shape
-    if k_cache.dim() != 4:
-        raise ValueError("k_cache must be 4-dimensional")
-    Hk = k_cache.shape[1 if kv_layout == "HND" else 2]
     dtype = nat.dtype_code(q)
-    pages, page, ks, vs = _cache(k_cache, v_cache, kv_layout, Hk, D, q.dtype)
+    pages, page, Hk, ks, vs = _cache(k_cache, v_cache, kv_layout, D, q.dtype)
     if Hk == 0 or Hq % Hk:
         raise ValueError(f"num_qo_heads {Hq} is not a multiple of num_kv_heads {Hk}")
-    if block_tables.dim() != 2 or block_tables.shape[0] != N or tuple(kv_lens.shape) != (N,):
+    if block_tables.dim() != 2 or block_tables.shape[0] != N or kv_lens.shape != (N,):
         raise ValueError(f"block_tables {tuple(block_tables.shape)} and kv_lens "
                          f"{tuple(kv_lens.shape)} do not fit {N} requests")
-    if block_tables.dtype != torch.int32 or kv_lens.dtype != torch.int32:
+    if not block_tables.dtype == kv_lens.dtype == torch.int32:
         raise TypeError("block_tables and kv_lens must be int32")
-    if not q.is_cuda:
-        raise RuntimeError("paged_decode_attention runs on the GPU")
-    same_device("paged_decode_attention", q.device, k_cache, v_cache, block_tables, kv_lens)
+    if not (0 <= q.get_device() == k_cache.get_device() == v_cache.get_device()
+            == block_tables.get_device() == kv_lens.get_device()):
+        refuse_devices("paged_decode_attention", q, k_cache, v_cache, block_tables, kv_lens)
     refuse_grad("paged_decode_attention", q, k_cache, v_cache)
     M = block_tables.shape[1]
-    if q.stride(2) != 1:
+    qn, qh, qd = q.stride()
+    if qd != 1:
         q = q.contiguous()
-    if M > 1 and block_tables.stride(1) != 1:
+        qn, qh, qd = q.stride()
+    row, entry = block_tables.stride()
+    if M > 1 and entry != 1:
         block_tables = block_tables.contiguous()
+        row = M
     kv_lens = kv_lens.contiguous()
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(D)
-    out = torch.empty(N, Hq, D, dtype=q.dtype, device=q.device)
-    if out.numel() == 0:
+    device = q.device
+    out = torch.empty((N, Hq, D), dtype=q.dtype, device=device)
+    if N * Hq * D == 0:
         return out
-    lib = nat.lib()
-    bytes_ = max(lib.va_paged_decode_workspace_size(dtype, N, Hq, Hk, D, M, page), 16)
-    work = torch.empty(bytes_, dtype=torch.uint8, device=q.device)
-    with nat.on_device(q.device):
-        rc = lib.va_paged_decode_attn(
-            dtype, nat.addr(q), q.stride(0), q.stride(1), nat.addr(k_cache), *ks,
-            nat.addr(v_cache), *vs, nat.addr(out), Hq * D, D, nat.addr(block_tables),
-            block_tables.stride(0), M, nat.addr(kv_lens), N, Hq, Hk, D, page, pages,
-            float(sm_scale), nat.addr(work), bytes_, nat.stream_addr(q.device))
+    bytes_ = _decode_workspace(dtype, N, Hq, Hk, D, M, page)
+    work = torch.empty(bytes_, dtype=torch.uint8, device=device)
+    with nat.on_device(device):
+        rc = nat.lib().va_paged_decode_attn(
+            dtype, q.data_ptr(), qn, qh, k_cache.data_ptr(), *ks, v_cache.data_ptr(), *vs,
+            out.data_ptr(), Hq * D, D, block_tables.data_ptr(), row, M, kv_lens.data_ptr(), N, Hq,
+            Hk, D, page, pages, float(sm_scale), work.data_ptr(), bytes_, nat.stream_addr(device))
     nat.check("va_paged_decode_attn", rc)
     return out
 

@@ -8,6 +8,7 @@ the per-head RMS norms that some models put before it.  Everything is computed
 in fp32 from angles reduced in 64 bits, and rounded once.
 """
 import ctypes
+import functools
 
 import torch
 
@@ -23,62 +24,63 @@ def refuse_grad(what, *tensors):
                     f"{what} has no backward pass: call it under torch.no_grad()")
 
 
-def same_device(what, device, *tensors):
+def refuse_devices(what, *tensors):
+    """The error for tensors that are not all on one GPU."""
+    if not tensors[0].is_cuda:
+        raise RuntimeError(f"{what} runs on the GPU")
     for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"{what}: tensors on {device} and {t.device}")
+        if t is not None and t.device != tensors[0].device:
+            raise ValueError(f"{what}: tensors on {tensors[0].device} and {t.device}")
 
 
-def _sections(mrope_section, half):
-    if mrope_section is None:
-        return 1, None
-    axes = len(mrope_section)
+@functools.lru_cache(maxsize=256)
+def _sections(section, half):
+    """(axes, their sections for the C call)."""
+    axes = len(section)
     if not 1 <= axes <= 4:
         raise ValueError(f"mrope_section has {axes} entries; 1 to 4 position axes are supported")
-    if any(n < 0 for n in mrope_section) or sum(mrope_section) != half:
-        raise ValueError(f"mrope_section {list(mrope_section)} does not add up to {half}")
-    return axes, (ctypes.c_int64 * axes)(*mrope_section)
+    if any(n < 0 for n in section) or sum(section) != half:
+        raise ValueError(f"mrope_section {list(section)} does not add up to {half}")
+    return axes, (ctypes.c_int64 * axes)(*section)
 
 
-def rotation_args(q, k, positions, inv_freq, q_weight, k_weight, mrope_section, tokens):
+def rotation_args(D, dtype, positions, inv_freq, q_weight, k_weight, mrope_section, tokens):
     """Checked arguments that both forms share: (positions, its axis stride, number of axes,
     sections, rotary_dim, weight type).  tokens: the shape of one axis' positions."""
-    D = q.shape[-1]
-    if k.shape[-1] != D:
-        raise ValueError(f"head_dim of q ({D}) and k ({k.shape[-1]}) differ")
-    if q.dtype != k.dtype:
-        raise ValueError(f"q ({q.dtype}) and k ({k.dtype}) must share a dtype")
-    if inv_freq.dim() != 1 or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be a contiguous float32 vector")
-    rot = 2 * inv_freq.shape[0]
-    if not 0 < rot <= D:
-        raise ValueError(f"inv_freq has {rot // 2} frequencies for a head_dim of {D}")
-    axes, sections = _sections(mrope_section, rot // 2)
+    half = inv_freq.shape[0]
+    if not 0 < 2 * half <= D:
+        raise ValueError(f"inv_freq has {half} frequencies for a head_dim of {D}")
+    if mrope_section is None:
+        axes, sections, shape = 1, None, tokens
+    else:
+        axes, sections = _sections(tuple(mrope_section), half)
+        shape = (axes, *tokens)
     if positions.dtype != torch.int64:
         if positions.dtype != torch.int32:
             raise TypeError(f"positions must be int64 or int32, not {positions.dtype}")
         positions = positions.long()
-    shape = tuple(tokens) if mrope_section is None else (axes, *tokens)
-    if tuple(positions.shape) != shape:
+    if positions.shape != shape:
         # (S,) for every row of the batch; (T,) of a step's tokens for every axis.
-        if tuple(positions.shape) != shape[:-2] + shape[-1:]:
+        if positions.shape != shape[:-2] + shape[-1:]:
             raise ValueError(f"positions {tuple(positions.shape)}: expected {shape}")
         positions = positions.unsqueeze(-2).expand(shape)
     if shape[-1] > 1 and positions.stride(-1) != 1:
         positions = positions.contiguous()
-    weight_type = q.dtype
+    weight_type = None
     for w in (q_weight, k_weight):
         if w is None:
             continue
-        if tuple(w.shape) != (D,) or not w.is_contiguous():
+        if w.shape != (D,) or not w.is_contiguous():
             raise ValueError(f"norm weights must be contiguous, of {D} values")
-        if w.dtype not in (q.dtype, torch.float32):
-            raise ValueError(f"norm weights of {w.dtype} for rows of {q.dtype}")
+        if w.dtype != dtype and w.dtype != torch.float32:
+            raise ValueError(f"norm weights of {w.dtype} for rows of {dtype}")
+        if weight_type is not None and w.dtype != weight_type:
+            raise ValueError("q_weight and k_weight must share a dtype")
         weight_type = w.dtype
-    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
-        raise ValueError("q_weight and k_weight must share a dtype")
-    return (positions, positions.stride(0) if mrope_section is not None else 0, axes, sections,
-            rot, nat.VA_F32 if weight_type == torch.float32 else nat.dtype_code(q))
+    return (positions, 0 if sections is None else positions.stride(0), axes, sections, 2 * half,
+            nat.VA_F32 if weight_type == torch.float32 else nat.DTYPES[dtype])
 
 
 def rows_like(x):
@@ -107,29 +109,43 @@ def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError("q and k must be (batch, heads, seq, head_dim)")
     B, Hq, S, D = q.shape
-    if (k.shape[0], k.shape[2]) != (B, S):
-        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} differ in batch or length")
+    Bk, Hk, Sk, Dk = k.shape
+    if Bk != B or Sk != S or Dk != D:
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} differ in batch, length or "
+                         "head_dim")
+    if q.dtype != k.dtype:
+        raise ValueError(f"q ({q.dtype}) and k ({k.dtype}) must share a dtype")
     dtype = nat.dtype_code(q)
     positions, spa, axes, sections, rot, wtype = rotation_args(
-        q, k, positions, inv_freq, q_weight, k_weight, mrope_section, (B, S))
-    if not q.is_cuda:
-        raise RuntimeError("qk_norm_rope runs on the GPU")
-    same_device("qk_norm_rope", q.device, k, positions, inv_freq, q_weight, k_weight)
+        D, q.dtype, positions, inv_freq, q_weight, k_weight, mrope_section, (B, S))
+    dev = q.get_device()
+    if not (0 <= dev == k.get_device() == positions.get_device() == inv_freq.get_device()
+            and (q_weight is None or q_weight.get_device() == dev)
+            and (k_weight is None or k_weight.get_device() == dev)):
+        refuse_devices("qk_norm_rope", q, k, positions, inv_freq, q_weight, k_weight)
     refuse_grad("qk_norm_rope", q, k, inv_freq, q_weight, k_weight)
-    if q.stride(3) != 1:
+    qb, qh, qs, qd = q.stride()
+    if qd != 1:
         q = q.contiguous()
-    if k.stride(3) != 1:
+        qb, qh, qs, qd = q.stride()
+    kb, kh, ks, kd = k.stride()
+    if kd != 1:
         k = k.contiguous()
+        kb, kh, ks, kd = k.stride()
     qo, ko = rows_like(q), rows_like(k)
-    if B * S == 0 or Hq == 0 or k.shape[1] == 0:
+    if B * S == 0 or Hq == 0 or Hk == 0:
         return qo, ko
-    with nat.on_device(q.device):
+    qob, qoh, qos, _ = qo.stride()
+    kob, koh, kos, _ = ko.stride()
+    device = q.device
+    with nat.on_device(device):
         rc = nat.lib().va_qk_norm_rope(
-            dtype, nat.addr(q), *q.stride()[:3], nat.addr(k), *k.stride()[:3], nat.addr(qo),
-            *qo.stride()[:3], nat.addr(ko), *ko.stride()[:3], B, Hq, k.shape[1], S, D,
-            nat.addr(positions), spa, positions.stride(-2), axes, sections, nat.addr(inv_freq),
-            rot, nat.addr(q_weight), nat.addr(k_weight), wtype, eps, attention_scaling,
-            int(interleaved), nat.stream_addr(q.device))
+            dtype, q.data_ptr(), qb, qh, qs, k.data_ptr(), kb, kh, ks, qo.data_ptr(), qob, qoh,
+            qos, ko.data_ptr(), kob, koh, kos, B, Hq, Hk, S, D, positions.data_ptr(), spa,
+            positions.stride(-2), axes, sections, inv_freq.data_ptr(), rot, nat.addr(q_weight),
+            nat.addr(k_weight), wtype, float(eps), float(attention_scaling),
+            1 if interleaved else 0,
+            nat.stream_addr(device))
     nat.check("va_qk_norm_rope", rc)
     return qo, ko
 
