@@ -32,6 +32,7 @@ __device__ inline float* part_row(const PagedArgs& a, int64_t slot, int64_t row)
 // Where a work-group's share begins and ends, and the request of its first unit.
 struct Place {
   PagedShare share;
+  uint32_t number;   // of the share
   uint32_t begin, end;
   uint32_t base;     // first unit of the request
   int32_t request, keys;
@@ -40,6 +41,17 @@ struct PlaceLds {
   uint32_t sum[kPagedWaves], base;
   int32_t request, keys;
 };
+
+// The share of a work-group.  Neighbouring work-groups take shares a quarter of
+// all apart: consecutive shares belong to one kv head for long, whose rows lie in
+// the same part of every token's and keep to some of the memory channels, and the
+// shares that start first got ahead of the others (36 to 44 us at one request of
+// 131072 keys).  us in order / in quarters: 32 + 8 heads, 131072 keys 114 / 102;
+// 16 + 16 heads, 40000 keys 75.3 / 68.9; 8 requests up to 32768 keys 47.4 / 45.5.
+__device__ inline uint32_t share_number(const PagedArgs& a) {
+  const uint32_t quarter = uint32_t(a.groups) / 4;
+  return blockIdx.x < 4 * quarter ? blockIdx.x % 4 * quarter + blockIdx.x / 4 : blockIdx.x;
+}
 
 // Sums the units of the requests (every work-group does, N lengths from L2) and
 // finds the request of the share's first unit.
@@ -65,7 +77,8 @@ __device__ inline Place locate(const PagedArgs& a, PlaceLds& lds) {
     total += lds.sum[i];
   }
   const PagedShare share(total, uint32_t(a.groups));
-  const uint32_t begin = share.begin(blockIdx.x);
+  const uint32_t number = share_number(a);
+  const uint32_t begin = share.begin(number);
   if (begin >= at && begin < at + mine)
     for (int32_t i = lo; i < lo + per && i < N; ++i) {
       if (per > 1) keys = paged_keys(a.lens[i], capacity);
@@ -79,7 +92,7 @@ __device__ inline Place locate(const PagedArgs& a, PlaceLds& lds) {
       at += n;
     }
   __syncthreads();
-  return Place{share, begin, share.begin(blockIdx.x + 1), lds.base, lds.request, lds.keys};
+  return Place{share, number, begin, share.begin(number + 1), lds.base, lds.request, lds.keys};
 }
 
 // Merges the waves' states of a segment's rows and writes them: to the output
@@ -219,12 +232,12 @@ __global__ __launch_bounds__(kPagedThreads) void paged_row_kernel(PagedArgs a) {
     if (lane == 0) sbad[wave] = bad;
     lds_barrier();
     finish<T, 1>(a, int(a.D), &sO[0][0][0], kRowMaxD, kRowTile * kRowMaxD, &sm[0][0], &sl[0][0], kRowTile,
-              rows, count == units, 2 * int64_t(blockIdx.x) + (u > begin), req, hk * a.G + r0,
+              rows, count == units, 2 * int64_t(pl.number) + (u > begin), req, hk * a.G + r0,
               keys == 0, sbad[0] || sbad[1] || sbad[2] || sbad[3]);
     if (c0 == 0 && threadIdx.x == 0)
       a.split[req * a.per_request + seg] =
           count == units ? make_int2(-1, -1)
-                         : make_int2(2 * int(blockIdx.x) + (u > begin),
+                         : make_int2(2 * int(pl.number) + (u > begin),
                                      int(pl.share.owner(u + units - 1)));
     u += count;
     if (u < end && u == base + units * a.per_request) {
@@ -308,7 +321,8 @@ template <int kTiles> struct Pages {
 //
 // kSplit: the units are dealt to the work-groups.  Otherwise a work-group of eight
 // waves takes a whole segment, and there is nothing to merge afterwards.
-template <typename T, int D, bool kWholeTiles, bool kSplit>
+// kStream: the values are read past the caches.
+template <typename T, int D, bool kWholeTiles, bool kSplit, bool kStream>
 __global__ __launch_bounds__(kSplit ? kPagedThreads : 2 * kPagedThreads, 2) void paged_tile_kernel(
     PagedArgs a) {
   constexpr bool k16 = sizeof(T) == 2;
@@ -328,7 +342,7 @@ __global__ __launch_bounds__(kSplit ? kPagedThreads : 2 * kPagedThreads, 2) void
   const int kg = lane / 16, c = lane % 16;
   const int64_t capacity = a.M * a.page;
   const uint32_t page = uint32_t(a.page);
-  Place pl{PagedShare(1, 1), 0, 0, 0, 0, 0};
+  Place pl{PagedShare(1, 1), 0, 0, 0, 0, 0, 0};
   if constexpr (kSplit) {
     pl = locate<kUnit>(a, place);
   } else {
@@ -434,11 +448,13 @@ __global__ __launch_bounds__(kSplit ? kPagedThreads : 2 * kPagedThreads, 2) void
 #pragma unroll
         for (int w = 0; w < kVW; w += kVW < 4 ? kVW : 4) {
           if constexpr (kVW >= 4) {
-            const u32x4_t x = *reinterpret_cast<const u32x4_t*>(
+            const u32x4_t* at = reinterpret_cast<const u32x4_t*>(
                 reinterpret_cast<const uint32_t*>(row) + w);
+            const u32x4_t x = kStream ? __builtin_nontemporal_load(at) : *at;
             vr[j][w] = x[0], vr[j][w + 1] = x[1], vr[j][w + 2] = x[2], vr[j][w + 3] = x[3];
           } else {
-            const u32x2_t x = *reinterpret_cast<const u32x2_t*>(row);
+            const u32x2_t* at = reinterpret_cast<const u32x2_t*>(row);
+            const u32x2_t x = kStream ? __builtin_nontemporal_load(at) : *at;
             vr[j][0] = x[0], vr[j][1] = x[1];
           }
         }
@@ -601,13 +617,13 @@ __global__ __launch_bounds__(kSplit ? kPagedThreads : 2 * kPagedThreads, 2) void
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) any_bad |= sbad[w] != 0;
     finish<T, 4, 64 * kWaves>(a, D, &sO[0][0][0], kStride, kTileHeads * kStride, &sm[0][0], &sl[0][0], kTileHeads,
-              rows, count == units, 2 * int64_t(blockIdx.x) + (u > begin), req, hk * a.G + r0,
+              rows, count == units, 2 * int64_t(pl.number) + (u > begin), req, hk * a.G + r0,
               keys == 0, any_bad);
     if (!kSplit) break;
     if (c0 == 0 && threadIdx.x == 0)
       a.split[req * a.per_request + seg] =
           count == units ? make_int2(-1, -1)
-                         : make_int2(2 * int(blockIdx.x) + (u > begin),
+                         : make_int2(2 * int(pl.number) + (u > begin),
                                      int(pl.share.owner(u + units - 1)));
     u += count;
     if (u < end && u == base + units * a.per_request) {
@@ -753,14 +769,25 @@ static bool whole_segments(int dtype, const PagedArgs& a) {
   return segments < 2048 && bytes <= (segments < 256 ? 256 << 10 : 512 << 10);
 }
 
-template <typename T, int D, bool kSplit>
+template <typename T, int D, bool kSplit, bool kStream>
 static void launch_tiles(const PagedArgs& a, hipStream_t stream) {
   const dim3 grid{unsigned(kSplit ? a.groups : a.N * a.per_request)};
   const dim3 block{kSplit ? kPagedThreads : 2 * kPagedThreads};
   if (a.page % 16 == 0)
-    hipLaunchKernelGGL((paged_tile_kernel<T, D, true, kSplit>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((paged_tile_kernel<T, D, true, kSplit, kStream>), grid, block, 0, stream, a);
   else
-    hipLaunchKernelGGL((paged_tile_kernel<T, D, false, kSplit>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((paged_tile_kernel<T, D, false, kSplit, kStream>), grid, block, 0, stream,
+                       a);
+}
+// Values that the Infinity Cache could not hold until the next step, if the tables
+// are full, are read past it (not keys: their rows are read in pieces of 64 bytes).
+// us without / with: 1 request, 131072 keys 60.6 / 57.3; 64 requests 101 / 93.6; 8
+// requests 45.2 / 40.5; 19 requests in fp32, 225 MB in turns, 23.7 / 24.9.
+template <typename T, int D> static void launch_split(const PagedArgs& a, hipStream_t stream) {
+  if (2 * a.N * a.Hk * a.M * a.page * D * int64_t(sizeof(T)) > (256 << 20))
+    launch_tiles<T, D, true, true>(a, stream);
+  else
+    launch_tiles<T, D, true, false>(a, stream);
 }
 
 template <typename T>
@@ -773,11 +800,12 @@ static hipError_t launch_paged_t(int dtype, PagedArgs& a, void* workspace, hipSt
                                     round256(8 * a.N * a.per_request));
   const dim3 grid{unsigned(a.groups)}, block{kPagedThreads};
   if (tiles && whole_segments(dtype, a)) {
-    a.D == 64 ? launch_tiles<T, 64, false>(a, stream) : launch_tiles<T, 128, false>(a, stream);
+    a.D == 64 ? launch_tiles<T, 64, false, false>(a, stream)
+              : launch_tiles<T, 128, false, false>(a, stream);
     return hipGetLastError();
   }
   if (tiles)
-    a.D == 64 ? launch_tiles<T, 64, true>(a, stream) : launch_tiles<T, 128, true>(a, stream);
+    a.D == 64 ? launch_split<T, 64>(a, stream) : launch_split<T, 128>(a, stream);
   else if (a.D <= 64)
     hipLaunchKernelGGL((paged_row_kernel<T, 1>), grid, block, 0, stream, a);
   else if (a.D <= 128)

@@ -111,15 +111,25 @@ typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 template <typename T> struct Piece {  // 8 features as they lie in memory
   u32x4_t w[sizeof(T) / 2];
 };
-template <typename T> __device__ inline Piece<T> load_piece(const T* p) {
+// kPast: past the caches, for data that is not used again soon.
+template <bool kPast, typename T> __device__ inline Piece<T> load_piece(const T* p) {
   Piece<T> r;
 #pragma unroll
-  for (int i = 0; i < int(sizeof(T) / 2); ++i) r.w[i] = reinterpret_cast<const u32x4_t*>(p)[i];
+  for (int i = 0; i < int(sizeof(T) / 2); ++i) {
+    const u32x4_t* at = reinterpret_cast<const u32x4_t*>(p) + i;
+    r.w[i] = kPast ? __builtin_nontemporal_load(at) : *at;
+  }
   return r;
 }
-template <typename T> __device__ inline void store_piece(T* p, const Piece<T>& r) {
+template <bool kPast, typename T> __device__ inline void store_piece(T* p, const Piece<T>& r) {
 #pragma unroll
-  for (int i = 0; i < int(sizeof(T) / 2); ++i) reinterpret_cast<u32x4_t*>(p)[i] = r.w[i];
+  for (int i = 0; i < int(sizeof(T) / 2); ++i) {
+    u32x4_t* at = reinterpret_cast<u32x4_t*>(p) + i;
+    if constexpr (kPast)
+      __builtin_nontemporal_store(r.w[i], at);
+    else
+      *at = r.w[i];
+  }
 }
 __device__ inline void unpack(const Piece<float>& r, float* x) {
 #pragma unroll
@@ -180,18 +190,20 @@ __device__ inline void load_weights(const RopeArgs& a, const void* w, int f0, in
 #pragma unroll
     for (int e = 0; e < 16; ++e) out[e] = 1.f;
   } else if (a.w_f32) {
-    unpack(load_piece(static_cast<const float*>(w) + f0), out);
-    unpack(load_piece(static_cast<const float*>(w) + f1), out + 8);
+    unpack(load_piece<false>(static_cast<const float*>(w) + f0), out);
+    unpack(load_piece<false>(static_cast<const float*>(w) + f1), out + 8);
   } else {
-    unpack(load_piece(static_cast<const T*>(w) + f0), out);
-    unpack(load_piece(static_cast<const T*>(w) + f1), out + 8);
+    unpack(load_piece<false>(static_cast<const T*>(w) + f0), out);
+    unpack(load_piece<false>(static_cast<const T*>(w) + f1), out + 8);
   }
 }
 
-// kCache: keys and values go to their slots.  kTokens tokens a work-group; U rows
-// of a lane are in flight: the first ones before the angles are made, which take
-// as long as they do, and each next one from the moment its place is free.
-template <typename T, int D, int kTokens, bool kCache>
+// kCache: keys and values go to their slots, past the caches: the next to read
+// them is the next step, after all other layers (8192 tokens 43.4 -> 41.9 us).
+// kStream: everything goes past them.  kTokens tokens a work-group; U rows of a
+// lane are in flight: the first ones before the angles are made, which take as
+// long as they do, and each next one from the moment its place is free.
+template <typename T, int D, int kTokens, bool kCache, bool kStream = false>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) void rope_kernel(RopeArgs a) {
   constexpr int kLanes = D / 16, kRows = 256 / kLanes, kHeads = kRows / kTokens;
   constexpr int U = 2;
@@ -221,8 +233,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) void rope_kernel(RopeA
     const T* from = static_cast<const T*>(rows.x) + b * rows.sb + (key ? h - a.Hq : h) * rows.sh +
                     s * rows.ss;
     if (value) from = static_cast<const T*>(a.v) + (h - a.Hq - a.Hk) * a.vh + s * a.vs;
-    p0[u] = load_piece(from + f0);
-    p1[u] = load_piece(from + f1);
+    p0[u] = load_piece<kStream>(from + f0);
+    p1[u] = load_piece<kStream>(from + f1);
   };
 #pragma unroll
   for (int u = 0; u < U; ++u) load(u, row % kHeads + u * kHeads);
@@ -300,9 +312,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) void rope_kernel(RopeA
         y0 = pack(y, T{});
         y1 = pack(y + 8, T{});
       }
-      if (!key || stored) {
-        store_piece(to + f0, y0);
-        store_piece(to + f1, y1);
+      if (kCache && key) {
+        if (stored) {
+          store_piece<true>(to + f0, y0);
+          store_piece<true>(to + f1, y1);
+        }
+      } else {
+        store_piece<kStream>(to + f0, y0);
+        store_piece<kStream>(to + f1, y1);
       }
     }
   }
@@ -328,7 +345,9 @@ __global__ __launch_bounds__(256) void write_element_kernel(WriteArgs a) {
 
 // The same in 16-byte pieces.  `lanes` lanes (a power of two up to 64) walk the
 // pieces of a token's keys and values, U tokens at a time with all their loads in
-// flight: a copy is bound by memory alone.
+// flight: a copy is bound by memory alone.  The stores go past the caches, as
+// above (32768 tokens of 4 heads of 128 in fp16: 29.8 -> 21.8 us; 613 tokens and
+// 131072 the same).
 constexpr int kWriteU = 4;
 __global__ __launch_bounds__(256) void write_piece_kernel(WriteArgs a, int es, int lanes) {
   const int per = 16 / es;                          // elements of a piece
@@ -363,8 +382,8 @@ __global__ __launch_bounds__(256) void write_piece_kernel(WriteArgs a, int es, i
 #pragma unroll
     for (int u = 0; u < kWriteU; ++u)
       if (real[u]) {
-        *piece(a.kc, ko[u] + to) = k[u];
-        *piece(a.vc, vo[u] + vto) = v[u];
+        __builtin_nontemporal_store(k[u], piece(a.kc, ko[u] + to));
+        __builtin_nontemporal_store(v[u], piece(a.vc, vo[u] + vto));
       }
   }
 }
@@ -384,12 +403,23 @@ static void launch_rope_pieces(const RopeArgs& a, hipStream_t stream) {
   // 4 heads of 128 in bf16, one token / four: 600 tokens 5.0 / 6.3, 1024 6.3 / 7.3,
   // 2333 13.1 / 11.3, 8192 34.6 / 27.0, 32760 138 / 101 (eight: 13.1, 26.2, 104).
   const int64_t tokens = a.B * a.S;
-  if (tokens >= 1536)
-    hipLaunchKernelGGL((rope_kernel<T, D, 4, kCache>), dim3(unsigned((tokens + 3) / 4)), dim3(256),
-                       0, stream, a);
-  else
+  if (tokens < 1536) {
     hipLaunchKernelGGL((rope_kernel<T, D, 1, kCache>), dim3(unsigned(tokens)), dim3(256), 0,
                        stream, a);
+    return;
+  }
+  const dim3 grid{unsigned((tokens + 3) / 4)};
+  // More than the Infinity Cache holds goes past it: with the producer before and a
+  // reader behind, 32760 tokens of 12 + 12 heads 224 -> 213 us, 32768 of 28 + 4 287 ->
+  // 258 (alone 87.7 -> 79.4, 97.9 -> 90.0); below that it costs the reader more than
+  // it saves (8192 tokens 60.7 -> 64.8).
+  if constexpr (!kCache) {
+    if (2 * tokens * (a.Hq + a.Hk) * D * int64_t(sizeof(T)) > (256 << 20)) {
+      hipLaunchKernelGGL((rope_kernel<T, D, 4, false, true>), grid, dim3(256), 0, stream, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((rope_kernel<T, D, 4, kCache>), grid, dim3(256), 0, stream, a);
 }
 
 template <typename T>
