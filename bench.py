@@ -17,7 +17,9 @@ the step over both, the roofline of the dominant kernel, and the CPU oracle
 timed on a bounded sample over every host core.
 
 Other modes (one JSON line each): --decode L (decode attention over an
-L-token KV cache), --tuner (the threshold tuner's recall/sparsity evaluation).
+L-token KV cache), --decode L --requests N (the decode step of N requests of up
+to L tokens over a paged cache), --tuner (the threshold tuner's recall/sparsity
+evaluation).
 """
 import argparse
 import json
@@ -62,6 +64,10 @@ def parse():
     ap.add_argument("--decode", type=int, default=None, metavar="L",
                     help="time decode attention (single_decode_with_kv_cache) over a KV cache "
                          "of L tokens with the workload's heads instead of the prefill")
+    ap.add_argument("--requests", type=int, default=None, metavar="N",
+                    help="with --decode L: time the step of N requests of L/4 to L tokens over a "
+                         "paged cache (paged_kv_plan, qk_norm_rope_to_cache, "
+                         "paged_decode_attention)")
     ap.add_argument("--tuner", action="store_true",
                     help="time the threshold tuner's recall/sparsity evaluation "
                          "(seg_pr_perHead) on the workload's shapes instead of the prefill")
@@ -661,6 +667,83 @@ def bench_decode(args, wl, dev):
             f.write(line + "\n")
 
 
+def bench_paged_step(args, wl, dev):
+    """One layer's decode step of N requests over a cache in pages of 16 tokens:
+    plan, norms and rotation with the write of keys and values, attention, with
+    the workload's heads; request lengths are drawn between L/4 and L.  `value`
+    is the eager step; `graph_us` the same step captured into a graph, as a
+    serving loop runs it.  HBM roofline of the step: every cached key and value
+    once."""
+    import vecattention_amd as va
+    L, N, Hq, Hk, D, page = args.decode, args.requests, wl.Hq, wl.Hk, wl.D, 16
+    g = torch.Generator().manual_seed(0)
+    lens = torch.randint(max(1, L // 4), L + 1, (N,), generator=g)
+    held, width = -(-lens // page), L // page + 2
+    pages = int(held.sum()) + N
+    ids = torch.randperm(pages, generator=g).int()
+    table = torch.full((N, width), -1, dtype=torch.int32)
+    table[torch.arange(width)[None] < held[:, None]] = ids[:int(held.sum())]
+    lens, table, free = lens.int().to(dev), table.to(dev), ids[int(held.sum()):].to(dev)
+    new = torch.ones(N, dtype=torch.int32, device=dev)
+    dg = torch.Generator(dev).manual_seed(1)
+    q, k, v = (torch.randn(N, H, D, generator=dg, device=dev).to(wl.dtype) for H in (Hq, Hk, Hk))
+    kc, vc = (torch.randn(pages, page, Hk, D, generator=dg, device=dev).to(wl.dtype)
+              for _ in range(2))
+    qw, kw = (torch.ones(D, dtype=wl.dtype, device=dev) for _ in range(2))
+    inv = (1e6 ** (-torch.arange(0, D, 2, dtype=torch.float64) / D)).float().to(dev)
+
+    def step():
+        p = va.paged_kv_plan(lens, new, table, free, page, N)
+        rq = va.qk_norm_rope_to_cache(q, k, v, kc, vc, p.slot_mapping, p.positions, inv, qw, kw)
+        return va.paged_decode_attention(rq, kc, vc, table, p.kv_lens)
+
+    def timed(fn, reps, warm):
+        for _ in range(warm):
+            fn()
+        torch.cuda.synchronize()
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        for _ in range(reps):
+            fn()
+        b.record()
+        torch.cuda.synchronize()
+        return a.elapsed_time(b) / reps
+
+    steps, warm = max(args.steps, 1) * 20, max(args.warmup, 1) * 5
+    ms = timed(step, steps, warm)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    graph_ms = timed(graph.replay, steps, warm)
+    es = torch.tensor([], dtype=wl.dtype).element_size()
+    gbs = 2 * int((lens + 1).sum()) * Hk * D * es / (graph_ms * 1e-3) / 1e9
+    result = {
+        "metric": "decode step latency over a paged cache (us)",
+        "value": round(ms * 1e3, 2),
+        "unit": "us",
+        "n_gpus": 1,
+        "steps": steps,
+        "warmup": warm,
+        "ms_per_step": round(ms, 5),
+        "higher_is_better": False,
+        "scaling": "weak",
+        "vs_baseline": None,
+        "dtype": {torch.bfloat16: "bf16", torch.float16: "fp16"}.get(wl.dtype, "fp32"),
+        "data": "synthetic (seeded N(0,1) q, K and V, random page order)",
+        "config": {"workload": f"paged-decode-{wl.name}-L{L}-N{N}", "requests": N, "Hq": Hq,
+                   "Hk": Hk, "D": D, "L": L, "page_size": page, "kv_layout": "NHD"},
+        "graph_us": round(graph_ms * 1e3, 2),
+        "roofline": {"bound": "hbm", "kernel": "paged_tile_kernel + paged_merge_kernel",
+                     "achieved": round(gbs, 1), "peak": HBM_PEAK_GBS, "unit": "GB/s",
+                     "frac": round(gbs / HBM_PEAK_GBS, 4), "traffic": None},
+    }
+    line = json.dumps(result)
+    print(line, flush=True)
+    if args.extra_json:
+        with open(args.extra_json, "a") as f:
+            f.write(line + "\n")
+
+
 # --------------------------------------------------------------------- main --
 
 def measure_prefill(args, wl, dev, with_cpu):
@@ -864,8 +947,10 @@ def main():
     if args.tuner:
         bench_tuner(args, wl, dev)
         return
+    if args.requests and not args.decode:
+        sys.exit("bench.py: --requests N goes with --decode L")
     if args.decode:
-        bench_decode(args, wl, dev)
+        (bench_paged_step if args.requests else bench_decode)(args, wl, dev)
         return
     extra = args.extra if args.extra is not None else ("B,D,E,A" if args.config == "C" else "none")
     extra = [] if extra.lower() == "none" else [x for x in extra.split(",") if x]
