@@ -550,6 +550,42 @@ def test_decode_streams_and_two_graphs():
             assert torch.equal(a, b)
 
 
+def test_refusals_on_the_gpu():
+    """What only shows with tensors on the GPU: other devices, and gradients."""
+    note("refusals")
+    g = gen(3)
+    q, k, v = (torch.randn(5, 2, 64, generator=g, device="cpu").to(DEV) for _ in range(3))
+    kc, vc = (torch.zeros(2, 16, 2, 64, device=DEV) for _ in range(2))
+    slots, pos, inv = torch.arange(5, device=DEV), torch.arange(5, device=DEV), freqs(64).to(DEV)
+    ok = (q, k, v, kc, vc, slots, pos, inv)
+    for i in range(1, 8):
+        bad = list(ok)
+        bad[i] = bad[i].cpu()
+        with pytest.raises(ValueError, match="tensors on"):
+            qk_norm_rope_to_cache(*bad)
+    w = torch.ones(64, device=DEV, requires_grad=True)
+    with pytest.raises(NotImplementedError, match="no backward"):
+        qk_norm_rope_to_cache(*ok, w, w)
+    with torch.no_grad():
+        qk_norm_rope_to_cache(*ok, w, w)
+    table, lens = torch.zeros(5, 1, dtype=torch.int32, device=DEV), torch.full(
+        (5,), 3, dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError, match="tensors on"):
+        paged_decode_attention(q, kc, vc, table.cpu(), lens)
+    with pytest.raises(NotImplementedError, match="no backward"):
+        paged_decode_attention(q.requires_grad_(), kc, vc, table, lens)
+    with pytest.raises(NotImplementedError, match="head_dim 320"):
+        paged_decode_attention(torch.zeros(1, 2, 320, device=DEV),
+                               *(torch.zeros(1, 16, 2, 320, device=DEV) for _ in range(2)),
+                               table[:1], lens[:1])
+    # nothing to do
+    empty = qk_norm_rope(torch.zeros(1, 2, 0, 64, device=DEV), torch.zeros(1, 2, 0, 64, device=DEV),
+                         torch.zeros(1, 0, dtype=torch.int64, device=DEV), inv)
+    assert empty[0].shape == (1, 2, 0, 64)
+    write_paged_kv(k[:0], v[:0], kc, vc, slots[:0])
+    assert paged_decode_attention(q.detach()[:0], kc, vc, table[:0], lens[:0]).shape == (0, 2, 64)
+
+
 # ---------------------------------------------------------------- together
 
 @pytest.mark.parametrize("dtype,layout", [(BF16, "NHD"), (F32, "HND")])

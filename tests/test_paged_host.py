@@ -326,12 +326,28 @@ def test_c_decode_errors(L):
 
 
 def test_operators_have_no_backward():
-    """The check comes after the device's, so it is seen through its own function here."""
-    from vecattention_amd.rotary import refuse_grad
-    w = torch.ones(4, requires_grad=True)
-    with pytest.raises(NotImplementedError, match="no backward"):
-        refuse_grad("x", None, w)
-    with torch.no_grad():
-        refuse_grad("x", w)
-    with torch.inference_mode():
-        refuse_grad("x", w)
+    """Refused after the device, so on the CPU the device speaks first; on a GPU
+    test_gpu_paged.py sees it."""
+    w = torch.ones(64, requires_grad=True)
+    with pytest.raises(RuntimeError, match="GPU"):
+        va.qk_norm_rope(**rope_ok(q_weight=w))
+
+
+def test_arguments_that_are_no_tensors_or_numbers():
+    with pytest.raises(TypeError, match="k must be a tensor"):
+        va.qk_norm_rope(**rope_ok(k=[1.0]))
+    with pytest.raises(TypeError, match="q_weight must be a tensor"):
+        va.qk_norm_rope(**rope_ok(q_weight=3))
+    with pytest.raises(TypeError):
+        va.qk_norm_rope(**rope_ok(mrope_section=7))
+    with pytest.raises(TypeError):
+        va.qk_norm_rope(**rope_ok(mrope_section=[16.5, 8, 8]))
+    with pytest.raises(TypeError):
+        va.paged_kv_plan(i32(3), i32(3), i32(3, 4), i32(5), 16.5, 8)
+    with pytest.raises(OverflowError):
+        va.paged_kv_plan(i32(3), i32(3), i32(3, 4), i32(5), 16, 1 << 70)
+    with pytest.raises(TypeError, match="arguments"):
+        nat._host_module().plan(1, 2)
+    with pytest.raises(KeyError):
+        va.write_paged_kv(torch.zeros(5, 2, 64), torch.zeros(5, 2, 64), torch.zeros(3, 16, 2, 64),
+                          torch.zeros(3, 16, 2, 64), torch.zeros(5, dtype=torch.int64), None)

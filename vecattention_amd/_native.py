@@ -207,3 +207,31 @@ _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device
 def on_device(device):
     """torch.cuda.device(device), without its bookkeeping when there is nothing to switch."""
     return _here if _current_device() == device.index else torch.cuda.device(device)
+
+
+_host = None
+
+
+def _host_module():
+    """The host module (csrc/host_calls.cpp), loaded once; raises if it is absent."""
+    global _host
+    if _host is None:
+        lib()
+        if not os.path.exists(os.path.join(_HERE, "_host.so")):
+            raise RuntimeError(
+                f"{_HERE}/_host.so is missing: build it with `python -m vecattention_amd.build`")
+        from . import _host as module
+        _host = module
+    return _host
+
+
+def host_call(name, on, *args):
+    """A call of the host module on the current stream of the tensor `on`'s GPU."""
+    call = getattr(_host or _host_module(), name)
+    dev = on.get_device()
+    if dev < 0:
+        return call(*args, 0)  # no GPU: the call refuses it
+    if dev == _current_device():
+        return call(*args, stream_addr(on.device) if _raw_stream is None else _raw_stream(dev))
+    with torch.cuda.device(dev):
+        return call(*args, stream_addr(on.device))

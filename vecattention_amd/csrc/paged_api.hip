@@ -108,7 +108,7 @@ int va_paged_plan(const int32_t* kv_lens, const int32_t* new_lens, int64_t N,
       va::launch_paged_plan(kv_lens, new_lens, N, block_tables, stn, M, free_pages, num_free,
                             free_head, page_size, num_tokens, kv_lens_out, qo_indptr, slot_mapping,
                             positions, request_ids, pages_taken,
-                            static_cast<int64_t*>(workspace), static_cast<hipStream_t>(stream)),
+                            static_cast<uint32_t*>(workspace), static_cast<hipStream_t>(stream)),
       "plan launch");
 }
 

@@ -633,19 +633,19 @@ __global__ __launch_bounds__(kSplit ? kPagedThreads : 2 * kPagedThreads, 2) void
   }
 }
 
-// Rows of segments that several work-groups share: one work-group of 256
-// threads per (segment, row).  The partials' weights 2^(m - M) go to LDS; kV
+// Rows of segments that several work-groups share: one work-group per
+// (segment, row).  The partials' weights 2^(m - M) go to LDS; kV
 // features a thread, as many partials side by side as that leaves threads for, U
 // of each thread's in flight (the first ones while the weights are computed);
 // then their sums, always in the same order.
 constexpr int kMostGroups = 2048;
-template <typename T, int kV>
-__global__ __launch_bounds__(kPagedThreads) void paged_merge_kernel(PagedArgs a) {
+template <typename T, int kV, int kThreads>
+__global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedArgs a) {
   typedef float vec __attribute__((ext_vector_type(kV)));
-  constexpr int U = 4;
+  constexpr int U = 4, kWaves = kThreads / 64;
   __shared__ float weight[kMostGroups + 1];
-  __shared__ vec sacc[kPagedThreads];
-  __shared__ float top[kPagedWaves], den[kPagedWaves];
+  __shared__ vec sacc[kThreads];
+  __shared__ float top[kWaves], den[kWaves];
   const int2 split = a.split[blockIdx.x];
   if (split.x < 0) return;  // written whole
   const uint32_t r = blockIdx.y, n = blockIdx.x / a.per_request;
@@ -653,7 +653,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_merge_kernel(PagedArgs a)
   const uint32_t head = (s - hk * a.tiles) * a.rows + r;
   if (head >= a.G) return;
   const int w0 = split.x / 2, parts = split.y - w0 + 1;
-  const int lanes = int(a.D) / kV, side = kPagedThreads / lanes;
+  const int lanes = int(a.D) / kV, side = kThreads / lanes;
   const int p = threadIdx.x / lanes, c = threadIdx.x - p * lanes;
   auto slot = [&](int i) { return int64_t(i == 0 ? split.x : 2 * (w0 + i)); };
   // Reads past the last partial read it again, with no weight.
@@ -667,7 +667,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_merge_kernel(PagedArgs a)
   };
   load(0);
   float m = -__builtin_inff();
-  for (int i = threadIdx.x; i < parts; i += kPagedThreads) {
+  for (int i = threadIdx.x; i < parts; i += kThreads) {
     const float2 ml = part_ml(a, slot(i))[r];
     if (!(ml.y == 0.f)) m = __builtin_fmaxf(m, ml.x);
   }
@@ -676,9 +676,9 @@ __global__ __launch_bounds__(kPagedThreads) void paged_merge_kernel(PagedArgs a)
   if (threadIdx.x % 64 == 0) top[threadIdx.x / 64] = m;
   lds_barrier();
 #pragma unroll
-  for (int w = 0; w < kPagedWaves; ++w) m = __builtin_fmaxf(m, top[w]);
+  for (int w = 0; w < kWaves; ++w) m = __builtin_fmaxf(m, top[w]);
   float l = 0.f;
-  for (int i = threadIdx.x; i < parts; i += kPagedThreads) {
+  for (int i = threadIdx.x; i < parts; i += kThreads) {
     const float2 ml = part_ml(a, slot(i))[r];
     const float f = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - m);  // 0: no key of any weight
     weight[i] = f;
@@ -709,7 +709,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_merge_kernel(PagedArgs a)
   for (int i = 1; i < side; ++i) acc += sacc[i * lanes + c];
   l = 0.f;
 #pragma unroll
-  for (int w = 0; w < kPagedWaves; ++w) l += den[w];
+  for (int w = 0; w < kWaves; ++w) l += den[w];
   T* out = static_cast<T*>(a.out) + n * a.on + (hk * a.G + head) * a.oh + c * kV;
 #pragma unroll
   for (int i = 0; i < kV; ++i) out[i] = Round<T>::store(acc[i] / l);
@@ -815,10 +815,12 @@ static hipError_t launch_paged_t(int dtype, PagedArgs& a, void* workspace, hipSt
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const dim3 segments{unsigned(a.N * a.per_request), unsigned(a.rows)};
-  if (a.D % 4 == 0)
-    hipLaunchKernelGGL((paged_merge_kernel<T, 4>), segments, block, 0, stream, a);
+  if (a.D % 4 != 0)
+    hipLaunchKernelGGL((paged_merge_kernel<T, 1, 256>), segments, dim3(256), 0, stream, a);
+  else if (a.D <= 128 && a.groups <= 8 * a.N * a.per_request)
+    hipLaunchKernelGGL((paged_merge_kernel<T, 4, 64>), segments, dim3(64), 0, stream, a);
   else
-    hipLaunchKernelGGL((paged_merge_kernel<T, 1>), segments, block, 0, stream, a);
+    hipLaunchKernelGGL((paged_merge_kernel<T, 4, 256>), segments, dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 

@@ -10,7 +10,7 @@ hipError_t launch_paged_plan(const int32_t* kv_lens, const int32_t* new_lens, in
                              const int32_t* free_pages, int64_t F, const int32_t* free_head,
                              int64_t page, int64_t tokens, int32_t* kv_out, int32_t* indptr,
                              int64_t* slots, int64_t* positions, int32_t* requests,
-                             int64_t* taken, int64_t* workspace, hipStream_t stream);
+                             int64_t* taken, uint32_t* workspace, hipStream_t stream);
 int64_t plan_workspace_bytes(int64_t N);
 
 constexpr int kRopeAxes = 4;

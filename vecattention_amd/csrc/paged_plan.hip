@@ -16,7 +16,7 @@
 
 namespace va {
 
-constexpr int kPlanLds = 2048;       // requests whose sums fit the LDS of a work-group (32 KB)
+constexpr int kPlanLds = 2048;       // requests whose sums fit the LDS of a work-group (16 KB)
 constexpr int kPlanThreads = 256;
 
 struct PlanArgs {
@@ -29,6 +29,7 @@ struct PlanArgs {
   int64_t F;
   const int32_t* free_head;
   uint32_t page;
+  uint32_t token_groups;
   int64_t tokens;
   int32_t* kv_out;
   int32_t* indptr;
@@ -42,55 +43,65 @@ __device__ inline PlanRow plan_row(const PlanArgs& a, int64_t i) {
   return PlanRow(a.kv_lens[i], a.new_lens[i], a.page, uint32_t(a.M));
 }
 
-// Exclusive sums of (x, y) over the work-group, and their totals in *tx, *ty.
+// Sums that end at 2^31 - 1 (still associative, for values up to that): no token
+// or entry behind it is ever looked up.
+constexpr uint32_t kMost = 0x7fffffffu;
+__device__ inline uint32_t plus(uint32_t a, uint32_t b) {
+  const uint32_t s = a + b;
+  return s < kMost ? s : kMost;
+}
+// As wave_inclusive_sum (lanes.h), with plus.
+__device__ inline uint32_t wave_inclusive_plus(uint32_t x) {
+#define VA_STEP(ctrl, rows) \
+  x = plus(x, uint32_t(__builtin_amdgcn_update_dpp(0, int(x), ctrl, rows, 0xf, false)))
+  VA_STEP(0x111, 0xf);  // row_shr:1, 2, 4, 8
+  VA_STEP(0x112, 0xf);
+  VA_STEP(0x114, 0xf);
+  VA_STEP(0x118, 0xf);
+  VA_STEP(0x142, 0xa);  // row_bcast:15 -> rows 1, 3
+  VA_STEP(0x143, 0xc);  // row_bcast:31 -> rows 2, 3
+#undef VA_STEP
+  return x;
+}
+
+// Exclusive sums of x and of y over the work-group, and their totals.
 template <int kThreads>
-__device__ inline void block_exclusive(int64_t& x, int64_t& y, int64_t* tx, int64_t* ty,
-                                       int64_t (*wave)[2]) {
+__device__ inline void block_exclusive(uint32_t& x, uint32_t& y, uint32_t* tx, uint32_t* ty,
+                                       uint2* wave) {
   const int lane = threadIdx.x % 64, w = threadIdx.x / 64;
-  int64_t sx = x, sy = y;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t ux = __shfl_up(sx, d), uy = __shfl_up(sy, d);
-    if (lane >= d) {
-      sx += ux;
-      sy += uy;
-    }
-  }
-  if (lane == 63) {
-    wave[w][0] = sx;
-    wave[w][1] = sy;
-  }
+  const uint32_t sx = wave_inclusive_plus(x), sy = wave_inclusive_plus(y);
+  if (lane == 63) wave[w] = make_uint2(sx, sy);
   __syncthreads();
-  int64_t bx = 0, by = 0, ax = 0, ay = 0;
+  uint32_t bx = 0, by = 0;
+  *tx = *ty = 0;
 #pragma unroll
   for (int i = 0; i < kThreads / 64; ++i) {
     if (i < w) {
-      bx += wave[i][0];
-      by += wave[i][1];
+      bx = plus(bx, wave[i].x);
+      by = plus(by, wave[i].y);
     }
-    ax += wave[i][0];
-    ay += wave[i][1];
+    *tx = plus(*tx, wave[i].x);
+    *ty = plus(*ty, wave[i].y);
   }
-  x = bx + sx - x;
-  y = by + sy - y;
-  *tx = ax;
-  *ty = ay;
+  // Exclusive: the lane before's sum.
+  const uint32_t ex = __shfl_up(sx, 1), ey = __shfl_up(sy, 1);
+  x = plus(bx, lane ? ex : 0u);
+  y = plus(by, lane ? ey : 0u);
 }
 
 // Outputs of one request: the length after the step and the row start.
 __device__ inline void plan_request(const PlanArgs& a, int64_t i, const PlanRow& r,
-                                    int64_t first_token) {
-  const uint32_t end = r.len + r.fresh;
-  a.kv_out[i] = int32_t(end < 0x7fffffffu ? end : 0x7fffffffu);
-  a.indptr[i] = int32_t(first_token < 0x7fffffff ? first_token : 0x7fffffff);
+                                    uint32_t first_token) {
+  a.kv_out[i] = int32_t(plus(r.len, r.fresh));
+  a.indptr[i] = int32_t(first_token);
 }
 
 // Largest i in [0, n) with start[i] <= x, where start[0] = 0 <= x < start[n]:
 // the request that holds x (requests that hold nothing are passed over).
-__device__ inline int64_t holder(const int64_t* start, int64_t n, int64_t x) {
-  int64_t lo = 0, hi = n;
+__device__ inline uint32_t holder(const uint32_t* start, uint32_t n, uint32_t x) {
+  uint32_t lo = 0, hi = n;
   while (hi - lo > 1) {
-    const int64_t mid = (lo + hi) >> 1;
+    const uint32_t mid = (lo + hi) >> 1;
     if (start[mid] <= x)
       lo = mid;
     else
@@ -99,86 +110,110 @@ __device__ inline int64_t holder(const int64_t* start, int64_t n, int64_t x) {
   return lo;
 }
 
-// The work-group's tokens and pages.  tok, pag: the sums, with the totals at [N].
-__device__ inline void plan_fill(const PlanArgs& a, const int64_t* tok, const int64_t* pag) {
-  const int64_t threads = int64_t(gridDim.x) * kPlanThreads;
-  const int64_t me = int64_t(blockIdx.x) * kPlanThreads + threadIdx.x;
+// The work-group's share.  tok, pag: the sums, with the totals at [N].  The first
+// `token_groups` work-groups take the tokens, kRun in a row to a thread, which makes
+// one search, and one division for each request and page that they reach (steps
+// of single tokens: kRun 1, all searches at once); the others take the new pages.
+template <int kRun>
+__device__ inline void plan_fill(const PlanArgs& a, const uint32_t* tok, const uint32_t* pag) {
+  const uint32_t N = uint32_t(a.N);
   const int64_t head = a.free_head ? int64_t(*a.free_head) : 0;
-  const int64_t ntok = tok[a.N], npag = pag[a.N];
-  for (int64_t t = me; t < a.tokens; t += threads) {
-    int64_t slot = -1, pos = 0;
-    int32_t req = -1;
-    if (t < ntok) {
-      const int64_t i = holder(tok, a.N, t);
+  const uint32_t ntok = tok[N], npag = pag[N];
+  if (blockIdx.x >= a.token_groups) {
+    const uint32_t threads = (gridDim.x - a.token_groups) * kPlanThreads;
+    const uint32_t me = (blockIdx.x - a.token_groups) * kPlanThreads + threadIdx.x;
+    for (uint32_t g = me; g < npag; g += threads) {
+      const uint32_t i = holder(pag, N, g);
       const PlanRow r = plan_row(a, i);
-      const uint32_t p = r.len + uint32_t(t - tok[i]);
-      slot = plan_slot(r, p, a.page, uint32_t(a.M), a.table + i * a.table_stride, a.free_pages,
-                       a.F, head + pag[i]);
-      pos = p;
-      req = int32_t(i);
+      a.table[int64_t(i) * a.table_stride + r.held + (g - pag[i])] =
+          free_page(a.free_pages, a.F, head + g);
     }
-    a.slots[t] = slot;
-    a.positions[t] = pos;
-    a.requests[t] = req;
+    if (me == 0) {
+      a.indptr[N] = int32_t(ntok);
+      *a.taken = npag;
+    }
+    return;
   }
-  for (int64_t g = me; g < npag; g += threads) {
-    const int64_t i = holder(pag, a.N, g);
-    const PlanRow r = plan_row(a, i);
-    a.table[i * a.table_stride + r.held + (g - pag[i])] = free_page(a.free_pages, a.F, head + g);
-  }
-  if (me == 0) {
-    a.indptr[a.N] = int32_t(ntok < 0x7fffffff ? ntok : 0x7fffffff);
-    *a.taken = npag;
+  const int64_t step = int64_t(a.token_groups) * kPlanThreads * kRun;
+  for (int64_t t0 = (int64_t(blockIdx.x) * kPlanThreads + threadIdx.x) * kRun; t0 < a.tokens;
+       t0 += step) {
+    uint32_t i = 0, next = 0, pos = 0, left = 0;  // request, its last token + 1, tokens left in page
+    int64_t slot = -1;
+#pragma unroll
+    for (int e = 0; e < kRun; ++e) {
+      const int64_t t64 = t0 + e;
+      if (t64 >= a.tokens) break;
+      const uint32_t t = uint32_t(t64);
+      const bool real = t < ntok;
+      if (real) {
+        if (e == 0 || t >= next || left == 0) {
+          if (e == 0 || t >= next) i = holder(tok, N, t);
+          next = tok[i + 1];
+          const PlanRow r = plan_row(a, i);
+          pos = r.len + (t - tok[i]);
+          slot = plan_slot(r, pos, a.page, uint32_t(a.M), a.table + int64_t(i) * a.table_stride,
+                           a.free_pages, a.F, head + pag[i]);
+          left = a.page - pos % a.page - 1;
+        } else {
+          ++pos;
+          --left;
+          slot = slot < 0 ? -1 : slot + 1;
+        }
+      }
+      a.slots[t64] = real ? slot : -1;
+      a.positions[t64] = real ? int64_t(pos) : 0;
+      a.requests[t64] = real ? int32_t(i) : -1;
+    }
   }
 }
 
+template <int kRun>
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
-  __shared__ int64_t tok[kPlanLds + 1], pag[kPlanLds + 1];
-  __shared__ int64_t wave[kPlanThreads / 64][2];
-  const int64_t per = (a.N + kPlanThreads - 1) / kPlanThreads;
-  const int64_t lo = threadIdx.x * per < a.N ? threadIdx.x * per : a.N;
-  const int64_t hi = lo + per < a.N ? lo + per : a.N;
-  int64_t x = 0, y = 0, tx, ty;
-  for (int64_t i = lo; i < hi; ++i) {
+  __shared__ uint32_t tok[kPlanLds + 1], pag[kPlanLds + 1];
+  __shared__ uint2 wave[kPlanThreads / 64];
+  const int per = int(a.N + kPlanThreads - 1) / kPlanThreads;
+  const int lo = int(threadIdx.x) * per, N = int(a.N);
+  uint32_t x = 0, y = 0, tx, ty;
+  for (int i = lo; i < lo + per && i < N; ++i) {
     const PlanRow r = plan_row(a, i);
-    x += r.fresh;
-    y += r.need;
+    x = plus(x, r.fresh);
+    y = plus(y, r.need);
   }
   block_exclusive<kPlanThreads>(x, y, &tx, &ty, wave);
-  for (int64_t i = lo; i < hi; ++i) {
+  for (int i = lo; i < lo + per && i < N; ++i) {
     const PlanRow r = plan_row(a, i);
     tok[i] = x;
     pag[i] = y;
     if (blockIdx.x == 0) plan_request(a, i, r, x);
-    x += r.fresh;
-    y += r.need;
+    x = plus(x, r.fresh);
+    y = plus(y, r.need);
   }
   if (threadIdx.x == 0) {
-    tok[a.N] = tx;
-    pag[a.N] = ty;
+    tok[N] = tx;
+    pag[N] = ty;
   }
   __syncthreads();
-  plan_fill(a, tok, pag);
+  plan_fill<kRun>(a, tok, pag);
 }
 
 // More requests than LDS holds: the sums of all of them, kThreads at a time.
 constexpr int kScanThreads = 1024;
-__global__ __launch_bounds__(kScanThreads) void plan_scan_kernel(PlanArgs a, int64_t* tok,
-                                                                 int64_t* pag) {
-  __shared__ int64_t wave[kScanThreads / 64][2];
-  int64_t bx = 0, by = 0;
+__global__ __launch_bounds__(kScanThreads) void plan_scan_kernel(PlanArgs a, uint32_t* tok,
+                                                                 uint32_t* pag) {
+  __shared__ uint2 wave[kScanThreads / 64];
+  uint32_t bx = 0, by = 0;
   for (int64_t base = 0; base < a.N; base += kScanThreads) {
     const int64_t i = base + threadIdx.x;
     const PlanRow r = i < a.N ? plan_row(a, i) : PlanRow(0, 0, 1, 0);
-    int64_t x = r.fresh, y = r.need, tx, ty;
+    uint32_t x = r.fresh, y = r.need, tx, ty;
     block_exclusive<kScanThreads>(x, y, &tx, &ty, wave);
     if (i < a.N) {
-      tok[i] = bx + x;
-      pag[i] = by + y;
-      plan_request(a, i, r, bx + x);
+      tok[i] = plus(bx, x);
+      pag[i] = plus(by, y);
+      plan_request(a, i, r, plus(bx, x));
     }
-    bx += tx;
-    by += ty;
+    bx = plus(bx, tx);
+    by = plus(by, ty);
     __syncthreads();  // `wave` is written again
   }
   if (threadIdx.x == 0) {
@@ -186,35 +221,45 @@ __global__ __launch_bounds__(kScanThreads) void plan_scan_kernel(PlanArgs a, int
     pag[a.N] = by;
   }
 }
-__global__ __launch_bounds__(kPlanThreads) void plan_fill_kernel(PlanArgs a, const int64_t* tok,
-                                                                 const int64_t* pag) {
-  plan_fill(a, tok, pag);
+__global__ __launch_bounds__(kPlanThreads) void plan_fill_kernel(PlanArgs a, const uint32_t* tok,
+                                                                 const uint32_t* pag) {
+  plan_fill<1>(a, tok, pag);
 }
 
-int64_t plan_workspace_bytes(int64_t N) { return N <= kPlanLds ? 0 : 16 * (N + 1); }
+int64_t plan_workspace_bytes(int64_t N) { return N <= kPlanLds ? 0 : 8 * (N + 1); }
 
 hipError_t launch_paged_plan(const int32_t* kv_lens, const int32_t* new_lens, int64_t N,
                              int32_t* table, int64_t table_stride, int64_t M,
                              const int32_t* free_pages, int64_t F, const int32_t* free_head,
                              int64_t page, int64_t tokens, int32_t* kv_out, int32_t* indptr,
                              int64_t* slots, int64_t* positions, int32_t* requests,
-                             int64_t* taken, int64_t* workspace, hipStream_t stream) {
-  const PlanArgs a{kv_lens, new_lens, N,      table,  table_stride, M,         free_pages, F,
-                   free_head, uint32_t(page), tokens, kv_out,       indptr,    slots,
-                   positions, requests,       taken};
-  // Four tokens a thread: fewer repeat the sums more often, more leave CUs idle.
-  int64_t groups = (tokens + 4 * kPlanThreads - 1) / (4 * kPlanThreads);
+                             int64_t* taken, uint32_t* workspace, hipStream_t stream) {
+  // Steps of single tokens, or prompts among them.
+  const int run = N <= kPlanLds && tokens > 4 * N ? 4 : 1;
+  int64_t groups = (tokens + run * kPlanThreads - 1) / (run * kPlanThreads);
   if (groups < 1) groups = 1;
   if (groups > 4096) groups = 4096;
-  if (N <= kPlanLds) {
-    hipLaunchKernelGGL(plan_kernel, dim3(unsigned(groups)), dim3(kPlanThreads), 0, stream, a);
-  } else {
+  int64_t page_groups = (tokens / page + N + 4 * kPlanThreads - 1) / (4 * kPlanThreads);
+  if (page_groups < 1) page_groups = 1;
+  if (page_groups > 1024) page_groups = 1024;
+  const PlanArgs a{kv_lens,   new_lens,       N,
+                   table,     table_stride,   M,
+                   free_pages, F,             free_head,
+                   uint32_t(page), uint32_t(groups), tokens,
+                   kv_out,    indptr,         slots,
+                   positions, requests,       taken};
+  const dim3 grid{unsigned(groups + page_groups)}, block{kPlanThreads};
+  if (N > kPlanLds) {
     hipLaunchKernelGGL(plan_scan_kernel, dim3(1), dim3(kScanThreads), 0, stream, a, workspace,
                        workspace + (N + 1));
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(plan_fill_kernel, dim3(unsigned(groups)), dim3(kPlanThreads), 0, stream, a,
-                       workspace, workspace + (N + 1));
+    hipLaunchKernelGGL(plan_fill_kernel, grid, block, 0, stream, a, workspace,
+                       workspace + (N + 1));
+  } else if (run == 4) {
+    hipLaunchKernelGGL(plan_kernel<4>, grid, block, 0, stream, a);
+  } else {
+    hipLaunchKernelGGL(plan_kernel<1>, grid, block, 0, stream, a);
   }
   return hipGetLastError();
 }
