@@ -132,7 +132,9 @@ def rope_inputs(B, Hq, Hk, S, D, dtype, seed, bshd=True):
     (1, 1, 1, 1, 128, 128, 1, True, True), (3, 5, 1, 9, 128, 64, 3, True, True),
     (1, 12, 12, 70, 80, 80, 1, True, False), (2, 3, 2, 11, 96, 34, 4, True, True),
     (1, 2, 1, 19, 256, 256, 1, True, True), (1, 40, 2, 130, 64, 32, 3, True, True),
-    (1, 1, 3, 5, 2, 2, 1, True, True), (1, 2, 2, 6, 512, 512, 1, False, False)])
+    (1, 1, 3, 5, 2, 2, 1, True, True), (1, 2, 2, 6, 512, 512, 1, False, False),
+    (1, 3, 2, 1701, 128, 128, 3, True, True), (2, 5, 1, 801, 64, 48, 1, True, False),
+    (1, 1, 1, 1537, 256, 128, 1, False, True)])
 def test_rope_matches_the_plain_form(B, Hq, Hk, S, D, rot, axes, norm, bshd, interleaved, dtype):
     note("rope", B, Hq, Hk, S, D, rot, axes, norm, bshd, interleaved, dtype)
     g = gen(S + D)
@@ -182,6 +184,21 @@ def test_rope_options_and_strides():
     q = torch.randn(B, Hq, D, S, generator=g).transpose(2, 3)
     got = qk_norm_rope(q.to(DEV), q.to(DEV), pos.to(DEV), freqs(D).to(DEV))
     within(got[0], *ref.rotate(q, pos.long(), freqs(D)), F32)
+
+
+def test_rope_more_than_the_cache_holds():
+    """Tensors of 278 MB, which go past the Infinity Cache, bit for bit as in two halves."""
+    note("rope, 278 MB")
+    S = 17001
+    q, k = (torch.randn(1, S, H, 128, device=DEV).bfloat16().transpose(1, 2) for H in (28, 4))
+    pos = torch.arange(S, device=DEV) + 7
+    w = (1 + 0.1 * torch.randn(128, device=DEV)).bfloat16()
+    inv = freqs(128).to(DEV)
+    whole = qk_norm_rope(q, k, pos, inv, w, w)
+    for part in (slice(0, 8000), slice(8000, S)):
+        half = qk_norm_rope(q[:, :, part], k[:, :, part], pos[part], inv, w, w)
+        for a, b in zip(whole, half):
+            assert torch.equal(a[:, :, part], b)
 
 
 def test_rope_far_positions_and_odd_values():
@@ -276,7 +293,8 @@ def test_write_strided_rows_and_caches():
 @pytest.mark.parametrize("T,Hq,Hk,D,rot,axes,norm,page,layout", [
     (1, 28, 4, 128, 128, 1, True, 16, "NHD"), (130, 32, 8, 128, 128, 1, True, 64, "HND"),
     (33, 8, 1, 64, 64, 3, False, 12, "NHD"), (16, 5, 5, 128, 64, 1, True, 1, "HND"),
-    (7, 40, 2, 96, 96, 1, True, 5, "NHD"), (300, 2, 2, 256, 256, 1, True, 32, "NHD")])
+    (7, 40, 2, 96, 96, 1, True, 5, "NHD"), (300, 2, 2, 256, 256, 1, True, 32, "NHD"),
+    (1538, 3, 2, 128, 128, 3, True, 16, "HND"), (1601, 2, 1, 64, 32, 1, False, 7, "NHD")])
 def test_rope_to_cache(T, Hq, Hk, D, rot, axes, norm, page, layout, dtype):
     """Queries and stored keys are those of the plain form, values are copied, other rows stay."""
     note("rope to cache", T, Hq, Hk, D, rot, axes, norm, page, layout, dtype)
@@ -389,6 +407,39 @@ def test_decode_many_requests(dtype):
     out = run_decode(*case, "NHD")
     within(out, *ref.decode(*case, "NHD"), dtype)
     assert torch.equal(out, run_decode(*case, "NHD"))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("D,page,extra", [(64, 16, 0), (128, 24, 0), (128, 16, 6), (64, 5, 20)])
+def test_decode_many_short_requests(D, page, extra, dtype):
+    """More segments than the GPU has CUs, tables of few pages: one wave or eight to a segment."""
+    note("paged decode, short requests", D, page, extra, dtype)
+    g = gen(D + page)
+    lens = torch.randint(0, 90, (140,), generator=g).tolist()
+    case = decode_case(lens, 6, 2, D, page, "NHD", dtype, seed=page, extra=extra)
+    bad = case[3].clone()
+    out = run_decode(*case, "NHD")
+    want, slack = ref.decode(*case, "NHD")
+    within(out, want, slack, dtype)
+    n = int(torch.tensor(lens).argmax())
+    bad[n, 0] = -1
+    out = run_decode(*case[:3], bad, case[4], "NHD").cpu()
+    assert bool(torch.isnan(out[n]).all())
+    keep = torch.arange(140) != n
+    within(out[keep], want[keep], slack[keep], dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_decode_forms_by_table_width(dtype):
+    """The same requests under tables of other widths take other forms of the kernel: one wave a
+    segment, eight, or the keys dealt out and merged, which also reads values past the caches."""
+    note("paged decode, forms", dtype)
+    q, kc, vc, table, lens = decode_case([40, 0, 17, 64] * 70, 4, 2, 64, 16, "NHD", dtype, seed=8)
+    want, slack = ref.decode(q, kc, vc, table, lens, "NHD")
+    for width in (4, 40, 64, 400, 9000):
+        wide = torch.full((280, width), -1, dtype=torch.int32)
+        wide[:, :4] = table[:, :4]
+        within(run_decode(q, kc, vc, wide, lens, "NHD"), want, slack, dtype)
 
 
 @pytest.mark.parametrize("D,dtype", [(128, BF16), (64, F32), (80, BF16)])

@@ -98,7 +98,7 @@ __device__ inline Place locate(const PagedArgs& a, PlaceLds& lds) {
 // Merges the waves' states of a segment's rows and writes them: to the output
 // (`whole`), or to a partial slot.  sO[wave][row][stride], sm/sl[wave][row];
 // kV features of a row a thread.
-template <typename T, int kV, int kThreads = kPagedThreads>
+template <typename T, int kV, int kThreads = kPagedThreads, int kStates = kPagedWaves>
 __device__ inline void finish(const PagedArgs& a, int D, const float* sO, int rstride,
                               int wstride, const float* sm, const float* sl, int mstride, int rows,
                               bool whole, int64_t slot, int64_t request, int64_t head, bool empty,
@@ -107,21 +107,21 @@ __device__ inline void finish(const PagedArgs& a, int D, const float* sO, int rs
   const int pieces = D / kV;
   for (int i = threadIdx.x; i < rows * pieces; i += kThreads) {
     const int r = i / pieces, f = (i - r * pieces) * kV;
-    float lw[kPagedWaves], mw[kPagedWaves], m = -__builtin_inff();
-    vec ow[kPagedWaves];
+    float lw[kStates], mw[kStates], m = -__builtin_inff();
+    vec ow[kStates];
 #pragma unroll
-    for (int w = 0; w < kPagedWaves; ++w) {
+    for (int w = 0; w < kStates; ++w) {
       lw[w] = sl[w * mstride + r];
       mw[w] = sm[w * mstride + r];
       ow[w] = *reinterpret_cast<const vec*>(sO + w * wstride + r * rstride + f);
     }
 #pragma unroll
-    for (int w = 0; w < kPagedWaves; ++w)
+    for (int w = 0; w < kStates; ++w)
       if (!(lw[w] == 0.f)) m = __builtin_fmaxf(m, mw[w]);
     float l = 0.f;
     vec o = vec(0.f);
 #pragma unroll
-    for (int w = 0; w < kPagedWaves; ++w) {
+    for (int w = 0; w < kStates; ++w) {
       const float c = __builtin_amdgcn_exp2f(mw[w] - m);
       if (lw[w] == 0.f) continue;  // no key seen, or none of any weight
       l += c * lw[w];
@@ -319,22 +319,22 @@ template <int kTiles> struct Pages {
 // the wait before one of them was read behind a branch, and a quarter of the
 // scores were stale.
 //
-// kSplit: the units are dealt to the work-groups.  Otherwise a work-group of eight
-// waves takes a whole segment, and there is nothing to merge afterwards.
+// kForm: the units are dealt to work-groups of four waves, or a work-group takes a
+// whole segment, with eight waves or one, and there is nothing to merge afterwards.
 // kStream: the values are read past the caches.
-template <typename T, int D, bool kWholeTiles, bool kSplit, bool kStream>
-__global__ __launch_bounds__(kSplit ? kPagedThreads : 2 * kPagedThreads, 2) void paged_tile_kernel(
-    PagedArgs a) {
-  constexpr bool k16 = sizeof(T) == 2;
-  constexpr int kWaves = kSplit ? kPagedWaves : 2 * kPagedWaves;
+enum PagedForm : int { kFormSplit = 4, kFormWhole = 8, kFormShort = 1 };  // and its waves
+template <typename T, int D, bool kWholeTiles, PagedForm kForm, bool kStream>
+__global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) {
+  constexpr bool k16 = sizeof(T) == 2, kSplit = kForm == kFormSplit;
+  constexpr int kWaves = kForm, kStates = kWaves < kPagedWaves ? kWaves : kPagedWaves;
   constexpr int kKeys = kStepKeys<T>, kTiles = kKeys / 16, kUnit = kWaves * kKeys;
   constexpr int kF = D / 16;                       // features of a lane in a row of V
   constexpr int kKL = k16 ? D / 32 : D / 16;       // 16-byte loads of a lane in a row of K
   constexpr int kVW = kF * int(sizeof(T)) / 4;     // words of a lane in a row of V
   constexpr int kStride = D + 4;
   __shared__ PlaceLds place;
-  __shared__ __align__(16) float sO[kPagedWaves][kTileHeads][kStride];
-  __shared__ float sm[kPagedWaves][kTileHeads], sl[kPagedWaves][kTileHeads];
+  __shared__ __align__(16) float sO[kStates][kTileHeads][kStride];
+  __shared__ float sm[kStates][kTileHeads], sl[kStates][kTileHeads];
   __shared__ int sbad[kWaves];
   __shared__ int2 srow[kWaves][kKeys];        // (page, row) of a step's keys, any page size
   const int lane = threadIdx.x % 64;
@@ -571,7 +571,7 @@ __global__ __launch_bounds__(kSplit ? kPagedThreads : 2 * kPagedThreads, 2) void
     if (u > begin) lds_barrier();  // the segment before has been read
     if (__any(bad)) bad = true;
     if (lane == 0) sbad[wave] = bad;
-    if constexpr (!kSplit) {
+    if constexpr (kForm == kFormWhole) {
       // The upper four waves' states join those of the lower four, lane by lane.
       f32x4_t* upper = reinterpret_cast<f32x4_t*>(&sO[0][0][0]) + (wave % kPagedWaves) * 64 * kF;
       if (wave >= kPagedWaves) {
@@ -600,7 +600,7 @@ __global__ __launch_bounds__(kSplit ? kPagedThreads : 2 * kPagedThreads, 2) void
       }
       lds_barrier();
     }
-    if (wave < kPagedWaves) {
+    if (wave < kStates) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -616,7 +616,7 @@ __global__ __launch_bounds__(kSplit ? kPagedThreads : 2 * kPagedThreads, 2) void
     bool any_bad = false;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) any_bad |= sbad[w] != 0;
-    finish<T, 4, 64 * kWaves>(a, D, &sO[0][0][0], kStride, kTileHeads * kStride, &sm[0][0], &sl[0][0], kTileHeads,
+    finish<T, 4, 64 * kWaves, kStates>(a, D, &sO[0][0][0], kStride, kTileHeads * kStride, &sm[0][0], &sl[0][0], kTileHeads,
               rows, count == units, 2 * int64_t(pl.number) + (u > begin), req, hk * a.G + r0,
               keys == 0, any_bad);
     if (!kSplit) break;
@@ -757,37 +757,51 @@ int64_t paged_attn_workspace(int dtype, PagedArgs a) {
   return rows < 0 || tiles < 0 ? -1 : rows > tiles ? rows : tiles;
 }
 
-// Whether every segment goes to a work-group of its own, from the most keys that
-// the table allows: up to 256 KB of keys and values a segment, up to 512 KB where
-// the segments fill the GPU, and not where they are so many and so short that most
-// waves have no keys.  us, split and merged / whole: 28 + 4 heads of 128 in bf16, 1
-// request: 512 keys 10.7 / 9.7, 1024 10.7 / 14.4; 64 requests: 1024 keys 23.2 /
-// 18.3, 2048 29.9 / 32.8; 16 + 16 heads, 256 requests: 256 keys 98.7 / 119.
-static bool whole_segments(int dtype, const PagedArgs& a) {
-  const int64_t segments = a.N * a.per_request;
-  const int64_t bytes = a.M * a.page * a.D * (dtype == kF32 ? 8 : 4);
-  return segments < 2048 && bytes <= (segments < 256 ? 256 << 10 : 512 << 10);
+// The form, by the segments and by the most keys that the tables allow a request.
+// A work-group a segment saves the merge and its launch, but takes the segment's
+// keys alone: eight waves up to 256 KB of keys and values, up to 512 KB where the
+// segments fill the GPU; one wave where they more than fill it and have few keys,
+// of which eight waves would get none or a step each.  us, split and merged / eight
+// waves / one wave, 28 + 4 heads of 128 in bf16:
+//   1 request, 512 keys 10.7 / 9.7 / -, 1024 keys 10.7 / 14.4 / -
+//   64 requests, 1024 keys 23.2 / 18.3 / -, 2048 keys 29.9 / 32.8 / -
+//   96 requests, 32 keys - / 9.8 / 6.6, 256 keys - / 16.3 / 16.5
+//   256 requests, 32 keys - / 21.1 / 9.4, 384 keys - / 39.8 / 31.8
+//   1000 requests, 384 keys 124 / - / 101.
+static PagedForm paged_form(int dtype, const PagedArgs& a) {
+  const int64_t segments = a.N * a.per_request, keys = a.M * a.page;
+  const int64_t bytes = keys * a.D * (dtype == kF32 ? 8 : 4);
+  if ((segments > 256 && keys <= 256 && bytes <= 128 << 10) ||
+      (segments >= 1024 && keys <= 384 && bytes <= 256 << 10))
+    return kFormShort;
+  if (segments < 2048 && bytes <= (segments < 256 ? 256 << 10 : 512 << 10)) return kFormWhole;
+  return kFormSplit;
 }
 
-template <typename T, int D, bool kSplit, bool kStream>
+template <typename T, int D, PagedForm kForm, bool kStream>
 static void launch_tiles(const PagedArgs& a, hipStream_t stream) {
-  const dim3 grid{unsigned(kSplit ? a.groups : a.N * a.per_request)};
-  const dim3 block{kSplit ? kPagedThreads : 2 * kPagedThreads};
+  const dim3 grid{unsigned(kForm == kFormSplit ? a.groups : a.N * a.per_request)};
+  const dim3 block{64 * kForm};
   if (a.page % 16 == 0)
-    hipLaunchKernelGGL((paged_tile_kernel<T, D, true, kSplit, kStream>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((paged_tile_kernel<T, D, true, kForm, kStream>), grid, block, 0, stream, a);
   else
-    hipLaunchKernelGGL((paged_tile_kernel<T, D, false, kSplit, kStream>), grid, block, 0, stream,
+    hipLaunchKernelGGL((paged_tile_kernel<T, D, false, kForm, kStream>), grid, block, 0, stream,
                        a);
 }
 // Values that the Infinity Cache could not hold until the next step, if the tables
 // are full, are read past it (not keys: their rows are read in pieces of 64 bytes).
 // us without / with: 1 request, 131072 keys 60.6 / 57.3; 64 requests 101 / 93.6; 8
 // requests 45.2 / 40.5; 19 requests in fp32, 225 MB in turns, 23.7 / 24.9.
-template <typename T, int D> static void launch_split(const PagedArgs& a, hipStream_t stream) {
-  if (2 * a.N * a.Hk * a.M * a.page * D * int64_t(sizeof(T)) > (256 << 20))
-    launch_tiles<T, D, true, true>(a, stream);
+template <typename T, int D>
+static void launch_form(PagedForm form, const PagedArgs& a, hipStream_t stream) {
+  if (form == kFormShort)
+    launch_tiles<T, D, kFormShort, false>(a, stream);
+  else if (form == kFormWhole)
+    launch_tiles<T, D, kFormWhole, false>(a, stream);
+  else if (2 * a.N * a.Hk * a.M * a.page * D * int64_t(sizeof(T)) > (256 << 20))
+    launch_tiles<T, D, kFormSplit, true>(a, stream);
   else
-    launch_tiles<T, D, true, false>(a, stream);
+    launch_tiles<T, D, kFormSplit, false>(a, stream);
 }
 
 template <typename T>
@@ -798,22 +812,23 @@ static hipError_t launch_paged_t(int dtype, PagedArgs& a, void* workspace, hipSt
   a.part = static_cast<float*>(workspace);
   a.split = reinterpret_cast<int2*>(static_cast<char*>(workspace) + need -
                                     round256(8 * a.N * a.per_request));
-  const dim3 grid{unsigned(a.groups)}, block{kPagedThreads};
-  if (tiles && whole_segments(dtype, a)) {
-    a.D == 64 ? launch_tiles<T, 64, false, false>(a, stream)
-              : launch_tiles<T, 128, false, false>(a, stream);
-    return hipGetLastError();
+  if (tiles) {
+    const PagedForm form = paged_form(dtype, a);
+    a.D == 64 ? launch_form<T, 64>(form, a, stream) : launch_form<T, 128>(form, a, stream);
+    if (form != kFormSplit) return hipGetLastError();
+  } else {
+    const dim3 grid{unsigned(a.groups)}, block{kPagedThreads};
+    if (a.D <= 64)
+      hipLaunchKernelGGL((paged_row_kernel<T, 1>), grid, block, 0, stream, a);
+    else if (a.D <= 128)
+      hipLaunchKernelGGL((paged_row_kernel<T, 2>), grid, block, 0, stream, a);
+    else
+      hipLaunchKernelGGL((paged_row_kernel<T, 4>), grid, block, 0, stream, a);
   }
-  if (tiles)
-    a.D == 64 ? launch_split<T, 64>(a, stream) : launch_split<T, 128>(a, stream);
-  else if (a.D <= 64)
-    hipLaunchKernelGGL((paged_row_kernel<T, 1>), grid, block, 0, stream, a);
-  else if (a.D <= 128)
-    hipLaunchKernelGGL((paged_row_kernel<T, 2>), grid, block, 0, stream, a);
-  else
-    hipLaunchKernelGGL((paged_row_kernel<T, 4>), grid, block, 0, stream, a);
-  hipError_t e = hipGetLastError();
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
+  // One wave a row where segments have few partials (64 requests of up to 16384 keys
+  // 6.3 -> 5.3 us), four where they may have many.
   const dim3 segments{unsigned(a.N * a.per_request), unsigned(a.rows)};
   if (a.D % 4 != 0)
     hipLaunchKernelGGL((paged_merge_kernel<T, 1, 256>), segments, dim3(256), 0, stream, a);
