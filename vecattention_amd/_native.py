@@ -231,7 +231,7 @@ def host_call(name, on, *args):
     dev = on.get_device()
     if dev < 0:
         return call(*args, 0)  # no GPU: the call refuses it
-    if dev == _current_device():
-        return call(*args, stream_addr(on.device) if _raw_stream is None else _raw_stream(dev))
+    if _raw_stream is not None and dev == _current_device():
+        return call(*args, _raw_stream(dev))
     with torch.cuda.device(dev):
         return call(*args, stream_addr(on.device))

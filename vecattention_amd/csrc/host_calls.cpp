@@ -9,6 +9,7 @@
 // torch's becomes the Python exception.
 #include <Python.h>
 
+#include <ATen/core/LegacyTypeDispatch.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
@@ -436,6 +437,7 @@ template <PyObject* (*f)(PyObject* const*), Py_ssize_t count>
 PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t n) {
   try {
     if (n != count) refuse(PyExc_TypeError, "%zd arguments, %zd expected", n, count);
+    at::AutoDispatchBelowADInplaceOrView below;  // nothing here is recorded
     return f(args);
   } catch (const Refused& r) {
     if (r.type) PyErr_SetString(r.type, r.text.c_str());

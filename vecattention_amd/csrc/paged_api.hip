@@ -124,8 +124,8 @@ int va_qk_norm_rope(int dtype, const void* q, int64_t sqb, int64_t sqh, int64_t 
   if (!q || !k || !q_out || !k_out) return api_error(VA_ERR_ARG, "null tensor pointer");
   if (B <= 0 || Hq <= 0 || Hk <= 0 || S <= 0 || D <= 0)
     return api_error(VA_ERR_ARG, "non-positive size");
-  if (!fits(B, S, kInt31) || !fits(B * S, Hq + Hk, int64_t(1) << 26))
-    return api_error(VA_ERR_UNSUPPORTED, "more than 2^26 rows in a call");
+  if (!fits(B, S, kInt31) || !fits(B * S, Hq + Hk, (int64_t(1) << 26) - 1))
+    return api_error(VA_ERR_UNSUPPORTED, "2^26 rows or more in a call");
   va::RopeArgs a{};
   const int rc = set_rotation(a, D, rotary_dim, positions, spa, spb, axes, sections, inv_freq,
                               q_weight, k_weight, dtype, weight_dtype, eps, scaling, interleaved);
@@ -152,8 +152,8 @@ int va_qk_norm_rope_to_cache(
   if (!q || !k || !v || !q_out || !k_cache || !v_cache || !slot_mapping)
     return api_error(VA_ERR_ARG, "null tensor pointer");
   if (T <= 0 || Hq <= 0 || Hk <= 0 || D <= 0) return api_error(VA_ERR_ARG, "non-positive size");
-  if (!fits(T, Hq + 2 * Hk, int64_t(1) << 26))
-    return api_error(VA_ERR_UNSUPPORTED, "more than 2^26 rows in a call");
+  if (!fits(T, Hq + 2 * Hk, (int64_t(1) << 26) - 1))
+    return api_error(VA_ERR_UNSUPPORTED, "2^26 rows or more in a call");
   if (const int rc = check_pages(num_pages, page_size)) return rc;
   va::RopeArgs a{};
   const int rc = set_rotation(a, D, rotary_dim, positions, spa, 0, axes, sections, inv_freq,
