@@ -58,6 +58,23 @@ __device__ inline uint32_t share_number(const PagedArgs& a) {
 template <int kUnit>
 __device__ inline Place locate(const PagedArgs& a, PlaceLds& lds) {
   const int64_t capacity = a.M * a.page;
+  if (a.N <= 64) {  // a lane a request, in every wave by itself
+    const int lane = threadIdx.x % 64;
+    const int32_t keys = lane < a.N ? paged_keys(a.lens[lane], capacity) : 0;
+    const uint32_t mine = lane < a.N ? a.per_request * paged_units(keys, kUnit) : 0;
+    const uint32_t sum = uint32_t(wave_inclusive_sum(int(mine)));
+    const PagedShare share(uint32_t(__builtin_amdgcn_readlane(int(sum), 63)), uint32_t(a.groups));
+    const uint32_t number = share_number(a), begin = share.begin(number);
+    const uint64_t here = __ballot(begin >= sum - mine && begin < sum);
+    const int at = here ? __builtin_ctzll(here) : 0;  // none: the share is empty
+    return Place{share,
+                 number,
+                 begin,
+                 share.begin(number + 1),
+                 uint32_t(__builtin_amdgcn_readlane(int(sum - mine), at)),
+                 at,
+                 __builtin_amdgcn_readlane(keys, at)};
+  }
   const int32_t N = int32_t(a.N), per = (N + kPagedThreads - 1) / kPagedThreads;
   const int32_t lo = int32_t(threadIdx.x) * per;
   uint32_t mine = 0;
@@ -633,13 +650,34 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
   }
 }
 
+// Maximum and sum over the wave, in every lane.  As row_sum's steps: pairs, quads'
+// halves, the mirrored quad and half of a DPP row; then across the four rows.
+template <int kCtrl> __device__ inline float dpp_of(float x) {
+  return bits_to_float(uint32_t(
+      __builtin_amdgcn_update_dpp(0, int(float_to_bits(x)), kCtrl, 0xf, 0xf, false)));
+}
+__device__ inline float wave_max(float x) {
+  x = __builtin_fmaxf(x, dpp_of<0xb1>(x));
+  x = __builtin_fmaxf(x, dpp_of<0x4e>(x));
+  x = __builtin_fmaxf(x, dpp_of<0x141>(x));
+  x = __builtin_fmaxf(x, dpp_of<0x140>(x));
+  return column_max(x);
+}
+__device__ inline float wave_sum(float x) {
+  x += dpp_of<0xb1>(x);
+  x += dpp_of<0x4e>(x);
+  x += dpp_of<0x141>(x);
+  x += dpp_of<0x140>(x);
+  return column_sum(x);
+}
+
 // Rows of segments that several work-groups share: one work-group per
-// (segment, row).  The partials' weights 2^(m - M) go to LDS; kV
-// features a thread, as many partials side by side as that leaves threads for, U
-// of each thread's in flight (the first ones while the weights are computed);
-// then their sums, always in the same order.
+// (segment, row).  The partials' weights 2^(m - M) go to LDS; kV features a thread,
+// as many partials side by side as that leaves threads for, U of each thread's in
+// flight (the first ones while the weights are computed); then their sums, always
+// in the same order.  kD: the head_dim, 0 for any.
 constexpr int kMostGroups = 2048;
-template <typename T, int kV, int kThreads>
+template <typename T, int kD, int kV, int kThreads>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedArgs a) {
   typedef float vec __attribute__((ext_vector_type(kV)));
   constexpr int U = 4, kWaves = kThreads / 64;
@@ -653,7 +691,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedArgs a) {
   const uint32_t head = (s - hk * a.tiles) * a.rows + r;
   if (head >= a.G) return;
   const int w0 = split.x / 2, parts = split.y - w0 + 1;
-  const int lanes = int(a.D) / kV, side = kThreads / lanes;
+  const int lanes = (kD ? kD : int(a.D)) / kV, side = kThreads / lanes;
   const int p = threadIdx.x / lanes, c = threadIdx.x - p * lanes;
   auto slot = [&](int i) { return int64_t(i == 0 ? split.x : 2 * (w0 + i)); };
   // Reads past the last partial read it again, with no weight.
@@ -665,28 +703,30 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedArgs a) {
       x[i] = reinterpret_cast<const vec*>(part_row(a, slot(at), r))[c];
     }
   };
+  const int me = threadIdx.x;
+  float2 mine = me < parts ? part_ml(a, slot(me))[r] : make_float2(0.f, 0.f);
   load(0);
-  float m = -__builtin_inff();
-  for (int i = threadIdx.x; i < parts; i += kThreads) {
+  float m = mine.y == 0.f ? -__builtin_inff() : mine.x;
+  for (int i = me + kThreads; i < parts; i += kThreads) {
     const float2 ml = part_ml(a, slot(i))[r];
     if (!(ml.y == 0.f)) m = __builtin_fmaxf(m, ml.x);
   }
+  m = wave_max(m);
+  if constexpr (kWaves > 1) {
+    if (me % 64 == 0) top[me / 64] = m;
+    lds_barrier();
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) m = __builtin_fmaxf(m, __shfl_xor(m, d));
-  if (threadIdx.x % 64 == 0) top[threadIdx.x / 64] = m;
-  lds_barrier();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) m = __builtin_fmaxf(m, top[w]);
-  float l = 0.f;
-  for (int i = threadIdx.x; i < parts; i += kThreads) {
-    const float2 ml = part_ml(a, slot(i))[r];
-    const float f = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - m);  // 0: no key of any weight
-    weight[i] = f;
-    l += f * ml.y;
+    for (int w = 0; w < kWaves; ++w) m = __builtin_fmaxf(m, top[w]);
   }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
-  if (threadIdx.x % 64 == 0) den[threadIdx.x / 64] = l;
+  float l = 0.f;
+  for (int i = me; i < parts; i += kThreads) {
+    if (i != me) mine = part_ml(a, slot(i))[r];
+    const float f = mine.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(mine.x - m);  // 0: no weight
+    weight[i] = f;
+    l += f * mine.y;
+  }
+  l = wave_sum(l);
+  if (me % 64 == 0) den[me / 64] = l;
   lds_barrier();
   vec acc = vec(0.f);
   for (int from = 0;; from += U * side) {
@@ -703,9 +743,10 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedArgs a) {
     }
     if (!more) break;
   }
-  sacc[threadIdx.x] = acc;
+  sacc[me] = acc;
   lds_barrier();
   if (p != 0) return;
+#pragma unroll 4
   for (int i = 1; i < side; ++i) acc += sacc[i * lanes + c];
   l = 0.f;
 #pragma unroll
@@ -804,6 +845,13 @@ static void launch_form(PagedForm form, const PagedArgs& a, hipStream_t stream) 
     launch_tiles<T, D, kFormSplit, false>(a, stream);
 }
 
+template <typename T, int kD, int kV, int kThreads>
+static void launch_merge(const PagedArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL((paged_merge_kernel<T, kD, kV, kThreads>),
+                     dim3(unsigned(a.N * a.per_request), unsigned(a.rows)), dim3(kThreads), 0,
+                     stream, a);
+}
+
 template <typename T>
 static hipError_t launch_paged_t(int dtype, PagedArgs& a, void* workspace, hipStream_t stream) {
   const bool tiles = tile_form(dtype, a);
@@ -829,13 +877,15 @@ static hipError_t launch_paged_t(int dtype, PagedArgs& a, void* workspace, hipSt
   if (e != hipSuccess) return e;
   // One wave a row where segments have few partials (64 requests of up to 16384 keys
   // 6.3 -> 5.3 us), four where they may have many.
-  const dim3 segments{unsigned(a.N * a.per_request), unsigned(a.rows)};
-  if (a.D % 4 != 0)
-    hipLaunchKernelGGL((paged_merge_kernel<T, 1, 256>), segments, dim3(256), 0, stream, a);
-  else if (a.D <= 128 && a.groups <= 8 * a.N * a.per_request)
-    hipLaunchKernelGGL((paged_merge_kernel<T, 4, 64>), segments, dim3(64), 0, stream, a);
+  const bool few = a.groups <= 8 * a.N * a.per_request;
+  if (a.D == 64)
+    few ? launch_merge<T, 64, 4, 64>(a, stream) : launch_merge<T, 64, 4, 256>(a, stream);
+  else if (a.D == 128)
+    few ? launch_merge<T, 128, 4, 64>(a, stream) : launch_merge<T, 128, 4, 256>(a, stream);
+  else if (a.D % 4 == 0)
+    launch_merge<T, 0, 4, 256>(a, stream);
   else
-    hipLaunchKernelGGL((paged_merge_kernel<T, 4, 256>), segments, dim3(256), 0, stream, a);
+    launch_merge<T, 0, 1, 256>(a, stream);
   return hipGetLastError();
 }
 
