@@ -64,10 +64,6 @@ def rounded(want, slack, dtype):
     return slack + HALF_STEP[dtype] * (want.abs() + slack) + SMALLEST[dtype]
 
 
-def slots_to_rows(slots, page):
-    return slots // page, slots % page
-
-
 def cache_rows(cache, layout):
     """(num_pages * page_size, Hk, D) of a cache."""
     x = cache if layout == "NHD" else cache.transpose(1, 2)

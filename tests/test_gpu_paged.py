@@ -528,6 +528,43 @@ def test_decode_values_that_are_not_finite(D, dtype):
     assert bool(((out.double() - want).abs() <= room)[ok].all())
 
 
+@pytest.mark.parametrize("D,dtype", [(128, F32), (72, F32), (128, BF16), (64, F16), (64, F32)])
+@pytest.mark.parametrize("lens", [[1, 17, 33, 45, 130], [20, 700], [5000], [3] * 300])
+def test_decode_infinite_values_by_masked_and_tiny_weights(lens, D, dtype):
+    """An infinite value of the last key is not met by the zero weights of the places behind it,
+    and one whose weight is too small for fp32 is infinite all the same."""
+    note("paged decode, infinite values", lens[:5], D, dtype)
+    q, kc, vc, table, l = decode_case(lens, 2, 2, D, 16, "NHD", dtype, seed=3, extra=0)
+    def row(c, n, t): return c[int(table[n, t // 16]), t % 16]  # noqa: E704
+    q[:] = 0
+    q[:, :, 0] = 1.0
+    high = []  # keys far above the others: 800 in their score's exponent of two
+    for n, L in enumerate(lens):
+        row(vc, n, L - 1)[0, 3] = math.inf
+        row(vc, n, 0)[1, 5] = -math.inf
+        high.append(L // 2)
+        row(kc, n, L // 2)[1, 0] = 560 * math.sqrt(D)
+    out = run_decode(q, kc, vc, table, l, "NHD").cpu()
+    for n, L in enumerate(lens):
+        v = ref.cache_rows(vc, "NHD")[table[n].long()[torch.arange(L) // 16] * 16 +
+                                      torch.arange(L) % 16].double()
+        k = ref.cache_rows(kc, "NHD")[table[n].long()[torch.arange(L) // 16] * 16 +
+                                      torch.arange(L) % 16].double()
+        p = torch.softmax((k * q[n].double()).sum(-1) / math.sqrt(D), 0)
+        want = (p[..., None] * v).sum(0)
+        assert want[0, 3] == math.inf and want[1, 5] == -math.inf
+        assert torch.equal(torch.isnan(out[n]), torch.isnan(want))
+        assert torch.equal(torch.isinf(out[n]), torch.isinf(want))
+        # Scores of size below 8 have weights as in the test above; head 1's are one key's value
+        # and others of at most 2^-24 (fp16's smallest weight) each.
+        size = (p[..., None] * v.abs()).sum(0)
+        u = 0.0 if dtype == F32 else ref.HALF_STEP[dtype]
+        tiny = L * 2.0 ** -24 * v[torch.isfinite(v)].abs().max() if dtype == F16 else 0.0
+        ok = torch.isfinite(want)
+        room = ref.rounded(want, (u + (300 + 2 * L) * 2.0 ** -22) * size + tiny, dtype)
+        assert bool(((out[n].double() - want).abs() <= room)[ok].all())
+
+
 def test_decode_strided_views():
     """Caches in one allocation, queries and tables cut from wider ones."""
     note("paged decode, strided")
@@ -619,6 +656,11 @@ def test_refusals_on_the_gpu():
         qk_norm_rope_to_cache(*ok, w, w)
     with torch.no_grad():
         qk_norm_rope_to_cache(*ok, w, w)
+    sparse = torch.zeros(5, 2, 128, device=DEV, requires_grad=True)[..., ::2]  # copied
+    with pytest.raises(NotImplementedError, match="no backward"):
+        write_paged_kv(k, sparse, kc, vc, slots)
+    with pytest.raises(NotImplementedError, match="no backward"):
+        qk_norm_rope_to_cache(q, sparse, v, kc, vc, slots, pos, inv)
     table, lens = torch.zeros(5, 1, dtype=torch.int32, device=DEV), torch.full(
         (5,), 3, dtype=torch.int32, device=DEV)
     with pytest.raises(ValueError, match="tensors on"):
@@ -635,6 +677,30 @@ def test_refusals_on_the_gpu():
     assert empty[0].shape == (1, 2, 0, 64)
     write_paged_kv(k[:0], v[:0], kc, vc, slots[:0])
     assert paged_decode_attention(q.detach()[:0], kc, vc, table[:0], lens[:0]).shape == (0, 2, 64)
+
+
+def test_writes_are_seen_by_autograd():
+    """A cache that a graph saved for its backward pass and that a call wrote is not used by it."""
+    note("versions")
+    k = torch.ones(5, 2, 64, device=DEV)
+    kc, vc = (torch.zeros(2, 16, 2, 64, device=DEV) for _ in range(2))
+    slots, table = torch.arange(5, device=DEV), torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    w = torch.ones(64, device=DEV, requires_grad=True)
+    for call in (lambda: write_paged_kv(k, k, kc, vc, slots),
+                 lambda: qk_norm_rope_to_cache(k, k, k, kc, vc, slots, slots, freqs(64).to(DEV))):
+        loss = (vc * w).sum()
+        with torch.no_grad():
+            call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    lens = torch.ones(1, dtype=torch.int32, device=DEV)
+    before = table._version
+    paged_kv_plan(lens, lens, table, lens, 16, 1)
+    assert table._version > before
+    with torch.inference_mode():
+        kc = torch.zeros(2, 16, 2, 64, device=DEV)
+        write_paged_kv(k, k, kc, kc.clone(), slots)
+        assert bool((kc[0, :5] == 1).all())
 
 
 # ---------------------------------------------------------------- together

@@ -160,6 +160,7 @@ def rope_ok(**over):
      ValueError),
     (dict(q_weight=torch.ones(32)), ValueError), (dict(q_weight=torch.ones(128)[::2]), ValueError),
     (dict(k_weight=torch.ones(64).half()), ValueError),
+    (dict(q=torch.zeros(2, 0, 5, 64)), ValueError), (dict(k=torch.zeros(2, 0, 5, 64)), ValueError),
     ({}, RuntimeError)])
 def test_rope_refusals(over, err):
     with pytest.raises(err):
@@ -190,6 +191,9 @@ CACHE_ERRORS = [
 
 @pytest.mark.parametrize("over,err", CACHE_ERRORS + [
     (dict(q=torch.zeros(4, 4, 64)), ValueError), (dict(q=torch.zeros(5, 4, 64).half()), ValueError),
+    (dict(q=torch.zeros(5, 0, 64)), ValueError),
+    (dict(k=torch.zeros(5, 0, 64), v=torch.zeros(5, 0, 64), k_cache=torch.zeros(3, 16, 0, 64),
+          v_cache=torch.zeros(3, 16, 0, 64)), ValueError),
     (dict(positions=torch.zeros(4, dtype=torch.int64)), ValueError)])
 def test_rope_to_cache_refusals(over, err):
     with pytest.raises(err):
@@ -316,7 +320,8 @@ def test_c_decode_errors(L):
                  dict(N=0), dict(Hq=0), dict(D=0), dict(M=-1), dict(Hq=5), dict(page=0),
                  dict(pages=0), dict(ws=P + 8)):
         assert c_decode(L, **over) == nat.VA_ERR_ARG, over
-    for over in (dict(D=257), dict(N=2 ** 22), dict(N=1000, M=2 ** 27), dict(M=2 ** 31)):
+    for over in (dict(D=257), dict(N=2 ** 22), dict(N=1000, M=2 ** 27), dict(M=2 ** 31),
+                 dict(M=2 ** 31 - 1, page=2 ** 31 - 1)):
         assert c_decode(L, **over) == nat.VA_ERR_UNSUPPORTED, over
     need = L.va_paged_decode_workspace_size(1, 3, 4, 2, 128, 8, 16)
     assert need > 0

@@ -100,6 +100,12 @@ void no_backward(const char* what, std::initializer_list<const at::Tensor*> tens
              what);
 }
 
+// Written behind autograd's back: what saved it for a backward pass has to notice.
+void written(std::initializer_list<const at::Tensor*> tensors) {
+  for (const at::Tensor* t : tensors)
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 // As nat.check(): the C call's code and message.
 void check(const char* fn, int rc) {
   if (rc == VA_OK) return;
@@ -298,6 +304,7 @@ PyObject* plan(PyObject* const* a) {
                       static_cast<int32_t*>(out[4].data_ptr()),
                       static_cast<int64_t*>(out[5].data_ptr()), address(work), bytes,
                       reinterpret_cast<void*>(integer(a[7]))));
+  written({&table});
   PyObject* tuple = PyTuple_New(6);
   if (!tuple) throw Refused{nullptr, ""};
   for (int i = 0; i < 6; ++i) PyTuple_SET_ITEM(tuple, i, THPVariable_Wrap(out[i]));
@@ -312,6 +319,7 @@ PyObject* rope(PyObject* const* a) {
   if (k_.size(0) != B || k_.size(2) != S || k_.size(3) != D)
     refuse(PyExc_ValueError, "q %s and k %s differ in batch, length or head_dim",
            shape(q_).c_str(), shape(k_).c_str());
+  if (Hq == 0 || Hk == 0) refuse(PyExc_ValueError, "q and k need a head each");
   if (q_.scalar_type() != k_.scalar_type())
     refuse(PyExc_ValueError, "q (%s) and k (%s) must share a dtype", name(q_), name(k_));
   const int dtype = dtype_code(q_);
@@ -320,7 +328,7 @@ PyObject* rope(PyObject* const* a) {
   one_gpu("qk_norm_rope", {&q_, &k_, &r.positions, &r.inv_freq, &r.qw, &r.kw});
   no_backward("qk_norm_rope", {&q_, &k_, &r.inv_freq, &r.qw, &r.kw});
   const at::Tensor q = rows(q_), k = rows(k_), qo = rows_like(q), ko = rows_like(k);
-  if (B && S && Hq && Hk)
+  if (B && S)
     check("va_qk_norm_rope",
           va_qk_norm_rope(
               dtype, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), k.data_ptr(),
@@ -349,6 +357,7 @@ PyObject* rope_to_cache(PyObject* const* a) {
   if (q_.scalar_type() != t.k.scalar_type())
     refuse(PyExc_ValueError, "q (%s) and k (%s) must share a dtype", name(q_), name(t.k));
   const int64_t Hq = q_.size(1);
+  if (Hq == 0 || t.Hk == 0) refuse(PyExc_ValueError, "q and k need a head each");
   const int dtype = dtype_code(q_);
   const Rotation r(t.D, q_, tensor(a[6], "positions"), tensor(a[7], "inv_freq"),
                    maybe(a[8], "q_weight"), maybe(a[9], "k_weight"), a[11], {t.T});
@@ -358,9 +367,10 @@ PyObject* rope_to_cache(PyObject* const* a) {
            (long long)t.Hk);
   one_gpu("qk_norm_rope_to_cache",
           {&q_, &t.k, &t.v, &kc, &vc, &t.slots, &r.positions, &r.inv_freq, &r.qw, &r.kw});
-  no_backward("qk_norm_rope_to_cache", {&q_, &t.k, &t.v, &kc, &vc, &r.inv_freq, &r.qw, &r.kw});
+  no_backward("qk_norm_rope_to_cache", {&q_, &tensor(a[1], "k"), &tensor(a[2], "v"), &kc, &vc,
+                                        &r.inv_freq, &r.qw, &r.kw});
   const at::Tensor q = rows(q_), out = rows_like(q);
-  if (t.T && Hq && t.Hk)
+  if (t.T)
     check("va_qk_norm_rope_to_cache",
           va_qk_norm_rope_to_cache(
               dtype, q.data_ptr(), q.stride(0), q.stride(1), t.k.data_ptr(), t.k.stride(0),
@@ -371,6 +381,7 @@ PyObject* rope_to_cache(PyObject* const* a) {
               r.axes, r.sections, static_cast<float*>(r.inv_freq.data_ptr()), r.rot,
               address(r.qw), address(r.kw), r.weight_type, float(real(a[10])),
               float(real(a[13])), truth(a[12]), reinterpret_cast<void*>(integer(a[15]))));
+  written({&kc, &vc});
   return THPVariable_Wrap(out);
 }
 
@@ -383,7 +394,7 @@ PyObject* write_kv(PyObject* const* a) {
     refuse(PyExc_ValueError, "a cache of %lld heads for keys of %lld", (long long)c.heads,
            (long long)t.Hk);
   one_gpu("write_paged_kv", {&t.k, &t.v, &kc, &vc, &t.slots});
-  no_backward("write_paged_kv", {&t.k, &t.v, &kc, &vc});
+  no_backward("write_paged_kv", {&tensor(a[0], "k"), &tensor(a[1], "v"), &kc, &vc});
   if (t.T && t.Hk && t.D)
     check("va_write_paged_kv",
           va_write_paged_kv(dtype, t.k.data_ptr(), t.k.stride(0), t.k.stride(1), t.v.data_ptr(),
@@ -391,6 +402,7 @@ PyObject* write_kv(PyObject* const* a) {
                             vc.data_ptr(), c.v[0], c.v[1], c.v[2], c.pages, c.page,
                             static_cast<int64_t*>(t.slots.data_ptr()), t.T, t.Hk, t.D,
                             reinterpret_cast<void*>(integer(a[6]))));
+  written({&kc, &vc});
   Py_RETURN_NONE;
 }
 

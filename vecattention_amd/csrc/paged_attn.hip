@@ -18,6 +18,8 @@
 #include "mfma.h"
 #include "paged_ops.h"
 
+#include <type_traits>
+
 namespace va {
 
 constexpr int kPagedThreads = 256, kPagedWaves = kPagedThreads / 64;
@@ -112,6 +114,12 @@ __device__ inline Place locate(const PagedArgs& a, PlaceLds& lds) {
   return Place{share, number, begin, share.begin(number + 1), lds.base, lds.request, lds.keys};
 }
 
+// w * x for a weight that is not zero, but may be too small for fp32: what is
+// infinite or not a number stays so.
+__device__ inline float weighed(float w, float x) {
+  return w != 0.f ? w * x : __builtin_fabsf(x) < __builtin_inff() ? 0.f : x;
+}
+
 // Merges the waves' states of a segment's rows and writes them: to the output
 // (`whole`), or to a partial slot.  sO[wave][row][stride], sm/sl[wave][row];
 // kV features of a row a thread.
@@ -142,7 +150,12 @@ __device__ inline void finish(const PagedArgs& a, int D, const float* sO, int rs
       const float c = __builtin_amdgcn_exp2f(mw[w] - m);
       if (lw[w] == 0.f) continue;  // no key seen, or none of any weight
       l += c * lw[w];
-      o += c * ow[w];
+      if (c != 0.f) {
+        o += c * ow[w];
+      } else {
+#pragma unroll
+        for (int e = 0; e < kV; ++e) o[e] += weighed(c, ow[w][e]);
+      }
     }
     if (bad) l = __builtin_nanf("");
     if (whole) {
@@ -230,8 +243,10 @@ __global__ __launch_bounds__(kPagedThreads) void paged_row_kernel(PagedArgs a) {
           const float ms = mnew == -__builtin_inff() ? 0.f : mnew;
           const float c1 = __builtin_amdgcn_exp2f(m[r] - ms), p1 = __builtin_amdgcn_exp2f(s - ms);
           l[r] = l[r] * c1 + p1;
+          const bool seen = s != -__builtin_inff();  // else a weight of 0 indeed
 #pragma unroll
-          for (int j = 0; j < NF; ++j) acc[r][j] = acc[r][j] * c1 + p1 * vf[j];
+          for (int j = 0; j < NF; ++j)
+            acc[r][j] = weighed(c1, acc[r][j]) + (seen ? weighed(p1, vf[j]) : p1 * vf[j]);
           m[r] = mnew;
         }
       }
@@ -278,8 +293,12 @@ __global__ __launch_bounds__(kPagedThreads) void paged_row_kernel(PagedArgs a) {
 //
 // 16-bit types round a weight to 8 (11) bits, which would cost as much accuracy
 // as the output's own rounding: it goes in as two parts, high + low, to 2^-16.
-// An infinite value would meet a low part of 0 or below and give NaN, so a
-// wave whose sums hold a NaN repeats its keys with the high part alone.
+//
+// Infinite values would meet weights of 0 and give NaN where they may not: the low
+// part of a weight (or one below 0), the weight of a key past the last, whose row
+// is the last key's, and weights too small for their type.  A wave whose sums hold
+// a NaN repeats its keys with the high part alone, zeros for rows past the last
+// key, and a smallest weight for every key that has one.
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
@@ -349,6 +368,7 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
   constexpr int kKL = k16 ? D / 32 : D / 16;       // 16-byte loads of a lane in a row of K
   constexpr int kVW = kF * int(sizeof(T)) / 4;     // words of a lane in a row of V
   constexpr int kStride = D + 4;
+  constexpr float kLeast = std::is_same_v<T, f16_t> ? 0x1p-24f : 0x1p-126f;  // weight of T
   __shared__ PlaceLds place;
   __shared__ __align__(16) float sO[kStates][kTileHeads][kStride];
   __shared__ float sm[kStates][kTileHeads], sl[kStates][kTileHeads];
@@ -480,8 +500,8 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
 
     f32x4_t acc[kF];
     float m, l;
-    bool high_only = false;
-    for (;;) {
+    auto walk = [&](auto again) {
+      constexpr bool repeat = decltype(again)::value;
       m = -__builtin_inff();
       l = 0.f;
 #pragma unroll
@@ -533,7 +553,13 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
           m = mn;
           l *= f;
 #pragma unroll
-          for (int x = 0; x < kF; ++x) acc[x] *= f;
+          for (int x = 0; x < kF; ++x) {
+            if constexpr (!repeat)
+              acc[x] *= f;
+            else
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[x][e] = weighed(f, acc[x][e]);
+          }
         }
         const float ms = m == -__builtin_inff() ? 0.f : m;
 #pragma unroll
@@ -541,8 +567,14 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
           const bool seen = p[j] != -__builtin_inff();
           p[j] = __builtin_amdgcn_exp2f(p[j] - ms);
           l += p[j];
-          // An infinite value of a key whose weight fp16 cannot hold is infinite all the same.
-          if (high_only && seen && p[j] < 0x1p-24f) p[j] = 0x1p-24f;
+          if (repeat && seen && p[j] < kLeast) p[j] = kLeast;
+        }
+        if constexpr (repeat) {
+#pragma unroll
+          for (int j = 0; j < kTiles * 4; ++j)
+            if (key0 + 16 * (j / 4) + 4 * kg + j % 4 > last)
+#pragma unroll
+              for (int w = 0; w < kVW; ++w) vr[j][w] = 0;
         }
         if constexpr (k16) {
           typedef typename Mfma16<T>::vec vec;
@@ -562,7 +594,7 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
             for (int j = 0; j < 4; ++j)
               av[j] = __builtin_amdgcn_perm(vr[2 * j + 1][x / 2], vr[2 * j][x / 2], sel);
             acc[x] = Mfma16<T>::run(__builtin_bit_cast(vec, av), hi, acc[x]);
-            if (!high_only) acc[x] = Mfma16<T>::run(__builtin_bit_cast(vec, av), lo, acc[x]);
+            if (!repeat) acc[x] = Mfma16<T>::run(__builtin_bit_cast(vec, av), lo, acc[x]);
           }
         } else {
 #pragma unroll
@@ -574,15 +606,14 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
         }
         if (i + 1 < steps) load_v(key0 + kUnit);
       }
-      if (!k16 || high_only) break;
-      bool nan = false;
+    };
+    walk(std::false_type{});
+    bool nan = false;
 #pragma unroll
-      for (int x = 0; x < kF; ++x)
+    for (int x = 0; x < kF; ++x)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) nan |= acc[x][e] != acc[x][e];
-      if (!__any(nan)) break;
-      high_only = true;
-    }
+      for (int e = 0; e < 4; ++e) nan |= acc[x][e] != acc[x][e];
+    if (__any(nan)) walk(std::true_type{});
     l = column_sum(l);
 
     if (u > begin) lds_barrier();  // the segment before has been read
@@ -610,7 +641,8 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
           const f32x4_t up = upper[x * 64 + lane];
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            acc[x][e] = (f == 0.f ? 0.f : f * acc[x][e]) + (g == 0.f ? 0.f : g * up[e]);
+            acc[x][e] = (l == 0.f ? 0.f : weighed(f, acc[x][e])) +
+                        (lu == 0.f ? 0.f : weighed(g, up[e]));
         }
         l = f * l + g * lu;
         m = mn;
@@ -721,9 +753,9 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedArgs a) {
   float l = 0.f;
   for (int i = me; i < parts; i += kThreads) {
     if (i != me) mine = part_ml(a, slot(i))[r];
-    const float f = mine.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(mine.x - m);  // 0: no weight
-    weight[i] = f;
-    l += f * mine.y;
+    const float f = __builtin_amdgcn_exp2f(mine.x - m);
+    weight[i] = mine.y == 0.f ? -1.f : f;  // -1: no weight at all
+    l += mine.y == 0.f ? 0.f : f * mine.y;
   }
   l = wave_sum(l);
   if (me % 64 == 0) den[me / 64] = l;
@@ -738,8 +770,11 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedArgs a) {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int at = from + p + i * side;
-      const float f = at < parts ? weight[at] : 0.f;
-      if (f != 0.f) acc += f * y[i];
+      const float f = at < parts ? weight[at] : -1.f;
+      if (f > 0.f) acc += f * y[i];
+      if (f == 0.f)
+#pragma unroll
+        for (int e = 0; e < kV; ++e) acc[e] += weighed(f, y[i][e]);
     }
     if (!more) break;
   }
@@ -778,6 +813,7 @@ static int64_t plan_form(PagedArgs& a, int64_t unit, int64_t tile, int64_t group
   a.tiles = int32_t((a.G + tile - 1) / tile);
   a.rows = int32_t((a.G + a.tiles - 1) / a.tiles);
   const int64_t longest = (a.M * a.page + unit - 1) / unit;
+  if (longest >= int64_t(1) << 31) return -1;  // nor does the product overflow
   const int64_t most = a.N * a.Hk * a.tiles * (longest > 1 ? longest : 1);  // units, at most
   if (most >= (int64_t(1) << 31)) return -1;
   a.groups = int32_t(most < groups ? most : groups);
