@@ -80,6 +80,22 @@ def test_plan_edges():
     plan_case([2 ** 31 - 1, 5], [9, 2], 1 << 20, 2048, [4, 5])       # lengths at the type's end
 
 
+def test_plan_outputs_are_tensors_of_their_own():
+    """Outputs of one allocation: written, copied and used in a graph one by one."""
+    note("plan outputs")
+    lens, new, table, free = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in (
+        [3, 0], [2, 9], [[1, 0, 0], [0, 0, 0]], [5, 6, 7, 8]))
+    step = paged_kv_plan(lens, new, table, free, 4, 13)
+    before = [t.clone() for t in step]
+    for i, t in enumerate(step):
+        t.add_(1)
+        for j, (a, b) in enumerate(zip(step, before)):
+            assert torch.equal(a, b + 1 if j <= i else b)
+        assert t.is_contiguous() and t._base is None
+        assert torch.equal(t.cpu(), (before[i] + 1).cpu()) and torch.equal(t[-1:], t[len(t) - 1:])
+    assert (step.positions.float().requires_grad_() * 2).sum().requires_grad
+
+
 def test_plan_long_prompts_and_replayed_graph():
     note("plan graph")
     g = gen(4)
@@ -700,6 +716,8 @@ def test_writes_are_seen_by_autograd():
     with torch.inference_mode():
         kc = torch.zeros(2, 16, 2, 64, device=DEV)
         write_paged_kv(k, k, kc, kc.clone(), slots)
+        step = paged_kv_plan(lens, lens, table, lens, 16, 3)
+        assert all(t.is_inference() and t.is_contiguous() for t in step)
         assert bool((kc[0, :5] == 1).all())
 
 

@@ -25,7 +25,8 @@ from . import _native as nat
 
 
 class PagedStep(NamedTuple):
-    """What a step needs to know, on the GPU (``paged_kv_plan``)."""
+    """What a step needs to know, on the GPU (``paged_kv_plan``).  The tensors of
+    the requests share one allocation, those of the tokens another."""
     kv_lens: torch.Tensor       # (N,) int32: lengths after the step
     qo_indptr: torch.Tensor     # (N + 1,) int32: first token of each request
     slot_mapping: torch.Tensor  # (num_tokens,) int64: slot of each token, -1 for none
