@@ -470,6 +470,17 @@ def test_decode_split_sequence(D, dtype):
     within(out, *ref.decode(q, kc, vc, table, lens, "NHD", 0.3), dtype)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("D", [6, 32, 40, 96, 160, 256])
+def test_decode_split_of_any_head_dim(D, dtype):
+    """Partial rows of several work-groups, merged in pieces of a row or whole rows."""
+    note("paged decode, split", D, dtype)
+    case = decode_case([4003, 1], 5, 1, D, 12, "HND", dtype, seed=D)
+    out = run_decode(*case, "HND")
+    within(out, *ref.decode(*case, "HND"), dtype)
+    assert torch.equal(out, run_decode(*case, "HND"))
+
+
 def test_decode_agrees_with_the_contiguous_cache():
     """One request on consecutive pages is what single_decode_with_kv_cache computes."""
     note("paged decode vs single")

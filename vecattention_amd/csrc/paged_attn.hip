@@ -263,9 +263,9 @@ __global__ __launch_bounds__(kPagedThreads) void paged_row_kernel(PagedArgs a) {
     }
     if (lane == 0) sbad[wave] = bad;
     lds_barrier();
-    finish<T, 1>(a, int(a.D), &sO[0][0][0], kRowMaxD, kRowTile * kRowMaxD, &sm[0][0], &sl[0][0], kRowTile,
-              rows, count == units, 2 * int64_t(pl.number) + (u > begin), req, hk * a.G + r0,
-              keys == 0, sbad[0] || sbad[1] || sbad[2] || sbad[3]);
+    finish<T, 1>(a, int(a.D), &sO[0][0][0], kRowMaxD, kRowTile * kRowMaxD, &sm[0][0], &sl[0][0],
+                 kRowTile, rows, count == units, 2 * int64_t(pl.number) + (u > begin), req,
+                 hk * a.G + r0, keys == 0, sbad[0] || sbad[1] || sbad[2] || sbad[3]);
     if (c0 == 0 && threadIdx.x == 0)
       a.split[req * a.per_request + seg] =
           count == units ? make_int2(-1, -1)
@@ -665,9 +665,10 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
     bool any_bad = false;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) any_bad |= sbad[w] != 0;
-    finish<T, 4, 64 * kWaves, kStates>(a, D, &sO[0][0][0], kStride, kTileHeads * kStride, &sm[0][0], &sl[0][0], kTileHeads,
-              rows, count == units, 2 * int64_t(pl.number) + (u > begin), req, hk * a.G + r0,
-              keys == 0, any_bad);
+    finish<T, 4, 64 * kWaves, kStates>(a, D, &sO[0][0][0], kStride, kTileHeads * kStride,
+                                       &sm[0][0], &sl[0][0], kTileHeads, rows, count == units,
+                                       2 * int64_t(pl.number) + (u > begin), req, hk * a.G + r0,
+                                       keys == 0, any_bad);
     if (!kSplit) break;
     if (c0 == 0 && threadIdx.x == 0)
       a.split[req * a.per_request + seg] =
@@ -707,9 +708,11 @@ __device__ inline float wave_sum(float x) {
 // (segment, row).  The partials' weights 2^(m - M) go to LDS; kV features a thread,
 // as many partials side by side as that leaves threads for, U of each thread's in
 // flight (the first ones while the weights are computed); then their sums, always
-// in the same order.  kD: the head_dim, 0 for any.
+// in the same order: across a wave's lanes in registers, then across the waves.  With
+// many partials 32 features a work-group keep all loads in flight at once (128 of 128
+// features, 28 rows: 6.3 -> 4.6 us).  kF: the features of a work-group, 0 for all of them.
 constexpr int kMostGroups = 2048;
-template <typename T, int kD, int kV, int kThreads>
+template <typename T, int kF, int kV, int kThreads>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedArgs a) {
   typedef float vec __attribute__((ext_vector_type(kV)));
   constexpr int U = 4, kWaves = kThreads / 64;
@@ -723,8 +726,9 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedArgs a) {
   const uint32_t head = (s - hk * a.tiles) * a.rows + r;
   if (head >= a.G) return;
   const int w0 = split.x / 2, parts = split.y - w0 + 1;
-  const int lanes = (kD ? kD : int(a.D)) / kV, side = kThreads / lanes;
-  const int p = threadIdx.x / lanes, c = threadIdx.x - p * lanes;
+  const int lanes = (kF ? kF : int(a.D)) / kV, side = kThreads / lanes;
+  const int p = threadIdx.x / lanes, c0 = threadIdx.x - p * lanes;
+  const int c = c0 + (kF ? int(blockIdx.z) * lanes : 0);
   auto slot = [&](int i) { return int64_t(i == 0 ? split.x : 2 * (w0 + i)); };
   // Reads past the last partial read it again, with no weight.
   vec x[U];
@@ -778,11 +782,28 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedArgs a) {
     }
     if (!more) break;
   }
-  sacc[me] = acc;
-  lds_barrier();
-  if (p != 0) return;
+  if constexpr (kF) {  // across the wave in registers, then the waves
+    constexpr int kLanes = kF / kV;
+    static_assert(kLanes == 8 || kLanes == 16 || kLanes == 32, "lanes of a row in a wave");
+#pragma unroll
+    for (int e = 0; e < kV; ++e) {
+      if constexpr (kLanes == 8) acc[e] += dpp_of<0x128>(acc[e]);  // row_ror:8
+      acc[e] = kLanes == 32 ? sum_halves(acc[e]) : column_sum(acc[e]);
+    }
+    if constexpr (kWaves > 1) {
+      if (me % 64 < kLanes) sacc[me / 64 * kLanes + c0] = acc;
+      lds_barrier();
+    }
+    if (p != 0) return;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) acc += sacc[w * kLanes + c0];
+  } else {
+    sacc[me] = acc;
+    lds_barrier();
+    if (p != 0) return;
 #pragma unroll 4
-  for (int i = 1; i < side; ++i) acc += sacc[i * lanes + c];
+    for (int i = 1; i < side; ++i) acc += sacc[i * lanes + c0];
+  }
   l = 0.f;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) l += den[w];
@@ -881,11 +902,12 @@ static void launch_form(PagedForm form, const PagedArgs& a, hipStream_t stream) 
     launch_tiles<T, D, kFormSplit, false>(a, stream);
 }
 
-template <typename T, int kD, int kV, int kThreads>
+template <typename T, int kF, int kV, int kThreads>
 static void launch_merge(const PagedArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL((paged_merge_kernel<T, kD, kV, kThreads>),
-                     dim3(unsigned(a.N * a.per_request), unsigned(a.rows)), dim3(kThreads), 0,
-                     stream, a);
+  hipLaunchKernelGGL((paged_merge_kernel<T, kF, kV, kThreads>),
+                     dim3(unsigned(a.N * a.per_request), unsigned(a.rows),
+                          unsigned(kF ? a.D / kF : 1)),
+                     dim3(kThreads), 0, stream, a);
 }
 
 template <typename T>
@@ -912,12 +934,14 @@ static hipError_t launch_paged_t(int dtype, PagedArgs& a, void* workspace, hipSt
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   // One wave a row where segments have few partials (64 requests of up to 16384 keys
-  // 6.3 -> 5.3 us), four where they may have many.
+  // 6.3 -> 5.3 us), four waves to 32 features where they may have many.
   const bool few = a.groups <= 8 * a.N * a.per_request;
-  if (a.D == 64)
-    few ? launch_merge<T, 64, 4, 64>(a, stream) : launch_merge<T, 64, 4, 256>(a, stream);
-  else if (a.D == 128)
-    few ? launch_merge<T, 128, 4, 64>(a, stream) : launch_merge<T, 128, 4, 256>(a, stream);
+  if (a.D == 64 && few)
+    launch_merge<T, 64, 4, 64>(a, stream);
+  else if (a.D == 128 && few)
+    launch_merge<T, 128, 4, 64>(a, stream);
+  else if (a.D % 32 == 0)
+    launch_merge<T, 32, 4, 256>(a, stream);
   else if (a.D % 4 == 0)
     launch_merge<T, 0, 4, 256>(a, stream);
   else
