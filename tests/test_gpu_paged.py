@@ -795,3 +795,59 @@ def test_prompts_then_generated_tokens(dtype, layout):
             move = ((K * query).abs().sum(-1) / math.sqrt(D)).max() * (2 * u + (D + 40) * 2.0 ** -24)
             rel = 2 * math.expm1(float(move)) + 2.0 ** -14
             within(out[n], want, rel * (w[..., None] * V.abs()).sum(0), dtype)
+
+
+@pytest.mark.parametrize("page", [16, 5])
+def test_a_whole_step_in_a_graph(page):
+    """Plan, rotation, writes and attention of a step in one graph that carries its state on the
+    GPU, replayed on a side stream with eager work between, against the same steps run eagerly."""
+    note("a step in a graph", page)
+    g = gen(31)
+    Hq, Hk, D, N, width, pages = 8, 2, 128, 5, 12, 64
+    inv = freqs(D).to(DEV)
+    qkv = [torch.randn(N, H, D, generator=g).bfloat16().to(DEV) for H in (Hq, Hk, Hk)]
+    free = torch.randperm(pages, generator=g).int().to(DEV)
+    ones = torch.ones(N, dtype=torch.int32, device=DEV)
+
+    def state():
+        return (torch.zeros(N, dtype=torch.int32, device=DEV),
+                torch.full((N, width), -1, dtype=torch.int32, device=DEV),
+                torch.zeros(1, dtype=torch.int32, device=DEV),
+                *(torch.zeros(pages, page, Hk, D, dtype=torch.bfloat16, device=DEV)
+                  for _ in range(4)))
+
+    def step(lens, table, head, kc, vc, kc2, vc2):
+        q, k, v = qkv
+        p = paged_kv_plan(lens, ones, table, free, page, N, head)
+        rq = qk_norm_rope_to_cache(q, k, v, kc, vc, p.slot_mapping, p.positions, inv)
+        pq, pk = qk_norm_rope(*(x.transpose(0, 1)[None] for x in (q, k)), p.positions, inv)
+        write_paged_kv(pk[0].transpose(0, 1), v, kc2, vc2, p.slot_mapping)
+        a = paged_decode_attention(rq, kc, vc, table, p.kv_lens)
+        b = paged_decode_attention(pq[0].transpose(0, 1), kc2, vc2, table, p.kv_lens)
+        lens.copy_(p.kv_lens)
+        head.add_(p.pages_taken)
+        return a, b
+
+    mine, theirs = state(), state()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*state())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a, b = step(*mine)
+    for i in range(page + 3):
+        fresh = [torch.randn(x.shape, generator=g).bfloat16().to(DEV) for x in qkv]
+        for x, y in zip(qkv, fresh):
+            x.copy_(y)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graph.replay()
+        torch.cuda.synchronize()
+        want = step(*theirs)
+        torch.cuda.synchronize()
+        assert int(theirs[0][0]) == i + 1
+        for x, y in zip((a, b, *mine), (*want, *theirs)):
+            assert torch.equal(x, y), i
+        assert torch.equal(a, b)
