@@ -436,7 +436,8 @@ int va_bf16_copy(const float* x, int64_t n, void* out, int32_t* inexact, void* s
  * do not suffice (*free_head + *pages_taken > num_free) the table entries and
  * slots without a page are -1, as is the slot of a token past the table's
  * end or in a page whose entry is negative.  workspace: of
- * va_paged_plan_workspace_size(N) bytes, 16-byte aligned (0: none).
+ * va_paged_plan_workspace_size(N) bytes, 16-byte aligned (0: none).  No output may
+ * overlap an input: every work-group reads all lengths for itself.
  */
 int64_t va_paged_plan_workspace_size(int64_t N);
 int va_paged_plan(const int32_t* kv_lens, const int32_t* new_lens, int64_t N,

@@ -43,6 +43,10 @@ __device__ inline PlanRow plan_row(const PlanArgs& a, int64_t i) {
   return PlanRow(a.kv_lens[i], a.new_lens[i], a.page, uint32_t(a.M));
 }
 
+__device__ inline int64_t plan_head(const PlanArgs& a) {
+  return a.free_head ? int64_t(*a.free_head) : 0;
+}
+
 // Sums that end at 2^31 - 1 (still associative, for values up to that): no token
 // or entry behind it is ever looked up.
 constexpr uint32_t kMost = 0x7fffffffu;
@@ -112,12 +116,13 @@ __device__ inline uint32_t holder(const uint32_t* start, uint32_t n, uint32_t x)
 
 // The work-group's share.  tok, pag: the sums, with the totals at [N].  The first
 // `token_groups` work-groups take the tokens, kRun in a row to a thread, which makes
-// one search, and one division for each request and page that they reach (steps
-// of single tokens: kRun 1, all searches at once); the others take the new pages.
+// one search, one division for each request and page that they reach, and 16-byte
+// stores (steps of single tokens: kRun 1, all searches at once); the others take the
+// new pages.
 template <int kRun>
-__device__ inline void plan_fill(const PlanArgs& a, const uint32_t* tok, const uint32_t* pag) {
+__device__ inline void plan_fill(const PlanArgs& a, const uint32_t* tok, const uint32_t* pag,
+                                 int64_t head) {
   const uint32_t N = uint32_t(a.N);
-  const int64_t head = a.free_head ? int64_t(*a.free_head) : 0;
   const uint32_t ntok = tok[N], npag = pag[N];
   if (blockIdx.x >= a.token_groups) {
     const uint32_t threads = (gridDim.x - a.token_groups) * kPlanThreads;
@@ -139,12 +144,12 @@ __device__ inline void plan_fill(const PlanArgs& a, const uint32_t* tok, const u
        t0 += step) {
     uint32_t i = 0, next = 0, pos = 0, left = 0;  // request, its last token + 1, tokens left in page
     int64_t slot = -1;
+    int64_t slots[kRun], positions[kRun];
+    int32_t requests[kRun];
 #pragma unroll
     for (int e = 0; e < kRun; ++e) {
-      const int64_t t64 = t0 + e;
-      if (t64 >= a.tokens) break;
-      const uint32_t t = uint32_t(t64);
-      const bool real = t < ntok;
+      const uint32_t t = uint32_t(t0 + e);
+      const bool real = t0 + e < a.tokens && t < ntok;
       if (real) {
         if (e == 0 || t >= next || left == 0) {
           if (e == 0 || t >= next) i = holder(tok, N, t);
@@ -160,9 +165,29 @@ __device__ inline void plan_fill(const PlanArgs& a, const uint32_t* tok, const u
           slot = slot < 0 ? -1 : slot + 1;
         }
       }
-      a.slots[t64] = real ? slot : -1;
-      a.positions[t64] = real ? int64_t(pos) : 0;
-      a.requests[t64] = real ? int32_t(i) : -1;
+      slots[e] = real ? slot : -1;
+      positions[e] = real ? int64_t(pos) : 0;
+      requests[e] = real ? int32_t(i) : -1;
+    }
+    if (kRun == 4 && t0 + kRun <= a.tokens) {
+      typedef int64_t long2_t __attribute__((ext_vector_type(2)));
+      typedef int32_t int4_t __attribute__((ext_vector_type(4)));
+#pragma unroll
+      for (int e = 0; e + 1 < kRun; e += 2) {
+        *reinterpret_cast<long2_t*>(a.slots + t0 + e) = long2_t{slots[e], slots[e + 1]};
+        *reinterpret_cast<long2_t*>(a.positions + t0 + e) =
+            long2_t{positions[e], positions[e + 1]};
+      }
+      *reinterpret_cast<int4_t*>(a.requests + t0) =
+          int4_t{requests[0], requests[1 % kRun], requests[2 % kRun], requests[3 % kRun]};
+    } else {
+#pragma unroll
+      for (int e = 0; e < kRun; ++e) {
+        if (t0 + e >= a.tokens) break;
+        a.slots[t0 + e] = slots[e];
+        a.positions[t0 + e] = positions[e];
+        a.requests[t0 + e] = requests[e];
+      }
     }
   }
 }
@@ -173,27 +198,30 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
   __shared__ uint2 wave[kPlanThreads / 64];
   const int per = int(a.N + kPlanThreads - 1) / kPlanThreads;
   const int lo = int(threadIdx.x) * per, N = int(a.N);
+  const int64_t head = plan_head(a);
   uint32_t x = 0, y = 0, tx, ty;
   for (int i = lo; i < lo + per && i < N; ++i) {
     const PlanRow r = plan_row(a, i);
+    tok[i] = r.fresh;  // read by this thread alone, below
+    pag[i] = r.need;
     x = plus(x, r.fresh);
     y = plus(y, r.need);
   }
   block_exclusive<kPlanThreads>(x, y, &tx, &ty, wave);
   for (int i = lo; i < lo + per && i < N; ++i) {
-    const PlanRow r = plan_row(a, i);
+    const uint32_t fresh = tok[i], need = pag[i];
     tok[i] = x;
     pag[i] = y;
-    if (blockIdx.x == 0) plan_request(a, i, r, x);
-    x = plus(x, r.fresh);
-    y = plus(y, r.need);
+    if (blockIdx.x == 0) plan_request(a, i, plan_row(a, i), x);
+    x = plus(x, fresh);
+    y = plus(y, need);
   }
   if (threadIdx.x == 0) {
     tok[N] = tx;
     pag[N] = ty;
   }
   __syncthreads();
-  plan_fill<kRun>(a, tok, pag);
+  plan_fill<kRun>(a, tok, pag, head);
 }
 
 // More requests than LDS holds: the sums of all of them, kThreads at a time.
@@ -223,7 +251,7 @@ __global__ __launch_bounds__(kScanThreads) void plan_scan_kernel(PlanArgs a, uin
 }
 __global__ __launch_bounds__(kPlanThreads) void plan_fill_kernel(PlanArgs a, const uint32_t* tok,
                                                                  const uint32_t* pag) {
-  plan_fill<1>(a, tok, pag);
+  plan_fill<1>(a, tok, pag, plan_head(a));
 }
 
 int64_t plan_workspace_bytes(int64_t N) { return N <= kPlanLds ? 0 : 8 * (N + 1); }
@@ -234,8 +262,10 @@ hipError_t launch_paged_plan(const int32_t* kv_lens, const int32_t* new_lens, in
                              int64_t page, int64_t tokens, int32_t* kv_out, int32_t* indptr,
                              int64_t* slots, int64_t* positions, int32_t* requests,
                              int64_t* taken, uint32_t* workspace, hipStream_t stream) {
-  // Steps of single tokens, or prompts among them.
-  const int run = N <= kPlanLds && tokens > 4 * N ? 4 : 1;
+  // Steps of single tokens, or prompts among them, whose tokens are stored by fours.
+  const bool whole = (reinterpret_cast<uintptr_t>(slots) | reinterpret_cast<uintptr_t>(positions) |
+                      reinterpret_cast<uintptr_t>(requests)) % 16 == 0;
+  const int run = N <= kPlanLds && tokens > 4 * N && whole ? 4 : 1;
   int64_t groups = (tokens + run * kPlanThreads - 1) / (run * kPlanThreads);
   if (groups < 1) groups = 1;
   if (groups > 4096) groups = 4096;
