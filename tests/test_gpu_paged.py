@@ -592,6 +592,50 @@ def test_decode_infinite_values_by_masked_and_tiny_weights(lens, D, dtype):
         assert bool(((out[n].double() - want).abs() <= room)[ok].all())
 
 
+def row_of(c, table, n, t, page):
+    return c[int(table[n, t // page]), t % page]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("lens,Hk,D,page", [([4101], 1, 128, 16), ([4101, 77], 2, 64, 24),
+                                            ([500], 2, 128, 16), ([250] * 150, 2, 64, 16),
+                                            ([900], 1, 72, 16)])
+def test_decode_small_weights_beside_a_great_one(lens, Hk, D, page, dtype):
+    """One key far above the others (an attention sink) whose value is 0: what the others' small
+    weights add up to is all of the output, in every form of the kernel."""
+    note("paged decode, sink", lens[:3], Hk, D, page, dtype)
+    N, g = len(lens), gen(D + page)
+    _, kc, vc, table, l = decode_case(lens, 2 * Hk, Hk, D, page, "NHD", dtype, seed=D, extra=0)
+    q = torch.zeros(N, 2 * Hk, D, dtype=dtype)
+    q[:, :, 0] = 1.0                       # a score is feature 0 of its key, exactly
+    for n, L in enumerate(lens):
+        for t in range(L):
+            row_of(kc, table, n, t, page)[:, 0] = (0.3 * torch.randn(Hk, generator=g)).to(dtype)
+    for gap, size in ((12.0, 1.0), (16.0, 1.0), (17.0, 1.0), (18.0, 1.0), (24.0, 500.0)):
+        k, v = kc.clone(), (size * (vc.abs() + 0.125)).to(dtype)
+        for n, L in enumerate(lens):
+            row_of(k, table, n, L // 3, page)[:, 0] = gap
+            row_of(v, table, n, L // 3, page)[:] = 0
+        out = run_decode(q, k, v, table, l, "NHD", sm_scale=1.0)
+        want, slack = torch.zeros(N, 2 * Hk, D).double(), torch.zeros(N, 2 * Hk, D).double()
+        for n, L in enumerate(lens):
+            t = torch.arange(L)
+            at = table[n].long()[t // page] * page + t % page
+            K, V = (ref.cache_rows(c, "NHD")[at].double().repeat_interleave(2, 1) for c in (k, v))
+            p = torch.softmax(K[..., 0], 0)
+            want[n] = (p[..., None] * V).sum(0)
+            # Roundings of 2^-24 each: scores of size below 25 in units of log2(e) (three for the
+            # scaled score, one for the difference, one step of exp2: below 200 in a weight and in
+            # the weights' sum together) and sums of at most 300 after one another (32 products of
+            # an instruction times 8 steps, the waves' and the work-groups' merges), of weights
+            # and of values: below 1000, 2^-14.  16-bit types' parts add at most 2^-18 of a weight
+            # and, in fp16, 2^-44 of the greatest one.
+            slack[n] = 2.0 ** -14 * want[n]
+            if dtype == F16:
+                slack[n] += L * 2.0 ** -44 * V.max()
+        within(out, want, slack, dtype)
+
+
 def test_decode_strided_views():
     """Caches in one allocation, queries and tables cut from wider ones."""
     note("paged decode, strided")

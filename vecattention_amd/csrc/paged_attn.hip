@@ -292,7 +292,13 @@ __global__ __launch_bounds__(kPagedThreads) void paged_row_kernel(PagedArgs a) {
 // but the waves' results at a segment's end goes through LDS.
 //
 // 16-bit types round a weight to 8 (11) bits, which would cost as much accuracy
-// as the output's own rounding: it goes in as two parts, high + low, to 2^-16.
+// as the output's own rounding: it goes in as two parts, high + low.  bf16 has the
+// exponents of fp32: to 2^-18 of the weight.  fp16 ends at 2^-24, and beside one key of
+// great weight the others' would be lost: its high part is that of 2^7 weights (at
+// most 2^15), its low part is held 2^12 times larger still and is summed by itself,
+// so that a weight is good to 2^-22 of itself or 2^-44, whatever is more, and a wave's
+// greatest weight is 1 or more.  (One sum for both parts would end at 2^-32, and keys
+// 24 nats below the greatest would be gone.)
 //
 // Infinite values would meet weights of 0 and give NaN where they may not: the low
 // part of a weight (or one below 0), the weight of a key past the last, whose row
@@ -368,7 +374,8 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
   constexpr int kKL = k16 ? D / 32 : D / 16;       // 16-byte loads of a lane in a row of K
   constexpr int kVW = kF * int(sizeof(T)) / 4;     // words of a lane in a row of V
   constexpr int kStride = D + 4;
-  constexpr float kLeast = std::is_same_v<T, f16_t> ? 0x1p-24f : 0x1p-126f;  // weight of T
+  constexpr bool kApart = std::is_same_v<T, f16_t>;  // the low parts are summed by themselves
+  constexpr float kLeast = kApart ? 0x1p-31f : 0x1p-126f;  // weight of T
   __shared__ PlaceLds place;
   __shared__ __align__(16) float sO[kStates][kTileHeads][kStride];
   __shared__ float sm[kStates][kTileHeads], sl[kStates][kTileHeads];
@@ -498,14 +505,17 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
       }
     };
 
-    f32x4_t acc[kF];
+    f32x4_t acc[kF], low[kApart ? kF : 1];
     float m, l;
     auto walk = [&](auto again) {
       constexpr bool repeat = decltype(again)::value;
       m = -__builtin_inff();
       l = 0.f;
 #pragma unroll
-      for (int f = 0; f < kF; ++f) acc[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      for (int f = 0; f < kF; ++f) {
+        acc[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        if constexpr (kApart) low[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      }
       if (steps > 0) {
         fetch(first);
         place();
@@ -554,6 +564,7 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
           l *= f;
 #pragma unroll
           for (int x = 0; x < kF; ++x) {
+            if constexpr (kApart) low[x] *= f;
             if constexpr (!repeat)
               acc[x] *= f;
             else
@@ -582,8 +593,13 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
           vec hi, lo;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            hi[j] = elem(p[j]);
-            lo[j] = elem(p[j] - float(hi[j]));
+            if constexpr (kApart) {
+              hi[j] = elem(p[j] * 0x1p7f);
+              lo[j] = elem(__builtin_fmaf(p[j], 0x1p19f, -0x1p12f * float(hi[j])));
+            } else {
+              hi[j] = elem(p[j]);
+              lo[j] = elem(p[j] - float(hi[j]));
+            }
           }
 #pragma unroll
           for (int x = 0; x < kF; ++x) {
@@ -594,7 +610,8 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
             for (int j = 0; j < 4; ++j)
               av[j] = __builtin_amdgcn_perm(vr[2 * j + 1][x / 2], vr[2 * j][x / 2], sel);
             acc[x] = Mfma16<T>::run(__builtin_bit_cast(vec, av), hi, acc[x]);
-            if (!repeat) acc[x] = Mfma16<T>::run(__builtin_bit_cast(vec, av), lo, acc[x]);
+            f32x4_t& rest = kApart ? low[kApart ? x : 0] : acc[x];
+            if (!repeat) rest = Mfma16<T>::run(__builtin_bit_cast(vec, av), lo, rest);
           }
         } else {
 #pragma unroll
@@ -605,6 +622,13 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
                                                             0, 0, 0);
         }
         if (i + 1 < steps) load_v(key0 + kUnit);
+      }
+      if constexpr (kApart) {
+#pragma unroll
+        for (int x = 0; x < kF; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            acc[x][e] = __builtin_fmaf(low[x][e], 0x1p-19f, acc[x][e] * 0x1p-7f);
       }
     };
     walk(std::false_type{});
