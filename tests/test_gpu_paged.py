@@ -636,6 +636,24 @@ def test_decode_small_weights_beside_a_great_one(lens, Hk, D, page, dtype):
         within(out, want, slack, dtype)
 
 
+def test_decode_scores_whose_steps_are_large():
+    """Scores of 2^27, whose neighbours lie 16 apart in powers of two: any weights of equal
+    values give that value."""
+    note("paged decode, large scores")
+    L, N = 300, 6                          # eight waves of 32 keys: the first has two steps
+    for dtype in (F16, BF16, F32):
+        q, kc, vc, table, l = decode_case([L] * N, 1, 1, 64, 16, "NHD", dtype, seed=1, extra=0)
+        q[:], kc[:], vc[:] = 0, 0, 1.0
+        q[:, 0, 0], q[:, 0, 1] = 2048.0, 1.0
+        for n in range(N):
+            for t in range(L):
+                row_of(kc, table, n, t, 16)[0, 0] = 4096.0
+                row_of(kc, table, n, t, 16)[0, 1] = float(n + t // 256)
+        out = run_decode(q, kc, vc, table, l, "NHD", sm_scale=16 / 1.4426950408889634)
+        # Both sums add the same 300 weights, each off by 2^-16 at most: below half a step of bf16.
+        assert bool(((out.float() - 1).abs() <= 2.0 ** -9).all()), (dtype, out[:, 0, 0])
+
+
 def test_decode_strided_views():
     """Caches in one allocation, queries and tables cut from wider ones."""
     note("paged decode, strided")

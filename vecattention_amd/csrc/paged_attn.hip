@@ -556,8 +556,9 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
           top = __builtin_fmaxf(top, p[j]);  // a NaN score stays out of m and poisons its weight
         }
         top = column_max(top);
-        // m trails the maximum by at most 8: weights stay below 2^8.
-        if (__any(top > m + 8.f)) {
+        // m trails the maximum by at most 8: weights stay within 2^8.  The difference is exact
+        // where it is near that; m + 8 rounds at scores of 2^27, to m + 16.
+        if (__any(top - m > 8.f)) {
           const float mn = __builtin_fmaxf(m, top);
           const float f = __builtin_amdgcn_exp2f(m - (mn == -__builtin_inff() ? 0.f : mn));
           m = mn;
