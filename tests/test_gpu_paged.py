@@ -654,6 +654,34 @@ def test_decode_scores_whose_steps_are_large():
         assert bool(((out.float() - 1).abs() <= 2.0 ** -9).all()), (dtype, out[:, 0, 0])
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("lens,Hq,D,page", [([3000], 8, 128, 16), ([700, 33, 2100], 4, 64, 24),
+                                            ([300, 64], 8, 128, 16), ([60] * 150, 4, 64, 16),
+                                            ([90, 500], 6, 40, 16)])
+def test_decode_finite_outputs_beside_others(lens, Hq, D, page, dtype):
+    """An infinite value, a NaN in a value or in a query reaches the outputs that the formula has
+    it in; all others stay as they are, bit for bit."""
+    note("paged decode, beside others", lens[:3], Hq, D, page, dtype)
+    q, kc, vc, table, l = decode_case(lens, Hq, 2, D, page, "NHD", dtype, seed=D, extra=0)
+    clean = run_decode(q, kc, vc, table, l, "NHD")
+    v, G = vc.clone(), Hq // 2
+    for n, L in enumerate(lens):
+        row_of(v, table, n, L // 2, page)[0, 3] = math.inf
+        row_of(v, table, n, L - 1, page)[0, 9] = -math.inf
+        row_of(v, table, n, L // 3, page)[1, 5] = math.nan
+    want = clean.clone()
+    want[:, :G, 3], want[:, :G, 9] = math.inf, -math.inf
+    out = run_decode(q, kc, v, table, l, "NHD")
+    assert bool(torch.isnan(out[:, G:, 5]).all())
+    out[:, G:, 5] = want[:, G:, 5]
+    assert torch.equal(out, want)
+    q[:, 1, 7] = math.nan
+    out = run_decode(q, kc, vc, table, l, "NHD")
+    assert bool(torch.isnan(out[:, 1]).all())
+    out[:, 1] = clean[:, 1]
+    assert torch.equal(out, clean)
+
+
 def test_decode_strided_views():
     """Caches in one allocation, queries and tables cut from wider ones."""
     note("paged decode, strided")

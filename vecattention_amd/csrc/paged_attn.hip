@@ -303,8 +303,10 @@ __global__ __launch_bounds__(kPagedThreads) void paged_row_kernel(PagedArgs a) {
 // Infinite values would meet weights of 0 and give NaN where they may not: the low
 // part of a weight (or one below 0), the weight of a key past the last, whose row
 // is the last key's, and weights too small for their type.  A wave whose sums hold
-// a NaN repeats its keys with the high part alone, zeros for rows past the last
-// key, and a smallest weight for every key that has one.
+// a NaN repeats its keys with zeros for rows past the last key and for values that
+// are not finite, so that all other sums come out as before, bit for bit; those
+// values go in by a product of their own, with a weight of 1 for every key that has
+// one, however small.
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
@@ -375,7 +377,6 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
   constexpr int kVW = kF * int(sizeof(T)) / 4;     // words of a lane in a row of V
   constexpr int kStride = D + 4;
   constexpr bool kApart = std::is_same_v<T, f16_t>;  // the low parts are summed by themselves
-  constexpr float kLeast = kApart ? 0x1p-31f : 0x1p-126f;  // weight of T
   __shared__ PlaceLds place;
   __shared__ __align__(16) float sO[kStates][kTileHeads][kStride];
   __shared__ float sm[kStates][kTileHeads], sl[kStates][kTileHeads];
@@ -574,12 +575,12 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
           }
         }
         const float ms = m == -__builtin_inff() ? 0.f : m;
+        float seen[kTiles * 4];  // 1 for a key that has a weight
 #pragma unroll
         for (int j = 0; j < kTiles * 4; ++j) {
-          const bool seen = p[j] != -__builtin_inff();
+          if constexpr (repeat) seen[j] = p[j] != -__builtin_inff() ? 1.f : 0.f;
           p[j] = __builtin_amdgcn_exp2f(p[j] - ms);
           l += p[j];
-          if (repeat && seen && p[j] < kLeast) p[j] = kLeast;
         }
         if constexpr (repeat) {
 #pragma unroll
@@ -591,9 +592,10 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
         if constexpr (k16) {
           typedef typename Mfma16<T>::vec vec;
           typedef typename Mfma16<T>::e elem;
-          vec hi, lo;
+          vec hi, lo, one;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
+            if constexpr (repeat) one[j] = elem(seen[j]);
             if constexpr (kApart) {
               hi[j] = elem(p[j] * 0x1p7f);
               lo[j] = elem(__builtin_fmaf(p[j], 0x1p19f, -0x1p12f * float(hi[j])));
@@ -606,21 +608,39 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
           for (int x = 0; x < kF; ++x) {
             // Feature x of the lane's eight keys: halves of words x / 2.
             const uint32_t sel = x % 2 ? 0x07060302u : 0x05040100u;
-            u32x4_t av;
+            u32x4_t av, odd;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 4; ++j) {
               av[j] = __builtin_amdgcn_perm(vr[2 * j + 1][x / 2], vr[2 * j][x / 2], sel);
+              if constexpr (repeat) {  // the halves whose exponent has every bit set
+                constexpr uint32_t kExp = kApart ? 0x7c00u : 0x7f80u;
+                odd[j] = ((av[j] & kExp) == kExp ? av[j] & 0xffffu : 0u) |
+                         ((av[j] >> 16 & kExp) == kExp ? av[j] & 0xffff0000u : 0u);
+                av[j] ^= odd[j];
+              }
+            }
             acc[x] = Mfma16<T>::run(__builtin_bit_cast(vec, av), hi, acc[x]);
             f32x4_t& rest = kApart ? low[kApart ? x : 0] : acc[x];
-            if (!repeat) rest = Mfma16<T>::run(__builtin_bit_cast(vec, av), lo, rest);
+            rest = Mfma16<T>::run(__builtin_bit_cast(vec, av), lo, rest);
+            if constexpr (repeat)
+              acc[x] = Mfma16<T>::run(__builtin_bit_cast(vec, odd), one, acc[x]);
           }
         } else {
 #pragma unroll
           for (int x = 0; x < kF; ++x)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              acc[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_to_float(vr[j][x]), p[j], acc[x],
-                                                            0, 0, 0);
+            for (int j = 0; j < 4; ++j) {
+              uint32_t v = vr[j][x], odd = 0;
+              if constexpr (repeat) {
+                odd = (v & 0x7f800000u) == 0x7f800000u ? v : 0u;
+                v ^= odd;
+              }
+              acc[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_to_float(v), p[j], acc[x], 0, 0,
+                                                            0);
+              if constexpr (repeat)
+                acc[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_to_float(odd), seen[j], acc[x],
+                                                              0, 0, 0);
+            }
         }
         if (i + 1 < steps) load_v(key0 + kUnit);
       }
