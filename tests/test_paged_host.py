@@ -356,3 +356,31 @@ def test_arguments_that_are_no_tensors_or_numbers():
     with pytest.raises(KeyError):
         va.write_paged_kv(torch.zeros(5, 2, 64), torch.zeros(5, 2, 64), torch.zeros(3, 16, 2, 64),
                           torch.zeros(3, 16, 2, 64), torch.zeros(5, dtype=torch.int64), None)
+
+
+def test_operators_have_no_forward_derivative():
+    """A tangent is refused, not dropped; where forward mode is off, the device speaks next."""
+    from torch.autograd import forward_ad as fw
+    x, kc, slots = torch.ones(5, 2, 64), torch.zeros(3, 16, 2, 64), torch.zeros(5, dtype=torch.int64)
+    inv, w = torch.ones(32), torch.ones(64)
+    table, lens = torch.zeros(5, 1, dtype=torch.int32), torch.ones(5, dtype=torch.int32)
+    calls = [(lambda q, k, f, u, v: va.qk_norm_rope(q[None], k[None], slots[:2], f, u, v),
+              [x, x, inv, w, w]),
+             (lambda q, k, v, c, d, f, u: va.qk_norm_rope_to_cache(q, k, v, c, d, slots, slots, f,
+                                                                   u, u),
+              [x, x, x, kc, kc, inv, w]),
+             (lambda k, v, c, d: va.write_paged_kv(k, v, c, d, slots), [x, x, kc, kc]),
+             (lambda k: va.write_paged_kv(k[..., ::2], x[..., ::2], kc[..., :32], kc[..., :32],
+                                          slots), [x]),  # a copied one
+             (lambda q, c, d: va.paged_decode_attention(q, c, d, table, lens), [x, kc, kc])]
+    with fw.dual_level():
+        for call, args in calls:
+            for i, a in enumerate(args):
+                dual = [fw.make_dual(b, torch.ones_like(b)) if i == j else b
+                        for j, b in enumerate(args)]
+                with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(*dual)
+                with fw._set_fwd_grad_enabled(False), pytest.raises(RuntimeError, match="the GPU"):
+                    call(*dual)
+            with pytest.raises(RuntimeError, match="the GPU"):
+                call(*args)

@@ -13,6 +13,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -83,7 +84,8 @@ int dtype_code(const at::Tensor& t) {
   }
 }
 
-// All on the first one's GPU, and nothing that autograd would want a backward of.
+// All on the first one's GPU, and nothing that autograd would want a derivative of:
+// a call runs below it, and would drop a tangent in silence.
 void one_gpu(const char* what, std::initializer_list<const at::Tensor*> tensors) {
   const at::Tensor& first = **tensors.begin();
   if (!first.is_cuda()) refuse(PyExc_RuntimeError, "%s runs on the GPU", what);
@@ -98,6 +100,14 @@ void no_backward(const char* what, std::initializer_list<const at::Tensor*> tens
     if (t->defined() && t->requires_grad())
       refuse(PyExc_NotImplementedError, "%s has no backward pass: call it under torch.no_grad()",
              what);
+}
+
+void no_tangent(const char* what, std::initializer_list<const at::Tensor*> tensors) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const at::Tensor* t : tensors)
+    if (t->defined() && t->_fw_grad(0).defined())
+      refuse(PyExc_NotImplementedError,
+             "%s has no forward-mode derivative: call it with tensors that have no tangent", what);
 }
 
 // Written behind autograd's back: what saved it for a backward pass has to notice.
@@ -351,8 +361,10 @@ PyObject* rope(PyObject* const* a) {
   const int dtype = dtype_code(q_);
   const Rotation r(D, q_, tensor(a[2], "positions"), tensor(a[3], "inv_freq"),
                    maybe(a[4], "q_weight"), maybe(a[5], "k_weight"), a[7], {B, S});
+  const auto inputs = {&q_, &k_, &r.inv_freq, &r.qw, &r.kw};
+  no_tangent("qk_norm_rope", inputs);
   one_gpu("qk_norm_rope", {&q_, &k_, &r.positions, &r.inv_freq, &r.qw, &r.kw});
-  no_backward("qk_norm_rope", {&q_, &k_, &r.inv_freq, &r.qw, &r.kw});
+  no_backward("qk_norm_rope", inputs);
   const at::Tensor q = rows(q_), k = rows(k_), qo = rows_like(q), ko = rows_like(k);
   if (B && S)
     check("va_qk_norm_rope",
@@ -391,10 +403,12 @@ PyObject* rope_to_cache(PyObject* const* a) {
   if (c.heads != t.Hk)
     refuse(PyExc_ValueError, "a cache of %lld heads for keys of %lld", (long long)c.heads,
            (long long)t.Hk);
+  const auto inputs = {&q_, &tensor(a[1], "k"), &tensor(a[2], "v"), &kc, &vc,
+                       &r.inv_freq, &r.qw, &r.kw};
+  no_tangent("qk_norm_rope_to_cache", inputs);
   one_gpu("qk_norm_rope_to_cache",
           {&q_, &t.k, &t.v, &kc, &vc, &t.slots, &r.positions, &r.inv_freq, &r.qw, &r.kw});
-  no_backward("qk_norm_rope_to_cache", {&q_, &tensor(a[1], "k"), &tensor(a[2], "v"), &kc, &vc,
-                                        &r.inv_freq, &r.qw, &r.kw});
+  no_backward("qk_norm_rope_to_cache", inputs);
   const at::Tensor q = rows(q_), out = rows_like(q);
   if (t.T)
     check("va_qk_norm_rope_to_cache",
@@ -419,8 +433,10 @@ PyObject* write_kv(PyObject* const* a) {
   if (c.heads != t.Hk)
     refuse(PyExc_ValueError, "a cache of %lld heads for keys of %lld", (long long)c.heads,
            (long long)t.Hk);
+  const auto inputs = {&tensor(a[0], "k"), &tensor(a[1], "v"), &kc, &vc};
+  no_tangent("write_paged_kv", inputs);
   one_gpu("write_paged_kv", {&t.k, &t.v, &kc, &vc, &t.slots});
-  no_backward("write_paged_kv", {&tensor(a[0], "k"), &tensor(a[1], "v"), &kc, &vc});
+  no_backward("write_paged_kv", inputs);
   if (t.T && t.Hk && t.D)
     check("va_write_paged_kv",
           va_write_paged_kv(dtype, t.k.data_ptr(), t.k.stride(0), t.k.stride(1), t.v.data_ptr(),
@@ -449,8 +465,10 @@ PyObject* decode(PyObject* const* a) {
            shape(table_).c_str(), shape(lens_).c_str(), (long long)N);
   if (table_.scalar_type() != at::kInt || lens_.scalar_type() != at::kInt)
     refuse(PyExc_TypeError, "block_tables and kv_lens must be int32");
+  const auto inputs = {&q_, &kc, &vc};
+  no_tangent("paged_decode_attention", inputs);
   one_gpu("paged_decode_attention", {&q_, &kc, &vc, &table_, &lens_});
-  no_backward("paged_decode_attention", {&q_, &kc, &vc});
+  no_backward("paged_decode_attention", inputs);
   const int64_t M = table_.size(1);
   const at::Tensor q = rows(q_), lens = lens_.contiguous(),
                    table = M > 1 && table_.stride(1) != 1 ? table_.contiguous() : table_;
