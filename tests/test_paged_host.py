@@ -384,3 +384,18 @@ def test_operators_have_no_forward_derivative():
                     call(*dual)
             with pytest.raises(RuntimeError, match="the GPU"):
                 call(*args)
+
+
+@pytest.mark.parametrize("bad", [None, [1.0], 3, "q"])
+def test_a_first_argument_that_is_no_tensor(bad):
+    """It chooses the GPU that the call runs on, and is refused as the others are."""
+    x, kc, slots, inv = (torch.zeros(5, 2, 64), torch.zeros(3, 16, 2, 64),
+                         torch.zeros(5, dtype=torch.int64), torch.ones(32))
+    for name, call in [
+            ("block_tables", lambda: va.paged_kv_plan(i32(3), i32(3), bad, i32(5), 16, 8)),
+            ("q", lambda: va.qk_norm_rope(bad, x[None], slots, inv)),
+            ("q", lambda: va.qk_norm_rope_to_cache(bad, x, x, kc, kc, slots, slots, inv)),
+            ("k", lambda: va.write_paged_kv(bad, x, kc, kc, slots)),
+            ("q", lambda: va.paged_decode_attention(bad, kc, kc, i32(5, 1), i32(5)))]:
+        with pytest.raises(TypeError, match=f"^{name} must be a tensor"):
+            call()

@@ -228,9 +228,9 @@ def _host_module():
 def host_call(name, on, *args):
     """A call of the host module on the current stream of the tensor `on`'s GPU."""
     call = getattr(_host or _host_module(), name)
-    dev = on.get_device()
+    dev = on.get_device() if isinstance(on, torch.Tensor) else -1
     if dev < 0:
-        return call(*args, 0)  # no GPU: the call refuses it
+        return call(*args, 0)  # no GPU, or no tensor: the call refuses it
     if _raw_stream is not None and dev == _current_device():
         return call(*args, _raw_stream(dev))
     with torch.cuda.device(dev):
