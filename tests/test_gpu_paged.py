@@ -887,6 +887,78 @@ def test_prompts_then_generated_tokens(dtype, layout):
             within(out[n], want, rel * (w[..., None] * V.abs()).sum(0), dtype)
 
 
+def test_image_prompt_then_generated_tokens():
+    """A prompt with an image, rotated over three axes, beside one of text; then generated tokens
+    at the positions behind each prompt's last, which for the first are not their indices."""
+    note("image prompt")
+    g = gen(23)
+    dtype, Hq, Hk, D, page, N = F32, 4, 2, 64, 16, 2
+    inv, sections = freqs(D), [8, 12, 12]
+    at = [torch.cat([torch.arange(5).expand(3, 5),
+                     5 + torch.stack([torch.zeros(24).long(), torch.arange(24) // 6,
+                                      torch.arange(24) % 6]),
+                     11 + torch.arange(7).expand(3, 7)], 1),     # 36 tokens, positions up to 17
+          torch.arange(21).expand(3, 21)]
+    lens = torch.zeros(N, dtype=torch.int32, device=DEV)
+    table = torch.full((N, 4), -1, dtype=torch.int32, device=DEV)
+    free = torch.randperm(8, generator=g).int().to(DEV)
+    head = torch.zeros(1, dtype=torch.int32, device=DEV)
+    deltas = torch.zeros(N, dtype=torch.int64, device=DEV)
+    kc, vc = (torch.full((8, page, Hk, D), math.nan, dtype=dtype, device=DEV) for _ in range(2))
+    K, V = [], []
+    for n in range(N):
+        S = at[n].shape[1]
+        new = torch.zeros(N, dtype=torch.int32, device=DEV)
+        new[n] = S
+        p = paged_kv_plan(lens, new, table, free, page, S, head)
+        head, lens = (head + p.pages_taken).int(), p.kv_lens
+        q, k, v = (torch.randn(1, H, S, D, generator=g, dtype=dtype) for H in (Hq, Hk, Hk))
+        ids = at[n][:, None].to(DEV)
+        _, rk = qk_norm_rope(q.to(DEV), k.to(DEV), ids, inv.to(DEV), mrope_section=sections)
+        write_paged_kv(rk[0].transpose(0, 1), v[0].transpose(0, 1).to(DEV), kc, vc, p.slot_mapping)
+        deltas[n] = ids.max() + 1 - S
+        K.append(ref.rotate(k[0], at[n][:, None], inv, sections=sections)[0].transpose(0, 1))
+        V.append(v[0].transpose(0, 1).double())
+    assert deltas.tolist() == [18 - 36, 0]
+    ones = torch.ones(N, dtype=torch.int32, device=DEV)
+    for step in range(3):
+        p = paged_kv_plan(lens, ones, table, free, page, N + 2, head)
+        head, lens = (head + p.pages_taken).int(), p.kv_lens
+        positions = p.positions + deltas[p.request_ids]
+        q, k, v = (torch.randn(N + 2, H, D, generator=g, dtype=dtype) for H in (Hq, Hk, Hk))
+        rq = qk_norm_rope_to_cache(*(x.to(DEV) for x in (q, k, v)), kc, vc, p.slot_mapping,
+                                   positions, inv.to(DEV))
+        out = paged_decode_attention(rq[:N], kc, vc, table, lens).cpu()
+        for n in range(N):
+            pos = int(at[n].max()) + 1 + step
+
+            def turned(x, pos):
+                return ref.rotate(x, torch.tensor([pos] * 3)[:, None], inv, sections=sections)[0]
+
+            def attend(pos):
+                keys = torch.cat([K[n], turned(k[n], pos)[None]]).repeat_interleave(Hq // Hk, 1)
+                s = (keys * turned(q[n], pos)).sum(-1) / math.sqrt(D)
+                return keys, torch.softmax(s, 0)
+
+            keys, w = attend(pos)
+            K[n] = torch.cat([K[n], turned(k[n], pos)[None]])
+            V[n] = torch.cat([V[n], v[n].double()[None]])
+            values = V[n].repeat_interleave(Hq // Hk, 1)
+            want = (w[..., None] * values).sum(0)
+            # The rotation is off by 32 roundings of the pairs' sizes, at most sqrt(2) of the rows'
+            # lengths: a score by twice that of their product and ref.decode's 2^-24 (D + 8).
+            size = (keys.norm(dim=-1) * q[n].double().norm(dim=-1)).max() / math.sqrt(D)
+            move = 2.0 ** -24 * (2 * 32 * math.sqrt(2) + D + 8) * float(size)
+            rel = 2 * math.expm1(move) + 2.0 ** -16
+            slack = rel * (w[..., None] * values.abs()).sum(0)
+            within(out[n], want, slack, dtype)
+            if n == 0:                           # and the bare index is another position
+                K[n], last = K[n][:-1], K[n][-1:]
+                bare = (attend(int(lens[0]) - 1)[1][..., None] * values).sum(0)
+                K[n] = torch.cat([K[n], last])
+                assert bool(((bare - want).abs() > 100 * slack).any())
+
+
 @pytest.mark.parametrize("page", [16, 5])
 def test_a_whole_step_in_a_graph(page):
     """Plan, rotation, writes and attention of a step in one graph that carries its state on the

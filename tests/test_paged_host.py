@@ -399,3 +399,47 @@ def test_a_first_argument_that_is_no_tensor(bad):
             ("q", lambda: va.paged_decode_attention(bad, kc, kc, i32(5, 1), i32(5)))]:
         with pytest.raises(TypeError, match=f"^{name} must be a tensor"):
             call()
+
+
+def test_the_documented_step_rotates_by_the_models_positions(monkeypatch):
+    """The documentation's step of a prompt with an image and of generated tokens, run with
+    recorders in place of the operators: a generated token's position is the one behind the
+    prompt's last, not its index."""
+    import glob
+    import re
+    blocks = [b for f in sorted(glob.glob(os.path.join(os.path.dirname(HERE), "*.md")))
+              for b in re.findall(r"```python\n(.*?)```", open(f).read(), re.S)
+              if "= paged_decode_attention(" in b]
+    assert len(blocks) == 1
+    N, S, i = 3, 36, 1
+    rotated = []
+
+    def plan(kv_lens, new_lens, tables, free_pages, page, num_tokens, head=None):
+        index = torch.full((N,), S)        # each request's next token, and one row of padding
+        return va.PagedStep(kv_lens, None, torch.cat([index, index[:1] * 0 - 1]),
+                            torch.cat([index, index[:1] * 0]),
+                            torch.tensor([0, 1, 2, -1], dtype=torch.int32), None)
+
+    def rotate(q, k, v, kc, vc, slots, positions, *more, **options):
+        rotated.append((positions, more, options))
+        return q
+
+    monkeypatch.setattr(va, "paged_kv_plan", plan)
+    monkeypatch.setattr(va, "qk_norm_rope", lambda q, k, *more, **options: (q, k))
+    monkeypatch.setattr(va, "qk_norm_rope_to_cache", rotate)
+    for name in ("write_paged_kv", "paged_decode_attention", "VecAttention_prefill"):
+        monkeypatch.setattr(va, name, lambda *args, **options: None)
+    # Five tokens of text, an image of 4 x 6, seven tokens of text behind its largest position.
+    at = torch.cat([torch.arange(5).expand(3, 5),
+                    5 + torch.stack([torch.zeros(24).long(), torch.arange(24) // 6,
+                                     torch.arange(24) % 6]),
+                    11 + torch.arange(7).expand(3, 7)], 1)[:, None]
+    x = torch.zeros(1, 2, S, 64)
+    exec(blocks[0].replace('"cuda"', '"cpu"'), dict(
+        torch=torch, num_pages=8, Hk=2, D=64, N=N, max_pages=4, i=i, num_tokens=N + 1, q=x, k=x,
+        v=x, kv_lens=None, new_lens=None, position_ids=at, q_norm=None, k_norm=None,
+        inv_freq=torch.ones(32), rotary_emb=type("", (), {"inv_freq": torch.ones(32)})))
+    (positions, _, options), = rotated
+    want = [S] * N
+    want[i] = int(at.max()) + 1
+    assert positions[:N].tolist() == want and "mrope_section" not in options

@@ -30,7 +30,7 @@ class PagedStep(NamedTuple):
     kv_lens: torch.Tensor       # (N,) int32: lengths after the step
     qo_indptr: torch.Tensor     # (N + 1,) int32: first token of each request
     slot_mapping: torch.Tensor  # (num_tokens,) int64: slot of each token, -1 for none
-    positions: torch.Tensor     # (num_tokens,) int64: position in its request
+    positions: torch.Tensor     # (num_tokens,) int64: its place among its request's tokens
     request_ids: torch.Tensor   # (num_tokens,) int32: its request, -1 for padding
     pages_taken: torch.Tensor   # (1,) int64: pages asked for
 
@@ -45,7 +45,10 @@ def paged_kv_plan(kv_lens, new_lens, block_tables, free_pages, page_size, num_to
     tokens need, taken from ``free_pages`` ((F,) int32) in the order of the
     requests, from entry ``free_head`` on (a one-element int32 tensor; None: 0).
     num_tokens: rows of the per-token outputs, at least sum(new_lens); further
-    rows are padding (request -1, position 0, slot -1).
+    rows are padding (request -1, position 0, slot -1).  ``positions`` count a
+    request's tokens; where the model's positions do not (the tokens of an image
+    cover fewer of them than their number), the rotation takes ``positions`` plus
+    the request's offset, indexed by ``request_ids``.
 
     Pages that the list no longer has give -1 entries and slots; then
     free_head + pages_taken exceeds F.  A token past the table's M pages has
@@ -74,7 +77,8 @@ def qk_norm_rope_to_cache(q, k, v, k_cache, v_cache, slot_mapping, positions, in
     their slots of the caches in the same launch.
 
     q: (T, Hq, D); k, v: (T, Hk, D); positions (T,), or with ``mrope_section``
-    (axes, T) ((T,): the same on every axis, as generated text has it);
+    (axes, T) ((T,): the same on every axis, as generated text has it; the
+    positions of the model, which behind an image are not the plan's);
     slot_mapping and caches as in ``write_paged_kv``.  Returns the rotated queries
     (T, Hq, D); those of tokens without a slot too.
     """
