@@ -796,6 +796,23 @@ def test_refusals_on_the_gpu():
     assert paged_decode_attention(q.detach()[:0], kc, vc, table[:0], lens[:0]).shape == (0, 2, 64)
 
 
+def test_rotation_has_no_backward():
+    """Each tensor of the rotation that wants a gradient is refused; without grad mode it runs."""
+    note("rotation, gradients")
+    g = gen(4)
+    q, k = (torch.randn(1, 2, 5, 64, generator=g).to(DEV) for _ in range(2))
+    w = torch.ones(64, device=DEV)
+    args = [q, k, torch.arange(5, device=DEV), freqs(64).to(DEV), w, w]
+    want = qk_norm_rope(*args)
+    for i in (0, 1, 3, 4, 5):
+        some = [a.clone().requires_grad_() if i == j else a for j, a in enumerate(args)]
+        with pytest.raises(NotImplementedError, match="no backward"):
+            qk_norm_rope(*some)
+        with torch.no_grad():
+            got = qk_norm_rope(*some)
+        assert all(torch.equal(a, b) and not a.requires_grad for a, b in zip(got, want))
+
+
 def test_writes_are_seen_by_autograd():
     """A cache that a graph saved for its backward pass and that a call wrote is not used by it."""
     note("versions")
