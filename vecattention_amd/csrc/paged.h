@@ -1,6 +1,6 @@
 // Index arithmetic of the paged key-value cache, shared by the plan, the cache
 // writes and the decode attention.  Host code compiles it too
-// (tests/test_paged_index.py runs it there).
+// (tests/test_paged_host.py runs it there).
 //
 // A cache holds num_pages pages of page_size slots; slot s is row s % page_size
 // of page s / page_size.  Row i of a block table lists the pages of request i in

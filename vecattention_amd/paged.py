@@ -11,6 +11,7 @@ and generated tokens alike:
    (``VecAttention_prefill``) wants the keys too, or ``qk_norm_rope_to_cache``
    for generated tokens;
 3. ``paged_decode_attention``: one new token of every request over its pages.
+   No operator attends from several new tokens of a request over its pages.
 
 A cache is (num_pages, page_size, num_kv_heads, head_dim) with kv_layout "NHD",
 (num_pages, num_kv_heads, page_size, head_dim) with "HND"; any strides with
@@ -99,7 +100,9 @@ def paged_decode_attention(q, k_cache, v_cache, block_tables, kv_lens, kv_layout
     num_kv_heads), zeros where kv_lens is 0 (or less).
 
     A request whose length exceeds its table's M pages, or whose table names a
-    page that the cache does not have, gives NaN.
+    page that the cache does not have, gives NaN.  Which form of the kernel runs
+    goes by M: tables cut to the step's longest request (``block_tables[:, :m]``)
+    are the faster ones for short requests.
     """
     return nat.host_call("decode", q, q, k_cache, v_cache, block_tables, kv_lens, kv_layout,
                          sm_scale)

@@ -19,7 +19,8 @@ def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e
     tensors in the same order of dimensions.
 
     q_weight, k_weight: (D,) norm weights in q's dtype or fp32 (None: no norm):
-    x * rsqrt(mean(x^2) + eps) * w over each head's row.
+    x * rsqrt(mean(x^2) + eps) * w over each head's row (a norm over the features of
+    all heads together is the caller's, who then passes no weights).
     positions: integers (B, S) or (S,), or with ``mrope_section`` (its entries
     are the frequencies that each position axis turns, at most four axes)
     (axes, B, S) or (axes, S).  inv_freq: fp32 (rotary_dim / 2,); features from
