@@ -513,6 +513,112 @@ int va_paged_decode_attn(int dtype, const void* q, int64_t sqn, int64_t sqh, con
                          int64_t page_size, int64_t num_pages, float softmax_scale,
                          void* workspace, int64_t workspace_bytes, void* stream);
 
+/*
+ * Rows that share pages: several answers to one prompt, the beams of a search.
+ * page_shares[p] (int32, one for each of the cache's num_pages pages) counts the
+ * rows that hold page p beyond the first: 0 for a page that one row holds and for
+ * a free one, so zeros are where a pool begins, and va_paged_plan, which takes
+ * pages of the free list, leaves it as it is.
+ *
+ * va_paged_fork: R rows of the next step from N rows of this one.  Row r goes on
+ * from row parents[r]: its length is min(kv_lens, keep_lens[r]) (keep_lens NULL:
+ * kv_lens; negative counts as 0) and its pages are that row's; a parent outside
+ * [0, N) makes an empty row.  Rows may have many children or none.  Entries of
+ * block_tables_out (R, M) behind a row's pages are -1.
+ * A row that ends inside a page that others hold too would write to theirs.  It
+ * gets a page of its own (the first of several such rows keeps the page if no
+ * other row holds it): copy_src[r], copy_dst[r] and copy_rows[r], its tokens in
+ * that page, say what va_copy_paged_kv has to copy; they are -1, -1 and 0 for the
+ * others.
+ * Pages whose last row went return to the free list: with head = *free_head (NULL:
+ * 0) within [0, num_free] and f freed pages, these take the entries from head - f
+ * on in ascending order, and the copies' pages are taken from there, in the order
+ * of the rows.  free_pages_out is the list after that and *free_head_out its first
+ * free entry.  Where the list ends, copy_dst and the table's entry are -1 and
+ * *free_head_out exceeds num_free; freed pages that would lie before entry 0 are
+ * dropped (a list with an entry for every page has room for all).  Entries that
+ * are not in [0, num_pages) are no pages: they are handed on, and counted nowhere.
+ * Results do not overlap the inputs.  N and R up to 65536.  workspace: of
+ * va_paged_fork_workspace_size bytes, 16-byte aligned.
+ */
+int64_t va_paged_fork_workspace_size(int64_t R, int64_t num_pages);
+int va_paged_fork(const int32_t* kv_lens, const int32_t* keep_lens, const int32_t* parents,
+                  int64_t N, int64_t R, const int32_t* block_tables, int64_t stn, int64_t M,
+                  const int32_t* page_shares, int64_t num_pages, const int32_t* free_pages,
+                  int64_t num_free, const int32_t* free_head, int64_t page_size,
+                  int32_t* kv_lens_out, int32_t* block_tables_out, int32_t* page_shares_out,
+                  int32_t* free_pages_out, int32_t* free_head_out, int32_t* copy_src,
+                  int32_t* copy_dst, int32_t* copy_rows, void* workspace, int64_t workspace_bytes,
+                  void* stream);
+
+/*
+ * The pages in use moved to the lowest numbers.  Of the pages that the tables'
+ * rows hold (t of them) and those of the free list from *free_head on, in
+ * ascending order, the first t are to be the tables': page copy_src[i] moves to
+ * page copy_dst[i] (both ascending; num_pages / 2 entries, -1 behind the
+ * *num_moves ones), which va_copy_paged_kv does.  Pages in neither place are not
+ * touched.  Results: tables with the new numbers (what is no page stays), the
+ * shares moved along, the free pages in ascending order at the list's end, and the
+ * first of them.  workspace: of va_paged_compact_workspace_size bytes, 16-byte
+ * aligned.
+ */
+int64_t va_paged_compact_workspace_size(int64_t num_pages);
+int va_paged_compact(const int32_t* kv_lens, int64_t N, const int32_t* block_tables, int64_t stn,
+                     int64_t M, const int32_t* page_shares, int64_t num_pages,
+                     const int32_t* free_pages, int64_t num_free, const int32_t* free_head,
+                     int64_t page_size, int32_t* block_tables_out, int32_t* page_shares_out,
+                     int32_t* free_pages_out, int32_t* free_head_out, int32_t* copy_src,
+                     int32_t* copy_dst, int32_t* num_moves, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
+/*
+ * Page src_pages[i] to page dst_pages[i] for i < C, in the key and the value cache
+ * of each of `layers` layers (host arrays of pointers; one set of strides for the
+ * keys and one for the values): its first rows[i] rows (NULL: all; at most
+ * page_size), the others stay as they are.  An entry with a page outside [0,
+ * num_pages) copies nothing.  The pages copied to are distinct and none of those
+ * copied from.
+ */
+int va_copy_paged_kv(int dtype, void* const* k_caches, void* const* v_caches, int64_t layers,
+                     int64_t skp, int64_t skn, int64_t skh, int64_t svp, int64_t svn, int64_t svh,
+                     int64_t num_pages, int64_t page_size, int64_t Hk, int64_t D,
+                     const int32_t* src_pages, const int32_t* dst_pages, const int32_t* rows,
+                     int64_t C, void* stream);
+
+/*
+ * Which rows begin with the same pages.  A group is a run of rows that hold tokens
+ * and have the same group_ids (NULL: the same first page).  prefix_lens[n]: tokens
+ * of the whole pages that all rows of n's group begin with, 0 in a group of one;
+ * group_rows[n]: the rows of the group that begins at row n, 0 where none with a
+ * shared prefix does.  N up to 65536.  workspace: of
+ * va_paged_prefix_workspace_size bytes, 16-byte aligned.
+ */
+int64_t va_paged_prefix_workspace_size(int64_t N);
+int va_paged_prefix(const int32_t* kv_lens, int64_t N, const int32_t* block_tables, int64_t stn,
+                    int64_t M, const int32_t* group_ids, int64_t page_size, int32_t* prefix_lens,
+                    int32_t* group_rows, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * va_paged_decode_attn for rows in groups that share their first pages
+ * (prefix_lens and group_rows as va_paged_prefix makes them, from these tables):
+ * the same results, but the keys of a group's prefix are read once for all of its
+ * rows, through the table of the group's first row.  Rows of a group have to hold
+ * prefix_lens tokens at least and list the same pages for them.  workspace: of
+ * va_paged_prefix_decode_workspace_size() bytes (-1: sizes that are not
+ * supported), 16-byte aligned; calls that may overlap need one each.
+ */
+int64_t va_paged_prefix_decode_workspace_size(int dtype, int64_t N, int64_t Hq, int64_t Hk,
+                                              int64_t D, int64_t M, int64_t page_size);
+int va_paged_prefix_decode_attn(int dtype, const void* q, int64_t sqn, int64_t sqh,
+                                const void* k_cache, int64_t skp, int64_t skn, int64_t skh,
+                                const void* v_cache, int64_t svp, int64_t svn, int64_t svh,
+                                void* out, int64_t son, int64_t soh, const int32_t* block_tables,
+                                int64_t stn, int64_t M, const int32_t* kv_lens,
+                                const int32_t* prefix_lens, const int32_t* group_rows, int64_t N,
+                                int64_t Hq, int64_t Hk, int64_t D, int64_t page_size,
+                                int64_t num_pages, float softmax_scale, void* workspace,
+                                int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,7 +10,9 @@ from .dispatch import (DiffusionStepContext, FastPrefillConfig, Full_prefill,
 from .tuner import seg_pr_perHead
 from .decode import single_decode_with_kv_cache
 from .rotary import qk_norm_rope
-from .paged import (PagedStep, paged_decode_attention, paged_kv_plan, qk_norm_rope_to_cache,
+from .paged import (PagedCompaction, PagedFork, PagedStep, SharedPrefix, copy_paged_kv,
+                    paged_decode_attention, paged_kv_compact, paged_kv_fork, paged_kv_plan,
+                    paged_kv_prefix, paged_prefix_decode_attention, qk_norm_rope_to_cache,
                     write_paged_kv)
 
 __all__ = [
@@ -31,4 +33,12 @@ __all__ = [
     "write_paged_kv",
     "qk_norm_rope_to_cache",
     "paged_decode_attention",
+    "PagedFork",
+    "paged_kv_fork",
+    "PagedCompaction",
+    "paged_kv_compact",
+    "copy_paged_kv",
+    "SharedPrefix",
+    "paged_kv_prefix",
+    "paged_prefix_decode_attention",
 ]

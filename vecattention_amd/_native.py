@@ -108,6 +108,21 @@ SIGNATURES = {
     "va_paged_decode_attn": (_int, [_int, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64,
                                     _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
                                     _i64, _i64, _i64, _i64, _f32, _vp, _i64, _vp]),
+    "va_paged_fork_workspace_size": (_i64, [_i64, _i64]),
+    "va_paged_fork": (_int, [_vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64,
+                             _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "va_paged_compact_workspace_size": (_i64, [_i64]),
+    "va_paged_compact": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp,
+                                _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "va_copy_paged_kv": (_int, [_int, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp]),
+    "va_paged_prefix_workspace_size": (_i64, [_i64]),
+    "va_paged_prefix": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp]),
+    "va_paged_prefix_decode_workspace_size": (_i64, [_int, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "va_paged_prefix_decode_attn": (_int, [_int, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp,
+                                           _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
+                                           _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64,
+                                           _f32, _vp, _i64, _vp]),
 }
 
 

@@ -21,6 +21,8 @@
 #include <cstdarg>
 #include <cstdio>
 #include <string>
+#include <utility>
+#include <vector>
 
 #include "../../include/vecattn.h"
 
@@ -448,7 +450,14 @@ PyObject* write_kv(PyObject* const* a) {
   Py_RETURN_NONE;
 }
 
-PyObject* decode(PyObject* const* a) {
+// Rows of a table, read: stride 1 within a row.
+at::Tensor table_rows(const at::Tensor& t) {
+  return t.size(1) > 1 && t.stride(1) != 1 ? t.contiguous() : t;
+}
+
+// Both decode attentions.  `prefix`: the second's two vectors, or null.
+at::Tensor attend(const char* what, PyObject* const* a, const at::Tensor* prefix,
+                  PyObject* layout, PyObject* sm_scale, PyObject* stream) {
   const at::Tensor &q_ = tensor(a[0], "q"), &kc = tensor(a[1], "k_cache"),
                    &vc = tensor(a[2], "v_cache"), &table_ = tensor(a[3], "block_tables"),
                    &lens_ = tensor(a[4], "kv_lens");
@@ -456,7 +465,7 @@ PyObject* decode(PyObject* const* a) {
     refuse(PyExc_ValueError, "q must be (requests, num_qo_heads, head_dim)");
   const int64_t N = q_.size(0), Hq = q_.size(1), D = q_.size(2);
   const int dtype = dtype_code(q_);
-  const Cache c(kc, vc, a[5], D, q_.scalar_type());
+  const Cache c(kc, vc, layout, D, q_.scalar_type());
   if (c.heads == 0 || Hq % c.heads)
     refuse(PyExc_ValueError, "num_qo_heads %lld is not a multiple of num_kv_heads %lld",
            (long long)Hq, (long long)c.heads);
@@ -465,28 +474,243 @@ PyObject* decode(PyObject* const* a) {
            shape(table_).c_str(), shape(lens_).c_str(), (long long)N);
   if (table_.scalar_type() != at::kInt || lens_.scalar_type() != at::kInt)
     refuse(PyExc_TypeError, "block_tables and kv_lens must be int32");
+  at::Tensor shared[2];
+  if (prefix) {
+    for (int i = 0; i < 2; ++i) {
+      if (prefix[i].dim() != 1 || prefix[i].size(0) != N)
+        refuse(PyExc_ValueError, "prefix_lens and group_rows must be of (%lld,)", (long long)N);
+      if (prefix[i].scalar_type() != at::kInt)
+        refuse(PyExc_TypeError, "prefix_lens and group_rows must be int32");
+      shared[i] = prefix[i].contiguous();
+    }
+  }
   const auto inputs = {&q_, &kc, &vc};
-  no_tangent("paged_decode_attention", inputs);
-  one_gpu("paged_decode_attention", {&q_, &kc, &vc, &table_, &lens_});
-  no_backward("paged_decode_attention", inputs);
+  no_tangent(what, inputs);
+  one_gpu(what, {&q_, &kc, &vc, &table_, &lens_, &shared[0], &shared[1]});
+  no_backward(what, inputs);
   const int64_t M = table_.size(1);
-  const at::Tensor q = rows(q_), lens = lens_.contiguous(),
-                   table = M > 1 && table_.stride(1) != 1 ? table_.contiguous() : table_;
-  const double scale = a[6] == Py_None ? 1.0 / std::sqrt(double(D)) : real(a[6]);
+  const at::Tensor q = rows(q_), lens = lens_.contiguous(), table = table_rows(table_);
+  const double scale = sm_scale == Py_None ? 1.0 / std::sqrt(double(D)) : real(sm_scale);
   const at::Tensor out = at::empty({N, Hq, D}, q.options());
-  if (N && Hq && D) {
-    int64_t bytes = va_paged_decode_workspace_size(dtype, N, Hq, c.heads, D, M, c.page);
-    if (bytes < 16) bytes = 16;
-    const at::Tensor work = at::empty({bytes}, q.options().dtype(at::kByte));
+  if (!N || !Hq || !D) return out;
+  int64_t bytes =
+      prefix ? va_paged_prefix_decode_workspace_size(dtype, N, Hq, c.heads, D, M, c.page)
+             : va_paged_decode_workspace_size(dtype, N, Hq, c.heads, D, M, c.page);
+  if (bytes < 16) bytes = 16;
+  const at::Tensor work = at::empty({bytes}, q.options().dtype(at::kByte));
+  int32_t* entries = static_cast<int32_t*>(table.data_ptr());
+  int32_t* counts = static_cast<int32_t*>(lens.data_ptr());
+  void* on = reinterpret_cast<void*>(integer(stream));
+  if (prefix)
+    check("va_paged_prefix_decode_attn",
+          va_paged_prefix_decode_attn(
+              dtype, q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), c.k[0], c.k[1], c.k[2],
+              vc.data_ptr(), c.v[0], c.v[1], c.v[2], out.data_ptr(), Hq * D, D, entries,
+              table.stride(0), M, counts, static_cast<int32_t*>(shared[0].data_ptr()),
+              static_cast<int32_t*>(shared[1].data_ptr()), N, Hq, c.heads, D, c.page, c.pages,
+              float(scale), work.data_ptr(), bytes, on));
+  else
     check("va_paged_decode_attn",
           va_paged_decode_attn(dtype, q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(),
                                c.k[0], c.k[1], c.k[2], vc.data_ptr(), c.v[0], c.v[1], c.v[2],
-                               out.data_ptr(), Hq * D, D, static_cast<int32_t*>(table.data_ptr()),
-                               table.stride(0), M, static_cast<int32_t*>(lens.data_ptr()), N, Hq,
-                               c.heads, D, c.page, c.pages, float(scale), work.data_ptr(), bytes,
-                               reinterpret_cast<void*>(integer(a[7]))));
+                               out.data_ptr(), Hq * D, D, entries, table.stride(0), M, counts, N,
+                               Hq, c.heads, D, c.page, c.pages, float(scale), work.data_ptr(),
+                               bytes, on));
+  return out;
+}
+
+PyObject* decode(PyObject* const* a) {
+  return THPVariable_Wrap(attend("paged_decode_attention", a, nullptr, a[5], a[6], a[7]));
+}
+
+PyObject* prefix_decode(PyObject* const* a) {
+  const at::Tensor prefix[2] = {tensor(a[5], "prefix_lens"), tensor(a[6], "group_rows")};
+  return THPVariable_Wrap(attend("paged_prefix_decode_attention", a, prefix, a[7], a[8], a[9]));
+}
+
+// Tables, lengths and the pool of pages of the calls that share them, checked.
+struct Pool {
+  at::Tensor lens, table, shares, free, head;
+  int64_t N, M, P, F, page;
+  Pool(const char* what, const at::Tensor& lens_, const at::Tensor& table_,
+       const at::Tensor& shares_, const at::Tensor& free_, PyObject* page_size,
+       const at::Tensor& head_) {
+    if (lens_.dim() != 1) refuse(PyExc_ValueError, "kv_lens must be a vector");
+    N = lens_.size(0);
+    if (table_.dim() != 2 || table_.size(0) != N)
+      refuse(PyExc_ValueError, "block_tables %s: expected (%lld, pages)", shape(table_).c_str(),
+             (long long)N);
+    if (shares_.dim() != 1 || free_.dim() != 1)
+      refuse(PyExc_ValueError, "page_shares and free_pages must be vectors");
+    if (head_.defined() && head_.numel() != 1)
+      refuse(PyExc_ValueError, "free_head must have one element");
+    for (const at::Tensor* t : {&lens_, &table_, &shares_, &free_, &head_})
+      if (t->defined() && t->scalar_type() != at::kInt)
+        refuse(PyExc_TypeError,
+               "lengths, block_tables, page_shares, free_pages and free_head must be int32");
+    page = integer(page_size);
+    if (page <= 0) refuse(PyExc_ValueError, "page_size %lld", (long long)page);
+    one_gpu(what, {&table_, &lens_, &shares_, &free_, &head_});
+    M = table_.size(1);
+    P = shares_.size(0);
+    F = free_.size(0);
+    lens = lens_.contiguous();
+    table = table_rows(table_);
+    shares = shares_.contiguous();
+    free = free_.contiguous();
+    head = head_;
   }
-  return THPVariable_Wrap(out);
+};
+int32_t* ints(const at::Tensor& t) { return static_cast<int32_t*>(address(t)); }
+
+PyObject* tuple_of(const at::Tensor* t, int n) {
+  PyObject* tuple = PyTuple_New(n);
+  if (!tuple) throw Refused{nullptr, ""};
+  for (int i = 0; i < n; ++i) PyTuple_SET_ITEM(tuple, i, THPVariable_Wrap(t[i]));
+  return tuple;
+}
+
+PyObject* fork(PyObject* const* a) {
+  const at::Tensor &parents_ = tensor(a[1], "parents"), keep_ = maybe(a[7], "keep_lens");
+  if (parents_.dim() != 1) refuse(PyExc_ValueError, "parents must be a vector");
+  const int64_t R = parents_.size(0);
+  if (keep_.defined() && (keep_.dim() != 1 || keep_.size(0) != R))
+    refuse(PyExc_ValueError, "keep_lens must have an entry for each of the %lld parents",
+           (long long)R);
+  for (const at::Tensor* t : {&parents_, &keep_})
+    if (t->defined() && t->scalar_type() != at::kInt)
+      refuse(PyExc_TypeError, "parents and keep_lens must be int32");
+  const Pool p("paged_kv_fork", tensor(a[0], "kv_lens"), tensor(a[2], "block_tables"),
+               tensor(a[3], "page_shares"), tensor(a[4], "free_pages"), a[5],
+               maybe(a[6], "free_head"));
+  one_gpu("paged_kv_fork", {&p.table, &parents_, &keep_});
+  const at::Tensor parents = parents_.contiguous();
+  const at::Tensor keep = keep_.defined() ? keep_.contiguous() : keep_;
+  // Of the rows, and of the pages: what one keeps does not hold the other's memory.
+  at::Tensor of_rows[5], of_pages[3], out[8];
+  together({{at::kInt, R}, {at::kInt, R}, {at::kInt, R}, {at::kInt, R}, {at::kInt, R * p.M}},
+           p.table.options(), of_rows);
+  together({{at::kInt, p.P}, {at::kInt, p.F}, {at::kInt, 1}}, p.table.options(), of_pages);
+  out[0] = of_rows[0];
+  out[1] = of_rows[4].view({R, p.M});
+  for (int i = 0; i < 3; ++i) out[2 + i] = of_pages[i];
+  for (int i = 0; i < 3; ++i) out[5 + i] = of_rows[1 + i];
+  const int64_t bytes = va_paged_fork_workspace_size(R, p.P);
+  const at::Tensor work = at::empty({bytes}, p.table.options().dtype(at::kByte));
+  check("va_paged_fork",
+        va_paged_fork(ints(p.lens), ints(keep), ints(parents), p.N, R, ints(p.table),
+                      p.table.stride(0), p.M, ints(p.shares), p.P, ints(p.free), p.F,
+                      ints(p.head), p.page, ints(out[0]), ints(out[1]), ints(out[2]),
+                      ints(out[3]), ints(out[4]), ints(out[5]), ints(out[6]), ints(out[7]),
+                      work.data_ptr(), bytes, reinterpret_cast<void*>(integer(a[8]))));
+  return tuple_of(out, 8);
+}
+
+PyObject* compact(PyObject* const* a) {
+  const Pool p("paged_kv_compact", tensor(a[0], "kv_lens"), tensor(a[1], "block_tables"),
+               tensor(a[2], "page_shares"), tensor(a[3], "free_pages"), a[4],
+               maybe(a[5], "free_head"));
+  const int64_t half = p.P / 2;
+  at::Tensor moves[3], of_pages[3], out[7];
+  together({{at::kInt, half}, {at::kInt, half}, {at::kInt, 1}}, p.table.options(), moves);
+  together({{at::kInt, p.P}, {at::kInt, p.F}, {at::kInt, 1}}, p.table.options(), of_pages);
+  out[0] = at::empty({p.N, p.M}, p.table.options());
+  for (int i = 0; i < 3; ++i) out[1 + i] = of_pages[i];
+  for (int i = 0; i < 3; ++i) out[4 + i] = moves[i];
+  const int64_t bytes = va_paged_compact_workspace_size(p.P);
+  const at::Tensor work = at::empty({bytes}, p.table.options().dtype(at::kByte));
+  check("va_paged_compact",
+        va_paged_compact(ints(p.lens), p.N, ints(p.table), p.table.stride(0), p.M, ints(p.shares),
+                         p.P, ints(p.free), p.F, ints(p.head), p.page, ints(out[0]), ints(out[1]),
+                         ints(out[2]), ints(out[3]), ints(out[4]), ints(out[5]), ints(out[6]),
+                         work.data_ptr(), bytes, reinterpret_cast<void*>(integer(a[6]))));
+  return tuple_of(out, 7);
+}
+
+PyObject* prefix(PyObject* const* a) {
+  const at::Tensor &lens_ = tensor(a[0], "kv_lens"), &table_ = tensor(a[1], "block_tables");
+  const at::Tensor ids_ = maybe(a[3], "group_ids");
+  if (lens_.dim() != 1) refuse(PyExc_ValueError, "kv_lens must be a vector");
+  const int64_t N = lens_.size(0);
+  if (table_.dim() != 2 || table_.size(0) != N)
+    refuse(PyExc_ValueError, "block_tables %s: expected (%lld, pages)", shape(table_).c_str(),
+           (long long)N);
+  if (ids_.defined() && (ids_.dim() != 1 || ids_.size(0) != N))
+    refuse(PyExc_ValueError, "group_ids must be of (%lld,)", (long long)N);
+  for (const at::Tensor* t : {&lens_, &table_, &ids_})
+    if (t->defined() && t->scalar_type() != at::kInt)
+      refuse(PyExc_TypeError, "kv_lens, block_tables and group_ids must be int32");
+  const int64_t page = integer(a[2]);
+  if (page <= 0) refuse(PyExc_ValueError, "page_size %lld", (long long)page);
+  one_gpu("paged_kv_prefix", {&table_, &lens_, &ids_});
+  const at::Tensor lens = lens_.contiguous(), table = table_rows(table_);
+  const at::Tensor ids = ids_.defined() ? ids_.contiguous() : ids_;
+  at::Tensor out[2];
+  together({{at::kInt, N}, {at::kInt, N}}, table.options(), out);
+  int64_t bytes = va_paged_prefix_workspace_size(N);
+  if (bytes < 16) bytes = 16;
+  const at::Tensor work = at::empty({bytes}, table.options().dtype(at::kByte));
+  check("va_paged_prefix",
+        va_paged_prefix(ints(lens), N, ints(table), table.stride(0), table.size(1), ints(ids),
+                        page, ints(out[0]), ints(out[1]), work.data_ptr(), bytes,
+                        reinterpret_cast<void*>(integer(a[4]))));
+  return tuple_of(out, 2);
+}
+
+// The caches of all layers: a tensor, or a list or tuple of tensors.
+std::vector<at::Tensor> layers(PyObject* o, const char* what) {
+  std::vector<at::Tensor> all;
+  if (THPVariable_Check(o)) {
+    all.push_back(THPVariable_Unpack(o));
+    return all;
+  }
+  if (!PyList_Check(o) && !PyTuple_Check(o))
+    refuse(PyExc_TypeError, "%s must be a tensor, or a list or tuple of tensors", what);
+  for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(o); ++i)
+    all.push_back(tensor(PySequence_Fast_GET_ITEM(o, i), what));
+  return all;
+}
+
+PyObject* copy(PyObject* const* a) {
+  const std::vector<at::Tensor> kc = layers(a[0], "k_caches"), vc = layers(a[1], "v_caches");
+  const at::Tensor &src_ = tensor(a[2], "src_pages"), &dst_ = tensor(a[3], "dst_pages");
+  const at::Tensor rows_ = maybe(a[4], "rows");
+  if (kc.empty() || kc.size() != vc.size())
+    refuse(PyExc_ValueError, "%zu k_caches and %zu v_caches", kc.size(), vc.size());
+  if (src_.dim() != 1 || dst_.sizes() != src_.sizes() ||
+      (rows_.defined() && rows_.sizes() != src_.sizes()))
+    refuse(PyExc_ValueError, "src_pages, dst_pages and rows must be vectors of one length");
+  for (const at::Tensor* t : {&src_, &dst_, &rows_})
+    if (t->defined() && t->scalar_type() != at::kInt)
+      refuse(PyExc_TypeError, "src_pages, dst_pages and rows must be int32");
+  const int dtype = dtype_code(kc[0]);
+  if (kc[0].dim() != 4)
+    refuse(PyExc_ValueError, "k_caches must be 4-dimensional, not %s", shape(kc[0]).c_str());
+  const int64_t D = kc[0].size(3);
+  const Cache c(kc[0], vc[0], a[5], D, kc[0].scalar_type());
+  for (size_t i = 0; i < kc.size(); ++i)
+    for (const auto& t : {std::make_pair(&kc[i], &kc[0]), std::make_pair(&vc[i], &vc[0])})
+      if (t.first->scalar_type() != t.second->scalar_type() ||
+          t.first->sizes() != t.second->sizes() || t.first->strides() != t.second->strides())
+        refuse(PyExc_ValueError, "the caches of all layers must have one shape, type and strides");
+  std::vector<void*> k, v;
+  for (size_t i = 0; i < kc.size(); ++i) {
+    no_tangent("copy_paged_kv", {&kc[i], &vc[i]});
+    one_gpu("copy_paged_kv", {&kc[0], &kc[i], &vc[i], &src_, &dst_, &rows_});
+    no_backward("copy_paged_kv", {&kc[i], &vc[i]});
+    k.push_back(kc[i].data_ptr());
+    v.push_back(vc[i].data_ptr());
+  }
+  const at::Tensor src = src_.contiguous(), dst = dst_.contiguous();
+  const at::Tensor rows = rows_.defined() ? rows_.contiguous() : rows_;
+  if (src.size(0) && c.heads && D)
+    check("va_copy_paged_kv",
+          va_copy_paged_kv(dtype, k.data(), v.data(), int64_t(k.size()), c.k[0], c.k[1], c.k[2],
+                           c.v[0], c.v[1], c.v[2], c.pages, c.page, c.heads, D, ints(src),
+                           ints(dst), ints(rows), src.size(0),
+                           reinterpret_cast<void*>(integer(a[6]))));
+  for (size_t i = 0; i < kc.size(); ++i) written({&kc[i], &vc[i]});
+  Py_RETURN_NONE;
 }
 
 template <PyObject* (*f)(PyObject* const*), Py_ssize_t count>
@@ -514,6 +738,11 @@ PyMethodDef methods[] = {method<plan, 8>("plan"),
                          method<rope_to_cache, 16>("rope_to_cache"),
                          method<write_kv, 7>("write_kv"),
                          method<decode, 8>("decode"),
+                         method<prefix_decode, 10>("prefix_decode"),
+                         method<fork, 9>("fork"),
+                         method<compact, 7>("compact"),
+                         method<prefix, 5>("prefix"),
+                         method<copy, 7>("copy"),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "vecattention_amd._host", nullptr, -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

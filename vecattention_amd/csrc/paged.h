@@ -45,6 +45,21 @@ struct PlanRow {
   }
 };
 
+// Pages that `len` tokens take of a table of `width` entries.
+__host__ __device__ inline uint32_t held_pages(int32_t len, uint32_t page, uint32_t width) {
+  if (len <= 0) return 0;
+  const uint32_t n = uint32_t(len) / page + (uint32_t(len) % page != 0);
+  return n < width ? n : width;
+}
+// The entry whose page holds tokens and has room for more, or -1: where a row's
+// next token goes beside some of its own.
+__host__ __device__ inline int64_t open_page(int32_t len, uint32_t page, uint32_t width) {
+  if (len <= 0 || uint32_t(len) % page == 0) return -1;
+  const uint32_t at = uint32_t(len) / page;
+  return at < width ? int64_t(at) : -1;
+}
+__host__ __device__ inline bool is_page(int32_t id, int64_t pages) { return id >= 0 && id < pages; }
+
 // Entry `at` of the list of free pages: -1 past its ends.
 __host__ __device__ inline int32_t free_page(const int32_t* free_pages, int64_t count, int64_t at) {
   return at >= 0 && at < count ? free_pages[at] : -1;

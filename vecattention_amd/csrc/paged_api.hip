@@ -269,4 +269,178 @@ int va_paged_decode_attn(int dtype, const void* q, int64_t sqn, int64_t sqh, con
                   "paged decode launch");
 }
 
+constexpr int64_t kMostGroups = int64_t(1) << 23;
+
+// Sizes of tables, lists and counts that the kernels take.
+static int check_share(int64_t N, int64_t R, int64_t M, int64_t P, int64_t F, int64_t page_size,
+                       int64_t stn, int64_t most) {
+  if (N < 0 || R < 0 || M < 0 || P < 0 || F < 0) return api_error(VA_ERR_ARG, "negative size");
+  if (page_size <= 0 || page_size >= kInt31)
+    return api_error(VA_ERR_ARG, "page_size %lld", (long long)page_size);
+  if (N > most || R > most)
+    return api_error(VA_ERR_UNSUPPORTED, "more than %lld rows", (long long)most);
+  if (M >= kInt31 || P >= kInt31 || F >= kInt31)
+    return api_error(VA_ERR_UNSUPPORTED, "sizes of 2^31 or more");
+  // A work-group for every 1024 entries of a row: a launch takes fewer than 2^32 threads.
+  if (!fits(N + R, M / 1024 + 1, kMostGroups))
+    return api_error(VA_ERR_UNSUPPORTED, "tables of 2^33 entries or more");
+  if (stn < 0) return api_error(VA_ERR_ARG, "negative stride");
+  return VA_OK;
+}
+static int check_workspace(const char* what, const void* workspace, int64_t bytes, int64_t need) {
+  if (need && (!workspace || bytes < need))
+    return api_error(VA_ERR_WORKSPACE, "%s needs %lld workspace bytes", what, (long long)need);
+  if (need && reinterpret_cast<uintptr_t>(workspace) % 16)
+    return api_error(VA_ERR_ARG, "workspace must be 16-byte aligned");
+  return VA_OK;
+}
+
+int64_t va_paged_fork_workspace_size(int64_t R, int64_t num_pages) {
+  return R < 0 || num_pages < 0 ? -1 : va::fork_workspace_bytes(R, num_pages);
+}
+
+int va_paged_fork(const int32_t* kv_lens, const int32_t* keep_lens, const int32_t* parents,
+                  int64_t N, int64_t R, const int32_t* block_tables, int64_t stn, int64_t M,
+                  const int32_t* page_shares, int64_t num_pages, const int32_t* free_pages,
+                  int64_t num_free, const int32_t* free_head, int64_t page_size,
+                  int32_t* kv_lens_out, int32_t* block_tables_out, int32_t* page_shares_out,
+                  int32_t* free_pages_out, int32_t* free_head_out, int32_t* copy_src,
+                  int32_t* copy_dst, int32_t* copy_rows, void* workspace, int64_t workspace_bytes,
+                  void* stream) {
+  if (const int rc =
+          check_share(N, R, M, num_pages, num_free, page_size, stn, va::kForkMostRows))
+    return rc;
+  if (!free_head_out || (N && !kv_lens) || (N && M && !block_tables) ||
+      (R && (!parents || !kv_lens_out || !copy_src || !copy_dst || !copy_rows)) ||
+      (R && M && !block_tables_out) || (num_pages && (!page_shares || !page_shares_out)) ||
+      (num_free && (!free_pages || !free_pages_out)))
+    return api_error(VA_ERR_ARG, "null pointer");
+  const int64_t need = va::fork_workspace_bytes(R, num_pages);
+  if (const int rc = check_workspace("the fork", workspace, workspace_bytes, need)) return rc;
+  const va::ForkArgs a{kv_lens,          keep_lens,       parents,        block_tables,
+                       stn,              N,               R,              M,
+                       page_shares,      num_pages,       free_pages,     num_free,
+                       free_head,        uint32_t(page_size), kv_lens_out, block_tables_out,
+                       page_shares_out,  free_pages_out,  free_head_out,  copy_src,
+                       copy_dst,         copy_rows};
+  return launched(va::launch_paged_fork(a, workspace, static_cast<hipStream_t>(stream)),
+                  "fork launch");
+}
+
+int64_t va_paged_compact_workspace_size(int64_t num_pages) {
+  return num_pages < 0 ? -1 : va::compact_workspace_bytes(num_pages);
+}
+
+int va_paged_compact(const int32_t* kv_lens, int64_t N, const int32_t* block_tables, int64_t stn,
+                     int64_t M, const int32_t* page_shares, int64_t num_pages,
+                     const int32_t* free_pages, int64_t num_free, const int32_t* free_head,
+                     int64_t page_size, int32_t* block_tables_out, int32_t* page_shares_out,
+                     int32_t* free_pages_out, int32_t* free_head_out, int32_t* copy_src,
+                     int32_t* copy_dst, int32_t* num_moves, void* workspace,
+                     int64_t workspace_bytes, void* stream) {
+  if (const int rc = check_share(N, 0, M, num_pages, num_free, page_size, stn, kMostGroups))
+    return rc;
+  if (!free_head_out || !num_moves || (N && !kv_lens) ||
+      (N && M && (!block_tables || !block_tables_out)) ||
+      (num_pages && (!page_shares || !page_shares_out)) ||
+      (num_pages > 1 && (!copy_src || !copy_dst)) ||
+      (num_free && (!free_pages || !free_pages_out)))
+    return api_error(VA_ERR_ARG, "null pointer");
+  const int64_t need = va::compact_workspace_bytes(num_pages);
+  if (const int rc = check_workspace("the compaction", workspace, workspace_bytes, need))
+    return rc;
+  const va::CompactArgs a{kv_lens,    block_tables,  stn,        N,
+                          M,          page_shares,   num_pages,  free_pages,
+                          num_free,   free_head,     uint32_t(page_size), block_tables_out,
+                          page_shares_out, free_pages_out, free_head_out, copy_src,
+                          copy_dst,   num_moves};
+  return launched(va::launch_paged_compact(a, workspace, static_cast<hipStream_t>(stream)),
+                  "compaction launch");
+}
+
+int64_t va_paged_prefix_workspace_size(int64_t N) {
+  return N < 0 ? -1 : va::prefix_workspace_bytes(N);
+}
+
+int va_paged_prefix(const int32_t* kv_lens, int64_t N, const int32_t* block_tables, int64_t stn,
+                    int64_t M, const int32_t* group_ids, int64_t page_size, int32_t* prefix_lens,
+                    int32_t* group_rows, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (const int rc = check_share(N, 0, M, 0, 0, page_size, stn, va::kPrefixMostRows)) return rc;
+  if (N == 0) return VA_OK;
+  if (!kv_lens || (M && !block_tables) || !prefix_lens || !group_rows)
+    return api_error(VA_ERR_ARG, "null pointer");
+  const int64_t need = va::prefix_workspace_bytes(N);
+  if (const int rc = check_workspace("the prefix", workspace, workspace_bytes, need)) return rc;
+  const va::PrefixArgs a{kv_lens, block_tables,        stn,         N,         M,
+                         group_ids, uint32_t(page_size), prefix_lens, group_rows};
+  return launched(va::launch_paged_prefix(a, workspace, static_cast<hipStream_t>(stream)),
+                  "prefix launch");
+}
+
+int va_copy_paged_kv(int dtype, void* const* k_caches, void* const* v_caches, int64_t layers,
+                     int64_t skp, int64_t skn, int64_t skh, int64_t svp, int64_t svn, int64_t svh,
+                     int64_t num_pages, int64_t page_size, int64_t Hk, int64_t D,
+                     const int32_t* src_pages, const int32_t* dst_pages, const int32_t* rows,
+                     int64_t C, void* stream) {
+  if (!dtype_ok(dtype)) return api_error(VA_ERR_ARG, "unknown dtype %d", dtype);
+  if (layers < 0 || C < 0 || Hk <= 0 || D <= 0)
+    return api_error(VA_ERR_ARG, "non-positive size");
+  if (const int rc = check_pages(num_pages, page_size)) return rc;
+  for (int64_t s : {skp, skn, skh, svp, svn, svh})
+    if (s < 0) return api_error(VA_ERR_ARG, "negative stride");
+  if (!fits(Hk, D, kInt31 - 1) || !fits(page_size, Hk * D, kInt31 - 1) || C >= kInt31 ||
+      !fits(C, page_size * Hk * D / 2048 + 1, kInt31 - 1))
+    return api_error(VA_ERR_UNSUPPORTED, "2^31 values of a page, or pieces, in a call");
+  if (layers == 0 || C == 0) return VA_OK;
+  if (!k_caches || !v_caches || !src_pages || !dst_pages)
+    return api_error(VA_ERR_ARG, "null pointer");
+  for (int64_t i = 0; i < layers; ++i)
+    if (!k_caches[i] || !v_caches[i]) return api_error(VA_ERR_ARG, "null cache pointer");
+  constexpr int64_t kMost = va::kCopyCaches / 2;
+  for (int64_t at = 0; at < layers; at += kMost) {
+    const int64_t n = layers - at < kMost ? layers - at : kMost;
+    va::CopyArgs a{};
+    for (int64_t i = 0; i < n; ++i) {
+      a.cache[i] = k_caches[at + i];
+      a.cache[n + i] = v_caches[at + i];
+    }
+    a.caches = int32_t(2 * n);
+    a.sp[0] = skp, a.sn[0] = skn, a.sh[0] = skh;
+    a.sp[1] = svp, a.sn[1] = svn, a.sh[1] = svh;
+    a.src = src_pages;
+    a.dst = dst_pages;
+    a.rows = rows;
+    a.C = C;
+    a.num_pages = num_pages;
+    a.page = int32_t(page_size);
+    a.heads = int32_t(Hk);
+    a.D = int32_t(D);
+    const int rc = launched(va::launch_copy_kv(dtype, a, static_cast<hipStream_t>(stream)),
+                            "page copy launch");
+    if (rc) return rc;
+  }
+  return VA_OK;
+}
+
+int64_t va_paged_prefix_decode_workspace_size(int dtype, int64_t N, int64_t Hq, int64_t Hk,
+                                              int64_t D, int64_t M, int64_t page_size) {
+  return va_paged_decode_workspace_size(dtype, N, Hq, Hk, D, M, page_size);
+}
+
+int va_paged_prefix_decode_attn(int dtype, const void* q, int64_t sqn, int64_t sqh,
+                                const void* k_cache, int64_t skp, int64_t skn, int64_t skh,
+                                const void* v_cache, int64_t svp, int64_t svn, int64_t svh,
+                                void* out, int64_t son, int64_t soh, const int32_t* block_tables,
+                                int64_t stn, int64_t M, const int32_t* kv_lens,
+                                const int32_t* prefix_lens, const int32_t* group_rows, int64_t N,
+                                int64_t Hq, int64_t Hk, int64_t D, int64_t page_size,
+                                int64_t num_pages, float softmax_scale, void* workspace,
+                                int64_t workspace_bytes, void* stream) {
+  if (!prefix_lens || !group_rows) return api_error(VA_ERR_ARG, "null pointer");
+  return va_paged_decode_attn(dtype, q, sqn, sqh, k_cache, skp, skn, skh, v_cache, svp, svn, svh,
+                              out, son, soh, block_tables, stn, M, kv_lens, N, Hq, Hk, D,
+                              page_size, num_pages, softmax_scale, workspace, workspace_bytes,
+                              stream);
+}
+
 }  // extern "C"

@@ -13,6 +13,65 @@ hipError_t launch_paged_plan(const int32_t* kv_lens, const int32_t* new_lens, in
                              int64_t* taken, uint32_t* workspace, hipStream_t stream);
 int64_t plan_workspace_bytes(int64_t N);
 
+// The next step's rows from this one's (paged_share.hip).
+struct ForkArgs {
+  const int32_t *kv_lens, *keep, *parents;  // (N), (R) or null, (R)
+  const int32_t* table;
+  int64_t table_stride, N, R, M;
+  const int32_t* shares;
+  int64_t P;
+  const int32_t* free_pages;
+  int64_t F;
+  const int32_t* free_head;
+  uint32_t page;
+  int32_t *kv_out, *table_out, *shares_out, *free_out, *head_out;
+  int32_t *copy_src, *copy_dst, *copy_rows;
+};
+constexpr int64_t kForkMostRows = 65536;
+int64_t fork_workspace_bytes(int64_t R, int64_t P);
+hipError_t launch_paged_fork(const ForkArgs& a, void* workspace, hipStream_t stream);
+
+struct CompactArgs {
+  const int32_t* kv_lens;
+  const int32_t* table;
+  int64_t table_stride, N, M;
+  const int32_t* shares;
+  int64_t P;
+  const int32_t* free_pages;
+  int64_t F;
+  const int32_t* free_head;
+  uint32_t page;
+  int32_t *table_out, *shares_out, *free_out, *head_out;
+  int32_t *copy_src, *copy_dst, *num_moves;
+};
+int64_t compact_workspace_bytes(int64_t P);
+hipError_t launch_paged_compact(const CompactArgs& a, void* workspace, hipStream_t stream);
+
+struct PrefixArgs {
+  const int32_t* kv_lens;
+  const int32_t* table;
+  int64_t table_stride, N, M;
+  const int32_t* ids;  // or null
+  uint32_t page;
+  int32_t *prefix_lens, *group_rows;
+};
+constexpr int64_t kPrefixMostRows = 65536;
+int64_t prefix_workspace_bytes(int64_t N);
+hipError_t launch_paged_prefix(const PrefixArgs& a, void* workspace, hipStream_t stream);
+
+// Rows of pages to other pages of each of `caches` caches, half of them with the
+// strides of the keys, the others with those of the values.
+constexpr int kCopyCaches = 64;
+struct CopyArgs {
+  void* cache[kCopyCaches];
+  int32_t caches;
+  int64_t sp[2], sn[2], sh[2];  // page, row and head strides of keys and values
+  const int32_t *src, *dst, *rows;
+  int64_t C, num_pages;
+  int32_t page, heads, D;
+};
+hipError_t launch_copy_kv(int dtype, const CopyArgs& a, hipStream_t stream);
+
 constexpr int kRopeAxes = 4;
 
 struct RopeRows {   // rows of one tensor: row (b, h, s) at base + b*sb + h*sh + s*ss

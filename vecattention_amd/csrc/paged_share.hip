@@ -1,0 +1,629 @@
+// Pages that several rows of a paged key-value cache hold: the next step's rows
+// from this one's (fork), the pages in use moved together (compact), and the
+// pages that neighbouring rows begin with (prefix).  Integer work on tables, a
+// count for each page and the list of free pages.
+//
+// shares[p] counts the rows that hold page p beyond the first: 0 for a page of
+// one row and for a free one, so that the plan, which takes pages off the free
+// list, has nothing to note.  A page whose last row goes has -1, which is how
+// the fork finds it.
+#include "common.h"
+#include "lanes.h"
+#include "paged_ops.h"
+
+namespace va {
+
+namespace {
+
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kChunk = 1024;       // table entries of a work-group
+constexpr int kPagesPer = 4096;    // pages of a work-group: 64 words of 64 bits
+
+__device__ inline int64_t head_of(const int32_t* head, int64_t F) {
+  const int64_t h = head ? *head : 0;
+  return h < 0 ? 0 : h > F ? F : h;
+}
+// For counts that other work-groups of the same launch change.
+__device__ inline int32_t load_agent(const int32_t* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline void add_agent(int32_t* p, int32_t v) {
+  __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// Whether any thread of the work-group has `x`.
+__device__ inline bool any_of(bool x) { return __syncthreads_or(x) != 0; }
+
+// Sum over a wave.
+__device__ inline int32_t wave_total(int32_t x) {
+  return __builtin_amdgcn_readlane(wave_inclusive_sum(x), 63);
+}
+// Exclusive sum over the work-group and the total.  `part`: kT / 64 values of LDS, which may be
+// written again after the next barrier.
+template <int kT>
+__device__ inline int32_t block_exclusive_sum(int32_t x, int32_t* part, int32_t* total) {
+  const int lane = threadIdx.x % 64, w = threadIdx.x / 64;
+  const int32_t s = wave_inclusive_sum(x);
+  if (lane == 63) part[w] = s;
+  __syncthreads();
+  int32_t before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < kT / 64; ++i) {
+    if (i < w) before += part[i];
+    all += part[i];
+  }
+  *total = all;
+  return before + s - x;
+}
+
+// ---------------------------------------------------------------------------
+// Fork.  With s1 = shares - (rows that held p) + (rows that hold it now), the
+// steps are: the new tables and s1 (fork_rows, fork_counts); the pages with s1 <
+// 0 and the rows that need a page of their own (fork_scan); who gets which page
+// (fork_place).  Rows keep a page that they would write to if they alone hold
+// it; where rows share it, the first of them keeps it if no row that has it whole
+// and no row outside the call holds it too.  All results are sums and ranks, so
+// they do not depend on the order of the atomics.
+struct ForkWork {
+  uint32_t* least;    // (P) first row that would write to a page
+  int32_t* writers;   // (P) and their number; both are set where a row writes alone
+  int32_t* rank;      // (R) number of the row's copy, -1 for none
+  int32_t* row_of;    // (R) row of each copy
+  uint64_t* gone;     // (P / 64) pages with s1 < 0
+  int32_t* counts;    // of them in each chunk of kPagesPer, then the number of copies
+};
+__host__ __device__ inline int64_t fork_chunks(int64_t P) {
+  return P > 0 ? (P + kPagesPer - 1) / kPagesPer : 1;
+}
+
+ForkWork fork_work(void* workspace, int64_t R, int64_t P) {
+  const int64_t chunks = fork_chunks(P);
+  ForkWork w;
+  w.gone = static_cast<uint64_t*>(workspace);
+  w.least = reinterpret_cast<uint32_t*>(w.gone + chunks * (kPagesPer / 64));
+  w.writers = reinterpret_cast<int32_t*>(w.least + P);
+  w.rank = w.writers + P;
+  w.row_of = w.rank + R;
+  w.counts = w.row_of + R;
+  return w;
+}
+
+// Row r's parent or -1, its length and pages.
+struct ForkRow {
+  int32_t parent, len;
+  uint32_t held, had;  // pages, and its parent's
+  __device__ ForkRow(const ForkArgs& a, int64_t r) {
+    parent = a.parents[r];
+    if (parent < 0 || parent >= a.N) {
+      parent = -1;
+      len = 0;
+      held = had = 0;
+      return;
+    }
+    const int32_t was = a.kv_lens[parent];
+    len = was > 0 ? was : 0;
+    if (a.keep) {
+      const int32_t most = a.keep[r] > 0 ? a.keep[r] : 0;
+      len = len < most ? len : most;
+    }
+    held = held_pages(len, a.page, uint32_t(a.M));
+    had = held_pages(was, a.page, uint32_t(a.M));
+  }
+  // The page that its next token goes into beside its own, or -1.
+  __device__ int32_t open(const ForkArgs& a) const {
+    const int64_t at = open_page(len, a.page, uint32_t(a.M));
+    if (parent < 0 || at < 0) return -1;
+    const int32_t id = a.table[parent * a.table_stride + at];
+    return is_page(id, a.P) ? id : -1;
+  }
+};
+
+// Work-groups [0, R * chunks): entries of the new tables; behind them copies of
+// the shares and of the free list.
+__global__ __launch_bounds__(kThreads) void fork_rows_kernel(ForkArgs a, ForkWork w,
+                                                             int64_t chunks) {
+  const int64_t g = blockIdx.x;
+  if (g < a.R * chunks) {
+    const int64_t r = g / chunks, first = (g - r * chunks) * kChunk;
+    const ForkRow row(a, r);
+    const int32_t* from = a.table + (row.parent < 0 ? 0 : row.parent) * a.table_stride;
+    for (int64_t k = first + threadIdx.x; k < first + kChunk && k < a.M; k += kThreads)
+      a.table_out[r * a.M + k] = k < row.held ? from[k] : -1;
+    if (first == 0 && threadIdx.x == 0) {
+      a.kv_out[r] = row.len;
+      const int32_t p = row.open(a);
+      if (p >= 0) {
+        w.least[p] = 0xffffffffu;
+        w.writers[p] = 0;
+      }
+    }
+    return;
+  }
+  const int64_t step = int64_t(gridDim.x - a.R * chunks) * kThreads;
+  for (int64_t i = (g - a.R * chunks) * kThreads + threadIdx.x; i < a.P + a.F; i += step) {
+    if (i < a.P)
+      a.shares_out[i] = a.shares[i];
+    else
+      a.free_out[i - a.P] = a.free_pages[i - a.P];
+  }
+}
+
+// What a page's count changes by: a row's first child stands for the row itself
+// in the pages that it keeps.  Work-groups [0, R * chunks) are the children's,
+// the others those of the rows that have none.
+__global__ __launch_bounds__(kThreads) void fork_counts_kernel(ForkArgs a, ForkWork w,
+                                                               int64_t chunks) {
+  const int64_t g = blockIdx.x, i = g / chunks, first = (g - i * chunks) * kChunk;
+  int64_t from, to;
+  int32_t parent, change;
+  if (i < a.R) {
+    const ForkRow row(a, i);
+    if (first == 0 && threadIdx.x == 0) {
+      const int32_t p = row.open(a);
+      if (p >= 0) {
+        atomicMin(w.least + p, uint32_t(i));
+        add_agent(w.writers + p, 1);
+      }
+    }
+    parent = row.parent;
+    if (parent < 0 || first >= row.had) return;
+    bool earlier = false;
+    for (int64_t j = threadIdx.x; j < i; j += kThreads) earlier |= a.parents[j] == parent;
+    if (any_of(earlier)) {
+      from = 0, to = row.held, change = 1;
+    } else {
+      from = row.held, to = row.had, change = -1;
+    }
+  } else {
+    parent = int32_t(i - a.R);
+    to = held_pages(a.kv_lens[parent], a.page, uint32_t(a.M));
+    if (first >= to) return;
+    bool child = false;
+    for (int64_t j = threadIdx.x; j < a.R; j += kThreads) child |= a.parents[j] == parent;
+    if (any_of(child)) return;
+    from = 0, change = -1;
+  }
+  if (from < first) from = first;
+  if (to > first + kChunk) to = first + kChunk;
+  for (int64_t k = from + threadIdx.x; k < to; k += kThreads) {
+    const int32_t id = a.table[parent * a.table_stride + k];
+    if (is_page(id, a.P)) add_agent(a.shares_out + id, change);
+  }
+}
+
+// The pages that went, 64 to a word, and how many of each chunk; the last
+// work-group numbers the rows' copies.
+__global__ __launch_bounds__(kThreads) void fork_scan_kernel(ForkArgs a, ForkWork w) {
+  __shared__ int32_t part[kWaves];
+  const int64_t chunks = gridDim.x - 1, g = blockIdx.x;
+  const int lane = threadIdx.x % 64;
+  if (g < chunks) {
+    int32_t mine = 0;
+    for (int64_t p = g * kPagesPer + threadIdx.x; p < (g + 1) * kPagesPer; p += kThreads) {
+      const bool gone = p < a.P && a.shares_out[p] < 0;
+      const uint64_t word = __ballot(gone);
+      if (lane == 0) w.gone[p / 64] = word;
+      if (gone) a.shares_out[p] = 0;
+      mine += gone;
+    }
+    int32_t total;
+    block_exclusive_sum<kThreads>(mine, part, &total);
+    if (threadIdx.x == 0) w.counts[g] = total;
+    return;
+  }
+  int32_t before = 0;
+  for (int64_t base = 0; base < a.R; base += kThreads) {
+    const int64_t r = base + threadIdx.x;
+    bool copies = false;
+    if (r < a.R) {
+      const ForkRow row(a, r);
+      const int32_t p = row.open(a);
+      if (p >= 0) {
+        const int32_t s = load_agent(a.shares_out + p);  // below 0, or made 0 by its chunk
+        copies = w.least[p] != uint32_t(r) || (s > 0 ? s : 0) + 1 > w.writers[p];
+      }
+    }
+    int32_t total;
+    const int32_t at = before + block_exclusive_sum<kThreads>(copies, part, &total);
+    if (r < a.R) w.rank[r] = copies ? at : -1;
+    if (copies) w.row_of[at] = int32_t(r);
+    before += total;
+    __syncthreads();  // `part` is written again
+  }
+  if (threadIdx.x == 0) w.counts[chunks] = before;
+}
+
+// Freed page j lies at head - freed + j of the list, copy j takes what is there.
+__global__ __launch_bounds__(kThreads) void fork_place_kernel(ForkArgs a, ForkWork w) {
+  __shared__ int32_t part[2][kWaves];
+  const int64_t chunks = fork_chunks(a.P), g = blockIdx.x;
+  const int lane = threadIdx.x % 64;
+  const int32_t taken = w.counts[chunks];
+  int32_t x = 0, y = 0, freed, before;
+  for (int64_t i = threadIdx.x; i < chunks; i += kThreads) {
+    x += w.counts[i];
+    if (i < g) y += w.counts[i];
+  }
+  block_exclusive_sum<kThreads>(x, part[0], &freed);
+  block_exclusive_sum<kThreads>(y, part[1], &before);
+  const int64_t head = head_of(a.free_head, a.F), top = head - freed;
+  if (g < chunks) {
+    if (w.counts[g] == 0) return;
+    for (int i = threadIdx.x / 64; i < kPagesPer / 64; i += kWaves) {
+      const uint64_t word = w.gone[g * (kPagesPer / 64) + i];
+      if (!(word >> lane & 1)) continue;
+      int32_t j = before;
+      for (int k = 0; k < i; ++k) j += __builtin_popcountll(w.gone[g * (kPagesPer / 64) + k]);
+      j += __builtin_popcountll(word & ((uint64_t(1) << lane) - 1));
+      const int32_t id = int32_t(g * kPagesPer + 64 * i + lane);
+      if (j < taken) {
+        const int32_t r = w.row_of[j];
+        const ForkRow row(a, r);
+        a.copy_dst[r] = id;
+        a.table_out[r * a.M + open_page(row.len, a.page, uint32_t(a.M))] = id;
+      } else if (top + j >= 0) {
+        a.free_out[top + j] = id;
+      }
+    }
+    return;
+  }
+  // Rows: kThreads to a work-group.
+  const int64_t r = (g - chunks) * kThreads + threadIdx.x;
+  if (r == 0) {
+    const int64_t left = top + taken;
+    *a.head_out = int32_t(left < 0 ? 0 : left < 0x7fffffff ? left : 0x7fffffff);
+  }
+  if (r >= a.R) return;
+  const ForkRow row(a, r);
+  const int32_t p = row.open(a), j = w.rank[r];
+  if (p >= 0 && w.least[p] == uint32_t(r)) {
+    // The copies' share in the page goes.
+    const int32_t copies = w.writers[p] - (j < 0), s = a.shares_out[p] - copies;
+    a.shares_out[p] = s > 0 ? s : 0;
+  }
+  a.copy_src[r] = j < 0 ? -1 : p;
+  a.copy_rows[r] = j < 0 ? 0 : int32_t(uint32_t(row.len) % a.page);
+  if (j < 0) {
+    a.copy_dst[r] = -1;
+  } else if (j >= freed) {
+    const int32_t id = free_page(a.free_pages, a.F, top + j);
+    a.copy_dst[r] = id;
+    a.table_out[r * a.M + open_page(row.len, a.page, uint32_t(a.M))] = id;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Compact.  U: the pages in the tables and the free ones, in order; the t in the
+// tables shall be the first t of U.  Those behind (movers) go to the free ones
+// among the first t (holes), in order.
+struct CompactWork {
+  uint32_t *used, *open;  // a bit for each page, 128 words to a chunk
+  int32_t* moved;         // (P) number of a page's move, -1 for none
+};
+CompactWork compact_work(void* workspace, int64_t P) {
+  const int64_t words = fork_chunks(P) * (kPagesPer / 32);
+  CompactWork w;
+  w.used = static_cast<uint32_t*>(workspace);
+  w.open = w.used + words;
+  w.moved = reinterpret_cast<int32_t*>(w.open + words);
+  return w;
+}
+
+__global__ __launch_bounds__(kThreads) void compact_clear_kernel(CompactArgs a, CompactWork w) {
+  const int64_t words = 2 * fork_chunks(a.P) * (kPagesPer / 32), half = a.P / 2;
+  const int64_t step = int64_t(gridDim.x) * kThreads;
+  for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x;
+       i < words + 2 * half + a.F + a.P; i += step) {
+    int64_t k = i;
+    if (k < words) {
+      w.used[k] = 0;
+    } else if ((k -= words) < half) {
+      a.copy_src[k] = -1;
+    } else if ((k -= half) < half) {
+      a.copy_dst[k] = -1;
+    } else if ((k -= half) < a.F) {
+      a.free_out[k] = a.free_pages[k];
+    } else {
+      a.shares_out[k - a.F] = a.shares[k - a.F];
+    }
+  }
+}
+
+__device__ inline void mark(uint32_t* bits, int32_t id, int64_t P) {
+  if (!is_page(id, P)) return;
+  const uint32_t bit = 1u << (id % 32);
+  if (!(bits[id / 32] & bit)) atomicOr(bits + id / 32, bit);
+}
+__global__ __launch_bounds__(kThreads) void compact_mark_kernel(CompactArgs a, CompactWork w,
+                                                                int64_t chunks) {
+  const int64_t g = blockIdx.x;
+  if (g < a.N * chunks) {
+    const int64_t n = g / chunks, first = (g - n * chunks) * kChunk;
+    int64_t to = held_pages(a.kv_lens[n], a.page, uint32_t(a.M));
+    if (to > first + kChunk) to = first + kChunk;
+    for (int64_t k = first + threadIdx.x; k < to; k += kThreads)
+      mark(w.used, a.table[n * a.table_stride + k], a.P);
+    return;
+  }
+  const int64_t step = int64_t(gridDim.x - a.N * chunks) * kThreads;
+  for (int64_t i = head_of(a.free_head, a.F) + (g - a.N * chunks) * kThreads + threadIdx.x;
+       i < a.F; i += step)
+    mark(w.open, a.free_pages[i], a.P);
+}
+
+// Where every page goes.  Each work-group counts all words for itself.
+__global__ __launch_bounds__(kThreads) void compact_place_kernel(CompactArgs a, CompactWork w) {
+  __shared__ int32_t part[6][kWaves];
+  constexpr int kWords = kPagesPer / 32;
+  const int64_t words = int64_t(gridDim.x) * kWords, mine = int64_t(blockIdx.x) * kWords;
+  // Words of a thread: a run of them, so that the boundary lies in one thread's.
+  const int64_t per = (words + kThreads - 1) / kThreads, lo = threadIdx.x * per;
+  const int64_t hi = lo + per < words ? lo + per : words;
+  int32_t u = 0, o = 0, ub = 0, ob = 0;
+  for (int64_t i = lo; i < hi; ++i) {
+    const uint32_t x = w.used[i], y = w.open[i] & ~x;
+    u += __builtin_popcount(x);
+    o += __builtin_popcount(y);
+    if (i < mine) {
+      ub += __builtin_popcount(x);
+      ob += __builtin_popcount(y);
+    }
+  }
+  int32_t t, free, used0, open0, moves;
+  const int32_t u0 = block_exclusive_sum<kThreads>(u, part[0], &t);
+  const int32_t o0 = block_exclusive_sum<kThreads>(o, part[1], &free);
+  block_exclusive_sum<kThreads>(ub, part[2], &used0);
+  block_exclusive_sum<kThreads>(ob, part[3], &open0);
+  // Holes: free pages of rank below t.
+  int32_t holes = 0;
+  if (u0 + o0 < t) {
+    int32_t rank = u0 + o0;
+    for (int64_t i = lo; i < hi && rank < t; ++i) {
+      const uint32_t x = w.used[i], y = w.open[i] & ~x;
+      const int32_t n = __builtin_popcount(x | y);
+      if (rank + n <= t) {
+        holes += __builtin_popcount(y);
+      } else {
+        uint32_t all = x | y;
+        for (int32_t k = rank; k < t; ++k) {
+          const uint32_t bit = all & -all;
+          if (y & bit) ++holes;
+          all ^= bit;
+        }
+      }
+      rank += n;
+    }
+  }
+  block_exclusive_sum<kThreads>(holes, part[4], &moves);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    *a.num_moves = moves;
+    *a.head_out = int32_t(a.F - free);
+  }
+  // The pages of this chunk: a wave takes 64 at a time.
+  const int lane = threadIdx.x % 64;
+  for (int i = threadIdx.x / 64; i < kWords / 2; i += kWaves) {
+    int32_t ru = used0, ro = open0;
+    uint64_t x = 0, y = 0;
+    // Two words to a lane: counts of the 64-page pieces before this one.
+    {
+      const int64_t k = mine + 2 * lane;
+      const uint32_t x0 = w.used[k], x1 = w.used[k + 1];
+      const uint32_t y0 = w.open[k] & ~x0, y1 = w.open[k + 1] & ~x1;
+      ru += wave_total(lane < i ? __builtin_popcount(x0) + __builtin_popcount(x1) : 0);
+      ro += wave_total(lane < i ? __builtin_popcount(y0) + __builtin_popcount(y1) : 0);
+      x = uint64_t(uint32_t(__builtin_amdgcn_readlane(int(x0), i))) |
+          uint64_t(uint32_t(__builtin_amdgcn_readlane(int(x1), i))) << 32;
+      y = uint64_t(uint32_t(__builtin_amdgcn_readlane(int(y0), i))) |
+          uint64_t(uint32_t(__builtin_amdgcn_readlane(int(y1), i))) << 32;
+    }
+    const uint64_t below = (uint64_t(1) << lane) - 1;
+    ru += __builtin_popcountll(x & below);
+    ro += __builtin_popcountll(y & below);
+    const int64_t p = int64_t(blockIdx.x) * kPagesPer + 64 * i + lane;
+    if (p >= a.P) continue;
+    const bool is_used = x >> lane & 1, is_open = y >> lane & 1;
+    const int32_t rank = ru + ro;
+    int32_t move = -1;
+    if (is_used && rank >= t) {
+      move = ru - (t - moves);
+      a.copy_src[move] = int32_t(p);
+    }
+    if (is_open && rank < t) a.copy_dst[ro] = int32_t(p);
+    if ((is_used || is_open) && rank >= t) a.free_out[a.F - free + (rank - t)] = int32_t(p);
+    w.moved[p] = move;
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void compact_tables_kernel(CompactArgs a, CompactWork w,
+                                                                  int64_t chunks) {
+  const int64_t g = blockIdx.x;
+  if (g < a.N * chunks) {
+    const int64_t n = g / chunks, first = (g - n * chunks) * kChunk;
+    const int64_t held = held_pages(a.kv_lens[n], a.page, uint32_t(a.M));
+    for (int64_t k = first + threadIdx.x; k < first + kChunk && k < a.M; k += kThreads) {
+      int32_t id = a.table[n * a.table_stride + k];
+      if (k < held && is_page(id, a.P)) {
+        const int32_t move = w.moved[id];
+        if (move >= 0) id = a.copy_dst[move];
+      }
+      a.table_out[n * a.M + k] = id;
+    }
+    return;
+  }
+  const int32_t moves = *a.num_moves;
+  const int64_t step = int64_t(gridDim.x - a.N * chunks) * kThreads;
+  for (int64_t i = (g - a.N * chunks) * kThreads + threadIdx.x; i < moves; i += step) {
+    const int32_t from = a.copy_src[i], to = a.copy_dst[i];
+    a.shares_out[to] = a.shares[from];
+    a.shares_out[from] = 0;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Prefix.  Row n goes with the row before it when both hold tokens and have the
+// same id (without ids: the same first page).
+__device__ inline bool joins(const PrefixArgs& a, int64_t n) {
+  if (n == 0 || a.kv_lens[n] <= 0 || a.kv_lens[n - 1] <= 0) return false;
+  if (a.ids) return a.ids[n] == a.ids[n - 1];
+  const int32_t id = a.M ? a.table[n * a.table_stride] : -1;
+  return id >= 0 && id == a.table[(n - 1) * a.table_stride];
+}
+
+// A work-group a row: the first row of its group, and the whole pages that the
+// two begin with.
+__global__ __launch_bounds__(kThreads) void prefix_rows_kernel(PrefixArgs a, int32_t* first,
+                                                               int32_t* pages) {
+  __shared__ int32_t best[kWaves];
+  const int64_t n = blockIdx.x;
+  const int lane = threadIdx.x % 64;
+  // The last row up to this one that does not join.
+  int32_t lead = 0;
+  for (int64_t i = threadIdx.x; i <= n; i += kThreads)
+    if (!joins(a, i)) lead = int32_t(i);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int32_t other = __shfl_xor(lead, d);
+    lead = lead > other ? lead : other;
+  }
+  if (lane == 0) best[threadIdx.x / 64] = lead;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) lead = lead > best[i] ? lead : best[i];
+  const int32_t len = a.kv_lens[n] > 0 ? a.kv_lens[n] : 0;
+  int64_t whole = uint32_t(len) / a.page;
+  if (whole > a.M) whole = a.M;
+  const int32_t *row = a.table + n * a.table_stride, *with = a.table + lead * a.table_stride;
+  int64_t same = whole;
+  for (int64_t k0 = 0; k0 < whole; k0 += 4 * kThreads) {
+    int64_t miss = whole;  // the thread's first entry that differs
+#pragma unroll
+    for (int e = 3; e >= 0; --e) {
+      const int64_t k = k0 + e * kThreads + threadIdx.x;
+      if (k < whole && (row[k] < 0 || row[k] != with[k])) miss = k;
+    }
+    if (any_of(miss < whole)) {
+      // The least over the work-group.
+      int32_t m = int32_t(miss);
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int32_t other = __shfl_xor(m, d);
+        m = m < other ? m : other;
+      }
+      if (lane == 0) best[threadIdx.x / 64] = m;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) m = m < best[i] ? m : best[i];
+      same = m;
+      break;
+    }
+  }
+  if (threadIdx.x == 0) {
+    first[n] = lead;
+    pages[n] = int32_t(same);
+  }
+}
+
+// A wave a row: the fewest pages over its group, and the group's rows.
+__global__ __launch_bounds__(kThreads) void prefix_groups_kernel(PrefixArgs a,
+                                                                 const int32_t* first,
+                                                                 const int32_t* pages) {
+  const int64_t n = int64_t(blockIdx.x) * kWaves + threadIdx.x / 64;
+  const int lane = threadIdx.x % 64;
+  if (n >= a.N) return;
+  const int32_t lead = first[n];
+  int32_t least = 0x7fffffff;
+  int64_t rows = 0;
+  for (int64_t base = lead; base < a.N; base += 64) {
+    const int64_t i = base + lane;
+    const bool in = i < a.N && first[i] == lead;
+    if (in) least = least < pages[i] ? least : pages[i];
+    const uint64_t all = __ballot(in);
+    rows += __builtin_popcountll(all);
+    if (all != ~uint64_t(0)) break;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int32_t other = __shfl_xor(least, d);
+    least = least < other ? least : other;
+  }
+  if (lane == 0) {
+    const int32_t len = rows > 1 ? int32_t(uint32_t(least) * a.page) : 0;
+    a.prefix_lens[n] = len;
+    a.group_rows[n] = n == lead && len > 0 ? int32_t(rows) : 0;
+  }
+}
+
+unsigned extra_groups(int64_t work) {
+  const int64_t g = (work + 4 * kThreads - 1) / (4 * kThreads);
+  return unsigned(g < 1 ? 1 : g > 1024 ? 1024 : g);
+}
+
+}  // namespace
+
+int64_t fork_workspace_bytes(int64_t R, int64_t P) {
+  const int64_t chunks = fork_chunks(P);
+  return 8 * chunks * (kPagesPer / 64) + 4 * (2 * P + 2 * R + chunks + 1);
+}
+
+hipError_t launch_paged_fork(const ForkArgs& a, void* workspace, hipStream_t stream) {
+  const ForkWork w = fork_work(workspace, a.R, a.P);
+  const int64_t per_row = a.M > 0 ? (a.M + kChunk - 1) / kChunk : 1;
+  hipLaunchKernelGGL(fork_rows_kernel, dim3(unsigned(a.R * per_row) + extra_groups(a.P + a.F)),
+                     dim3(kThreads), 0, stream, a, w, per_row);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  if (a.R + a.N > 0) {
+    hipLaunchKernelGGL(fork_counts_kernel, dim3(unsigned((a.R + a.N) * per_row)), dim3(kThreads),
+                       0, stream, a, w, per_row);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  const int64_t chunks = fork_chunks(a.P);
+  hipLaunchKernelGGL(fork_scan_kernel, dim3(unsigned(chunks + 1)), dim3(kThreads), 0, stream, a,
+                     w);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const int64_t rows = a.R > 0 ? (a.R + kThreads - 1) / kThreads : 1;
+  hipLaunchKernelGGL(fork_place_kernel, dim3(unsigned(chunks + rows)), dim3(kThreads), 0, stream,
+                     a, w);
+  return hipGetLastError();
+}
+
+int64_t compact_workspace_bytes(int64_t P) {
+  return 8 * fork_chunks(P) * (kPagesPer / 32) + 4 * P;
+}
+
+hipError_t launch_paged_compact(const CompactArgs& a, void* workspace, hipStream_t stream) {
+  const CompactWork w = compact_work(workspace, a.P);
+  const int64_t per_row = a.M > 0 ? (a.M + kChunk - 1) / kChunk : 1;
+  const int64_t chunks = fork_chunks(a.P);
+  hipLaunchKernelGGL(compact_clear_kernel, dim3(extra_groups(3 * a.P + a.F)), dim3(kThreads), 0,
+                     stream, a, w);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(compact_mark_kernel, dim3(unsigned(a.N * per_row) + extra_groups(a.F)),
+                     dim3(kThreads), 0, stream, a, w, per_row);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(compact_place_kernel, dim3(unsigned(chunks)), dim3(kThreads), 0, stream, a, w);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(compact_tables_kernel, dim3(unsigned(a.N * per_row) + extra_groups(a.P / 2)),
+                     dim3(kThreads), 0, stream, a, w, per_row);
+  return hipGetLastError();
+}
+
+int64_t prefix_workspace_bytes(int64_t N) { return 8 * N; }
+
+hipError_t launch_paged_prefix(const PrefixArgs& a, void* workspace, hipStream_t stream) {
+  int32_t* first = static_cast<int32_t*>(workspace);
+  int32_t* pages = first + a.N;
+  hipLaunchKernelGGL(prefix_rows_kernel, dim3(unsigned(a.N)), dim3(kThreads), 0, stream, a, first,
+                     pages);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(prefix_groups_kernel, dim3(unsigned((a.N + kWaves - 1) / kWaves)),
+                     dim3(kThreads), 0, stream, a, first, pages);
+  return hipGetLastError();
+}
+
+}  // namespace va

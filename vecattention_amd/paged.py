@@ -13,6 +13,14 @@ and generated tokens alike:
 3. ``paged_decode_attention``: one new token of every request over its pages.
    No operator attends from several new tokens of a request over its pages.
 
+Rows of the batch may hold the same pages: several answers to one prompt, the
+beams of a search.  Between two steps ``paged_kv_fork`` makes the next rows from
+the present ones (rows go on, are forked, cut back or dropped) and
+``copy_paged_kv`` copies what it lists in all layers; ``paged_kv_prefix`` finds
+what rows begin with in common, once a step, and then
+``paged_prefix_decode_attention`` reads it once for all of them.
+``paged_kv_compact`` moves the pages in use together.
+
 A cache is (num_pages, page_size, num_kv_heads, head_dim) with kv_layout "NHD",
 (num_pages, num_kv_heads, page_size, head_dim) with "HND"; any strides with
 contiguous features.  Nothing waits for the GPU or is kept between calls, so the
@@ -108,5 +116,117 @@ def paged_decode_attention(q, k_cache, v_cache, block_tables, kv_lens, kv_layout
                          sm_scale)
 
 
+class PagedFork(NamedTuple):
+    """The next step's rows (``paged_kv_fork``).  The tensors of the rows share one
+    allocation, those of the pages another."""
+    kv_lens: torch.Tensor       # (R,) int32
+    block_tables: torch.Tensor  # (R, M) int32, -1 behind a row's pages
+    page_shares: torch.Tensor   # (num_pages,) int32
+    free_pages: torch.Tensor    # (F,) int32
+    free_head: torch.Tensor     # (1,) int32: its first free entry
+    copy_src: torch.Tensor      # (R,) int32: page that the row's last tokens are in, -1 for no copy
+    copy_dst: torch.Tensor      # (R,) int32: page that they are to be in, -1 for no copy
+    copy_rows: torch.Tensor     # (R,) int32: how many of them
+
+
+def paged_kv_fork(kv_lens, parents, block_tables, page_shares, free_pages, page_size,
+                  free_head=None, keep_lens=None):
+    """The rows of the next step from those of this one, with the pages they share.
+
+    kv_lens (N,), block_tables (N, M): the rows as they are.  parents: (R,), the row
+    that each new row goes on from; one that several name is forked, one that none
+    names is dropped, and a parent outside [0, N) (-1) makes an empty row.
+    keep_lens: (R,), tokens that a new row keeps at most (None: all of them).
+    page_shares: (num_pages,), the rows that hold each page beyond the first; zeros
+    to begin with.  free_pages and free_head: the list that ``paged_kv_plan`` takes
+    from.  All int32.  Nothing is written in place: the results replace them.
+
+    Pages are shared, not copied, but for the one that a row's next tokens go into:
+    where rows would share a page that is not full, each but one gets its own
+    (``copy_src``, ``copy_dst``, ``copy_rows`` are what ``copy_paged_kv`` then copies
+    in every layer).  Pages that no row holds any more return to the free list, in
+    front of ``free_head`` and in ascending order, and the copies take theirs from
+    there.  Where the list ends they get -1 (``paged_decode_attention`` answers NaN
+    for such a row) and the new ``free_head`` exceeds the list; a list with an entry
+    for every page of the cache has room for all that return.  At most 65536 rows.
+    """
+    return PagedFork._make(nat.host_call("fork", block_tables, kv_lens, parents, block_tables,
+                                         page_shares, free_pages, page_size, free_head,
+                                         keep_lens))
+
+
+class PagedCompaction(NamedTuple):
+    """Pages moved together (``paged_kv_compact``)."""
+    block_tables: torch.Tensor  # (N, M) int32
+    page_shares: torch.Tensor   # (num_pages,) int32
+    free_pages: torch.Tensor    # (F,) int32: the free ones at its end, in ascending order
+    free_head: torch.Tensor     # (1,) int32: its first free entry
+    copy_src: torch.Tensor      # (num_pages // 2,) int32: pages to move, -1 behind them
+    copy_dst: torch.Tensor      # (num_pages // 2,) int32: where to
+    num_moves: torch.Tensor     # (1,) int32
+
+
+def paged_kv_compact(kv_lens, block_tables, page_shares, free_pages, page_size, free_head=None):
+    """The pages of the tables to the lowest numbers of those pages and the free ones.
+
+    Arguments as for ``paged_kv_fork``.  Pages that are neither in the tables' rows
+    nor in the list from ``free_head`` on stay where they are and keep their numbers,
+    so the tables have to be all that may be renumbered.  ``copy_paged_kv(k_caches,
+    v_caches, c.copy_src, c.copy_dst)`` moves the rows of every layer.
+    """
+    return PagedCompaction._make(nat.host_call("compact", block_tables, kv_lens, block_tables,
+                                               page_shares, free_pages, page_size, free_head))
+
+
+def copy_paged_kv(k_caches, v_caches, src_pages, dst_pages, rows=None, kv_layout="NHD"):
+    """Pages to other pages of the same caches, in place, all layers in one launch.
+
+    k_caches, v_caches: the cache of one layer, or lists of those of all layers (one
+    shape, type and strides).  src_pages, dst_pages: (C,) int32; an entry with a page
+    outside the cache (-1) copies nothing.  The pages copied to must be distinct, and
+    none of them copied from.  rows: (C,) int32, the tokens at the beginning of each
+    page that are copied (None: all); the rows behind them stay.
+    """
+    one = k_caches[0] if isinstance(k_caches, (list, tuple)) and k_caches else k_caches
+    nat.host_call("copy", one, k_caches, v_caches, src_pages, dst_pages, rows, kv_layout)
+
+
+class SharedPrefix(NamedTuple):
+    """What neighbouring rows begin with in common (``paged_kv_prefix``)."""
+    prefix_lens: torch.Tensor  # (N,) int32: tokens that the row's group shares, in whole pages
+    group_rows: torch.Tensor   # (N,) int32: rows of the group that begins here, else 0
+
+
+def paged_kv_prefix(kv_lens, block_tables, page_size, group_ids=None):
+    """Which rows begin with the same pages, for ``paged_prefix_decode_attention``.
+
+    Rows that follow each other, hold tokens and have the same group_ids ((N,) int32)
+    are a group; without group_ids, rows whose first page is the same (a system
+    prompt that all requests begin with makes one group of them: ids say which larger
+    parts to share instead).  ``prefix_lens`` are the tokens of the whole pages that
+    all rows of a group begin with, 0 where a row is alone.  What it finds stays true
+    while rows grow; after a fork or a compaction it has to be found anew.
+    """
+    return SharedPrefix._make(nat.host_call("prefix", block_tables, kv_lens, block_tables,
+                                            page_size, group_ids))
+
+
+def paged_prefix_decode_attention(q, k_cache, v_cache, block_tables, kv_lens, prefix,
+                                  kv_layout="NHD", sm_scale=None):
+    """``paged_decode_attention`` for rows that share the beginnings of their pages.
+
+    prefix: ``paged_kv_prefix`` of these rows (a pair of prefix_lens and group_rows).
+    The keys and values of a group's prefix are read once, for the query heads of all
+    of its rows together, and every row's own keys after them; otherwise arguments and
+    result are those of ``paged_decode_attention``.  Rows of a group hold at least
+    prefix_lens tokens, and list the same pages for them.
+    """
+    prefix_lens, group_rows = prefix
+    return nat.host_call("prefix_decode", q, q, k_cache, v_cache, block_tables, kv_lens,
+                         prefix_lens, group_rows, kv_layout, sm_scale)
+
+
 __all__ = ["PagedStep", "paged_kv_plan", "write_paged_kv", "qk_norm_rope_to_cache",
-           "paged_decode_attention"]
+           "paged_decode_attention", "PagedFork", "paged_kv_fork", "PagedCompaction",
+           "paged_kv_compact", "copy_paged_kv", "SharedPrefix", "paged_kv_prefix",
+           "paged_prefix_decode_attention"]
