@@ -202,8 +202,8 @@ int va_write_paged_kv(int dtype, const void* k, int64_t skt, int64_t skh, const 
   return launched(va::launch_write_kv(dtype, a, static_cast<hipStream_t>(stream)), "write launch");
 }
 
-int64_t va_paged_decode_workspace_size(int dtype, int64_t N, int64_t Hq, int64_t Hk, int64_t D,
-                                       int64_t M, int64_t page_size) {
+static int64_t decode_workspace(int dtype, int64_t N, int64_t Hq, int64_t Hk, int64_t D, int64_t M,
+                                int64_t page_size, bool prefix) {
   if (!dtype_ok(dtype) || N <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk || D <= 0 || M < 0 ||
       page_size <= 0 || page_size >= kInt31 || M >= kInt31 || !fits(N, Hq, int64_t(1) << 23))
     return -1;
@@ -214,16 +214,23 @@ int64_t va_paged_decode_workspace_size(int dtype, int64_t N, int64_t Hq, int64_t
   a.D = D;
   a.M = M;
   a.page = page_size;
-  return va::paged_attn_workspace(dtype, a);
+  return prefix ? va::prefix_attn_workspace(dtype, a) : va::paged_attn_workspace(dtype, a);
 }
 
-int va_paged_decode_attn(int dtype, const void* q, int64_t sqn, int64_t sqh, const void* k_cache,
-                         int64_t skp, int64_t skn, int64_t skh, const void* v_cache, int64_t svp,
-                         int64_t svn, int64_t svh, void* out, int64_t son, int64_t soh,
-                         const int32_t* block_tables, int64_t stn, int64_t M,
-                         const int32_t* kv_lens, int64_t N, int64_t Hq, int64_t Hk, int64_t D,
-                         int64_t page_size, int64_t num_pages, float softmax_scale,
-                         void* workspace, int64_t workspace_bytes, void* stream) {
+int64_t va_paged_decode_workspace_size(int dtype, int64_t N, int64_t Hq, int64_t Hk, int64_t D,
+                                       int64_t M, int64_t page_size) {
+  return decode_workspace(dtype, N, Hq, Hk, D, M, page_size, false);
+}
+
+// Both decode attentions: without prefix_lens and group_rows, the plain one.
+static int decode_attn(int dtype, const void* q, int64_t sqn, int64_t sqh, const void* k_cache,
+                       int64_t skp, int64_t skn, int64_t skh, const void* v_cache, int64_t svp,
+                       int64_t svn, int64_t svh, void* out, int64_t son, int64_t soh,
+                       const int32_t* block_tables, int64_t stn, int64_t M,
+                       const int32_t* kv_lens, const int32_t* prefix_lens,
+                       const int32_t* group_rows, int64_t N, int64_t Hq, int64_t Hk, int64_t D,
+                       int64_t page_size, int64_t num_pages, float softmax_scale,
+                       void* workspace, int64_t workspace_bytes, void* stream) {
   if (!dtype_ok(dtype)) return api_error(VA_ERR_ARG, "unknown dtype %d", dtype);
   if (!q || !k_cache || !v_cache || !out || !kv_lens || (M && !block_tables))
     return api_error(VA_ERR_ARG, "null tensor pointer");
@@ -232,7 +239,8 @@ int va_paged_decode_attn(int dtype, const void* q, int64_t sqn, int64_t sqh, con
   if (Hq % Hk) return api_error(VA_ERR_ARG, "num q heads not a multiple of kv heads");
   if (D > 256) return api_error(VA_ERR_UNSUPPORTED, "head_dim %lld > 256", (long long)D);
   if (const int rc = check_pages(num_pages, page_size)) return rc;
-  const int64_t need = va_paged_decode_workspace_size(dtype, N, Hq, Hk, D, M, page_size);
+  const int64_t need =
+      decode_workspace(dtype, N, Hq, Hk, D, M, page_size, prefix_lens != nullptr);
   if (need < 0)
     return api_error(VA_ERR_UNSUPPORTED, "2^23 query rows, or 2^31 work units, in a call");
   if (!workspace || workspace_bytes < need)
@@ -265,8 +273,24 @@ int va_paged_decode_attn(int dtype, const void* q, int64_t sqn, int64_t sqh, con
   a.page = page_size;
   a.num_pages = num_pages;
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
-  return launched(va::launch_paged_attn(dtype, a, workspace, static_cast<hipStream_t>(stream)),
+  a.prefix_lens = prefix_lens;
+  a.group_rows = group_rows;
+  const auto on = static_cast<hipStream_t>(stream);
+  return launched(prefix_lens ? va::launch_prefix_attn(dtype, a, workspace, on)
+                              : va::launch_paged_attn(dtype, a, workspace, on),
                   "paged decode launch");
+}
+
+int va_paged_decode_attn(int dtype, const void* q, int64_t sqn, int64_t sqh, const void* k_cache,
+                         int64_t skp, int64_t skn, int64_t skh, const void* v_cache, int64_t svp,
+                         int64_t svn, int64_t svh, void* out, int64_t son, int64_t soh,
+                         const int32_t* block_tables, int64_t stn, int64_t M,
+                         const int32_t* kv_lens, int64_t N, int64_t Hq, int64_t Hk, int64_t D,
+                         int64_t page_size, int64_t num_pages, float softmax_scale,
+                         void* workspace, int64_t workspace_bytes, void* stream) {
+  return decode_attn(dtype, q, sqn, sqh, k_cache, skp, skn, skh, v_cache, svp, svn, svh, out, son,
+                     soh, block_tables, stn, M, kv_lens, nullptr, nullptr, N, Hq, Hk, D,
+                     page_size, num_pages, softmax_scale, workspace, workspace_bytes, stream);
 }
 
 constexpr int64_t kMostGroups = int64_t(1) << 23;
@@ -424,7 +448,7 @@ int va_copy_paged_kv(int dtype, void* const* k_caches, void* const* v_caches, in
 
 int64_t va_paged_prefix_decode_workspace_size(int dtype, int64_t N, int64_t Hq, int64_t Hk,
                                               int64_t D, int64_t M, int64_t page_size) {
-  return va_paged_decode_workspace_size(dtype, N, Hq, Hk, D, M, page_size);
+  return decode_workspace(dtype, N, Hq, Hk, D, M, page_size, true);
 }
 
 int va_paged_prefix_decode_attn(int dtype, const void* q, int64_t sqn, int64_t sqh,
@@ -437,10 +461,9 @@ int va_paged_prefix_decode_attn(int dtype, const void* q, int64_t sqn, int64_t s
                                 int64_t num_pages, float softmax_scale, void* workspace,
                                 int64_t workspace_bytes, void* stream) {
   if (!prefix_lens || !group_rows) return api_error(VA_ERR_ARG, "null pointer");
-  return va_paged_decode_attn(dtype, q, sqn, sqh, k_cache, skp, skn, skh, v_cache, svp, svn, svh,
-                              out, son, soh, block_tables, stn, M, kv_lens, N, Hq, Hk, D,
-                              page_size, num_pages, softmax_scale, workspace, workspace_bytes,
-                              stream);
+  return decode_attn(dtype, q, sqn, sqh, k_cache, skp, skn, skh, v_cache, svp, svn, svh, out, son,
+                     soh, block_tables, stn, M, kv_lens, prefix_lens, group_rows, N, Hq, Hk, D,
+                     page_size, num_pages, softmax_scale, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

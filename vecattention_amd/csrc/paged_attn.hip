@@ -55,14 +55,30 @@ __device__ inline uint32_t share_number(const PagedArgs& a) {
   return blockIdx.x < 4 * quarter ? blockIdx.x % 4 * quarter + blockIdx.x / 4 : blockIdx.x;
 }
 
+// The keys that a row's own pass skips: with kState, those it shares.
+template <bool kState>
+__device__ inline int32_t skipped(const PagedArgs& a, int64_t n, int64_t capacity) {
+  if constexpr (kState) {
+    const int32_t shared = shared_keys(a.prefix_lens[n], capacity), len = a.lens[n];
+    return len <= 0 ? 0 : shared < len ? shared : len;
+  }
+  return 0;
+}
+// The keys of a row's pass (paged_keys).
+template <bool kState>
+__device__ inline int32_t row_keys(const PagedArgs& a, int64_t n, int64_t capacity) {
+  const int32_t keys = paged_keys(a.lens[n], capacity);
+  return kState && keys > 0 ? keys - skipped<kState>(a, n, capacity) : keys;
+}
+
 // Sums the units of the requests (every work-group does, N lengths from L2) and
 // finds the request of the share's first unit.
-template <int kUnit>
+template <int kUnit, bool kState = false>
 __device__ inline Place locate(const PagedArgs& a, PlaceLds& lds) {
   const int64_t capacity = a.M * a.page;
   if (a.N <= 64) {  // a lane a request, in every wave by itself
     const int lane = threadIdx.x % 64;
-    const int32_t keys = lane < a.N ? paged_keys(a.lens[lane], capacity) : 0;
+    const int32_t keys = lane < a.N ? row_keys<kState>(a, lane, capacity) : 0;
     const uint32_t mine = lane < a.N ? a.per_request * paged_units(keys, kUnit) : 0;
     const uint32_t sum = uint32_t(wave_inclusive_sum(int(mine)));
     const PagedShare share(uint32_t(__builtin_amdgcn_readlane(int(sum), 63)), uint32_t(a.groups));
@@ -82,7 +98,7 @@ __device__ inline Place locate(const PagedArgs& a, PlaceLds& lds) {
   uint32_t mine = 0;
   int32_t keys = 0;
   for (int32_t i = lo; i < lo + per && i < N; ++i) {
-    keys = paged_keys(a.lens[i], capacity);
+    keys = row_keys<kState>(a, i, capacity);
     mine += a.per_request * paged_units(keys, kUnit);
   }
   const int lane = threadIdx.x % 64, w = threadIdx.x / 64;
@@ -100,7 +116,7 @@ __device__ inline Place locate(const PagedArgs& a, PlaceLds& lds) {
   const uint32_t begin = share.begin(number);
   if (begin >= at && begin < at + mine)
     for (int32_t i = lo; i < lo + per && i < N; ++i) {
-      if (per > 1) keys = paged_keys(a.lens[i], capacity);
+      if (per > 1) keys = row_keys<kState>(a, i, capacity);
       const uint32_t n = a.per_request * paged_units(keys, kUnit);
       if (begin < at + n) {
         lds.request = i;
@@ -121,9 +137,11 @@ __device__ inline float weighed(float w, float x) {
 }
 
 // Merges the waves' states of a segment's rows and writes them: to the output
-// (`whole`), or to a partial slot.  sO[wave][row][stride], sm/sl[wave][row];
-// kV features of a row a thread.
-template <typename T, int kV, int kThreads = kPagedThreads, int kStates = kPagedWaves>
+// (`whole`), or to a partial slot; with kState to the rows' states where the segment
+// begins here (`whole`).  sO[wave][row][stride], sm/sl[wave][row]; kV features of a row
+// a thread.
+template <typename T, int kV, int kThreads = kPagedThreads, int kStates = kPagedWaves,
+          bool kState = false>
 __device__ inline void finish(const PagedArgs& a, int D, const float* sO, int rstride,
                               int wstride, const float* sm, const float* sl, int mstride, int rows,
                               bool whole, int64_t slot, int64_t request, int64_t head, bool empty,
@@ -158,7 +176,11 @@ __device__ inline void finish(const PagedArgs& a, int D, const float* sO, int rs
       }
     }
     if (bad) l = __builtin_nanf("");
-    if (whole) {
+    if (kState && whole) {
+      const int64_t row = request * a.Hk * a.G + head + r;
+      if (f == 0) a.state_ml[row] = make_float2(m, l);
+      *reinterpret_cast<vec*>(a.state + row * a.D + f) = o;
+    } else if (whole) {
       // No key: 0.  Keys without weight (scores of -infinity alone): 0/0, as the formula has it.
       struct alignas(sizeof(T) * kV) Row { T x[kV]; } y;
 #pragma unroll
@@ -367,7 +389,9 @@ template <int kTiles> struct Pages {
 // whole segment, with eight waves or one, and there is nothing to merge afterwards.
 // kStream: the values are read past the caches.
 enum PagedForm : int { kFormSplit = 4, kFormWhole = 8, kFormShort = 1 };  // and its waves
-template <typename T, int D, bool kWholeTiles, PagedForm kForm, bool kStream>
+//
+// kState: a row's keys from `skipped` on, and states instead of outputs.
+template <typename T, int D, bool kWholeTiles, PagedForm kForm, bool kStream, bool kState = false>
 __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) {
   constexpr bool k16 = sizeof(T) == 2, kSplit = kForm == kFormSplit;
   constexpr int kWaves = kForm, kStates = kWaves < kPagedWaves ? kWaves : kPagedWaves;
@@ -389,10 +413,10 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
   const uint32_t page = uint32_t(a.page);
   Place pl{PagedShare(1, 1), 0, 0, 0, 0, 0, 0};
   if constexpr (kSplit) {
-    pl = locate<kUnit>(a, place);
+    pl = locate<kUnit, kState>(a, place);
   } else {
     pl.request = int32_t(blockIdx.x / uint32_t(a.per_request));
-    pl.keys = paged_keys(a.lens[pl.request], capacity);
+    pl.keys = row_keys<kState>(a, pl.request, capacity);
     pl.begin = (blockIdx.x - pl.request * a.per_request) * paged_units(pl.keys, kUnit);
     pl.end = pl.begin + 1;  // all of the segment's units
   }
@@ -420,8 +444,9 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
                         : u32x4_t{0, 0, 0, 0};
     }
     bool bad = keys < 0;
-    const uint32_t last = keys > 0 ? uint32_t(keys) - 1 : 0;
-    const uint32_t first = c0 * kUnit + wave * kKeys;
+    const uint32_t skip = uint32_t(skipped<kState>(a, req, capacity));
+    const uint32_t last = skip + (keys > 0 ? uint32_t(keys) - 1 : 0);
+    const uint32_t first = skip + c0 * kUnit + wave * kKeys;
     int steps = 0;
     if (keys > 0 && first <= last) {
       const uint32_t left = (last - first) / kUnit + 1;
@@ -710,10 +735,10 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
     bool any_bad = false;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) any_bad |= sbad[w] != 0;
-    finish<T, 4, 64 * kWaves, kStates>(a, D, &sO[0][0][0], kStride, kTileHeads * kStride,
-                                       &sm[0][0], &sl[0][0], kTileHeads, rows, count == units,
-                                       2 * int64_t(pl.number) + (u > begin), req, hk * a.G + r0,
-                                       keys == 0, any_bad);
+    finish<T, 4, 64 * kWaves, kStates, kState>(
+        a, D, &sO[0][0][0], kStride, kTileHeads * kStride, &sm[0][0], &sl[0][0], kTileHeads, rows,
+        kState ? c0 == 0 : count == units, 2 * int64_t(pl.number) + (!kState && u > begin), req,
+        hk * a.G + r0, keys == 0, any_bad);
     if (!kSplit) break;
     if (c0 == 0 && threadIdx.x == 0)
       a.split[req * a.per_request + seg] =
@@ -723,7 +748,7 @@ __global__ __launch_bounds__(64 * kForm, 2) void paged_tile_kernel(PagedArgs a) 
     u += count;
     if (u < end && u == base + units * a.per_request) {
       base = u;
-      keys = paged_keys(a.lens[++req], capacity);
+      keys = row_keys<kState>(a, ++req, capacity);
     }
   }
 }
@@ -861,7 +886,7 @@ static int64_t round256(int64_t x) { return (x + 255) / 256 * 256; }
 
 // Whether the matrix-core form takes these rows: whole 16-byte pieces, and
 // offsets within a page of 31 bits.
-static bool tile_form(int dtype, const PagedArgs& a) {
+bool paged_tile_form(int dtype, const PagedArgs& a) {
   if (a.D != 64 && a.D != 128) return false;
   const int64_t es = dtype == kF32 ? 4 : 2, piece = 16 / es;
   for (const void* p : {a.q, a.k, a.v})
@@ -957,7 +982,7 @@ static void launch_merge(const PagedArgs& a, hipStream_t stream) {
 
 template <typename T>
 static hipError_t launch_paged_t(int dtype, PagedArgs& a, void* workspace, hipStream_t stream) {
-  const bool tiles = tile_form(dtype, a);
+  const bool tiles = paged_tile_form(dtype, a);
   const int64_t need = tiles ? plan_tiles(dtype, a) : plan_rows(a);
   if (need < 0) return hipErrorInvalidValue;
   a.part = static_cast<float*>(workspace);
@@ -991,6 +1016,30 @@ static hipError_t launch_paged_t(int dtype, PagedArgs& a, void* workspace, hipSt
     launch_merge<T, 0, 4, 256>(a, stream);
   else
     launch_merge<T, 0, 1, 256>(a, stream);
+  return hipGetLastError();
+}
+
+// States of the rows' own keys: always dealt evenly, since the tables' width says
+// nothing about how many there are.
+int64_t paged_states_workspace(int dtype, PagedArgs& a) { return plan_tiles(dtype, a); }
+
+template <typename T, int D>
+static void launch_states(const PagedArgs& a, hipStream_t stream) {
+  const dim3 grid{unsigned(a.groups)}, block{64 * kFormSplit};
+  if (a.page % 16 == 0)
+    hipLaunchKernelGGL((paged_tile_kernel<T, D, true, kFormSplit, false, true>), grid, block, 0,
+                       stream, a);
+  else
+    hipLaunchKernelGGL((paged_tile_kernel<T, D, false, kFormSplit, false, true>), grid, block, 0,
+                       stream, a);
+}
+
+hipError_t launch_paged_states(int dtype, PagedArgs& a, hipStream_t stream) {
+  const bool wide = a.D == 128;
+  if (dtype == kBF16)
+    wide ? launch_states<bf16_t, 128>(a, stream) : launch_states<bf16_t, 64>(a, stream);
+  else
+    wide ? launch_states<f16_t, 128>(a, stream) : launch_states<f16_t, 64>(a, stream);
   return hipGetLastError();
 }
 

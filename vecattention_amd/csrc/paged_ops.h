@@ -135,10 +135,33 @@ struct PagedArgs {
   float* part;               // partial rows, see paged_attn.hip
   int2* split;               // per segment: first slot and last work-group, -1 written whole
   FastDiv by_page;
+  // Attention of rows that share their first keys (paged_prefix.hip): those keys of
+  // row n, and the rows of the group that begins there.  Its kernels leave states (m,
+  // l) and unnormalised rows of D: `state` one for each (request, query head).
+  const int32_t *prefix_lens, *group_rows;
+  float2* state_ml;
+  float* state;
 };
+
+// Keys of a prefix that are computed for its rows together: whole tiles of them.
+constexpr int kPrefixTile = 64;
+__host__ __device__ inline int32_t shared_keys(int32_t prefix, int64_t capacity) {
+  const int64_t n = prefix < capacity ? prefix : capacity;
+  return n <= 0 ? 0 : int32_t(n / kPrefixTile * kPrefixTile);
+}
 // Workspace bytes for these sizes (N, Hk, G, D, M, page), -1 where the units do
 // not fit 31 bits.
 int64_t paged_attn_workspace(int dtype, PagedArgs a);
 hipError_t launch_paged_attn(int dtype, PagedArgs a, void* workspace, hipStream_t stream);
+
+// The matrix-core form with 16-bit rows, whether it takes these tensors; and its
+// states of every row's own keys (from shared_keys on), `states` work-groups beyond
+// the first of a segment having slots of the partial rows.
+bool paged_tile_form(int dtype, const PagedArgs& a);
+int64_t paged_states_workspace(int dtype, PagedArgs& a);
+hipError_t launch_paged_states(int dtype, PagedArgs& a, hipStream_t stream);
+
+int64_t prefix_attn_workspace(int dtype, PagedArgs a);
+hipError_t launch_prefix_attn(int dtype, PagedArgs a, void* workspace, hipStream_t stream);
 
 }  // namespace va

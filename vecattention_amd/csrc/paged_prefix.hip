@@ -1,0 +1,718 @@
+// Decode attention of rows that share the first pages of a paged cache: the keys
+// that a group of rows shares are read, and multiplied, once for all of its rows.
+//   out[n, h] = sum_j softmax_j(q[n, h] . K[n, j] * scale) V[n, j]
+// splits at the prefix: with m the running maximum, l = sum_j 2^(s_j - m) and o =
+// sum_j 2^(s_j - m) V_j over the prefix and over the row's own keys, in log2 units,
+//   out = (o_p 2^(m_p - m) + o_r 2^(m_r - m)) / (l_p 2^(m_p - m) + l_r 2^(m_r - m)).
+//
+// Three launches: the prefixes (here), the rows' own keys (paged_attn.hip's tile
+// kernel, kState) and the merge.  A prefix's rows are the query heads of a kv head of
+// all its requests, 128 to a tile: a work-group takes one, each wave 32 of its rows,
+// and walks 64 keys a step as dense attention does (attn_dense.hip): K and V tiles go
+// to a ring of three LDS slots, S^T = K Q^T and O^T += V^T P^T on 32x32x16 matrix
+// instructions, weights from the scores' registers.  The steps of all (group, kv head,
+// tile) segments are dealt evenly to the work-groups (PagedShare), since the lengths
+// are known to the GPU only.
+#include "attn_common.h"
+#include "lanes.h"
+#include "mfma.h"
+#include "paged_ops.h"
+
+namespace va {
+
+namespace {
+
+constexpr int kThreads = 256, kWaves = 4;
+constexpr int kRows = 128;       // rows of a tile
+constexpr int kMostGroups = 512;
+constexpr int kIdKeys = 1024;    // keys whose page ids lie in LDS, for pages of any size
+
+// Where a state lies: that of a segment's first share with its row, (request, query
+// head); those of the shares that go on with a segment by the share.
+struct SharedArgs {
+  PagedArgs a;
+  FastDiv by_g;
+  float2* first_ml;   // (N * Hq)
+  float* first;       // (N * Hq, D)
+  float2* more_ml;    // (groups * kRows)
+  float* more;        // (groups * kRows, D)
+  int4* record;       // (N * Hq): first and last share of the row's segment, its place there
+  int32_t groups;
+  uint32_t least;     // steps of a share, at least
+};
+
+__device__ inline uint32_t plus(uint32_t a, uint32_t b) {
+  const uint32_t s = a + b;
+  return s < a ? 0xffffffffu : s;
+}
+
+// Rows and shared keys of the group that begins at row n, and its steps.
+struct Group {
+  int32_t first, rows, keys;
+  uint32_t tiles, steps;  // per (kv head, tile): steps
+  uint32_t base;          // number of its first step
+};
+__device__ inline Group group_at(const PagedArgs& a, int64_t n) {
+  Group g{int32_t(n), 0, 0, 0, 0, 0};
+  if (n >= a.N) return g;
+  const int64_t rows = a.group_rows[n] < a.N - n ? a.group_rows[n] : a.N - n;
+  if (rows <= 0) return g;
+  g.keys = shared_keys(a.prefix_lens[n], a.M * a.page);
+  g.rows = int32_t(rows);
+  g.tiles = uint32_t((rows * a.G + kRows - 1) / kRows);
+  g.steps = uint32_t(g.keys / kPrefixTile);
+  return g;
+}
+__device__ inline uint32_t all_steps(const PagedArgs& a, const Group& g) {
+  const uint64_t n = uint64_t(a.Hk) * g.tiles * g.steps;
+  return n < 0xffffffffu ? uint32_t(n) : 0xffffffffu;
+}
+
+// The steps of the groups in order: every thread holds the sum before its rows.
+struct Steps {
+  int32_t lo, hi;
+  uint32_t before, mine, total;
+};
+struct StepsLds {
+  uint32_t sum[kWaves];
+  Group found;
+};
+__device__ inline Steps count_steps(const PagedArgs& a, StepsLds& lds) {
+  const int32_t N = int32_t(a.N), per = (N + kThreads - 1) / kThreads;
+  const int lane = threadIdx.x % 64, w = threadIdx.x / 64;
+  Steps s;
+  s.lo = int32_t(threadIdx.x) * per < N ? int32_t(threadIdx.x) * per : N;
+  s.hi = s.lo + per < N ? s.lo + per : N;
+  s.mine = 0;
+  for (int32_t i = s.lo; i < s.hi; ++i) s.mine = plus(s.mine, all_steps(a, group_at(a, i)));
+  uint32_t x = s.mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t y = __shfl_up(x, d);
+    if (lane >= d) x = plus(x, y);
+  }
+  if (lane == 63) lds.sum[w] = x;
+  const uint32_t up = __shfl_up(x, 1);
+  __syncthreads();
+  s.before = lane ? up : 0;
+  s.total = 0;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    if (i < w) s.before = plus(s.before, lds.sum[i]);
+    s.total = plus(s.total, lds.sum[i]);
+  }
+  return s;
+}
+// The group of step u.
+__device__ inline Group find_step(const PagedArgs& a, const Steps& s, uint32_t u, StepsLds& lds) {
+  __syncthreads();  // the one found before has been read
+  if (u >= s.before && u - s.before < s.mine) {
+    uint32_t at = s.before;
+    for (int32_t i = s.lo; i < s.hi; ++i) {
+      Group g = group_at(a, i);
+      const uint32_t n = all_steps(a, g);
+      if (u - at < n) {
+        g.base = at;
+        lds.found = g;
+        break;
+      }
+      at = plus(at, n);
+    }
+  }
+  __syncthreads();
+  return lds.found;
+}
+
+// Shares: as many as give each `least` steps.
+__device__ inline PagedShare shares_of(const SharedArgs& x, uint32_t total) {
+  const uint32_t n = total / x.least;
+  return PagedShare(total, n < 1 ? 1 : n < uint32_t(x.groups) ? n : uint32_t(x.groups));
+}
+
+// 16 bytes a lane from `base` (uniform) + `offset` into LDS from base + kOffset on, as
+// copy16_row_to_lds_at.
+template <uint32_t kOffset>
+__device__ inline void copy16_at(uint32_t lds_base, uint64_t base, uint32_t offset) {
+  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 sc1"
+               :
+               : "s"(lds_base), "v"(offset), "s"(base), "n"(kOffset)
+               : "memory", "scc");
+}
+// The same with an address for each lane.
+template <uint32_t kOffset>
+__device__ inline void copy16_from(uint32_t lds_base, uint64_t address) {
+  asm volatile("s_add_u32 m0, %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off sc1"
+               :
+               : "s"(lds_base), "v"(address), "n"(kOffset)
+               : "memory", "scc");
+}
+
+template <typename T> constexpr bool kIsF16 = std::is_same_v<T, f16_t>;
+
+// w * x for a weight that is not zero, but may be too small for fp32.
+__device__ inline float weighed(float w, float x) {
+  return w != 0.f ? w * x : __builtin_fabsf(x) < __builtin_inff() ? 0.f : x;
+}
+
+// kWhole: pages of a multiple of 16 tokens, so that the 16 keys that a wave copies of
+// a tile lie in one.
+template <typename T, int D, bool kWhole>
+__global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void prefix_tile_kernel(SharedArgs x) {
+  using M = Mfma<T>;
+  using vec = typename M::vec;
+  constexpr int kRowBytes = 2 * D, NCH = D / 8;
+  constexpr uint32_t TB = uint32_t(kTileKeys * kRowBytes);
+  constexpr int RPC = 1024 / kRowBytes, H = kTileKeys * kRowBytes / 1024 / kWaves;
+  constexpr int NQK = D / 16, NB = D / 32, NPV = 4 * NB;
+  // fp16 holds weights down to 2^-24: those of 2^7 more are held, at most 2^15 of them.
+  constexpr float kBias = kIsF16<T> ? 7.f : 0.f;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[3 * TB];
+  __shared__ StepsLds lds;
+  __shared__ int sbad[kWaves], snan[kWaves];
+  __shared__ int32_t sid[kWhole ? 1 : kIdKeys + 2];
+  const PagedArgs& a = x.a;
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
+  const int l32 = lane % 32, hh = lane / 32;
+  const uint32_t page = uint32_t(a.page);
+
+  const Steps all = count_steps(a, lds);
+  const PagedShare share = shares_of(x, all.total);
+  // Neighbouring shares to one XCD.
+  const uint32_t eighth = share.groups / 8;
+  const uint32_t number = blockIdx.x < 8 * eighth
+                              ? blockIdx.x % 8 * eighth + blockIdx.x / 8
+                              : blockIdx.x;
+  if (number >= share.groups || all.total == 0) return;
+  const uint32_t begin = share.begin(number), end = share.begin(number + 1);
+
+  // ---- copies: copy c of this wave fills tile rows [(wave*H + c)*RPC, +RPC), the lane
+  // row crow + c*RPC, of which it fetches chunk p ^ chunk_swizzle(row).
+  const uint32_t crow = uint32_t(wave * H * RPC + lane / NCH);
+  const uint32_t c0off = uint32_t(16 * ((lane % NCH) ^ chunk_swizzle<D>(int(crow))));
+  constexpr uint32_t kXorStep = D == 128 ? 16 : 32;
+  static_assert(H * RPC == 16, "a wave copies 16 keys of a tile");
+  const uint32_t lds_copy_base =
+      uint32_t(__builtin_amdgcn_readfirstlane(int(lds_addr(smem) + uint32_t(wave * H * 1024))));
+  const uint32_t kn2 = uint32_t(a.kn) * 2, vn2 = uint32_t(a.vn) * 2;
+
+  // ---- LDS read offsets, as in dense attention.
+  const uint32_t k0 = uint32_t(l32 * kRowBytes + 16 * (hh ^ chunk_swizzle<D>(l32)));
+  uint32_t v0[2];
+  {
+    const int j = (lane % 16) / 4, g2 = 2 * ((lane / 16) % 2) + (lane % 4) / 2;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int R = 8 * r + 4 * hh + j;
+      v0[r] = uint32_t(R * kRowBytes + 16 * (g2 ^ chunk_swizzle<D>(R)) + 8 * (lane % 2));
+    }
+  }
+
+  Group grp = find_step(a, all, begin, lds);
+  for (uint32_t u = begin; u < end;) {
+    if (u - grp.base >= uint32_t(a.Hk) * grp.tiles * grp.steps) grp = find_step(a, all, u, lds);
+    const uint32_t seg = (u - grp.base) / grp.steps, t0 = (u - grp.base) - seg * grp.steps;
+    const uint32_t count = end - u < grp.steps - t0 ? end - u : grp.steps - t0;
+    const uint32_t hk = seg / grp.tiles, tile = seg - hk * grp.tiles;
+    const uint32_t rows = uint32_t(grp.rows) * uint32_t(a.G) - tile * kRows;  // from this tile on
+    const bool active = uint32_t(32 * wave) < rows;  // uniform
+    const uint32_t place = uint32_t(32 * wave + l32);
+    const uint32_t row = tile * kRows + (place < rows ? place : rows - 1);
+    const uint32_t in = x.by_g.div(row);
+    const int64_t request = grp.first + in, head = hk * a.G + (row - in * uint32_t(a.G));
+    const int32_t* table = a.table + int64_t(grp.first) * a.table_stride;
+    const T* kbase = static_cast<const T*>(a.k) + int64_t(hk) * a.kh;
+    const T* vbase = static_cast<const T*>(a.v) + int64_t(hk) * a.vh;
+    bool bad = false;
+
+    vec qreg[NQK];
+    {
+      const T* qp = static_cast<const T*>(a.q) + request * a.qn + head * a.qh;
+#pragma unroll
+      for (int s = 0; s < NQK; ++s)
+        qreg[s] = __builtin_bit_cast(vec, *reinterpret_cast<const uint4*>(qp + 16 * s + 8 * hh));
+    }
+
+    // Page ids are read as scalars, ahead of the copies that use them (a vector load would
+    // make the compiler wait for all copies in flight).
+    typedef const __attribute__((address_space(4))) int32_t* scalar_ptr;
+    const scalar_ptr ids = (scalar_ptr)(uintptr_t)table;
+    struct At { int64_t id; uint32_t in; };
+    auto key_of = [&](uint32_t t) {  // the wave's first key of tile t, at most the last tile's
+      const uint32_t last = t0 + count - 1;
+      return uint32_t(__builtin_amdgcn_readfirstlane(
+          int((t < last ? t : last) * kTileKeys + uint32_t(16 * wave))));
+    };
+    auto find = [&](uint32_t t) {
+      const uint32_t key = key_of(t), p = a.by_page.div(key);
+      return At{ids[p], key - p * page};
+    };
+    auto check = [&](At at) {
+      if (at.id < 0 || at.id >= a.num_pages) {
+        bad = true;
+        at.id = 0;
+      }
+      return at;
+    };
+    // Pages of any size: the ids of kIdKeys keys in LDS.
+    uint32_t id_first = 0;
+    auto fill_ids = [&](uint32_t t) {
+      if constexpr (!kWhole) {
+        const uint32_t from = t * kTileKeys, to = (t0 + count) * kTileKeys;
+        const uint32_t stop = to - from < kIdKeys ? to : from + kIdKeys;
+        id_first = a.by_page.div(from);
+        const uint32_t n = a.by_page.div(stop - 1) - id_first + 1;
+        for (uint32_t i = tid; i < n; i += kThreads) {
+          int32_t id = table[id_first + i];
+          if (id < 0 || id >= a.num_pages) {
+            bad = true;
+            id = 0;
+          }
+          sid[i] = id;
+        }
+        __syncthreads();
+      }
+    };
+    auto copy = [&](auto base_tag, auto c_tag, const T* from, int64_t sp, uint32_t row_bytes,
+                    const At& at, uint32_t t) {
+      constexpr int c = decltype(c_tag)::value;
+      uint32_t ch = c0off;
+      asm volatile("" : "+v"(ch));  // formed at each copy
+      if constexpr (kWhole) {
+        const uint64_t base = reinterpret_cast<uint64_t>(from + at.id * sp) +
+                              uint64_t(at.in + uint32_t(c * RPC)) * row_bytes;
+        copy16_at<decltype(base_tag)::value + c * 1024u>(
+            lds_copy_base, base, uint32_t(lane / NCH) * row_bytes + (ch ^ (c * kXorStep)));
+      } else {
+        const uint32_t last = t0 + count - 1;
+        const uint32_t key = (t < last ? t : last) * kTileKeys + crow + uint32_t(c * RPC);
+        const uint32_t p = a.by_page.div(key);
+        const uint64_t row_at = reinterpret_cast<uint64_t>(from + sid[p - id_first] * sp) +
+                                uint64_t(key - p * page) * row_bytes;
+        copy16_from<decltype(base_tag)::value + c * 1024u>(lds_copy_base,
+                                                           row_at + (ch ^ (c * kXorStep)));
+      }
+    };
+
+    f32x16_t o[NB];
+    float mneg, lsum;
+    auto kread = [&](const unsigned char* kb, uint32_t kx, int i) {
+      return __builtin_bit_cast(vec, *reinterpret_cast<const uint4*>(
+                                         kb + (kx ^ uint32_t(32 * (i % NQK))) +
+                                         i / NQK * 32 * kRowBytes));
+    };
+    auto vread = [&](const unsigned char* vb, uint32_t va, uint32_t vb1, int f) {
+      const int sub = f / NB, i = f % NB;
+      const unsigned char* p0 = vb + (va ^ uint32_t(64 * i)) + sub * 16 * kRowBytes;
+      const unsigned char* p1 = vb + (vb1 ^ uint32_t(64 * i)) + sub * 16 * kRowBytes;
+      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4_t*)(p0));
+      const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4_t*)(p1));
+      const s16x4_t both[2] = {lo, hi};
+      return __builtin_bit_cast(vec, both);
+    };
+
+    // The steps of the segment.  `again`: values that are not finite go in by a product
+    // of their own, with a weight of 1 for every key that has one, however small, and
+    // leave the others' sums as they were.
+    auto walk = [&](auto again) {
+      constexpr bool repeat = decltype(again)::value;
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
+      mneg = __builtin_inff();  // -(running maximum), less kBias
+      lsum = 0.f;
+      fill_ids(t0);
+      At now{}, next{};
+      if constexpr (kWhole) now = check(find(t0)), next = find(t0 + 1);
+      static_for<H>([&](auto c) { copy(lds_off<0>{}, c, kbase, a.kp, kn2, now, t0); });
+      static_for<H>([&](auto c) { copy(lds_off<TB>{}, c, vbase, a.vp, vn2, now, t0); });
+      auto step = [&](uint32_t t, auto r_tag) {
+        constexpr int r = decltype(r_tag)::value;
+        constexpr uint32_t k_this = uint32_t((2 * r) % 3) * TB;
+        constexpr uint32_t v_this = uint32_t((2 * r + 1) % 3) * TB;
+        constexpr uint32_t k_next = uint32_t((2 * r + 2) % 3) * TB;
+        constexpr uint32_t v_next = k_this;
+        if constexpr (!kWhole)
+          if (t > t0 && (t + 1 - t0) % (kIdKeys / kTileKeys) == 0 && t + 1 < t0 + count) {
+            __syncthreads();
+            fill_ids(t + 1);
+          }
+        if constexpr (kWhole) now = check(next), next = find(t + 2);
+        auto kcopies = [&](auto c) { copy(lds_off<k_next>{}, c, kbase, a.kp, kn2, now, t + 1); };
+        auto vcopies = [&](auto c) { copy(lds_off<v_next>{}, c, vbase, a.vp, vn2, now, t + 1); };
+        vm_lds_barrier_keep<H>();  // K(t) landed; every wave is done with V(t-1)
+        if (!active) {
+          static_for<H>(kcopies);
+          vm_lds_barrier_keep<H>();
+          static_for<H>(vcopies);
+          return;
+        }
+        f32x16_t sc[2];
+        {
+          const unsigned char* kb = smem + k_this;
+          uint32_t kx = k0;
+          asm volatile("" : "+v"(kx));
+          constexpr int kAhead = 2;
+          vec kf[2 * NQK];
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) kf[i] = kread(kb, kx, i);
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sc[hf][e] = 0.f;
+          __builtin_amdgcn_s_setprio(2);
+#pragma unroll
+          for (int i = 0; i < 2 * NQK; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (i + kAhead < 2 * NQK) kf[i + kAhead] = kread(kb, kx, i + kAhead);
+            sc[i / NQK] = M::run(kf[i], qreg[i % NQK], sc[i / NQK]);
+            static_for<H>([&](auto c) {
+              if (c * 2 * NQK / H == i) kcopies(c);
+            });
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          __builtin_amdgcn_s_setprio(0);
+        }
+        float tmax;
+        {
+          float u0 = max3_plain(sc[0][0], sc[0][1], sc[0][2]), u1 = sc[0][3];
+#pragma unroll
+          for (int e = 4; e < 32; e += 4) {
+            u0 = max3_plain(u0, sc[e / 16][e % 16], sc[e / 16][e % 16 + 1]);
+            u1 = max3_plain(u1, sc[e / 16][e % 16 + 2], sc[e / 16][e % 16 + 3]);
+          }
+          tmax = max_plain(u0, u1);
+        }
+        // The maximum moves when a score exceeds it by more than the slack.  Compared is the
+        // exponent that the score's weight would have, and scores are scaled and rounded as
+        // the maximum is: where the steps of both are larger than the slack (2^27 and more),
+        // a fused multiplication's exact product lies tens of powers of two beside them.
+        const float lead = tmax * a.scale_log2 + mneg;
+        const bool first = mneg == __builtin_inff();
+        if (__builtin_amdgcn_ballot_w64(first ? tmax > -__builtin_inff()
+                                              : lead > kRescaleSlack + kBias)) {
+          tmax = max_halves(tmax);
+          const float top = tmax * a.scale_log2;
+          float to = kBias - top;  // of this tile
+          if (!(to < mneg)) to = mneg;
+          const float alpha = to == mneg ? 1.f : __builtin_amdgcn_exp2f(to - mneg);
+#pragma unroll
+          for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              o[i][e] = repeat ? weighed(alpha, o[i][e]) : o[i][e] * alpha;
+          lsum *= alpha;
+          mneg = to;
+        }
+        const float bias = mneg == __builtin_inff() ? 0.f : mneg;  // no score yet: weights of 0
+        vec bfrag[4], one[repeat ? 4 : 1];
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          __builtin_amdgcn_sched_barrier(0);
+          float pr[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float s = sc[f / 2][8 * (f % 2) + e];
+            pr[e] = __builtin_amdgcn_exp2f(s * a.scale_log2 + bias);
+          }
+          bfrag[f] = M::pack(pr);
+          if constexpr (repeat) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              pr[e] = sc[f / 2][8 * (f % 2) + e] * a.scale_log2 != -__builtin_inff() ? 1.f : 0.f;
+            one[f] = M::pack(pr);
+          }
+        }
+        vm_lds_barrier_keep<H>();  // V(t) landed; every wave is done with K(t)
+        uint32_t va = v0[0], vb1 = v0[1];
+        asm volatile("" : "+v"(va), "+v"(vb1));
+        const unsigned char* vb = smem + v_this;
+        constexpr int kVAhead = 2;
+        vec vf[NPV];
+#pragma unroll
+        for (int f = 0; f < kVAhead; ++f) vf[f] = vread(vb, va, vb1, f);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int f = 0; f < NPV; ++f) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (f + kVAhead < NPV) vf[f + kVAhead] = vread(vb, va, vb1, f + kVAhead);
+          if constexpr (repeat) {
+            typedef uint16_t half8 __attribute__((ext_vector_type(8)));
+            constexpr uint16_t kExp = kIsF16<T> ? 0x7c00 : 0x7f80;
+            half8 fine = __builtin_bit_cast(half8, vf[f]), odd;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              odd[e] = (fine[e] & kExp) == kExp ? fine[e] : uint16_t(0);
+              fine[e] ^= odd[e];
+            }
+            o[f % NB] = M::run(__builtin_bit_cast(vec, fine), bfrag[f / NB], o[f % NB]);
+            o[f % NB] = M::run(__builtin_bit_cast(vec, odd), one[f / NB], o[f % NB]);
+          } else {
+            o[f % NB] = M::run(vf[f], bfrag[f / NB], o[f % NB]);
+          }
+          static_for<H>([&](auto c) {
+            if (c * NPV / H == f) vcopies(c);
+          });
+#pragma unroll
+          for (int j = f * 16 / NPV; j < (f + 1) * 16 / NPV; ++j)
+            lsum = M::add_pair(bfrag[j / 4], j % 4, lsum);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(0);
+      };
+      const uint32_t stop = t0 + count;
+      for (uint32_t t = t0; t < stop; t += 3) {
+        step(t, std::integral_constant<int, 0>{});
+        if (t + 1 < stop) step(t + 1, std::integral_constant<int, 1>{});
+        if (t + 2 < stop) step(t + 2, std::integral_constant<int, 2>{});
+      }
+      vm_lds_barrier();  // the last copies have landed
+    };
+    walk(std::false_type{});
+    bool nan = false;
+    if (active) {
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) nan |= o[i][e] != o[i][e];
+    }
+    if (lane == 0) sbad[wave] = 0;
+    if (__any(nan) && lane == 0) snan[wave] = 1;
+    if (!__any(nan) && lane == 0) snan[wave] = 0;
+    if (__any(bad) && lane == 0) sbad[wave] = 1;
+    lds_barrier();
+    const bool some_nan = snan[0] | snan[1] | snan[2] | snan[3];
+    const bool some_bad = sbad[0] | sbad[1] | sbad[2] | sbad[3];
+    if (some_nan && !some_bad) walk(std::true_type{});
+    float l = sum_halves(lsum);
+    if (some_bad) l = __builtin_nanf("");
+    if (active && place < rows) {
+      const bool starts = t0 == 0;
+      const int64_t q_row = request * a.Hk * a.G + head;
+      const int64_t to = starts ? q_row : int64_t(number) * kRows + place;
+      float* out = (starts ? x.first : x.more) + to * D;
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<float4*>(out + 32 * i + 8 * g + 4 * hh) =
+              make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
+      if (hh == 0) {
+        (starts ? x.first_ml : x.more_ml)[to] = make_float2(-mneg, l);
+        if (starts)
+          x.record[q_row] = make_int4(int(number), int(share.owner(u + grp.steps - 1)), int(place),
+                                      0);
+      }
+    }
+    lds_barrier();  // the flags have been read
+    u += count;
+  }
+}
+
+// Joins the states of a (request, query head): those of the prefix's shares, then
+// those of its own keys, always in this order.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void prefix_merge_kernel(SharedArgs x) {
+  constexpr int kLanes = D / 4, kSide = kThreads / kLanes, U = 4, kMost = 2 * kMostGroups + 2;
+  typedef float vec4 __attribute__((ext_vector_type(4)));
+  __shared__ float weight[kMost];
+  __shared__ vec4 sacc[kThreads];
+  __shared__ float top[kWaves], den[kWaves];
+  const PagedArgs& a = x.a;
+  const int64_t row = blockIdx.x;
+  const uint32_t Hq = uint32_t(a.Hk * a.G), n = uint32_t(row) / Hq, head = uint32_t(row) - n * Hq;
+  T* out = static_cast<T*>(a.out) + n * a.on + head * a.oh;
+  const int c = threadIdx.x % kLanes, side = threadIdx.x / kLanes;
+  if (a.lens[n] <= 0) {
+    if (side == 0)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[4 * c + e] = Round<T>::store(0.f);
+    return;
+  }
+  // The prefix's shares, and those of the row's own segment.
+  int pre = 0, pre_from = 0, place = 0;
+  if (shared_keys(a.prefix_lens[n], a.M * a.page) > 0) {
+    const int4 r = x.record[row];
+    pre_from = r.x < 0 ? 0 : r.x < x.groups ? r.x : x.groups - 1;
+    const int last = r.y < pre_from ? pre_from : r.y < x.groups ? r.y : x.groups - 1;
+    place = r.z & (kRows - 1);
+    pre = last - pre_from + 1;
+  }
+  const uint32_t hk = head / uint32_t(a.G), in = head - hk * uint32_t(a.G);
+  const uint32_t tile = in / uint32_t(a.rows), r = in - tile * uint32_t(a.rows);
+  const int2 split = a.split[int64_t(n) * a.per_request + hk * uint32_t(a.tiles) + tile];
+  const int own_from = split.x < 0 ? 0 : split.x / 2;
+  const int parts = pre + 1 + (split.x < 0 ? 0 : split.y - own_from);
+  const int64_t slots = 2 * int64_t(a.groups);
+  auto ml = [&](int i) {
+    if (i < pre)
+      return i == 0 ? x.first_ml[row] : x.more_ml[int64_t(pre_from + i) * kRows + place];
+    i -= pre;
+    return i == 0 ? a.state_ml[row]
+                  : reinterpret_cast<const float2*>(a.part)[2 * (own_from + i) * a.rows + r];
+  };
+  auto state = [&](int i) {
+    const float* p;
+    if (i < pre) {
+      p = i == 0 ? x.first + row * D : x.more + (int64_t(pre_from + i) * kRows + place) * D;
+    } else {
+      i -= pre;
+      p = i == 0 ? a.state + row * D
+                 : a.part + 2 * slots * a.rows + (int64_t(2 * (own_from + i)) * a.rows + r) * D;
+    }
+    return reinterpret_cast<const vec4*>(p)[c];
+  };
+  const int me = threadIdx.x;
+  float m = -__builtin_inff();
+  for (int i = me; i < parts; i += kThreads) {
+    const float2 y = ml(i);
+    if (!(y.y == 0.f)) m = __builtin_fmaxf(m, y.x);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) m = __builtin_fmaxf(m, __shfl_xor(m, d));
+  if (me % 64 == 0) top[me / 64] = m;
+  lds_barrier();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) m = __builtin_fmaxf(m, top[w]);
+  float l = 0.f;
+  for (int i = me; i < parts; i += kThreads) {
+    const float2 y = ml(i);
+    const float f = __builtin_amdgcn_exp2f(y.x - m);
+    weight[i] = y.y == 0.f ? -1.f : f;  // -1: no weight at all
+    l += y.y == 0.f ? 0.f : f * y.y;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
+  if (me % 64 == 0) den[me / 64] = l;
+  lds_barrier();
+  vec4 acc = vec4(0.f);
+  for (int from = side; from < parts; from += U * kSide) {
+    vec4 y[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      y[i] = state(from + i * kSide < parts ? from + i * kSide : parts - 1);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const float f = from + i * kSide < parts ? weight[from + i * kSide] : -1.f;
+      if (f > 0.f) acc += f * y[i];
+      if (f == 0.f || f != f)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += f != f ? f : weighed(f, y[i][e]);
+    }
+  }
+  sacc[me] = acc;
+  lds_barrier();
+  if (side != 0) return;
+#pragma unroll
+  for (int i = 1; i < kSide; ++i) acc += sacc[i * kLanes + c];
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) l += den[w];
+  struct alignas(sizeof(T) * 4) Out { T v[4]; } y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y.v[e] = Round<T>::store(acc[e] / l);
+  *reinterpret_cast<Out*>(out + 4 * c) = y;
+}
+
+int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
+
+// Work-groups for the prefixes: no more than there can be steps.
+int64_t prefix_groups(const PagedArgs& a) {
+  const int64_t tiles = a.N * a.G / kRows + a.N;
+  const int64_t steps = a.Hk * tiles * (a.M * a.page / kPrefixTile);
+  return steps < 1 ? 1 : steps < kMostGroups ? steps : kMostGroups;
+}
+
+template <typename T, int D>
+hipError_t launch_prefix(const SharedArgs& x, hipStream_t stream) {
+  const dim3 grid{unsigned(x.groups)}, block{kThreads};
+  if (x.a.page % 16 == 0)
+    hipLaunchKernelGGL((prefix_tile_kernel<T, D, true>), grid, block, 0, stream, x);
+  else
+    hipLaunchKernelGGL((prefix_tile_kernel<T, D, false>), grid, block, 0, stream, x);
+  return hipGetLastError();
+}
+template <typename T, int D>
+hipError_t launch_join(const SharedArgs& x, hipStream_t stream) {
+  hipLaunchKernelGGL((prefix_merge_kernel<T, D>), dim3(unsigned(x.a.N * x.a.Hk * x.a.G)),
+                     dim3(kThreads), 0, stream, x);
+  return hipGetLastError();
+}
+
+// Whether the prefix is computed once: 16-bit rows that the matrix-core form takes, a
+// scale that orders scores as the products are ordered, and tables that could share a
+// tile of keys.
+bool shares_prefix(int dtype, const PagedArgs& a) {
+  return dtype != kF32 && a.N > 1 && a.M * a.page >= kPrefixTile && a.scale_log2 >= 0.f &&
+         a.kn < (int64_t(1) << 26) && a.vn < (int64_t(1) << 26) && paged_tile_form(dtype, a);
+}
+
+// The regions of the workspace, behind those of the rows' own keys (`own` bytes).
+int64_t lay_out(PagedArgs& a, SharedArgs* x, char* work, int64_t own) {
+  const int64_t rows = a.N * a.Hk * a.G, groups = prefix_groups(a);
+  int64_t at = own;
+  auto take = [&](int64_t bytes) {
+    char* p = work + at;
+    at += round256(bytes);
+    return p;
+  };
+  char* p[7];
+  p[0] = take(8 * rows);
+  p[1] = take(4 * rows * a.D);
+  p[2] = take(8 * rows);
+  p[3] = take(4 * rows * a.D);
+  p[4] = take(8 * groups * kRows);
+  p[5] = take(4 * groups * kRows * a.D);
+  p[6] = take(16 * rows);
+  if (x) {
+    a.state_ml = reinterpret_cast<float2*>(p[0]);
+    a.state = reinterpret_cast<float*>(p[1]);
+    x->first_ml = reinterpret_cast<float2*>(p[2]);
+    x->first = reinterpret_cast<float*>(p[3]);
+    x->more_ml = reinterpret_cast<float2*>(p[4]);
+    x->more = reinterpret_cast<float*>(p[5]);
+    x->record = reinterpret_cast<int4*>(p[6]);
+    x->groups = int32_t(groups);
+    x->by_g = FastDiv(uint32_t(a.G));
+    x->least = 4;
+    x->a = a;
+  }
+  return at;
+}
+
+}  // namespace
+
+int64_t prefix_attn_workspace(int dtype, PagedArgs a) {
+  const int64_t plain = paged_attn_workspace(dtype, a);
+  if (plain < 0 || dtype == kF32 || (a.D != 64 && a.D != 128)) return plain;
+  const int64_t own = paged_states_workspace(dtype, a);
+  if (own < 0) return -1;
+  const int64_t all = lay_out(a, nullptr, nullptr, own);
+  return all > plain ? all : plain;
+}
+
+hipError_t launch_prefix_attn(int dtype, PagedArgs a, void* workspace, hipStream_t stream) {
+  if (!shares_prefix(dtype, a)) return launch_paged_attn(dtype, a, workspace, stream);
+  char* work = static_cast<char*>(workspace);
+  const int64_t own = paged_states_workspace(dtype, a);
+  if (own < 0) return hipErrorInvalidValue;
+  a.part = reinterpret_cast<float*>(work);
+  a.split = reinterpret_cast<int2*>(work + own - round256(8 * a.N * a.per_request));
+  SharedArgs x{};
+  lay_out(a, &x, work, own);
+  const bool wide = a.D == 128, bf = dtype == kBF16;
+  hipError_t e = bf ? (wide ? launch_prefix<bf16_t, 128>(x, stream)
+                            : launch_prefix<bf16_t, 64>(x, stream))
+                    : (wide ? launch_prefix<f16_t, 128>(x, stream)
+                            : launch_prefix<f16_t, 64>(x, stream));
+  if (e != hipSuccess) return e;
+  e = launch_paged_states(dtype, x.a, stream);
+  if (e != hipSuccess) return e;
+  return bf ? (wide ? launch_join<bf16_t, 128>(x, stream) : launch_join<bf16_t, 64>(x, stream))
+            : (wide ? launch_join<f16_t, 128>(x, stream) : launch_join<f16_t, 64>(x, stream));
+}
+
+}  // namespace va
