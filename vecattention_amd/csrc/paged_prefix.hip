@@ -24,21 +24,21 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kRows = 128;       // rows of a tile
-constexpr int kMostGroups = 512;
+constexpr int kMostGroups = 768;  // three a CU
 constexpr int kIdKeys = 1024;    // keys whose page ids lie in LDS, for pages of any size
 
-// Where a state lies: that of a segment's first share with its row, (request, query
-// head); those of the shares that go on with a segment by the share.
+// Where a state lies: that of the first piece with its row, (request, query head); those
+// of the others in slots of `stride` rows.
 struct SharedArgs {
   PagedArgs a;
   FastDiv by_g;
   float2* first_ml;   // (N * Hq)
   float* first;       // (N * Hq, D)
-  float2* more_ml;    // (groups * kRows)
-  float* more;        // (groups * kRows, D)
-  int4* record;       // (N * Hq): first and last share of the row's segment, its place there
-  int32_t groups;
-  uint32_t least;     // steps of a share, at least
+  float2* more_ml;    // (groups slots)
+  float* more;
+  int4* record;       // (N * Hq): pieces of the row behind its first, their slots' first, its row
+  int32_t groups, stride;  // stride: rows of a tile that there can be
+  uint32_t least;          // steps of a piece, at least
 };
 
 __device__ inline uint32_t plus(uint32_t a, uint32_t b) {
@@ -46,87 +46,122 @@ __device__ inline uint32_t plus(uint32_t a, uint32_t b) {
   return s < a ? 0xffffffffu : s;
 }
 
-// Rows and shared keys of the group that begins at row n, and its steps.
+// Rows and shared keys of the group that begins at row n: `tiles` tiles of rows for
+// each kv head, `steps` steps of each.
 struct Group {
-  int32_t first, rows, keys;
-  uint32_t tiles, steps;  // per (kv head, tile): steps
-  uint32_t base;          // number of its first step
+  int32_t first, rows;
+  uint32_t tiles, steps;
 };
 __device__ inline Group group_at(const PagedArgs& a, int64_t n) {
-  Group g{int32_t(n), 0, 0, 0, 0, 0};
+  Group g{int32_t(n), 0, 0, 0};
   if (n >= a.N) return g;
   const int64_t rows = a.group_rows[n] < a.N - n ? a.group_rows[n] : a.N - n;
   if (rows <= 0) return g;
-  g.keys = shared_keys(a.prefix_lens[n], a.M * a.page);
   g.rows = int32_t(rows);
-  g.tiles = uint32_t((rows * a.G + kRows - 1) / kRows);
-  g.steps = uint32_t(g.keys / kPrefixTile);
+  g.steps = uint32_t(shared_keys(a.prefix_lens[n], a.M * a.page) / kPrefixTile);
+  g.tiles = g.steps ? uint32_t((rows * a.G + kRows - 1) / kRows) : 0;
   return g;
 }
-__device__ inline uint32_t all_steps(const PagedArgs& a, const Group& g) {
-  const uint64_t n = uint64_t(a.Hk) * g.tiles * g.steps;
-  return n < 0xffffffffu ? uint32_t(n) : 0xffffffffu;
+__device__ inline uint32_t uniform(uint32_t x) {
+  return uint32_t(__builtin_amdgcn_readfirstlane(int(x)));
 }
 
-// The steps of the groups in order: every thread holds the sum before its rows.
-struct Steps {
-  int32_t lo, hi;
-  uint32_t before, mine, total;
-};
-struct StepsLds {
-  uint32_t sum[kWaves];
+// A piece: some steps of a tile of rows of a kv head.  Every work-group counts them
+// for itself.  The pieces of a group are numbered by kv head, then range of keys, then
+// tile, so that work-groups of neighbouring numbers, which run on one XCD at a time,
+// read the same keys from its L2 (in the order of tiles, then ranges, 131072 keys of
+// 448 rows of 4 kv heads came from the fabric four times, at the most that it gives).
+struct Sum { uint32_t pieces, more; };  // `more`: those that are not the first of their rows
+struct PiecesLds {
+  uint2 sum[kWaves];
+  Sum before[kThreads], mine[kThreads];
   Group found;
+  Sum at;
 };
-__device__ inline Steps count_steps(const PagedArgs& a, StepsLds& lds) {
-  const int32_t N = int32_t(a.N), per = (N + kThreads - 1) / kThreads;
+struct Pieces {
+  uint32_t length, count;  // steps of a piece, at most; all pieces
+};
+__device__ inline Sum pieces_of(const PagedArgs& a, const Group& g, uint32_t length) {
+  const uint32_t segments = uint32_t(a.Hk) * g.tiles;
+  if (!segments) return Sum{0, 0};
+  const uint32_t ranges = (g.steps - 1) / length + 1;
+  const uint64_t n = uint64_t(segments) * ranges;
+  const uint32_t all = n < 0xffffffffu ? uint32_t(n) : 0xffffffffu;
+  return Sum{all, all - segments};
+}
+// Sums over the work-group of two values, and over the threads before.
+__device__ inline uint2 block_sum(uint2 x, uint2* part, uint2* before) {
   const int lane = threadIdx.x % 64, w = threadIdx.x / 64;
-  Steps s;
-  s.lo = int32_t(threadIdx.x) * per < N ? int32_t(threadIdx.x) * per : N;
-  s.hi = s.lo + per < N ? s.lo + per : N;
-  s.mine = 0;
-  for (int32_t i = s.lo; i < s.hi; ++i) s.mine = plus(s.mine, all_steps(a, group_at(a, i)));
-  uint32_t x = s.mine;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t y = __shfl_up(x, d);
-    if (lane >= d) x = plus(x, y);
+    const uint32_t u = __shfl_up(x.x, d), v = __shfl_up(x.y, d);
+    if (lane >= d) x = make_uint2(plus(x.x, u), plus(x.y, v));
   }
-  if (lane == 63) lds.sum[w] = x;
-  const uint32_t up = __shfl_up(x, 1);
+  __syncthreads();  // the sums before have been read
+  if (lane == 63) part[w] = x;
+  const uint32_t u = __shfl_up(x.x, 1), v = __shfl_up(x.y, 1);
   __syncthreads();
-  s.before = lane ? up : 0;
-  s.total = 0;
+  uint2 b = lane ? make_uint2(u, v) : make_uint2(0, 0), total = make_uint2(0, 0);
 #pragma unroll
   for (int i = 0; i < kWaves; ++i) {
-    if (i < w) s.before = plus(s.before, lds.sum[i]);
-    s.total = plus(s.total, lds.sum[i]);
+    if (i < w) b = make_uint2(plus(b.x, part[i].x), plus(b.y, part[i].y));
+    total = make_uint2(plus(total.x, part[i].x), plus(total.y, part[i].y));
   }
-  return s;
+  *before = b;
+  return make_uint2(uniform(total.x), uniform(total.y));
 }
-// The group of step u.
-__device__ inline Group find_step(const PagedArgs& a, const Steps& s, uint32_t u, StepsLds& lds) {
+__device__ inline int32_t run_of(const PagedArgs& a) {
+  return (int32_t(a.N) + kThreads - 1) / kThreads;
+}
+__device__ inline Pieces count_pieces(const PagedArgs& a, uint32_t groups, uint32_t least,
+                                      PiecesLds& lds) {
+  const int32_t N = int32_t(a.N), per = run_of(a), lo = int32_t(threadIdx.x) * per;
+  uint2 mine = make_uint2(0, 0), before;
+  for (int32_t i = lo; i < lo + per && i < N; ++i) {
+    const Group g = group_at(a, i);
+    const uint64_t segments = uint64_t(a.Hk) * g.tiles, steps = segments * g.steps;
+    mine = make_uint2(plus(mine.x, steps < 0xffffffffu ? uint32_t(steps) : 0xffffffffu),
+                      plus(mine.y, uint32_t(segments)));
+  }
+  const uint2 all = block_sum(mine, lds.sum, &before);
+  // A work-group one piece, where there are fewer segments than work-groups.
+  const uint32_t spare = all.y < groups / 2 ? groups - all.y : groups / 2;
+  Pieces p;
+  p.length = all.x / (spare ? spare : 1) + 1;
+  if (p.length < least) p.length = least;
+  mine = make_uint2(0, 0);
+  for (int32_t i = lo; i < lo + per && i < N; ++i) {
+    const Sum s = pieces_of(a, group_at(a, i), p.length);
+    mine = make_uint2(plus(mine.x, s.pieces), plus(mine.y, s.more));
+  }
+  p.count = block_sum(mine, lds.sum, &before).x;
+  lds.before[threadIdx.x] = Sum{before.x, before.y};
+  lds.mine[threadIdx.x] = Sum{mine.x, mine.y};
+  return p;
+}
+// The group of a piece, and the pieces before the group.
+__device__ inline Group find_piece(const PagedArgs& a, uint32_t piece, uint32_t length,
+                                   PiecesLds& lds, Sum* before) {
   __syncthreads();  // the one found before has been read
-  if (u >= s.before && u - s.before < s.mine) {
-    uint32_t at = s.before;
-    for (int32_t i = s.lo; i < s.hi; ++i) {
-      Group g = group_at(a, i);
-      const uint32_t n = all_steps(a, g);
-      if (u - at < n) {
-        g.base = at;
+  const int32_t per = run_of(a), lo = int32_t(threadIdx.x) * per;
+  Sum at = lds.before[threadIdx.x];
+  if (piece >= at.pieces && piece - at.pieces < lds.mine[threadIdx.x].pieces) {
+    for (int32_t i = lo; i < lo + per && i < a.N; ++i) {
+      const Group g = group_at(a, i);
+      const Sum n = pieces_of(a, g, length);
+      if (piece - at.pieces < n.pieces) {
         lds.found = g;
+        lds.at = at;
         break;
       }
-      at = plus(at, n);
+      at = Sum{plus(at.pieces, n.pieces), plus(at.more, n.more)};
     }
   }
   __syncthreads();
-  return lds.found;
-}
-
-// Shares: as many as give each `least` steps.
-__device__ inline PagedShare shares_of(const SharedArgs& x, uint32_t total) {
-  const uint32_t n = total / x.least;
-  return PagedShare(total, n < 1 ? 1 : n < uint32_t(x.groups) ? n : uint32_t(x.groups));
+  *before = Sum{uniform(lds.at.pieces), uniform(lds.at.more)};
+  const Group g = lds.found;  // in scalar registers
+  return Group{int32_t(uniform(uint32_t(g.first))), int32_t(uniform(uint32_t(g.rows))),
+               uniform(g.tiles), uniform(g.steps)};
 }
 
 // 16 bytes a lane from `base` (uniform) + `offset` into LDS from base + kOffset on, as
@@ -157,7 +192,7 @@ __device__ inline float weighed(float w, float x) {
 // kWhole: pages of a multiple of 16 tokens, so that the 16 keys that a wave copies of
 // a tile lie in one.
 template <typename T, int D, bool kWhole>
-__global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void prefix_tile_kernel(SharedArgs x) {
+__global__ __launch_bounds__(kThreads, D == 128 ? (kWhole ? 3 : 2) : 4) void prefix_tile_kernel(SharedArgs x) {
   using M = Mfma<T>;
   using vec = typename M::vec;
   constexpr int kRowBytes = 2 * D, NCH = D / 8;
@@ -167,8 +202,8 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void prefix_tile_kernel
   // fp16 holds weights down to 2^-24: those of 2^7 more are held, at most 2^15 of them.
   constexpr float kBias = kIsF16<T> ? 7.f : 0.f;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[3 * TB];
-  __shared__ StepsLds lds;
-  __shared__ int sbad[kWaves], snan[kWaves];
+  __shared__ PiecesLds lds;
+  __shared__ int sbad[kWaves];
   __shared__ int32_t sid[kWhole ? 1 : kIdKeys + 2];
   const PagedArgs& a = x.a;
   const int tid = threadIdx.x;
@@ -176,15 +211,12 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void prefix_tile_kernel
   const int l32 = lane % 32, hh = lane / 32;
   const uint32_t page = uint32_t(a.page);
 
-  const Steps all = count_steps(a, lds);
-  const PagedShare share = shares_of(x, all.total);
-  // Neighbouring shares to one XCD.
-  const uint32_t eighth = share.groups / 8;
+  const Pieces all = count_pieces(a, uint32_t(x.groups), x.least, lds);
+  // Neighbouring pieces to one XCD.
+  const uint32_t eighth = uint32_t(x.groups) / 8;
   const uint32_t number = blockIdx.x < 8 * eighth
                               ? blockIdx.x % 8 * eighth + blockIdx.x / 8
                               : blockIdx.x;
-  if (number >= share.groups || all.total == 0) return;
-  const uint32_t begin = share.begin(number), end = share.begin(number + 1);
 
   // ---- copies: copy c of this wave fills tile rows [(wave*H + c)*RPC, +RPC), the lane
   // row crow + c*RPC, of which it fetches chunk p ^ chunk_swizzle(row).
@@ -195,6 +227,7 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void prefix_tile_kernel
   const uint32_t lds_copy_base =
       uint32_t(__builtin_amdgcn_readfirstlane(int(lds_addr(smem) + uint32_t(wave * H * 1024))));
   const uint32_t kn2 = uint32_t(a.kn) * 2, vn2 = uint32_t(a.vn) * 2;
+  const uint32_t krow = uint32_t(lane / NCH) * kn2, vrow = uint32_t(lane / NCH) * vn2;
 
   // ---- LDS read offsets, as in dense attention.
   const uint32_t k0 = uint32_t(l32 * kRowBytes + 16 * (hh ^ chunk_swizzle<D>(l32)));
@@ -208,18 +241,28 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void prefix_tile_kernel
     }
   }
 
-  Group grp = find_step(a, all, begin, lds);
-  for (uint32_t u = begin; u < end;) {
-    if (u - grp.base >= uint32_t(a.Hk) * grp.tiles * grp.steps) grp = find_step(a, all, u, lds);
-    const uint32_t seg = (u - grp.base) / grp.steps, t0 = (u - grp.base) - seg * grp.steps;
-    const uint32_t count = end - u < grp.steps - t0 ? end - u : grp.steps - t0;
-    const uint32_t hk = seg / grp.tiles, tile = seg - hk * grp.tiles;
+  for (uint32_t piece = number; piece < all.count; piece += uint32_t(x.groups)) {
+    Sum before;
+    const Group grp = find_piece(a, piece, all.length, lds, &before);
+    const uint32_t ranges = (grp.steps - 1) / all.length + 1;
+    const uint32_t at = piece - before.pieces, hk = at / (ranges * grp.tiles);
+    const uint32_t in_head = at - hk * ranges * grp.tiles, range = in_head / grp.tiles;
+    const uint32_t tile = in_head - range * grp.tiles, t0 = range * all.length;
+    const uint32_t count = grp.steps - t0 < all.length ? grp.steps - t0 : all.length;
+    // The slots of the segment's further pieces.
+    const uint32_t slots = before.more + (hk * grp.tiles + tile) * (ranges - 1);
     const uint32_t rows = uint32_t(grp.rows) * uint32_t(a.G) - tile * kRows;  // from this tile on
     const bool active = uint32_t(32 * wave) < rows;  // uniform
-    const uint32_t place = uint32_t(32 * wave + l32);
-    const uint32_t row = tile * kRows + (place < rows ? place : rows - 1);
-    const uint32_t in = x.by_g.div(row);
-    const int64_t request = grp.first + in, head = hk * a.G + (row - in * uint32_t(a.G));
+    // The lane's row: request first + row / G, head row % G of the kv head.
+    auto place_of = [&](uint32_t& place, int64_t& request, int64_t& head) {
+      uint32_t l = uint32_t(l32);
+      asm volatile("" : "+v"(l));  // formed where it is used
+      place = uint32_t(32 * wave) + l;
+      const uint32_t row = tile * kRows + (place < rows ? place : rows - 1);
+      const uint32_t in = x.by_g.div(row);
+      request = grp.first + in;
+      head = hk * a.G + (row - in * uint32_t(a.G));
+    };
     const int32_t* table = a.table + int64_t(grp.first) * a.table_stride;
     const T* kbase = static_cast<const T*>(a.k) + int64_t(hk) * a.kh;
     const T* vbase = static_cast<const T*>(a.v) + int64_t(hk) * a.vh;
@@ -227,32 +270,36 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void prefix_tile_kernel
 
     vec qreg[NQK];
     {
+      uint32_t place;
+      int64_t request, head;
+      place_of(place, request, head);
       const T* qp = static_cast<const T*>(a.q) + request * a.qn + head * a.qh;
 #pragma unroll
       for (int s = 0; s < NQK; ++s)
         qreg[s] = __builtin_bit_cast(vec, *reinterpret_cast<const uint4*>(qp + 16 * s + 8 * hh));
     }
+#pragma unroll
+    for (int s = 0; s < NQK; ++s) asm volatile("" ::"v"(qreg[s]));  // landed before the copies
 
     // Page ids are read as scalars, ahead of the copies that use them (a vector load would
     // make the compiler wait for all copies in flight).
     typedef const __attribute__((address_space(4))) int32_t* scalar_ptr;
     const scalar_ptr ids = (scalar_ptr)(uintptr_t)table;
-    struct At { int64_t id; uint32_t in; };
-    auto key_of = [&](uint32_t t) {  // the wave's first key of tile t, at most the last tile's
+    struct Next { int32_t id; uint32_t in; };
+    struct At { uint64_t k, v; };  // addresses of the wave's first key
+    auto find = [&](uint32_t t) {  // of tile t, at most the last one
       const uint32_t last = t0 + count - 1;
-      return uint32_t(__builtin_amdgcn_readfirstlane(
-          int((t < last ? t : last) * kTileKeys + uint32_t(16 * wave))));
+      const uint32_t key = (t < last ? t : last) * kTileKeys + uint32_t(16 * wave);
+      const uint32_t p = a.by_page.div(key);
+      return Next{ids[p], key - p * page};
     };
-    auto find = [&](uint32_t t) {
-      const uint32_t key = key_of(t), p = a.by_page.div(key);
-      return At{ids[p], key - p * page};
-    };
-    auto check = [&](At at) {
-      if (at.id < 0 || at.id >= a.num_pages) {
+    auto check = [&](Next n) {
+      if (uint32_t(n.id) >= uint32_t(a.num_pages)) {
         bad = true;
-        at.id = 0;
+        n.id = 0;
       }
-      return at;
+      return At{reinterpret_cast<uint64_t>(kbase + n.id * a.kp) + n.in * kn2,
+                reinterpret_cast<uint64_t>(vbase + n.id * a.vp) + n.in * vn2};
     };
     // Pages of any size: the ids of kIdKeys keys in LDS.
     uint32_t id_first = 0;
@@ -273,25 +320,29 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void prefix_tile_kernel
         __syncthreads();
       }
     };
-    auto copy = [&](auto base_tag, auto c_tag, const T* from, int64_t sp, uint32_t row_bytes,
-                    const At& at, uint32_t t) {
+    auto copy = [&](auto base_tag, auto c_tag, uint64_t at, const T* from, int64_t sp,
+                    uint32_t row_bytes, uint32_t row_at, uint32_t t) {
       constexpr int c = decltype(c_tag)::value;
       uint32_t ch = c0off;
       asm volatile("" : "+v"(ch));  // formed at each copy
       if constexpr (kWhole) {
-        const uint64_t base = reinterpret_cast<uint64_t>(from + at.id * sp) +
-                              uint64_t(at.in + uint32_t(c * RPC)) * row_bytes;
         copy16_at<decltype(base_tag)::value + c * 1024u>(
-            lds_copy_base, base, uint32_t(lane / NCH) * row_bytes + (ch ^ (c * kXorStep)));
+            lds_copy_base, at + uint32_t(c * RPC) * row_bytes, row_at + (ch ^ (c * kXorStep)));
       } else {
         const uint32_t last = t0 + count - 1;
         const uint32_t key = (t < last ? t : last) * kTileKeys + crow + uint32_t(c * RPC);
         const uint32_t p = a.by_page.div(key);
-        const uint64_t row_at = reinterpret_cast<uint64_t>(from + sid[p - id_first] * sp) +
-                                uint64_t(key - p * page) * row_bytes;
+        const uint64_t row = reinterpret_cast<uint64_t>(from + sid[p - id_first] * sp) +
+                             (key - p * page) * row_bytes;
         copy16_from<decltype(base_tag)::value + c * 1024u>(lds_copy_base,
-                                                           row_at + (ch ^ (c * kXorStep)));
+                                                           row + (ch ^ (c * kXorStep)));
       }
+    };
+    auto copy_k = [&](auto base_tag, auto c_tag, const At& at, uint32_t t) {
+      copy(base_tag, c_tag, at.k, kbase, a.kp, kn2, krow, t);
+    };
+    auto copy_v = [&](auto base_tag, auto c_tag, const At& at, uint32_t t) {
+      copy(base_tag, c_tag, at.v, vbase, a.vp, vn2, vrow, t);
     };
 
     f32x16_t o[NB];
@@ -313,11 +364,7 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void prefix_tile_kernel
       return __builtin_bit_cast(vec, both);
     };
 
-    // The steps of the segment.  `again`: values that are not finite go in by a product
-    // of their own, with a weight of 1 for every key that has one, however small, and
-    // leave the others' sums as they were.
-    auto walk = [&](auto again) {
-      constexpr bool repeat = decltype(again)::value;
+    {
 #pragma unroll
       for (int i = 0; i < NB; ++i)
 #pragma unroll
@@ -325,11 +372,13 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void prefix_tile_kernel
       mneg = __builtin_inff();  // -(running maximum), less kBias
       lsum = 0.f;
       fill_ids(t0);
-      At now{}, next{};
+      At now{};
+      Next next{};
       if constexpr (kWhole) now = check(find(t0)), next = find(t0 + 1);
-      static_for<H>([&](auto c) { copy(lds_off<0>{}, c, kbase, a.kp, kn2, now, t0); });
-      static_for<H>([&](auto c) { copy(lds_off<TB>{}, c, vbase, a.vp, vn2, now, t0); });
-      auto step = [&](uint32_t t, auto r_tag) {
+      static_for<H>([&](auto c) { copy_k(lds_off<0>{}, c, now, t0); });
+      static_for<H>([&](auto c) { copy_v(lds_off<TB>{}, c, now, t0); });
+      // Waves without rows copy, and meet the others at the barriers.
+      auto step = [&](uint32_t t, auto r_tag, auto active_tag) {
         constexpr int r = decltype(r_tag)::value;
         constexpr uint32_t k_this = uint32_t((2 * r) % 3) * TB;
         constexpr uint32_t v_this = uint32_t((2 * r + 1) % 3) * TB;
@@ -340,16 +389,17 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void prefix_tile_kernel
             __syncthreads();
             fill_ids(t + 1);
           }
-        if constexpr (kWhole) now = check(next), next = find(t + 2);
-        auto kcopies = [&](auto c) { copy(lds_off<k_next>{}, c, kbase, a.kp, kn2, now, t + 1); };
-        auto vcopies = [&](auto c) { copy(lds_off<v_next>{}, c, vbase, a.vp, vn2, now, t + 1); };
+        if constexpr (kWhole) now = check(next);
+        auto kcopies = [&](auto c) { copy_k(lds_off<k_next>{}, c, now, t + 1); };
+        auto vcopies = [&](auto c) { copy_v(lds_off<v_next>{}, c, now, t + 1); };
         vm_lds_barrier_keep<H>();  // K(t) landed; every wave is done with V(t-1)
-        if (!active) {
+        if constexpr (!decltype(active_tag)::value) {
           static_for<H>(kcopies);
+          if constexpr (kWhole) next = find(t + 2);
           vm_lds_barrier_keep<H>();
           static_for<H>(vcopies);
           return;
-        }
+        } else {
         f32x16_t sc[2];
         {
           const unsigned char* kb = smem + k_this;
@@ -376,6 +426,7 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void prefix_tile_kernel
           __builtin_amdgcn_sched_barrier(0);
           __builtin_amdgcn_s_setprio(0);
         }
+        if constexpr (kWhole) next = find(t + 2);  // here by the next barrier
         float tmax;
         {
           float u0 = max3_plain(sc[0][0], sc[0][1], sc[0][2]), u1 = sc[0][3];
@@ -403,12 +454,12 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void prefix_tile_kernel
           for (int i = 0; i < NB; ++i)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-              o[i][e] = repeat ? weighed(alpha, o[i][e]) : o[i][e] * alpha;
+              o[i][e] *= alpha;
           lsum *= alpha;
           mneg = to;
         }
         const float bias = mneg == __builtin_inff() ? 0.f : mneg;  // no score yet: weights of 0
-        vec bfrag[4], one[repeat ? 4 : 1];
+        vec bfrag[4];
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
           __builtin_amdgcn_sched_barrier(0);
@@ -419,12 +470,6 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void prefix_tile_kernel
             pr[e] = __builtin_amdgcn_exp2f(s * a.scale_log2 + bias);
           }
           bfrag[f] = M::pack(pr);
-          if constexpr (repeat) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              pr[e] = sc[f / 2][8 * (f % 2) + e] * a.scale_log2 != -__builtin_inff() ? 1.f : 0.f;
-            one[f] = M::pack(pr);
-          }
         }
         vm_lds_barrier_keep<H>();  // V(t) landed; every wave is done with K(t)
         uint32_t va = v0[0], vb1 = v0[1];
@@ -439,20 +484,7 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void prefix_tile_kernel
         for (int f = 0; f < NPV; ++f) {
           __builtin_amdgcn_sched_barrier(0);
           if (f + kVAhead < NPV) vf[f + kVAhead] = vread(vb, va, vb1, f + kVAhead);
-          if constexpr (repeat) {
-            typedef uint16_t half8 __attribute__((ext_vector_type(8)));
-            constexpr uint16_t kExp = kIsF16<T> ? 0x7c00 : 0x7f80;
-            half8 fine = __builtin_bit_cast(half8, vf[f]), odd;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              odd[e] = (fine[e] & kExp) == kExp ? fine[e] : uint16_t(0);
-              fine[e] ^= odd[e];
-            }
-            o[f % NB] = M::run(__builtin_bit_cast(vec, fine), bfrag[f / NB], o[f % NB]);
-            o[f % NB] = M::run(__builtin_bit_cast(vec, odd), one[f / NB], o[f % NB]);
-          } else {
-            o[f % NB] = M::run(vf[f], bfrag[f / NB], o[f % NB]);
-          }
+          o[f % NB] = M::run(vf[f], bfrag[f / NB], o[f % NB]);
           static_for<H>([&](auto c) {
             if (c * NPV / H == f) vcopies(c);
           });
@@ -462,38 +494,35 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void prefix_tile_kernel
         }
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_setprio(0);
+        }
       };
-      const uint32_t stop = t0 + count;
-      for (uint32_t t = t0; t < stop; t += 3) {
-        step(t, std::integral_constant<int, 0>{});
-        if (t + 1 < stop) step(t + 1, std::integral_constant<int, 1>{});
-        if (t + 2 < stop) step(t + 2, std::integral_constant<int, 2>{});
-      }
+      auto steps = [&](auto active_tag) {
+        const uint32_t stop = t0 + count;
+        for (uint32_t t = t0; t < stop; t += 3) {
+          step(t, std::integral_constant<int, 0>{}, active_tag);
+          if (t + 1 < stop) step(t + 1, std::integral_constant<int, 1>{}, active_tag);
+          if (t + 2 < stop) step(t + 2, std::integral_constant<int, 2>{}, active_tag);
+        }
+      };
+      if (active)
+        steps(std::true_type{});
+      else
+        steps(std::false_type{});
       vm_lds_barrier();  // the last copies have landed
-    };
-    walk(std::false_type{});
-    bool nan = false;
-    if (active) {
-#pragma unroll
-      for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) nan |= o[i][e] != o[i][e];
     }
-    if (lane == 0) sbad[wave] = 0;
-    if (__any(nan) && lane == 0) snan[wave] = 1;
-    if (!__any(nan) && lane == 0) snan[wave] = 0;
-    if (__any(bad) && lane == 0) sbad[wave] = 1;
+    const bool lane_bad = __any(bad);
+    if (lane == 0) sbad[wave] = lane_bad;
     lds_barrier();
-    const bool some_nan = snan[0] | snan[1] | snan[2] | snan[3];
-    const bool some_bad = sbad[0] | sbad[1] | sbad[2] | sbad[3];
-    if (some_nan && !some_bad) walk(std::true_type{});
     float l = sum_halves(lsum);
-    if (some_bad) l = __builtin_nanf("");
-    if (active && place < rows) {
-      const bool starts = t0 == 0;
+    if (sbad[0] | sbad[1] | sbad[2] | sbad[3]) l = __builtin_nanf("");
+    uint32_t place;
+    int64_t request, head;
+    place_of(place, request, head);
+    const uint32_t slot = slots + range - 1;
+    if (active && place < rows && (range == 0 || slot < uint32_t(x.groups))) {
       const int64_t q_row = request * a.Hk * a.G + head;
-      const int64_t to = starts ? q_row : int64_t(number) * kRows + place;
-      float* out = (starts ? x.first : x.more) + to * D;
+      const int64_t to = range == 0 ? q_row : int64_t(slot) * x.stride + place;
+      float* out = (range == 0 ? x.first : x.more) + to * D;
 #pragma unroll
       for (int i = 0; i < NB; ++i)
 #pragma unroll
@@ -501,116 +530,197 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void prefix_tile_kernel
           *reinterpret_cast<float4*>(out + 32 * i + 8 * g + 4 * hh) =
               make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
       if (hh == 0) {
-        (starts ? x.first_ml : x.more_ml)[to] = make_float2(-mneg, l);
-        if (starts)
-          x.record[q_row] = make_int4(int(number), int(share.owner(u + grp.steps - 1)), int(place),
-                                      0);
+        (range == 0 ? x.first_ml : x.more_ml)[to] = make_float2(-mneg, l);
+        if (range == 0) x.record[q_row] = make_int4(int(ranges) - 1, int(slots), int(place), 0);
       }
     }
-    lds_barrier();  // the flags have been read
-    u += count;
   }
+}
+
+// One row's state over its first `keys` keys in fp32, a wave a key: for rows whose
+// values are not finite, which the matrix products' rounded weights (0 for a key far
+// below the others) would make NaN of.  To sm, sl and so of each wave.
+template <typename T, int D>
+__device__ void row_state(const PagedArgs& a, int64_t n, uint32_t head, uint32_t hk, int32_t keys,
+                          float (&sm)[kWaves], float (&sl)[kWaves], float (*so)[D]) {
+  constexpr int NF = D / 64, U = 4;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const T* qp = static_cast<const T*>(a.q) + n * a.qn + int64_t(head) * a.qh;
+  const int32_t* table = a.table + n * a.table_stride;
+  float q[NF], acc[NF], m = -__builtin_inff(), l = 0.f;
+#pragma unroll
+  for (int j = 0; j < NF; ++j) q[j] = to_f32(qp[lane + 64 * j]), acc[j] = 0.f;
+  for (int32_t k0 = U * wave; k0 < keys; k0 += U * kWaves) {
+    float kf[U][NF], vf[U][NF];
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const uint32_t key = uint32_t(k0 + i), p = a.by_page.div(key);  // keys: whole tiles
+      int64_t id = table[p];
+      if (!is_page(int32_t(id), a.num_pages)) id = 0, bad = true;
+      const uint32_t in = key - p * uint32_t(a.page);
+      const T* kr = static_cast<const T*>(a.k) + id * a.kp + in * a.kn + int64_t(hk) * a.kh;
+      const T* vr = static_cast<const T*>(a.v) + id * a.vp + in * a.vn + int64_t(hk) * a.vh;
+#pragma unroll
+      for (int j = 0; j < NF; ++j) {
+        kf[i][j] = to_f32(kr[lane + 64 * j]);
+        vf[i][j] = to_f32(vr[lane + 64 * j]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < NF; ++j) s += q[j] * kf[i][j];
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
+      s = bad ? __builtin_nanf("") : s * a.scale_log2;
+      const float top = __builtin_fmaxf(m, s), ms = top == -__builtin_inff() ? 0.f : top;
+      const float f = __builtin_amdgcn_exp2f(m - ms), w = __builtin_amdgcn_exp2f(s - ms);
+      l = l * f + w;
+#pragma unroll
+      for (int j = 0; j < NF; ++j)
+        acc[j] = weighed(f, acc[j]) +
+                 (s != -__builtin_inff() ? weighed(w, vf[i][j]) : w * vf[i][j]);
+      m = top;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NF; ++j) so[wave][lane + 64 * j] = acc[j];
+  if (lane == 0) sm[wave] = m, sl[wave] = l;
 }
 
 // Joins the states of a (request, query head): those of the prefix's shares, then
 // those of its own keys, always in this order.
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void prefix_merge_kernel(SharedArgs x) {
-  constexpr int kLanes = D / 4, kSide = kThreads / kLanes, U = 4, kMost = 2 * kMostGroups + 2;
+  constexpr int kLanes = D / 4, kSide = kThreads / kLanes, U = 4;
+  constexpr int kMost = 2 * kMostGroups + 2 + kWaves;
   typedef float vec4 __attribute__((ext_vector_type(4)));
   __shared__ float weight[kMost];
   __shared__ vec4 sacc[kThreads];
-  __shared__ float top[kWaves], den[kWaves];
+  __shared__ float top[kWaves], den[kWaves], sm[kWaves], sl[kWaves];
   const PagedArgs& a = x.a;
   const int64_t row = blockIdx.x;
   const uint32_t Hq = uint32_t(a.Hk * a.G), n = uint32_t(row) / Hq, head = uint32_t(row) - n * Hq;
   T* out = static_cast<T*>(a.out) + n * a.on + head * a.oh;
-  const int c = threadIdx.x % kLanes, side = threadIdx.x / kLanes;
+  const int c = threadIdx.x % kLanes, side = threadIdx.x / kLanes, me = threadIdx.x;
   if (a.lens[n] <= 0) {
     if (side == 0)
 #pragma unroll
       for (int e = 0; e < 4; ++e) out[4 * c + e] = Round<T>::store(0.f);
     return;
   }
-  // The prefix's shares, and those of the row's own segment.
+  // The prefix's pieces, and those of the row's own segment.
   int pre = 0, pre_from = 0, place = 0;
-  if (shared_keys(a.prefix_lens[n], a.M * a.page) > 0) {
+  const int32_t shared = shared_keys(a.prefix_lens[n], a.M * a.page);
+  if (shared > 0) {
     const int4 r = x.record[row];
-    pre_from = r.x < 0 ? 0 : r.x < x.groups ? r.x : x.groups - 1;
-    const int last = r.y < pre_from ? pre_from : r.y < x.groups ? r.y : x.groups - 1;
-    place = r.z & (kRows - 1);
-    pre = last - pre_from + 1;
+    pre_from = r.y >= 0 && r.y < x.groups ? r.y : 0;
+    pre = 1 + (r.x < 0 ? 0 : r.x < x.groups - pre_from ? r.x : x.groups - pre_from);
+    place = r.z >= 0 && r.z < x.stride ? r.z : 0;
   }
   const uint32_t hk = head / uint32_t(a.G), in = head - hk * uint32_t(a.G);
   const uint32_t tile = in / uint32_t(a.rows), r = in - tile * uint32_t(a.rows);
   const int2 split = a.split[int64_t(n) * a.per_request + hk * uint32_t(a.tiles) + tile];
   const int own_from = split.x < 0 ? 0 : split.x / 2;
-  const int parts = pre + 1 + (split.x < 0 ? 0 : split.y - own_from);
+  const int own = 1 + (split.x < 0 ? 0 : split.y - own_from);
   const int64_t slots = 2 * int64_t(a.groups);
+  // Part i: `own` of them from i = 0 on, those of the prefix behind; with `exact` these are
+  // the waves' states of row_state, in place of weights not used yet.
+  bool exact = false;
+  auto so = [&]() { return reinterpret_cast<float(*)[D]>(&sacc[0]); };
   auto ml = [&](int i) {
-    if (i < pre)
-      return i == 0 ? x.first_ml[row] : x.more_ml[int64_t(pre_from + i) * kRows + place];
-    i -= pre;
-    return i == 0 ? a.state_ml[row]
-                  : reinterpret_cast<const float2*>(a.part)[2 * (own_from + i) * a.rows + r];
+    if (i < own)
+      return i == 0 ? a.state_ml[row]
+                    : reinterpret_cast<const float2*>(a.part)[2 * (own_from + i) * a.rows + r];
+    i -= own;
+    if (exact) return make_float2(sm[i], sl[i]);
+    return i == 0 ? x.first_ml[row] : x.more_ml[int64_t(pre_from + i - 1) * x.stride + place];
   };
   auto state = [&](int i) {
     const float* p;
-    if (i < pre) {
-      p = i == 0 ? x.first + row * D : x.more + (int64_t(pre_from + i) * kRows + place) * D;
-    } else {
-      i -= pre;
+    if (i < own) {
       p = i == 0 ? a.state + row * D
                  : a.part + 2 * slots * a.rows + (int64_t(2 * (own_from + i)) * a.rows + r) * D;
+    } else {
+      i -= own;
+      p = i == 0 ? x.first + row * D : x.more + (int64_t(pre_from + i - 1) * x.stride + place) * D;
     }
     return reinterpret_cast<const vec4*>(p)[c];
   };
-  const int me = threadIdx.x;
-  float m = -__builtin_inff();
-  for (int i = me; i < parts; i += kThreads) {
-    const float2 y = ml(i);
-    if (!(y.y == 0.f)) m = __builtin_fmaxf(m, y.x);
-  }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) m = __builtin_fmaxf(m, __shfl_xor(m, d));
-  if (me % 64 == 0) top[me / 64] = m;
-  lds_barrier();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) m = __builtin_fmaxf(m, top[w]);
-  float l = 0.f;
-  for (int i = me; i < parts; i += kThreads) {
-    const float2 y = ml(i);
-    const float f = __builtin_amdgcn_exp2f(y.x - m);
-    weight[i] = y.y == 0.f ? -1.f : f;  // -1: no weight at all
-    l += y.y == 0.f ? 0.f : f * y.y;
-  }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
-  if (me % 64 == 0) den[me / 64] = l;
-  lds_barrier();
-  vec4 acc = vec4(0.f);
-  for (int from = side; from < parts; from += U * kSide) {
-    vec4 y[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i)
-      y[i] = state(from + i * kSide < parts ? from + i * kSide : parts - 1);
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const float f = from + i * kSide < parts ? weight[from + i * kSide] : -1.f;
-      if (f > 0.f) acc += f * y[i];
-      if (f == 0.f || f != f)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] += f != f ? f : weighed(f, y[i][e]);
+  float l;
+  auto weights = [&](int parts) {
+    float m = -__builtin_inff();
+    for (int i = me; i < parts; i += kThreads) {
+      const float2 y = ml(i);
+      if (!(y.y == 0.f)) m = __builtin_fmaxf(m, y.x);
     }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) m = __builtin_fmaxf(m, __shfl_xor(m, d));
+    if (me % 64 == 0) top[me / 64] = m;
+    lds_barrier();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) m = __builtin_fmaxf(m, top[w]);
+    l = 0.f;
+    for (int i = me; i < parts; i += kThreads) {
+      const float2 y = ml(i);
+      const float f = __builtin_amdgcn_exp2f(y.x - m);
+      weight[i] = y.y == 0.f ? -1.f : f;  // -1: no weight at all
+      l += y.y == 0.f ? 0.f : f * y.y;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
+    if (me % 64 == 0) den[me / 64] = l;
+    lds_barrier();
+    l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) l += den[w];
+  };
+  auto add = [&](vec4& acc, float f, vec4 y) {
+    if (f > 0.f) acc += f * y;
+    if (f == 0.f || f != f)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += f != f ? f : weighed(f, y[e]);
+  };
+  auto gather = [&](int parts) {
+    vec4 acc = vec4(0.f);
+    for (int from = side; from < parts; from += U * kSide) {
+      vec4 y[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        y[i] = state(from + i * kSide < parts ? from + i * kSide : parts - 1);
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        add(acc, from + i * kSide < parts ? weight[from + i * kSide] : -1.f, y[i]);
+    }
+    sacc[me] = acc;
+    lds_barrier();
+    acc = sacc[c];
+#pragma unroll
+    for (int i = 1; i < kSide; ++i) acc += sacc[i * kLanes + c];
+    return acc;
+  };
+  weights(own + pre);
+  vec4 acc = gather(own + pre);
+  bool nan = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) nan |= acc[e] != acc[e];
+  if (pre > 0 && l == l && __syncthreads_or(nan)) {
+    // (The row's own table lists the same pages.)
+    row_state<T, D>(a, n, head, hk, shared, sm, sl, so());
+    exact = true;
+    __syncthreads();
+    vec4 rest[kWaves];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) rest[w] = *reinterpret_cast<const vec4*>(&so()[w][4 * c]);
+    __syncthreads();
+    weights(own + kWaves);
+    acc = gather(own);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) add(acc, weight[own + w], rest[w]);
   }
-  sacc[me] = acc;
-  lds_barrier();
   if (side != 0) return;
-#pragma unroll
-  for (int i = 1; i < kSide; ++i) acc += sacc[i * kLanes + c];
-  l = 0.f;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) l += den[w];
   struct alignas(sizeof(T) * 4) Out { T v[4]; } y;
 #pragma unroll
   for (int e = 0; e < 4; ++e) y.v[e] = Round<T>::store(acc[e] / l);
@@ -653,6 +763,7 @@ bool shares_prefix(int dtype, const PagedArgs& a) {
 // The regions of the workspace, behind those of the rows' own keys (`own` bytes).
 int64_t lay_out(PagedArgs& a, SharedArgs* x, char* work, int64_t own) {
   const int64_t rows = a.N * a.Hk * a.G, groups = prefix_groups(a);
+  const int64_t stride = a.N * a.G < kRows ? a.N * a.G : kRows;
   int64_t at = own;
   auto take = [&](int64_t bytes) {
     char* p = work + at;
@@ -664,8 +775,8 @@ int64_t lay_out(PagedArgs& a, SharedArgs* x, char* work, int64_t own) {
   p[1] = take(4 * rows * a.D);
   p[2] = take(8 * rows);
   p[3] = take(4 * rows * a.D);
-  p[4] = take(8 * groups * kRows);
-  p[5] = take(4 * groups * kRows * a.D);
+  p[4] = take(8 * groups * stride);
+  p[5] = take(4 * groups * stride * a.D);
   p[6] = take(16 * rows);
   if (x) {
     a.state_ml = reinterpret_cast<float2*>(p[0]);
@@ -676,6 +787,7 @@ int64_t lay_out(PagedArgs& a, SharedArgs* x, char* work, int64_t own) {
     x->more = reinterpret_cast<float*>(p[5]);
     x->record = reinterpret_cast<int4*>(p[6]);
     x->groups = int32_t(groups);
+    x->stride = int32_t(stride);
     x->by_g = FastDiv(uint32_t(a.G));
     x->least = 4;
     x->a = a;
