@@ -618,6 +618,274 @@ __global__ __launch_bounds__(kThreads) void prefix_groups_kernel(PrefixArgs a,
   }
 }
 
+// ---------------------------------------------------------------------------
+// The same for small batches and pools in one work-group, with the counts in LDS:
+// the launches and the reads that wait for one another are what such a call takes
+// (us, 8 rows: fork @F@, compaction of 12 rows @C@, prefixes of 8 rows @P@).
+constexpr int kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64;
+constexpr int kSmallRows = 256;
+constexpr int kSmallPages = 8192;       // 32 KB of counts
+constexpr int64_t kSmallEntries = 32768;
+constexpr int32_t kGone = -(1 << 30);   // the count of a page that no row holds any more
+
+__global__ __launch_bounds__(kSmallThreads) void fork_small_kernel(ForkArgs a, FastDiv by_m) {
+  __shared__ int32_t s[kSmallPages];
+  __shared__ int32_t parent[kSmallRows], held[kSmallRows], had[kSmallRows], ends[kSmallRows];
+  __shared__ int32_t old_held[kSmallRows], freed[kSmallRows];
+  __shared__ uint8_t is_first[kSmallRows], kids[kSmallRows];
+  __shared__ int32_t part[2][kSmallWaves];
+  const int t = threadIdx.x, lane = t % 64, wave = t / 64;
+  const int R = int(a.R), N = int(a.N), P = int(a.P), F = int(a.F);
+  const uint32_t M = uint32_t(a.M);
+  const int64_t head = head_of(a.free_head, a.F);
+  for (int p = t; p < P; p += kSmallThreads) s[p] = a.shares[p];
+  int32_t len = 0;
+  if (t < R) {
+    const ForkRow row(a, t);
+    parent[t] = row.parent;
+    held[t] = int32_t(row.held);
+    had[t] = int32_t(row.had);
+    ends[t] = row.open(a);
+    len = row.len;
+    a.kv_out[t] = len;
+  } else if (t >= kSmallRows && t < kSmallRows + N) {
+    old_held[t - kSmallRows] = int32_t(held_pages(a.kv_lens[t - kSmallRows], a.page, M));
+    kids[t - kSmallRows] = 0;
+  }
+  __syncthreads();
+  bool not_least = false;
+  const int32_t end = t < R ? ends[t] : -1;
+  if (t < R) {
+    bool first = true;
+    for (int j = 0; j < t; ++j) {
+      first = first && parent[j] != parent[t];
+      not_least |= ends[j] == end;
+    }
+    is_first[t] = first;
+    if (parent[t] >= 0) kids[parent[t]] = 1;
+  }
+  __syncthreads();
+  for (uint32_t e = t; e < uint32_t(R) * M; e += kSmallThreads) {
+    const uint32_t r = by_m.div(e), k = e - r * M;
+    int32_t id = -1;
+    const bool in = int32_t(k) < held[r];
+    if (in || (is_first[r] && int32_t(k) < had[r])) {
+      id = a.table[parent[r] * a.table_stride + k];
+      if (is_page(id, P) && !(in && is_first[r])) atomicAdd(&s[id], in ? 1 : -1);
+    }
+    a.table_out[e] = in ? id : -1;
+  }
+  for (uint32_t e = t; e < uint32_t(N) * M; e += kSmallThreads) {
+    const uint32_t n = by_m.div(e), k = e - n * M;
+    if (kids[n] || int32_t(k) >= old_held[n]) continue;
+    const int32_t id = a.table[n * a.table_stride + k];
+    if (is_page(id, P)) atomicAdd(&s[id], -1);
+  }
+  __syncthreads();
+  // The pages that went: a run of whole words of 64 to a wave.
+  const int run = (P + kSmallThreads - 1) / kSmallThreads * 64, from = wave * run;
+  int32_t mine = 0;
+  for (int p = from + lane; p < from + run; p += 64) {
+    const bool gone = p < P && s[p] < 0;
+    if (gone) s[p] = kGone;
+    mine += __builtin_popcountll(__ballot(gone));
+  }
+  if (lane == 0) part[0][wave] = mine;
+  __syncthreads();
+  int32_t before = 0, nf = 0;
+#pragma unroll
+  for (int i = 0; i < kSmallWaves; ++i) {
+    if (i < wave) before += part[0][i];
+    nf += part[0][i];
+  }
+  // Rows that get a page of their own leave the shared one: all but the first, then the first
+  // if somebody holds it still.
+  bool copies = end >= 0 && not_least;
+  if (copies) atomicSub(&s[end], 1);
+  __syncthreads();
+  if (end >= 0 && !not_least && s[end] > 0) {
+    copies = true;
+    --s[end];
+  }
+  const uint64_t word = __ballot(copies);
+  if (lane == 0) part[1][wave] = __builtin_popcountll(word);
+  __syncthreads();
+  int32_t rank = 0, nt = 0;
+#pragma unroll
+  for (int i = 0; i < kSmallWaves; ++i) {
+    if (i < wave) rank += part[1][i];
+    nt += part[1][i];
+  }
+  rank += __builtin_popcountll(word & ((uint64_t(1) << lane) - 1));
+  const int64_t top = head - nf;
+  for (int p = from + lane; p < from + run; p += 64) {
+    const int32_t v = p < P ? s[p] : 0;
+    const bool gone = v < kGone / 2;
+    const uint64_t all = __ballot(gone);
+    const int32_t j = before + __builtin_popcountll(all & ((uint64_t(1) << lane) - 1));
+    before += __builtin_popcountll(all);
+    if (p < P) a.shares_out[p] = v > 0 ? v : 0;
+    if (gone) {
+      if (j < nt)
+        freed[j] = p;
+      else if (top + j >= 0)
+        a.free_out[top + j] = p;
+    }
+  }
+  for (int i = t; i < F; i += kSmallThreads)
+    if (i < top + nt || i >= head) a.free_out[i] = a.free_pages[i];
+  __syncthreads();
+  if (t == 0) *a.head_out = int32_t(top + nt < 0 ? 0 : top + nt);
+  if (t >= R) return;
+  int32_t to = -1;
+  if (copies) {
+    to = rank < nf ? freed[rank] : free_page(a.free_pages, a.F, top + rank);
+    a.table_out[uint32_t(t) * M + uint32_t(open_page(len, a.page, M))] = to;
+  }
+  a.copy_src[t] = copies ? end : -1;
+  a.copy_dst[t] = to;
+  a.copy_rows[t] = copies ? int32_t(uint32_t(len) % a.page) : 0;
+}
+
+__global__ __launch_bounds__(kSmallThreads) void compact_small_kernel(CompactArgs a,
+                                                                      FastDiv by_m) {
+  constexpr int kWords = kSmallPages / 32;
+  __shared__ uint32_t used[kWords], open[kWords];
+  __shared__ int32_t pu[kWords], po[kWords], part[3][kSmallWaves];
+  __shared__ int32_t hole[kSmallPages / 2];
+  const int t = threadIdx.x;
+  const int N = int(a.N), P = int(a.P), F = int(a.F), half = P / 2;
+  const uint32_t M = uint32_t(a.M);
+  const int64_t head = head_of(a.free_head, a.F);
+  for (int i = t; i < kWords; i += kSmallThreads) used[i] = open[i] = 0;
+  __syncthreads();
+  for (uint32_t e = t; e < uint32_t(N) * M; e += kSmallThreads) {
+    const uint32_t n = by_m.div(e), k = e - n * M;
+    if (k >= held_pages(a.kv_lens[n], a.page, M)) continue;
+    const int32_t id = a.table[n * a.table_stride + k];
+    if (is_page(id, P)) atomicOr(&used[id / 32], 1u << (id % 32));
+  }
+  for (int64_t i = head + t; i < F; i += kSmallThreads) {
+    const int32_t id = a.free_pages[i];
+    if (is_page(id, P)) atomicOr(&open[id / 32], 1u << (id % 32));
+  }
+  __syncthreads();
+  uint32_t x = 0, y = 0;
+  if (t < kWords) {
+    x = used[t];
+    y = open[t] & ~x;
+    open[t] = y;
+  }
+  const int32_t nx = __builtin_popcount(x), ny = __builtin_popcount(y);
+  int32_t total, free, moves;
+  const int32_t ux = block_exclusive_sum<kSmallThreads>(nx, part[0], &total);
+  const int32_t uy = block_exclusive_sum<kSmallThreads>(ny, part[1], &free);
+  int32_t holes = 0;
+  if (t < kWords) {
+    pu[t] = ux;
+    po[t] = uy;
+    uint32_t all = x | y;
+    const int32_t rank = ux + uy, n = nx + ny;
+    if (rank + n <= total) {
+      holes = ny;
+    } else {
+      for (int32_t k = rank; k < total; ++k) {
+        const uint32_t bit = all & -all;
+        holes += (y & bit) != 0;
+        all ^= bit;
+      }
+    }
+  }
+  block_exclusive_sum<kSmallThreads>(holes, part[2], &moves);
+  auto ranks = [&](int p, int32_t* ru, int32_t* ro) {
+    const uint32_t below = (1u << (p % 32)) - 1;
+    *ru = pu[p / 32] + __builtin_popcount(used[p / 32] & below);
+    *ro = po[p / 32] + __builtin_popcount(open[p / 32] & below);
+  };
+  auto has = [](const uint32_t* bits, int p) { return (bits[p / 32] >> (p % 32) & 1) != 0; };
+  __syncthreads();
+  for (int p = t; p < P; p += kSmallThreads) {
+    int32_t ru, ro;
+    ranks(p, &ru, &ro);
+    const bool is_used = has(used, p), is_open = has(open, p);
+    if (is_open && ru + ro < total) {
+      hole[ro] = p;
+      a.copy_dst[ro] = p;
+    }
+    if ((is_used || is_open) && ru + ro >= total)
+      a.free_out[F - free + (ru + ro - total)] = p;
+    if (is_used && ru + ro >= total) a.copy_src[ru - (total - moves)] = p;
+  }
+  for (int i = t; i < F - free; i += kSmallThreads) a.free_out[i] = a.free_pages[i];
+  for (int i = moves + t; i < half; i += kSmallThreads) a.copy_src[i] = a.copy_dst[i] = -1;
+  if (t == 0) {
+    *a.num_moves = moves;
+    *a.head_out = F - free;
+  }
+  __syncthreads();
+  // The new number of a page.
+  auto place = [&](int p) {
+    int32_t ru, ro;
+    ranks(p, &ru, &ro);
+    return ru + ro >= total ? hole[ru - (total - moves)] : p;
+  };
+  for (int p = t; p < P; p += kSmallThreads) {
+    int32_t ru, ro;
+    ranks(p, &ru, &ro);
+    if (has(open, p) && ru + ro < total) continue;  // a hole: its new page writes it
+    const int32_t v = a.shares[p];
+    const bool moved = has(used, p) && ru + ro >= total;
+    a.shares_out[p] = moved ? 0 : v;
+    if (moved) a.shares_out[hole[ru - (total - moves)]] = v;
+  }
+  for (uint32_t e = t; e < uint32_t(N) * M; e += kSmallThreads) {
+    const uint32_t n = by_m.div(e), k = e - n * M;
+    int32_t id = a.table[n * a.table_stride + k];
+    if (k < held_pages(a.kv_lens[n], a.page, M) && is_page(id, P)) id = place(id);
+    a.table_out[e] = id;
+  }
+}
+
+// Up to 64 rows: a lane a row for the groups, a wave a row for the pages.
+__global__ __launch_bounds__(kSmallThreads) void prefix_small_kernel(PrefixArgs a) {
+  __shared__ int32_t pages[64];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, N = int(a.N);
+  const uint64_t leads = __ballot(lane < N && !joins(a, lane));
+  for (int n = wave; n < N; n += kSmallWaves) {
+    const int lead = 63 - __builtin_clzll(leads & (~uint64_t(0) >> (63 - n)));
+    const int32_t len = a.kv_lens[n] > 0 ? a.kv_lens[n] : 0;
+    int64_t whole = uint32_t(len) / a.page;
+    if (whole > a.M) whole = a.M;
+    const int32_t *row = a.table + n * a.table_stride, *with = a.table + lead * a.table_stride;
+    int64_t same = whole;
+    constexpr int kPer = 4;
+    for (int64_t k0 = 0; k0 < whole; k0 += 64 * kPer) {
+      uint64_t miss[kPer];
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const int64_t k = k0 + 64 * e + lane;
+        miss[e] = __ballot(k < whole && (row[k] < 0 || row[k] != with[k]));
+      }
+      bool found = false;
+#pragma unroll
+      for (int e = kPer - 1; e >= 0; --e)
+        if (miss[e]) same = k0 + 64 * e + __builtin_ctzll(miss[e]), found = true;
+      if (found) break;
+    }
+    if (lane == 0) pages[n] = int32_t(same);
+  }
+  __syncthreads();
+  if (wave != 0 || lane >= N) return;
+  const int lead = 63 - __builtin_clzll(leads & (~uint64_t(0) >> (63 - lane)));
+  const uint64_t later = lead < 63 ? leads >> (lead + 1) << (lead + 1) : 0;
+  const int end = later ? __builtin_ctzll(later) : N, rows = end - lead;
+  int32_t least = pages[lead];
+  for (int i = lead + 1; i < end; ++i) least = least < pages[i] ? least : pages[i];
+  const int32_t len = rows > 1 ? int32_t(uint32_t(least) * a.page) : 0;
+  a.prefix_lens[lane] = len;
+  a.group_rows[lane] = lane == lead && len > 0 ? rows : 0;
+}
+
 unsigned extra_groups(int64_t work) {
   const int64_t g = (work + 4 * kThreads - 1) / (4 * kThreads);
   return unsigned(g < 1 ? 1 : g > 1024 ? 1024 : g);
@@ -631,6 +899,12 @@ int64_t fork_workspace_bytes(int64_t R, int64_t P) {
 }
 
 hipError_t launch_paged_fork(const ForkArgs& a, void* workspace, hipStream_t stream) {
+  if (a.N <= kSmallRows && a.R <= kSmallRows && a.P <= kSmallPages &&
+      a.F <= 2 * kSmallPages && (a.N + a.R) * a.M <= kSmallEntries) {
+    hipLaunchKernelGGL(fork_small_kernel, dim3(1), dim3(kSmallThreads), 0, stream, a,
+                       FastDiv(uint32_t(a.M > 0 ? a.M : 1)));
+    return hipGetLastError();
+  }
   const ForkWork w = fork_work(workspace, a.R, a.P);
   const int64_t per_row = a.M > 0 ? (a.M + kChunk - 1) / kChunk : 1;
   hipLaunchKernelGGL(fork_rows_kernel, dim3(unsigned(a.R * per_row + a.N) + extra_groups(a.P + a.F)),
@@ -660,6 +934,11 @@ int64_t compact_workspace_bytes(int64_t P) {
 }
 
 hipError_t launch_paged_compact(const CompactArgs& a, void* workspace, hipStream_t stream) {
+  if (a.P <= kSmallPages && a.F <= 2 * kSmallPages && a.N * a.M <= kSmallEntries) {
+    hipLaunchKernelGGL(compact_small_kernel, dim3(1), dim3(kSmallThreads), 0, stream, a,
+                       FastDiv(uint32_t(a.M > 0 ? a.M : 1)));
+    return hipGetLastError();
+  }
   const CompactWork w = compact_work(workspace, a.P);
   const int64_t per_row = a.M > 0 ? (a.M + kChunk - 1) / kChunk : 1;
   const int64_t chunks = fork_chunks(a.P);
@@ -685,6 +964,10 @@ hipError_t launch_paged_compact(const CompactArgs& a, void* workspace, hipStream
 int64_t prefix_workspace_bytes(int64_t N) { return 8 * N; }
 
 hipError_t launch_paged_prefix(const PrefixArgs& a, void* workspace, hipStream_t stream) {
+  if (a.N <= 64 && a.N * a.M <= kSmallEntries) {
+    hipLaunchKernelGGL(prefix_small_kernel, dim3(1), dim3(kSmallThreads), 0, stream, a);
+    return hipGetLastError();
+  }
   int32_t* first = static_cast<int32_t*>(workspace);
   int32_t* pages = first + a.N;
   hipLaunchKernelGGL(prefix_rows_kernel, dim3(unsigned(a.N)), dim3(kThreads), 0, stream, a, first,
