@@ -154,12 +154,10 @@ __host__ __device__ inline int32_t shared_keys(int32_t prefix, int64_t capacity)
 int64_t paged_attn_workspace(int dtype, PagedArgs a);
 hipError_t launch_paged_attn(int dtype, PagedArgs a, void* workspace, hipStream_t stream);
 
-// The matrix-core form with 16-bit rows, whether it takes these tensors; and its
-// states of every row's own keys (from shared_keys on), `states` work-groups beyond
-// the first of a segment having slots of the partial rows.
+// Whether the matrix-core form takes these tensors; its work for the states of every
+// row's own keys (from shared_keys on), and the bytes of the partial rows.
 bool paged_tile_form(int dtype, const PagedArgs& a);
 int64_t paged_states_workspace(int dtype, PagedArgs& a);
-hipError_t launch_paged_states(int dtype, PagedArgs& a, hipStream_t stream);
 
 int64_t prefix_attn_workspace(int dtype, PagedArgs a);
 hipError_t launch_prefix_attn(int dtype, PagedArgs a, void* workspace, hipStream_t stream);

@@ -17,6 +17,7 @@
 #include "lanes.h"
 #include "mfma.h"
 #include "paged_ops.h"
+#include "paged_tile.h"
 
 namespace va {
 
@@ -24,7 +25,7 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kRows = 128;       // rows of a tile
-constexpr int kMostGroups = 768;  // three a CU
+constexpr int kMostGroups = 512;  // of the prefixes: two a CU  // three a CU
 constexpr int kIdKeys = 1024;    // keys whose page ids lie in LDS, for pages of any size
 
 // Where a state lies: that of the first piece with its row, (request, query head); those
@@ -113,22 +114,67 @@ __device__ inline uint2 block_sum(uint2 x, uint2* part, uint2* before) {
 __device__ inline int32_t run_of(const PagedArgs& a) {
   return (int32_t(a.N) + kThreads - 1) / kThreads;
 }
+// Steps of a piece: a work-group one piece, where there are fewer segments than work-groups.
+__device__ inline uint32_t piece_length(uint32_t steps, uint32_t segments, uint32_t groups,
+                                        uint32_t least) {
+  const uint32_t spare = segments < groups / 2 ? groups - segments : groups / 2;
+  const uint32_t n = steps / (spare ? spare : 1) + 1;
+  return n < least ? least : n;
+}
+__device__ inline uint2 steps_of(const PagedArgs& a, const Group& g) {  // and segments
+  const uint64_t segments = uint64_t(a.Hk) * g.tiles, steps = segments * g.steps;
+  return make_uint2(steps < 0xffffffffu ? uint32_t(steps) : 0xffffffffu, uint32_t(segments));
+}
+// Up to 64 rows are a lane each, in every wave by itself.
+__device__ inline uint2 wave_sum(uint2 x) {
+  const int lane = threadIdx.x % 64;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t u = __shfl_up(x.x, d), v = __shfl_up(x.y, d);
+    if (lane >= d) x = make_uint2(plus(x.x, u), plus(x.y, v));
+  }
+  return x;
+}
+__device__ inline uint32_t lane_of(uint32_t x, int lane) {
+  return uint32_t(__builtin_amdgcn_readlane(int(x), lane));
+}
+struct LanePieces {
+  Group g;
+  Sum before, mine;
+};
+__device__ inline Pieces count_in_lanes(const PagedArgs& a, uint32_t groups, uint32_t least,
+                                        LanePieces* to) {
+  to->g = group_at(a, threadIdx.x % 64);
+  const uint2 all = wave_sum(steps_of(a, to->g));
+  Pieces p;
+  p.length = piece_length(lane_of(all.x, 63), lane_of(all.y, 63), groups, least);
+  to->mine = pieces_of(a, to->g, p.length);
+  const uint2 sum = wave_sum(make_uint2(to->mine.pieces, to->mine.more));
+  p.count = lane_of(sum.x, 63);
+  const uint32_t u = __shfl_up(sum.x, 1), v = __shfl_up(sum.y, 1);
+  to->before = threadIdx.x % 64 ? Sum{u, v} : Sum{0, 0};
+  return p;
+}
+__device__ inline Group find_in_lanes(const LanePieces& l, uint32_t piece, Sum* before) {
+  const uint64_t here =
+      __ballot(piece >= l.before.pieces && piece - l.before.pieces < l.mine.pieces);
+  const int at = here ? __builtin_ctzll(here) : 0;  // (piece is below the sum)
+  *before = Sum{lane_of(l.before.pieces, at), lane_of(l.before.more, at)};
+  return Group{at, int32_t(lane_of(uint32_t(l.g.rows), at)), lane_of(l.g.tiles, at),
+               lane_of(l.g.steps, at)};
+}
+
 __device__ inline Pieces count_pieces(const PagedArgs& a, uint32_t groups, uint32_t least,
                                       PiecesLds& lds) {
   const int32_t N = int32_t(a.N), per = run_of(a), lo = int32_t(threadIdx.x) * per;
   uint2 mine = make_uint2(0, 0), before;
   for (int32_t i = lo; i < lo + per && i < N; ++i) {
-    const Group g = group_at(a, i);
-    const uint64_t segments = uint64_t(a.Hk) * g.tiles, steps = segments * g.steps;
-    mine = make_uint2(plus(mine.x, steps < 0xffffffffu ? uint32_t(steps) : 0xffffffffu),
-                      plus(mine.y, uint32_t(segments)));
+    const uint2 n = steps_of(a, group_at(a, i));
+    mine = make_uint2(plus(mine.x, n.x), plus(mine.y, n.y));
   }
   const uint2 all = block_sum(mine, lds.sum, &before);
-  // A work-group one piece, where there are fewer segments than work-groups.
-  const uint32_t spare = all.y < groups / 2 ? groups - all.y : groups / 2;
   Pieces p;
-  p.length = all.x / (spare ? spare : 1) + 1;
-  if (p.length < least) p.length = least;
+  p.length = piece_length(all.x, all.y, groups, least);
   mine = make_uint2(0, 0);
   for (int32_t i = lo; i < lo + per && i < N; ++i) {
     const Sum s = pieces_of(a, group_at(a, i), p.length);
@@ -184,39 +230,43 @@ __device__ inline void copy16_from(uint32_t lds_base, uint64_t address) {
 
 template <typename T> constexpr bool kIsF16 = std::is_same_v<T, f16_t>;
 
-// w * x for a weight that is not zero, but may be too small for fp32.
-__device__ inline float weighed(float w, float x) {
-  return w != 0.f ? w * x : __builtin_fabsf(x) < __builtin_inff() ? 0.f : x;
-}
-
 // kWhole: pages of a multiple of 16 tokens, so that the 16 keys that a wave copies of
 // a tile lie in one.
+template <typename T, int D, bool kWhole> struct PrefixLds {
+  static constexpr uint32_t kTileBytes = uint32_t(kTileKeys * 2 * D);
+  __attribute__((aligned(1024))) unsigned char tiles[3 * kTileBytes];
+  PiecesLds pieces;
+  int bad[kWaves];
+  int32_t ids[kWhole ? 1 : kIdKeys + 2];
+};
 template <typename T, int D, bool kWhole>
-__global__ __launch_bounds__(kThreads, D == 128 ? (kWhole ? 3 : 2) : 4) void prefix_tile_kernel(SharedArgs x) {
+__device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D, kWhole>& shared,
+                                            uint32_t block) {
   using M = Mfma<T>;
   using vec = typename M::vec;
   constexpr int kRowBytes = 2 * D, NCH = D / 8;
-  constexpr uint32_t TB = uint32_t(kTileKeys * kRowBytes);
+  constexpr uint32_t TB = PrefixLds<T, D, kWhole>::kTileBytes;
   constexpr int RPC = 1024 / kRowBytes, H = kTileKeys * kRowBytes / 1024 / kWaves;
   constexpr int NQK = D / 16, NB = D / 32, NPV = 4 * NB;
   // fp16 holds weights down to 2^-24: those of 2^7 more are held, at most 2^15 of them.
   constexpr float kBias = kIsF16<T> ? 7.f : 0.f;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[3 * TB];
-  __shared__ PiecesLds lds;
-  __shared__ int sbad[kWaves];
-  __shared__ int32_t sid[kWhole ? 1 : kIdKeys + 2];
+  unsigned char* smem = shared.tiles;
+  PiecesLds& lds = shared.pieces;
+  auto& sbad = shared.bad;
+  auto& sid = shared.ids;
   const PagedArgs& a = x.a;
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
   const int l32 = lane % 32, hh = lane / 32;
   const uint32_t page = uint32_t(a.page);
 
-  const Pieces all = count_pieces(a, uint32_t(x.groups), x.least, lds);
+  const bool few = a.N <= 64;
+  LanePieces lanes;
+  const Pieces all = few ? count_in_lanes(a, uint32_t(x.groups), x.least, &lanes)
+                         : count_pieces(a, uint32_t(x.groups), x.least, lds);
   // Neighbouring pieces to one XCD.
   const uint32_t eighth = uint32_t(x.groups) / 8;
-  const uint32_t number = blockIdx.x < 8 * eighth
-                              ? blockIdx.x % 8 * eighth + blockIdx.x / 8
-                              : blockIdx.x;
+  const uint32_t number = block < 8 * eighth ? block % 8 * eighth + block / 8 : block;
 
   // ---- copies: copy c of this wave fills tile rows [(wave*H + c)*RPC, +RPC), the lane
   // row crow + c*RPC, of which it fetches chunk p ^ chunk_swizzle(row).
@@ -243,7 +293,9 @@ __global__ __launch_bounds__(kThreads, D == 128 ? (kWhole ? 3 : 2) : 4) void pre
 
   for (uint32_t piece = number; piece < all.count; piece += uint32_t(x.groups)) {
     Sum before;
-    const Group grp = find_piece(a, piece, all.length, lds, &before);
+    if (few && piece != number) __syncthreads();  // the piece before is done with its flags
+    const Group grp = few ? find_in_lanes(lanes, piece, &before)
+                          : find_piece(a, piece, all.length, lds, &before);
     const uint32_t ranges = (grp.steps - 1) / all.length + 1;
     const uint32_t at = piece - before.pieces, hk = at / (ranges * grp.tiles);
     const uint32_t in_head = at - hk * ranges * grp.tiles, range = in_head / grp.tiles;
@@ -370,6 +422,7 @@ __global__ __launch_bounds__(kThreads, D == 128 ? (kWhole ? 3 : 2) : 4) void pre
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
       mneg = __builtin_inff();  // -(running maximum), less kBias
+      bool far = false;         // for some row, 2^16 or more
       lsum = 0.f;
       fill_ids(t0);
       At now{};
@@ -437,10 +490,7 @@ __global__ __launch_bounds__(kThreads, D == 128 ? (kWhole ? 3 : 2) : 4) void pre
           }
           tmax = max_plain(u0, u1);
         }
-        // The maximum moves when a score exceeds it by more than the slack.  Compared is the
-        // exponent that the score's weight would have, and scores are scaled and rounded as
-        // the maximum is: where the steps of both are larger than the slack (2^27 and more),
-        // a fused multiplication's exact product lies tens of powers of two beside them.
+        // The maximum moves when a score's weight would exceed 2 to the slack.
         const float lead = tmax * a.scale_log2 + mneg;
         const bool first = mneg == __builtin_inff();
         if (__builtin_amdgcn_ballot_w64(first ? tmax > -__builtin_inff()
@@ -457,20 +507,28 @@ __global__ __launch_bounds__(kThreads, D == 128 ? (kWhole ? 3 : 2) : 4) void pre
               o[i][e] *= alpha;
           lsum *= alpha;
           mneg = to;
+          far = __any(mneg < -0x1p16f);
         }
         const float bias = mneg == __builtin_inff() ? 0.f : mneg;  // no score yet: weights of 0
+        // Scores are scaled and rounded as the maximum is where its steps are large: a fused
+        // multiplication's exact product would lie tens of powers of two beside it from 2^27
+        // on.  Below 2^16 the two are within 2^-8 of each other.
         vec bfrag[4];
+        auto weights = [&](auto exponent) {
 #pragma unroll
-        for (int f = 0; f < 4; ++f) {
-          __builtin_amdgcn_sched_barrier(0);
-          float pr[8];
+          for (int f = 0; f < 4; ++f) {
+            __builtin_amdgcn_sched_barrier(0);
+            float pr[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float s = sc[f / 2][8 * (f % 2) + e];
-            pr[e] = __builtin_amdgcn_exp2f(s * a.scale_log2 + bias);
+            for (int e = 0; e < 8; ++e)
+              pr[e] = __builtin_amdgcn_exp2f(exponent(sc[f / 2][8 * (f % 2) + e]));
+            bfrag[f] = M::pack(pr);
           }
-          bfrag[f] = M::pack(pr);
-        }
+        };
+        if (far)
+          weights([&](float s) { return s * a.scale_log2 + bias; });
+        else
+          weights([&](float s) { return __builtin_fmaf(s, a.scale_log2, bias); });
         vm_lds_barrier_keep<H>();  // V(t) landed; every wave is done with K(t)
         uint32_t va = v0[0], vb1 = v0[1];
         asm volatile("" : "+v"(va), "+v"(vb1));
@@ -537,6 +595,22 @@ __global__ __launch_bounds__(kThreads, D == 128 ? (kWhole ? 3 : 2) : 4) void pre
   }
 }
 
+// The prefixes' work-groups, then those of the rows' own keys: what is left of the GPU
+// beside the ones is taken by the others.
+template <typename T, int D, bool kWhole>
+__global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void prefix_kernel(SharedArgs x) {
+  __shared__ union Lds {
+    __device__ Lds() {}
+    PrefixLds<T, D, kWhole> prefix;
+    TileLds<T, D, kFormSplit> own;
+  } lds;
+  if (blockIdx.x < uint32_t(x.groups))
+    prefix_tile<T, D, kWhole>(x, lds.prefix, blockIdx.x);
+  else
+    paged_tile<T, D, kWhole, kFormSplit, false, true>(x.a, lds.own,
+                                                      blockIdx.x - uint32_t(x.groups));
+}
+
 // One row's state over its first `keys` keys in fp32, a wave a key: for rows whose
 // values are not finite, which the matrix products' rounded weights (0 for a key far
 // below the others) would make NaN of.  To sm, sl and so of each wave.
@@ -595,7 +669,7 @@ __device__ void row_state(const PagedArgs& a, int64_t n, uint32_t head, uint32_t
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void prefix_merge_kernel(SharedArgs x) {
   constexpr int kLanes = D / 4, kSide = kThreads / kLanes, U = 4;
-  constexpr int kMost = 2 * kMostGroups + 2 + kWaves;
+  constexpr int kMost = 2 * 512 + 2 + kWaves;
   typedef float vec4 __attribute__((ext_vector_type(4)));
   __shared__ float weight[kMost];
   __shared__ vec4 sacc[kThreads];
@@ -738,11 +812,11 @@ int64_t prefix_groups(const PagedArgs& a) {
 
 template <typename T, int D>
 hipError_t launch_prefix(const SharedArgs& x, hipStream_t stream) {
-  const dim3 grid{unsigned(x.groups)}, block{kThreads};
+  const dim3 grid{unsigned(x.groups + x.a.groups)}, block{kThreads};
   if (x.a.page % 16 == 0)
-    hipLaunchKernelGGL((prefix_tile_kernel<T, D, true>), grid, block, 0, stream, x);
+    hipLaunchKernelGGL((prefix_kernel<T, D, true>), grid, block, 0, stream, x);
   else
-    hipLaunchKernelGGL((prefix_tile_kernel<T, D, false>), grid, block, 0, stream, x);
+    hipLaunchKernelGGL((prefix_kernel<T, D, false>), grid, block, 0, stream, x);
   return hipGetLastError();
 }
 template <typename T, int D>
@@ -816,12 +890,10 @@ hipError_t launch_prefix_attn(int dtype, PagedArgs a, void* workspace, hipStream
   SharedArgs x{};
   lay_out(a, &x, work, own);
   const bool wide = a.D == 128, bf = dtype == kBF16;
-  hipError_t e = bf ? (wide ? launch_prefix<bf16_t, 128>(x, stream)
+  const hipError_t e = bf ? (wide ? launch_prefix<bf16_t, 128>(x, stream)
                             : launch_prefix<bf16_t, 64>(x, stream))
                     : (wide ? launch_prefix<f16_t, 128>(x, stream)
                             : launch_prefix<f16_t, 64>(x, stream));
-  if (e != hipSuccess) return e;
-  e = launch_paged_states(dtype, x.a, stream);
   if (e != hipSuccess) return e;
   return bf ? (wide ? launch_join<bf16_t, 128>(x, stream) : launch_join<bf16_t, 64>(x, stream))
             : (wide ? launch_join<f16_t, 128>(x, stream) : launch_join<f16_t, 64>(x, stream));
