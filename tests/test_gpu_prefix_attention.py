@@ -19,7 +19,7 @@ def note(*a):
     print("[case]", *a, flush=True)
 
 
-def make(groups, Hq, Hk, D, page, layout, dtype, seed=0, gap=0, scale=1.0):
+def make(groups, Hq, Hk, D, page, layout, dtype, seed=0):
     """Rows in groups [(prefix tokens, [own tokens of each row])]: the prefix's whole pages are
     shared, the rest of it is each row's own copy, as a fork leaves it.  Returns q, caches, tables
     and lengths on the CPU."""
@@ -36,7 +36,7 @@ def make(groups, Hq, Hk, D, page, layout, dtype, seed=0, gap=0, scale=1.0):
             rows.append((base + list(range(used, used + more)))[:held])
             used += more
             lens.append(length)
-    width = max([len(r) for r in rows] + [1]) + gap
+    width = max([len(r) for r in rows] + [1])
     pages = used + 3
     order = torch.randperm(pages, generator=g)
     table = torch.full((len(rows), width), -1, dtype=torch.int32)
@@ -44,8 +44,17 @@ def make(groups, Hq, Hk, D, page, layout, dtype, seed=0, gap=0, scale=1.0):
         table[n, :len(r)] = order[torch.tensor(r, dtype=torch.long)].int()
     shape = (pages, page, Hk, D) if layout == "NHD" else (pages, Hk, page, D)
     kc, vc = (torch.randn(shape, generator=g).to(dtype) for _ in range(2))
-    q = (scale * torch.randn(len(rows), Hq, D, generator=g)).to(dtype)
+    q = torch.randn(len(rows), Hq, D, generator=g).to(dtype)
     return q, kc, vc, table, torch.tensor(lens, dtype=torch.int32)
+
+
+def widened(table, kc, layout="NHD"):
+    """The same table with room for longer requests: so much that the prefix is computed once (the
+    form goes by the tables' width), however few keys there are."""
+    page, Hk = (kc.shape[1], kc.shape[2]) if layout == "NHD" else (kc.shape[2], kc.shape[1])
+    width = -(-(130 << 20) // (4 * len(table) * page * Hk * kc.shape[3]))
+    more = torch.full((len(table), max(width - table.shape[1], 0)), -1, dtype=torch.int32)
+    return torch.cat([table, more.to(table.device)], 1)
 
 
 def room(q, kc, vc, table, lens, layout, scale=None):
@@ -61,9 +70,9 @@ def room(q, kc, vc, table, lens, layout, scale=None):
     return want, slack
 
 
-def run(q, kc, vc, table, lens, layout="NHD", page=None, ids=None, scale=None):
-    page = page or kc.shape[1 if layout == "NHD" else 2]
-    d_table, d_lens = table.to(DEV), lens.to(DEV)
+def run(q, kc, vc, table, lens, layout="NHD", ids=None, scale=None, wide=True):
+    page = kc.shape[1 if layout == "NHD" else 2]
+    d_table, d_lens = (widened(table, kc, layout) if wide else table).to(DEV), lens.to(DEV)
     prefix = paged_kv_prefix(d_lens, d_table, page, None if ids is None else ids.to(DEV))
     out = paged_prefix_decode_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), d_table, d_lens, prefix,
                                         kv_layout=layout, sm_scale=scale)
@@ -71,10 +80,10 @@ def run(q, kc, vc, table, lens, layout="NHD", page=None, ids=None, scale=None):
     return out, prefix
 
 
-def check(case, layout="NHD", ids=None, scale=None):
+def check(case, layout="NHD", ids=None, scale=None, wide=True):
     q, kc, vc, table, lens = case
     note("attend", list(q.shape), list(kc.shape), layout, q.dtype, "rows", len(lens))
-    out, prefix = run(q, kc, vc, table, lens, layout, None, ids, scale)
+    out, prefix = run(q, kc, vc, table, lens, layout, ids, scale, wide)
     want, slack = room(q, kc, vc, table, lens, layout, scale)
     assert out.dtype == q.dtype and out.shape == want.shape
     off = (out.double().cpu() - want).abs()
@@ -104,7 +113,9 @@ CASES = [
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("groups,Hq,Hk,D,page,layout", CASES)
 def test_matches_the_plain_form(groups, Hq, Hk, D, page, layout, dtype):
-    check(make(groups, Hq, Hk, D, page, layout, dtype, len(groups) + Hq), layout)
+    case = make(groups, Hq, Hk, D, page, layout, dtype, len(groups) + Hq)
+    check(case, layout)
+    check(case, layout, wide=False)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
@@ -139,6 +150,7 @@ def test_agrees_with_the_unshared_form():
     note("unshared")
     q, kc, vc, table, lens = (t.to(DEV) for t in make([(5000, [60, 7, 900, 1]), (64, [3, 3])], 28,
                                                       4, 128, 16, "NHD", BF16, 5))
+    table = widened(table, kc)
     shared = paged_prefix_decode_attention(q, kc, vc, table, lens, paged_kv_prefix(lens, table, 16))
     plain = paged_decode_attention(q, kc, vc, table, lens)
     assert float((shared.double() - plain.double()).norm() / plain.double().norm()) < 2.0 ** -8
@@ -188,7 +200,7 @@ def test_pages_that_cannot_be_read(dtype):
     q, kc, vc, table, lens = case
     want, slack = room(*case, "NHD")
     for n, k, bad in ((0, 3, 10 ** 6), (3, 7, kc.shape[0]), (1, 40, -1), (5, 0, -7)):
-        broken = table.clone()
+        broken = widened(table, kc)
         rows = [n]
         if n in (0, 3) and k < (40 if n == 0 else 8):  # a page that the whole group shares
             rows = [0, 1, 2] if n == 0 else [3, 4]
@@ -204,7 +216,7 @@ def test_pages_that_cannot_be_read(dtype):
                 assert bool(((out[r] - want[r]).abs()
                              <= ref.rounded(want, slack, dtype)[r]).all()), (n, r)
     short = table[:, :30].contiguous()  # tables narrower than the lengths
-    out, _ = run(q, kc, vc, short, lens)
+    out, _ = run(q, kc, vc, short, lens, wide=False)
     assert bool(torch.isnan(out[:3]).all()) and bool(torch.isfinite(out[3:]).all())
 
 
@@ -278,8 +290,7 @@ def test_strided_views():
     tall[::2] = kc.to(DEV)
     odd = torch.zeros(kc.numel() + 1, dtype=BF16, device=DEV)[1:].view(kc.shape)
     odd.copy_(kc)
-    d_table = torch.full((5, table.shape[1] + 9), 3, dtype=torch.int32, device=DEV)
-    d_table[:, :table.shape[1]] = table.to(DEV)
+    d_table = widened(table, kc).to(DEV)
     pairs = torch.stack([lens, lens + 1], 1).to(DEV)
     prefix = paged_kv_prefix(pairs[:, 0], d_table, 16)
     doubled = [torch.stack([t, t], 1)[:, 0] for t in prefix]
@@ -300,7 +311,7 @@ def test_offsets_past_32_bits():
     big_v = torch.zeros(400000, 16, 2, 128, dtype=BF16, device=DEV)
     at = 400000 - P
     big_k[at:], big_v[at:] = kc.to(DEV), vc.to(DEV)
-    far = torch.where(table >= 0, table + at, table).to(DEV)
+    far = widened(torch.where(table >= 0, table + at, table), kc).to(DEV)
     d_lens = lens.to(DEV)
     out = paged_prefix_decode_attention(q.to(DEV), big_k, big_v, far, d_lens,
                                         paged_kv_prefix(d_lens, far, 16))
@@ -312,7 +323,9 @@ def test_streams_and_two_graphs():
     """Two captured graphs and eager calls on another stream, each with a workspace of its own."""
     note("graphs")
     cases = [[t.to(DEV) for t in make([(3000 + 100 * s, [60, 7, 300, 1]), (640, [3, 3])], 8, 2, 128,
-                                      16, "NHD", BF16, s, gap=30 - 7 * s)] for s in (0, 1)]
+                                      16, "NHD", BF16, s)] for s in (0, 1)]
+    for case in cases:
+        case[3] = widened(case[3], case[1])
     want = []
     for q, kc, vc, table, lens in cases:
         want.append(paged_prefix_decode_attention(q, kc, vc, table, lens,
@@ -345,6 +358,7 @@ def test_same_bits_every_time():
     note("same bits")
     q, kc, vc, table, lens = (t.to(DEV) for t in make([(9000, [60, 7, 300, 1]), (640, [3, 3])], 28,
                                                       4, 128, 16, "NHD", BF16, 3))
+    table = widened(table, kc)
     prefix = paged_kv_prefix(lens, table, 16)
     want = paged_prefix_decode_attention(q, kc, vc, table, lens, prefix)
     for _ in range(5):

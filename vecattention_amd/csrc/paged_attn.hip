@@ -398,8 +398,11 @@ static hipError_t launch_paged_t(int dtype, PagedArgs& a, void* workspace, hipSt
 }
 
 // States of rows' own keys: always dealt evenly, since the tables' width says nothing
-// about how many there are.
-int64_t paged_states_workspace(int dtype, PagedArgs& a) { return plan_tiles(dtype, a); }
+// about how many there are, to one work-group a CU, which the prefixes' work-groups
+// join (paged_prefix.hip).
+int64_t paged_states_workspace(int dtype, PagedArgs& a) {
+  return plan_form(a, dtype == kF32 ? kTileUnit<float> : kTileUnit<bf16_t>, kTileHeads, 256);
+}
 
 hipError_t launch_paged_attn(int dtype, PagedArgs a, void* workspace, hipStream_t stream) {
   if (dtype == kBF16) return launch_paged_t<bf16_t>(dtype, a, workspace, stream);

@@ -480,16 +480,20 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
           __builtin_amdgcn_s_setprio(0);
         }
         if constexpr (kWhole) next = find(t + 2);  // here by the next barrier
-        float tmax;
-        {
-          float u0 = max3_plain(sc[0][0], sc[0][1], sc[0][2]), u1 = sc[0][3];
+        // The maximum's instructions are inline assembly, before which the compiler leaves no
+        // wait for the matrix instructions: 11 wait states after the last one.
+        float tmax = 0.f;
+        static_for<2>([&](auto half) {
+          constexpr int hf = decltype(half)::value;
+          if constexpr (hf == 1) asm volatile("s_nop 10" : "+v"(sc[1]));
+          float u0 = max3_plain(sc[hf][0], sc[hf][1], sc[hf][2]), u1 = sc[hf][3];
 #pragma unroll
-          for (int e = 4; e < 32; e += 4) {
-            u0 = max3_plain(u0, sc[e / 16][e % 16], sc[e / 16][e % 16 + 1]);
-            u1 = max3_plain(u1, sc[e / 16][e % 16 + 2], sc[e / 16][e % 16 + 3]);
+          for (int e = 4; e < 16; e += 4) {
+            u0 = max3_plain(u0, sc[hf][e], sc[hf][e + 1]);
+            u1 = max3_plain(u1, sc[hf][e + 2], sc[hf][e + 3]);
           }
-          tmax = max_plain(u0, u1);
-        }
+          tmax = hf == 0 ? max_plain(u0, u1) : max3_plain(tmax, u0, u1);
+        });
         // The maximum moves when a score's weight would exceed 2 to the slack.
         const float lead = tmax * a.scale_log2 + mneg;
         const bool first = mneg == __builtin_inff();
@@ -595,8 +599,10 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
   }
 }
 
-// The prefixes' work-groups, then those of the rows' own keys: what is left of the GPU
-// beside the ones is taken by the others.
+// The work-groups of the rows' own keys, which are the shorter ones, then those of the
+// prefixes, which take their places as they end.  us, 40 rows of 6 prompts / 64 rows of
+// 131072 keys: in this order 26.1 / 158, own keys behind 30.1 / 164, own keys in a launch
+// of their own 32.1 / 171.
 template <typename T, int D, bool kWhole>
 __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void prefix_kernel(SharedArgs x) {
   __shared__ union Lds {
@@ -604,19 +610,19 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void prefix_kernel(Shar
     PrefixLds<T, D, kWhole> prefix;
     TileLds<T, D, kFormSplit> own;
   } lds;
-  if (blockIdx.x < uint32_t(x.groups))
-    prefix_tile<T, D, kWhole>(x, lds.prefix, blockIdx.x);
+  const uint32_t own = uint32_t(x.a.groups);
+  if (blockIdx.x < own)
+    paged_tile<T, D, kWhole, kFormSplit, false, true>(x.a, lds.own, blockIdx.x);
   else
-    paged_tile<T, D, kWhole, kFormSplit, false, true>(x.a, lds.own,
-                                                      blockIdx.x - uint32_t(x.groups));
+    prefix_tile<T, D, kWhole>(x, lds.prefix, blockIdx.x - own);
 }
 
 // One row's state over its first `keys` keys in fp32, a wave a key: for rows whose
 // values are not finite, which the matrix products' rounded weights (0 for a key far
 // below the others) would make NaN of.  To sm, sl and so of each wave.
-template <typename T, int D>
+template <typename T, int D, int kW>
 __device__ void row_state(const PagedArgs& a, int64_t n, uint32_t head, uint32_t hk, int32_t keys,
-                          float (&sm)[kWaves], float (&sl)[kWaves], float (*so)[D]) {
+                          float (&sm)[kW], float (&sl)[kW], float (*so)[D]) {
   constexpr int NF = D / 64, U = 4;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const T* qp = static_cast<const T*>(a.q) + n * a.qn + int64_t(head) * a.qh;
@@ -624,7 +630,7 @@ __device__ void row_state(const PagedArgs& a, int64_t n, uint32_t head, uint32_t
   float q[NF], acc[NF], m = -__builtin_inff(), l = 0.f;
 #pragma unroll
   for (int j = 0; j < NF; ++j) q[j] = to_f32(qp[lane + 64 * j]), acc[j] = 0.f;
-  for (int32_t k0 = U * wave; k0 < keys; k0 += U * kWaves) {
+  for (int32_t k0 = U * wave; k0 < keys; k0 += U * kW) {
     float kf[U][NF], vf[U][NF];
     bool bad = false;
 #pragma unroll
@@ -666,20 +672,28 @@ __device__ void row_state(const PagedArgs& a, int64_t n, uint32_t head, uint32_t
 
 // Joins the states of a (request, query head): those of the prefix's shares, then
 // those of its own keys, always in this order.
+constexpr int kJoinThreads = 128;
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void prefix_merge_kernel(SharedArgs x) {
-  constexpr int kLanes = D / 4, kSide = kThreads / kLanes, U = 4;
-  constexpr int kMost = 2 * 512 + 2 + kWaves;
+__global__ __launch_bounds__(kJoinThreads) void prefix_merge_kernel(SharedArgs x) {
+  constexpr int kW = kJoinThreads / 64;
+  constexpr int kLanes = D / 4, kSide = kJoinThreads / kLanes, U = 8;
+  constexpr int kMost = 2 * 512 + 2 + kW;
   typedef float vec4 __attribute__((ext_vector_type(4)));
   __shared__ float weight[kMost];
-  __shared__ vec4 sacc[kThreads];
-  __shared__ float top[kWaves], den[kWaves], sm[kWaves], sl[kWaves];
+  __shared__ vec4 sacc[kJoinThreads];
+  __shared__ float top[kW], den[kW], sm[kW], sl[kW];
   const PagedArgs& a = x.a;
   const int64_t row = blockIdx.x;
   const uint32_t Hq = uint32_t(a.Hk * a.G), n = uint32_t(row) / Hq, head = uint32_t(row) - n * Hq;
   T* out = static_cast<T*>(a.out) + n * a.on + head * a.oh;
   const int c = threadIdx.x % kLanes, side = threadIdx.x / kLanes, me = threadIdx.x;
-  if (a.lens[n] <= 0) {
+  const uint32_t hk = head / uint32_t(a.G), in = head - hk * uint32_t(a.G);
+  const uint32_t tile = in / uint32_t(a.rows), r = in - tile * uint32_t(a.rows);
+  // Read together, whatever is needed of them.
+  const int32_t len = a.lens[n], prefix = a.prefix_lens[n];
+  const int4 record = x.record[row];
+  const int2 split = a.split[int64_t(n) * a.per_request + hk * uint32_t(a.tiles) + tile];
+  if (len <= 0) {
     if (side == 0)
 #pragma unroll
       for (int e = 0; e < 4; ++e) out[4 * c + e] = Round<T>::store(0.f);
@@ -687,16 +701,13 @@ __global__ __launch_bounds__(kThreads) void prefix_merge_kernel(SharedArgs x) {
   }
   // The prefix's pieces, and those of the row's own segment.
   int pre = 0, pre_from = 0, place = 0;
-  const int32_t shared = shared_keys(a.prefix_lens[n], a.M * a.page);
+  const int32_t shared = shared_keys(prefix, a.M * a.page);
   if (shared > 0) {
-    const int4 r = x.record[row];
-    pre_from = r.y >= 0 && r.y < x.groups ? r.y : 0;
-    pre = 1 + (r.x < 0 ? 0 : r.x < x.groups - pre_from ? r.x : x.groups - pre_from);
-    place = r.z >= 0 && r.z < x.stride ? r.z : 0;
+    pre_from = record.y >= 0 && record.y < x.groups ? record.y : 0;
+    pre = 1 + (record.x < 0 ? 0
+                            : record.x < x.groups - pre_from ? record.x : x.groups - pre_from);
+    place = record.z >= 0 && record.z < x.stride ? record.z : 0;
   }
-  const uint32_t hk = head / uint32_t(a.G), in = head - hk * uint32_t(a.G);
-  const uint32_t tile = in / uint32_t(a.rows), r = in - tile * uint32_t(a.rows);
-  const int2 split = a.split[int64_t(n) * a.per_request + hk * uint32_t(a.tiles) + tile];
   const int own_from = split.x < 0 ? 0 : split.x / 2;
   const int own = 1 + (split.x < 0 ? 0 : split.y - own_from);
   const int64_t slots = 2 * int64_t(a.groups);
@@ -726,7 +737,7 @@ __global__ __launch_bounds__(kThreads) void prefix_merge_kernel(SharedArgs x) {
   float l;
   auto weights = [&](int parts) {
     float m = -__builtin_inff();
-    for (int i = me; i < parts; i += kThreads) {
+    for (int i = me; i < parts; i += kJoinThreads) {
       const float2 y = ml(i);
       if (!(y.y == 0.f)) m = __builtin_fmaxf(m, y.x);
     }
@@ -735,9 +746,9 @@ __global__ __launch_bounds__(kThreads) void prefix_merge_kernel(SharedArgs x) {
     if (me % 64 == 0) top[me / 64] = m;
     lds_barrier();
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) m = __builtin_fmaxf(m, top[w]);
+    for (int w = 0; w < kW; ++w) m = __builtin_fmaxf(m, top[w]);
     l = 0.f;
-    for (int i = me; i < parts; i += kThreads) {
+    for (int i = me; i < parts; i += kJoinThreads) {
       const float2 y = ml(i);
       const float f = __builtin_amdgcn_exp2f(y.x - m);
       weight[i] = y.y == 0.f ? -1.f : f;  // -1: no weight at all
@@ -749,7 +760,7 @@ __global__ __launch_bounds__(kThreads) void prefix_merge_kernel(SharedArgs x) {
     lds_barrier();
     l = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) l += den[w];
+    for (int w = 0; w < kW; ++w) l += den[w];
   };
   auto add = [&](vec4& acc, float f, vec4 y) {
     if (f > 0.f) acc += f * y;
@@ -757,16 +768,22 @@ __global__ __launch_bounds__(kThreads) void prefix_merge_kernel(SharedArgs x) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[e] += f != f ? f : weighed(f, y[e]);
   };
-  auto gather = [&](int parts) {
+  vec4 y[U];
+  auto load = [&](int from, int parts) {
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      y[i] = state(from + i * kSide < parts ? from + i * kSide : parts - 1);
+  };
+  auto gather = [&](int parts) {  // the first ones are loaded
     vec4 acc = vec4(0.f);
     for (int from = side; from < parts; from += U * kSide) {
-      vec4 y[U];
+      vec4 z[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) z[i] = y[i];
+      if (from + U * kSide < parts) load(from + U * kSide, parts);
 #pragma unroll
       for (int i = 0; i < U; ++i)
-        y[i] = state(from + i * kSide < parts ? from + i * kSide : parts - 1);
-#pragma unroll
-      for (int i = 0; i < U; ++i)
-        add(acc, from + i * kSide < parts ? weight[from + i * kSide] : -1.f, y[i]);
+        add(acc, from + i * kSide < parts ? weight[from + i * kSide] : -1.f, z[i]);
     }
     sacc[me] = acc;
     lds_barrier();
@@ -775,6 +792,7 @@ __global__ __launch_bounds__(kThreads) void prefix_merge_kernel(SharedArgs x) {
     for (int i = 1; i < kSide; ++i) acc += sacc[i * kLanes + c];
     return acc;
   };
+  load(side, own + pre);
   weights(own + pre);
   vec4 acc = gather(own + pre);
   bool nan = false;
@@ -782,30 +800,31 @@ __global__ __launch_bounds__(kThreads) void prefix_merge_kernel(SharedArgs x) {
   for (int e = 0; e < 4; ++e) nan |= acc[e] != acc[e];
   if (pre > 0 && l == l && __syncthreads_or(nan)) {
     // (The row's own table lists the same pages.)
-    row_state<T, D>(a, n, head, hk, shared, sm, sl, so());
+    row_state<T, D, kW>(a, n, head, hk, shared, sm, sl, so());
     exact = true;
     __syncthreads();
-    vec4 rest[kWaves];
+    vec4 rest[kW];
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) rest[w] = *reinterpret_cast<const vec4*>(&so()[w][4 * c]);
+    for (int w = 0; w < kW; ++w) rest[w] = *reinterpret_cast<const vec4*>(&so()[w][4 * c]);
     __syncthreads();
-    weights(own + kWaves);
+    load(side, own);
+    weights(own + kW);
     acc = gather(own);
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) add(acc, weight[own + w], rest[w]);
+    for (int w = 0; w < kW; ++w) add(acc, weight[own + w], rest[w]);
   }
   if (side != 0) return;
-  struct alignas(sizeof(T) * 4) Out { T v[4]; } y;
+  struct alignas(sizeof(T) * 4) Out { T v[4]; } z;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) y.v[e] = Round<T>::store(acc[e] / l);
-  *reinterpret_cast<Out*>(out + 4 * c) = y;
+  for (int e = 0; e < 4; ++e) z.v[e] = Round<T>::store(acc[e] / l);
+  *reinterpret_cast<Out*>(out + 4 * c) = z;
 }
 
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 
 // Work-groups for the prefixes: no more than there can be steps.
 int64_t prefix_groups(const PagedArgs& a) {
-  const int64_t tiles = a.N * a.G / kRows + a.N;
+  const int64_t tiles = a.N * a.G / kRows + (a.N + 1) / 2;  // groups have two rows at least
   const int64_t steps = a.Hk * tiles * (a.M * a.page / kPrefixTile);
   return steps < 1 ? 1 : steps < kMostGroups ? steps : kMostGroups;
 }
@@ -822,16 +841,22 @@ hipError_t launch_prefix(const SharedArgs& x, hipStream_t stream) {
 template <typename T, int D>
 hipError_t launch_join(const SharedArgs& x, hipStream_t stream) {
   hipLaunchKernelGGL((prefix_merge_kernel<T, D>), dim3(unsigned(x.a.N * x.a.Hk * x.a.G)),
-                     dim3(kThreads), 0, stream, x);
+                     dim3(kJoinThreads), 0, stream, x);
   return hipGetLastError();
 }
 
 // Whether the prefix is computed once: 16-bit rows that the matrix-core form takes, a
-// scale that orders scores as the products are ordered, and tables that could share a
-// tile of keys.
+// scale that orders scores as the products are ordered, and enough to read if every row
+// did so for itself, to the tables' width, which the two launches here cost less than.
+// us, every row for itself / shared, 28 query and 4 kv heads of 128 in bf16: 8 rows of
+// 4096 keys (68 MB) 17.6 / 24, of 8192 (135 MB) 28.8 / 25, 64 rows of 1024 keys (143 MB)
+// 23.6 / 33, of 2048 (277 MB) 37.8 / 34; 16 and 16 heads of 64: 8 rows of 2048 keys (69 MB)
+// 18.7 / 17.6, of 4096 25.0 / 17.6.
 bool shares_prefix(int dtype, const PagedArgs& a) {
-  return dtype != kF32 && a.N > 1 && a.M * a.page >= kPrefixTile && a.scale_log2 >= 0.f &&
-         a.kn < (int64_t(1) << 26) && a.vn < (int64_t(1) << 26) && paged_tile_form(dtype, a);
+  const double bytes = 4.0 * double(a.N * a.Hk * a.D) * double(a.M * a.page);
+  return dtype != kF32 && a.N > 1 && bytes > double(128 << 20) && a.M * a.page >= kPrefixTile &&
+         a.scale_log2 >= 0.f && a.kn < (int64_t(1) << 26) && a.vn < (int64_t(1) << 26) &&
+         paged_tile_form(dtype, a);
 }
 
 // The regions of the workspace, behind those of the rows' own keys (`own` bytes).
@@ -863,7 +888,7 @@ int64_t lay_out(PagedArgs& a, SharedArgs* x, char* work, int64_t own) {
     x->groups = int32_t(groups);
     x->stride = int32_t(stride);
     x->by_g = FastDiv(uint32_t(a.G));
-    x->least = 4;
+    x->least = 2;
     x->a = a;
   }
   return at;
