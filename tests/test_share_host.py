@@ -350,3 +350,18 @@ def test_c_attend_errors(L):
     assert c_attend(L, ws=None) == nat.VA_ERR_WORKSPACE
     assert c_attend(L, wsb=need - 1) == nat.VA_ERR_WORKSPACE
     assert L.va_paged_prefix_decode_workspace_size(1, 3, 5, 2, 128, 8, 16) == -1
+
+
+def test_no_matrix_result_of_shared_prefixes_is_read_too_soon(tmp_path, monkeypatch):
+    import asm_hazards
+    # Passes + 3 for 16-bit operands, of which 32x32x16 takes 8.
+    monkeypatch.setattr(asm_hazards, "NEED", {**asm_hazards.NEED, "v_mfma_f32_32x32x16_bf16": 11,
+                                              "v_mfma_f32_32x32x16_f16": 11})
+    from vecattention_amd import build
+    csrc = os.path.join(os.path.dirname(build.__file__), "csrc")
+    out = tmp_path / "paged_prefix.s"
+    subprocess.run([build.hipcc(), *build.FLAGS, "--cuda-device-only", "-S",
+                    os.path.join(csrc, "paged_prefix.hip"), "-o", str(out)], check=True,
+                   capture_output=True)
+    count, early = asm_hazards.early_reads(out.read_text())
+    assert count > 300 and early == []
