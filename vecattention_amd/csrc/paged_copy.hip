@@ -6,8 +6,9 @@
 // thread, all loads before the stores.
 //
 // us, 1500 pages of 32 KB in eight caches (786 MB read and written): 233 with every
-// piece's place found by two divisions, which made it 70 us of arithmetic; @LINEAR@ where
-// pages are blocks without gaps, whose pieces need none.
+// piece's place found by two divisions, which made it 70 us of arithmetic; 158 (5.0 TB/s,
+// a large copy's rate) where pages are blocks without gaps, whose pieces need none.  Last
+// pages of eight rows in 4 layers: 5.1, the launch.
 #include "common.h"
 #include "paged_ops.h"
 

@@ -5,14 +5,29 @@
 // sum_j 2^(s_j - m) V_j over the prefix and over the row's own keys, in log2 units,
 //   out = (o_p 2^(m_p - m) + o_r 2^(m_r - m)) / (l_p 2^(m_p - m) + l_r 2^(m_r - m)).
 //
-// Three launches: the prefixes (here), the rows' own keys (paged_attn.hip's tile
-// kernel, kState) and the merge.  A prefix's rows are the query heads of a kv head of
-// all its requests, 128 to a tile: a work-group takes one, each wave 32 of its rows,
-// and walks 64 keys a step as dense attention does (attn_dense.hip): K and V tiles go
-// to a ring of three LDS slots, S^T = K Q^T and O^T += V^T P^T on 32x32x16 matrix
-// instructions, weights from the scores' registers.  The steps of all (group, kv head,
-// tile) segments are dealt evenly to the work-groups (PagedShare), since the lengths
-// are known to the GPU only.
+// Two launches: the rows' own keys (paged_tile.h, kState) and the prefixes beside each
+// other, then the merge.  A prefix's rows are the query heads of a kv head of all its
+// requests, 128 to a tile; a piece of work is a tile and a range of keys, dealt so that
+// every work-group has one (the lengths are known to the GPU only: each work-group
+// counts the pieces for itself).  A wave takes 32 rows and walks 64 keys a step as dense
+// attention does (attn_dense.hip): K and V tiles go to a ring of three LDS slots, S^T =
+// K Q^T and O^T += V^T P^T on 32x32x16 matrix instructions, weights from the scores'
+// registers, rounded once to 16 bits (each weight by half a step at most, the same in the
+// sum of the values and in the weights' own sum, which puts an output off by about as
+// much as its own rounding; two parts a weight, as for the own keys, would double the
+// products).  Only whole 64-key tiles of a prefix are walked here, without masks; what is
+// left of it comes with the row's own keys.
+//
+// us, bf16, D 128: 64 rows of 28 query and 4 kv heads that share 131072 keys: 152 for
+// 120 GFLOP (790 TFLOP/s; the rows' tiles hold 8/7 of that): 30 at any length (launches,
+// counting, 33 MB of states written and read again), then steps at 1000 TFLOP/s and more,
+// where the matrix cores' power is the bound, as in dense attention.  Every row for
+// itself: 2466.  40 rows of 32 query and 8 kv heads in six groups of 8192 keys: 34 for
+// 96 MB (19 at a copy's rate), where every row for itself takes 67.
+// Tried, and no faster: rings of four and six slots; two to eight K and V fragments read
+// ahead; three work-groups a CU; the keys of a step between two waves where a tile has 64
+// rows at most (a half step takes 0.8 of a whole one: 162 -> 184 with twice the steps a
+// piece); ranges that begin their walks at different steps.
 #include "attn_common.h"
 #include "lanes.h"
 #include "mfma.h"
@@ -25,7 +40,7 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kRows = 128;       // rows of a tile
-constexpr int kMostGroups = 512;  // of the prefixes: two a CU  // three a CU
+constexpr int kMostGroups = 512;  // of the prefixes: two a CU
 constexpr int kIdKeys = 1024;    // keys whose page ids lie in LDS, for pages of any size
 
 // Where a state lies: that of the first piece with its row, (request, query head); those
