@@ -70,8 +70,9 @@ __device__ inline int32_t block_exclusive_sum(int32_t x, int32_t* part, int32_t*
 // they do not depend on the order of the atomics.
 struct ForkWork {
   uint32_t* least;    // (P) first row that would write to a page
-  int32_t* writers;   // (P) and their number; both are set where a row writes alone
+  int32_t* writers;   // (P) and their number; both are set where a row writes
   uint8_t* first;     // (R) no row before it has its parent; (N) behind it: rows with children
+  int32_t* end;       // (R) page that the row would write to, -1 for none
   int32_t* rank;      // (R) number of the row's copy, -1 for none
   int32_t* row_of;    // (R) row of each copy
   uint64_t* gone;     // (P / 64) pages with s1 < 0
@@ -87,7 +88,8 @@ ForkWork fork_work(void* workspace, int64_t R, int64_t P) {
   w.gone = static_cast<uint64_t*>(workspace);
   w.least = reinterpret_cast<uint32_t*>(w.gone + chunks * (kPagesPer / 64));
   w.writers = reinterpret_cast<int32_t*>(w.least + P);
-  w.rank = w.writers + P;
+  w.end = w.writers + P;
+  w.rank = w.end + R;
   w.row_of = w.rank + R;
   w.counts = w.row_of + R;
   w.first = reinterpret_cast<uint8_t*>(w.counts + chunks + 1);
@@ -143,6 +145,7 @@ __global__ __launch_bounds__(kThreads) void fork_rows_kernel(ForkArgs a, ForkWor
       w.first[r] = !earlier;
       a.kv_out[r] = row.len;
       const int32_t p = row.open(a);
+      w.end[r] = p;
       if (p >= 0) {
         w.least[p] = 0xffffffffu;
         w.writers[p] = 0;
@@ -179,7 +182,7 @@ __global__ __launch_bounds__(kThreads) void fork_counts_kernel(ForkArgs a, ForkW
   if (i < a.R) {
     const ForkRow row(a, i);
     if (first == 0 && threadIdx.x == 0) {
-      const int32_t p = row.open(a);
+      const int32_t p = w.end[i];
       if (p >= 0) {
         atomicMin(w.least + p, uint32_t(i));
         add_agent(w.writers + p, 1);
@@ -230,8 +233,7 @@ __global__ __launch_bounds__(kThreads) void fork_scan_kernel(ForkArgs a, ForkWor
     const int64_t r = base + threadIdx.x;
     bool copies = false;
     if (r < a.R) {
-      const ForkRow row(a, r);
-      const int32_t p = row.open(a);
+      const int32_t p = w.end[r];
       if (p >= 0) {
         const int32_t s = load_agent(a.shares_out + p);  // below 0, or made 0 by its chunk
         copies = w.least[p] != uint32_t(r) || (s > 0 ? s : 0) + 1 > w.writers[p];
@@ -277,9 +279,8 @@ __global__ __launch_bounds__(kThreads) void fork_place_kernel(ForkArgs a, ForkWo
       const int32_t id = int32_t(g * kPagesPer + 64 * i + lane);
       if (j < taken) {
         const int32_t r = w.row_of[j];
-        const ForkRow row(a, r);
         a.copy_dst[r] = id;
-        a.table_out[r * a.M + open_page(row.len, a.page, uint32_t(a.M))] = id;
+        a.table_out[r * a.M + open_page(a.kv_out[r], a.page, uint32_t(a.M))] = id;
       } else if (top + j >= 0) {
         a.free_out[top + j] = id;
       }
@@ -293,21 +294,20 @@ __global__ __launch_bounds__(kThreads) void fork_place_kernel(ForkArgs a, ForkWo
     *a.head_out = int32_t(left < 0 ? 0 : left < 0x7fffffff ? left : 0x7fffffff);
   }
   if (r >= a.R) return;
-  const ForkRow row(a, r);
-  const int32_t p = row.open(a), j = w.rank[r];
+  const int32_t p = w.end[r], j = w.rank[r], len = a.kv_out[r];
   if (p >= 0 && w.least[p] == uint32_t(r)) {
     // The copies' share in the page goes.
     const int32_t copies = w.writers[p] - (j < 0), s = a.shares_out[p] - copies;
     a.shares_out[p] = s > 0 ? s : 0;
   }
   a.copy_src[r] = j < 0 ? -1 : p;
-  a.copy_rows[r] = j < 0 ? 0 : int32_t(uint32_t(row.len) % a.page);
+  a.copy_rows[r] = j < 0 ? 0 : int32_t(uint32_t(len) % a.page);
   if (j < 0) {
     a.copy_dst[r] = -1;
   } else if (j >= freed) {
     const int32_t id = free_page(a.free_pages, a.F, top + j);
     a.copy_dst[r] = id;
-    a.table_out[r * a.M + open_page(row.len, a.page, uint32_t(a.M))] = id;
+    a.table_out[r * a.M + open_page(len, a.page, uint32_t(a.M))] = id;
   }
 }
 
@@ -631,14 +631,18 @@ __global__ __launch_bounds__(kThreads) void prefix_groups_kernel(PrefixArgs a,
 constexpr int kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64;
 constexpr int kSmallRows = 256;
 constexpr int kSmallPages = 8192;       // 32 KB of counts
-constexpr int64_t kSmallEntries = 32768;
+// Table entries, above which the general forms are as fast.  us, here / general: fork (rows
+// before and after), 8 rows of 2048 entries 14.2 / 19, 64 of 256 15.2 / 19, 32 of 1024 24 /
+// 20.5; compaction, 16384 entries 17.6 / 21, 32768 32 / 22; prefixes, 16384 entries 7.4 to
+// 10.0 / 9.5, 32768 11.5 to 17.6 / 9.5.
+constexpr int64_t kSmallForkEntries = 32768, kSmallEntries = 16384;
 constexpr int32_t kGone = -(1 << 30);   // the count of a page that no row holds any more
 
 __global__ __launch_bounds__(kSmallThreads) void fork_small_kernel(ForkArgs a, FastDiv by_m) {
   __shared__ int32_t s[kSmallPages];
   __shared__ int32_t parent[kSmallRows], held[kSmallRows], had[kSmallRows], ends[kSmallRows];
   __shared__ int32_t old_held[kSmallRows], freed[kSmallRows];
-  __shared__ uint8_t is_first[kSmallRows], kids[kSmallRows];
+  __shared__ uint8_t is_first[kSmallRows], kids[kSmallRows], later[kSmallRows];
   __shared__ int32_t part[2][kSmallWaves];
   const int t = threadIdx.x, lane = t % 64, wave = t / 64;
   const int R = int(a.R), N = int(a.N), P = int(a.P), F = int(a.F);
@@ -652,6 +656,8 @@ __global__ __launch_bounds__(kSmallThreads) void fork_small_kernel(ForkArgs a, F
     held[t] = int32_t(row.held);
     had[t] = int32_t(row.had);
     ends[t] = row.open(a);
+    is_first[t] = 1;
+    later[t] = 0;
     len = row.len;
     a.kv_out[t] = len;
   } else if (t >= kSmallRows && t < kSmallRows + N) {
@@ -659,18 +665,27 @@ __global__ __launch_bounds__(kSmallThreads) void fork_small_kernel(ForkArgs a, F
     kids[t - kSmallRows] = 0;
   }
   __syncthreads();
-  bool not_least = false;
+  // Whether a row before has the same parent, or ends in the same page: four threads a row.
   const int32_t end = t < R ? ends[t] : -1;
-  if (t < R) {
-    bool first = true;
-    for (int j = 0; j < t; ++j) {
-      first = first && parent[j] != parent[t];
-      not_least |= ends[j] == end;
+  {
+    constexpr int kParts = kSmallThreads / kSmallRows;
+    const int r = t % kSmallRows, run = (R + kParts - 1) / kParts, j0 = t / kSmallRows * run;
+    const int stop = j0 + run < R ? j0 + run : R;
+    if (r < R) {
+      const int32_t p = parent[r], at = ends[r];
+      int same = 0, writes = 0;
+#pragma unroll 8
+      for (int j = j0; j < stop; ++j) {
+        same |= int(j < r) & int(parent[j] == p);
+        writes |= int(j < r) & int(ends[j] == at);
+      }
+      if (same) is_first[r] = 0;
+      if (writes) later[r] = 1;
+      if (t < R && p >= 0) kids[p] = 1;
     }
-    is_first[t] = first;
-    if (parent[t] >= 0) kids[parent[t]] = 1;
   }
   __syncthreads();
+  const bool not_least = t < R && later[t] != 0;
   for (uint32_t e = t; e < uint32_t(R) * M; e += kSmallThreads) {
     const uint32_t r = by_m.div(e), k = e - r * M;
     int32_t id = -1;
@@ -901,12 +916,12 @@ unsigned extra_groups(int64_t work) {
 
 int64_t fork_workspace_bytes(int64_t R, int64_t P) {
   const int64_t chunks = fork_chunks(P);
-  return 8 * chunks * (kPagesPer / 64) + 4 * (2 * P + 2 * R + chunks + 1) + R + kForkMostRows;
+  return 8 * chunks * (kPagesPer / 64) + 4 * (2 * P + 3 * R + chunks + 1) + R + kForkMostRows;
 }
 
 hipError_t launch_paged_fork(const ForkArgs& a, void* workspace, hipStream_t stream) {
   if (a.N <= kSmallRows && a.R <= kSmallRows && a.P <= kSmallPages &&
-      a.F <= 2 * kSmallPages && (a.N + a.R) * a.M <= kSmallEntries) {
+      a.F <= 2 * kSmallPages && (a.N + a.R) * a.M <= kSmallForkEntries) {
     hipLaunchKernelGGL(fork_small_kernel, dim3(1), dim3(kSmallThreads), 0, stream, a,
                        FastDiv(uint32_t(a.M > 0 ? a.M : 1)));
     return hipGetLastError();
