@@ -52,7 +52,9 @@ def widened(table, kc, layout="NHD"):
     """The same table with room for longer requests: so much that the prefix is computed once (the
     form goes by the tables' width), however few keys there are."""
     page, Hk = (kc.shape[1], kc.shape[2]) if layout == "NHD" else (kc.shape[2], kc.shape[1])
-    width = -(-(130 << 20) // (4 * len(table) * page * Hk * kc.shape[3]))
+    D = kc.shape[3]
+    most = (260 if kc.dtype == F32 and D == 128 else 130) << 20
+    width = -(-most // (4 * len(table) * page * Hk * D))
     more = torch.full((len(table), max(width - table.shape[1], 0)), -1, dtype=torch.int32)
     return torch.cat([table, more.to(table.device)], 1)
 

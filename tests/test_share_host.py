@@ -354,9 +354,11 @@ def test_c_attend_errors(L):
 
 def test_no_matrix_result_of_shared_prefixes_is_read_too_soon(tmp_path, monkeypatch):
     import asm_hazards
-    # Passes + 3 for 16-bit operands, of which 32x32x16 takes 8.
+    # Passes + 3 for 16-bit operands, of which 32x32x16 takes 8; passes + 2 for fp32 ones, of which
+    # 32x32x2 takes 16.
     monkeypatch.setattr(asm_hazards, "NEED", {**asm_hazards.NEED, "v_mfma_f32_32x32x16_bf16": 11,
-                                              "v_mfma_f32_32x32x16_f16": 11})
+                                              "v_mfma_f32_32x32x16_f16": 11,
+                                              "v_mfma_f32_32x32x2_f32": 18})
     from vecattention_amd import build
     csrc = os.path.join(os.path.dirname(build.__file__), "csrc")
     out = tmp_path / "paged_prefix.s"

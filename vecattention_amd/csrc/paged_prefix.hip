@@ -244,6 +244,7 @@ __device__ inline void copy16_from(uint32_t lds_base, uint64_t address) {
 }
 
 template <typename T> constexpr bool kIsF16 = std::is_same_v<T, f16_t>;
+template <typename T> constexpr bool kIsF32 = std::is_same_v<T, float>;
 
 // kWhole: pages of a multiple of 16 tokens, so that the 16 keys that a wave copies of
 // a tile lie in one.
@@ -614,20 +615,207 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
   }
 }
 
+// The same in fp32.  A wave takes 32 rows and walks 32 keys at a time by itself, rows of K
+// and V going from memory to the registers of the lane that multiplies them: S^T = K Q^T
+// in D/2 v_mfma_f32_32x32x2_f32 (lane l: key or row l % 32, features from l / 32 * D / 2
+// on), O^T += V^T P^T in D/2 more, weights from the scores' registers.  Where a tile has 64
+// (32) rows at most, two (four) waves take turns at the same rows' keys.  Bound by the fp32
+// matrix cores: 8192 cycles for 32 keys of D 128, beside which loads and exponentials are
+// little (64 rows of 28 and 4 heads of 128 over 8192 keys: 135 us for 7.5 GFLOP, of which 45
+// at any length; every row for itself 307).
+template <int D> struct PrefixLdsF32 {
+  PiecesLds pieces;
+  float2 ml[kWaves][64];
+  float o[3][32 * D];
+};
+template <int D>
+__device__ __forceinline__ void prefix_tile_f32(const SharedArgs& x, PrefixLdsF32<D>& shared,
+                                                uint32_t block) {
+  constexpr int NB = D / 32, NQ = D / 8, kStep = 32;
+  PiecesLds& lds = shared.pieces;
+  const PagedArgs& a = x.a;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  const int l32 = lane % 32, hh = lane / 32;
+  const bool few = a.N <= 64;
+  LanePieces lanes;
+  const Pieces all = few ? count_in_lanes(a, uint32_t(x.groups), x.least, &lanes)
+                         : count_pieces(a, uint32_t(x.groups), x.least, lds);
+  // Neighbouring pieces to one XCD.
+  const uint32_t eighth = uint32_t(x.groups) / 8;
+  const uint32_t number = block < 8 * eighth ? block % 8 * eighth + block / 8 : block;
+  for (uint32_t piece = number; piece < all.count; piece += uint32_t(x.groups)) {
+    Sum before;
+    if (few && piece != number) __syncthreads();  // the piece before is done with the LDS
+    const Group grp = few ? find_in_lanes(lanes, piece, &before)
+                          : find_piece(a, piece, all.length, lds, &before);
+    const uint32_t ranges = (grp.steps - 1) / all.length + 1;
+    const uint32_t at = piece - before.pieces, hk = at / (ranges * grp.tiles);
+    const uint32_t in_head = at - hk * ranges * grp.tiles, range = in_head / grp.tiles;
+    const uint32_t tile = in_head - range * grp.tiles, t0 = range * all.length;
+    const uint32_t count = grp.steps - t0 < all.length ? grp.steps - t0 : all.length;
+    const uint32_t slots = before.more + (hk * grp.tiles + tile) * (ranges - 1);
+    const uint32_t rows = uint32_t(grp.rows) * uint32_t(a.G) - tile * kRows;
+    const int blocks = rows > 64 ? 4 : rows > 32 ? 2 : 1, parts = kWaves / blocks;
+    const int block_of = wave % blocks, part = wave / blocks;
+    const bool active = uint32_t(32 * block_of) < rows;  // uniform
+    const uint32_t place = uint32_t(32 * block_of + l32);
+    const uint32_t row = tile * kRows + (place < rows ? place : rows - 1);
+    const uint32_t in = x.by_g.div(row);
+    const int64_t request = grp.first + in;
+    const int64_t head = hk * a.G + (row - in * uint32_t(a.G));
+    const int32_t* table = a.table + int64_t(grp.first) * a.table_stride;
+    const float* kbase = static_cast<const float*>(a.k) + int64_t(hk) * a.kh + hh * (D / 2);
+    const float* vbase = static_cast<const float*>(a.v) + int64_t(hk) * a.vh + l32;
+
+    float m = -__builtin_inff(), l = 0.f;
+    f32x16_t o[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
+    if (active) {
+      const float* qp = static_cast<const float*>(a.q) + request * a.qn + head * a.qh + hh * (D / 2);
+      float4 q[NQ];
+#pragma unroll
+      for (int c = 0; c < NQ; ++c) q[c] = reinterpret_cast<const float4*>(qp)[c];
+      const uint32_t end = 2 * (t0 + count), from = 2 * t0 + uint32_t(part);
+      bool bad = false;
+      // The lane's key of 32-key tile t (the last one for those behind it): its page entry,
+      // read ahead, and its place there.
+      auto key_of = [&](uint32_t t) { return (t < end ? t : end - 1) * kStep + uint32_t(l32); };
+      auto entry = [&](uint32_t t) { return table[a.by_page.div(key_of(t))]; };
+      struct Key { int32_t id; uint32_t in; };
+      auto place_of = [&](uint32_t t, int32_t id) {
+        if (!is_page(id, a.num_pages)) {
+          bad = true;
+          id = 0;
+        }
+        const uint32_t key = key_of(t);
+        return Key{id, key - a.by_page.div(key) * uint32_t(a.page)};
+      };
+      float4 k[NQ];
+      auto load_k = [&](const Key& at) {
+        const float* p = kbase + at.id * a.kp + int64_t(at.in) * a.kn;
+#pragma unroll
+        for (int c = 0; c < NQ; ++c) k[c] = reinterpret_cast<const float4*>(p)[c];
+      };
+      Key now = place_of(from, entry(from));
+      load_k(now);
+      int32_t next_id = entry(from + parts);
+      for (uint32_t t = from; t < end; t += parts) {
+        // Row 8 (e / 4) + 4 hh + e % 4 of the tile: the key whose weight is the lane's e-th.
+        float v[16][NB];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int j = 8 * (e / 4) + 4 * hh + e % 4;
+          const int64_t id = __shfl(now.id, j);
+          const float* p = vbase + id * a.vp + int64_t(__shfl(now.in, j)) * a.vn;
+#pragma unroll
+          for (int i = 0; i < NB; ++i) v[e][i] = p[32 * i];
+        }
+        f32x16_t sc;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[e] = 0.f;
+#pragma unroll
+        for (int c = 0; c < NQ; ++c) {
+          sc = __builtin_amdgcn_mfma_f32_32x32x2f32(k[c].x, q[c].x, sc, 0, 0, 0);
+          sc = __builtin_amdgcn_mfma_f32_32x32x2f32(k[c].y, q[c].y, sc, 0, 0, 0);
+          sc = __builtin_amdgcn_mfma_f32_32x32x2f32(k[c].z, q[c].z, sc, 0, 0, 0);
+          sc = __builtin_amdgcn_mfma_f32_32x32x2f32(k[c].w, q[c].w, sc, 0, 0, 0);
+        }
+        now = place_of(t + parts, next_id);
+        load_k(now);
+        next_id = entry(t + 2 * parts);
+        float top = m;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          sc[e] *= a.scale_log2;
+          top = __builtin_fmaxf(top, sc[e]);
+        }
+        top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+        const float base = top == -__builtin_inff() ? 0.f : top;
+        if (__any(top != m)) {
+          const float alpha = __builtin_amdgcn_exp2f(m - base);
+          l *= alpha;
+#pragma unroll
+          for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
+          m = top;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float w = __builtin_amdgcn_exp2f(sc[e] - base);
+          l += w;
+#pragma unroll
+          for (int i = 0; i < NB; ++i)
+            o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[e][i], w, o[i], 0, 0, 0);
+        }
+      }
+      l += __shfl_xor(l, 32);
+      if (__any(bad)) l = __builtin_nanf("");
+    }
+    if (parts > 1) {  // the states of the same rows, in the order of the waves
+      if (part > 0) {
+        shared.ml[wave][lane] = make_float2(m, l);
+        float* to = shared.o[wave - blocks];
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) to[(16 * i + e) * 64 + lane] = o[i][e];
+      }
+      __syncthreads();
+      if (part > 0) continue;
+      for (int w = wave + blocks; w < kWaves; w += blocks) {
+        const float2 y = shared.ml[w][lane];
+        const float top = __builtin_fmaxf(m, y.x), base = top == -__builtin_inff() ? 0.f : top;
+        const float f = __builtin_amdgcn_exp2f(m - base), g = __builtin_amdgcn_exp2f(y.x - base);
+        const float* from = shared.o[w - blocks];
+        l = l * f + y.y * g;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            o[i][e] = o[i][e] * f + from[(16 * i + e) * 64 + lane] * g;
+        m = top;
+      }
+    }
+    const uint32_t slot = slots + range - 1;
+    if (active && place < rows && (range == 0 || slot < uint32_t(x.groups))) {
+      const int64_t q_row = request * a.Hk * a.G + head;
+      const int64_t to = range == 0 ? q_row : int64_t(slot) * x.stride + place;
+      float* out = (range == 0 ? x.first : x.more) + to * D;
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<float4*>(out + 32 * i + 8 * g + 4 * hh) =
+              make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
+      if (hh == 0) {
+        (range == 0 ? x.first_ml : x.more_ml)[to] = make_float2(m, l);
+        if (range == 0) x.record[q_row] = make_int4(int(ranges) - 1, int(slots), int(place), 0);
+      }
+    }
+  }
+}
+
 // The work-groups of the rows' own keys, which are the shorter ones, then those of the
 // prefixes, which take their places as they end.  us, 40 rows of 6 prompts / 64 rows of
 // 131072 keys: in this order 26.1 / 158, own keys behind 30.1 / 164, own keys in a launch
 // of their own 32.1 / 171.
 template <typename T, int D, bool kWhole>
-__global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void prefix_kernel(SharedArgs x) {
+__global__ __launch_bounds__(kThreads, kIsF32<T> ? 1 : D == 128 ? 2 : 3) void prefix_kernel(
+    SharedArgs x) {
   __shared__ union Lds {
     __device__ Lds() {}
-    PrefixLds<T, D, kWhole> prefix;
+    std::conditional_t<kIsF32<T>, PrefixLdsF32<D>, PrefixLds<T, D, kWhole>> prefix;
     TileLds<T, D, kFormSplit> own;
   } lds;
   const uint32_t own = uint32_t(x.a.groups);
   if (blockIdx.x < own)
     paged_tile<T, D, kWhole, kFormSplit, false, true>(x.a, lds.own, blockIdx.x);
+  else if constexpr (kIsF32<T>)
+    prefix_tile_f32<D>(x, lds.prefix, blockIdx.x - own);
   else
     prefix_tile<T, D, kWhole>(x, lds.prefix, blockIdx.x - own);
 }
@@ -859,17 +1047,28 @@ hipError_t launch_join(const SharedArgs& x, hipStream_t stream) {
                      dim3(kJoinThreads), 0, stream, x);
   return hipGetLastError();
 }
+template <typename T>
+hipError_t launch_both(const SharedArgs& x, hipStream_t stream) {
+  const bool wide = x.a.D == 128;
+  const hipError_t e = wide ? launch_prefix<T, 128>(x, stream) : launch_prefix<T, 64>(x, stream);
+  if (e != hipSuccess) return e;
+  return wide ? launch_join<T, 128>(x, stream) : launch_join<T, 64>(x, stream);
+}
 
-// Whether the prefix is computed once: 16-bit rows that the matrix-core form takes, a
-// scale that orders scores as the products are ordered, and enough to read if every row
-// did so for itself, to the tables' width, which the two launches here cost less than.
+// Whether the prefix is computed once: rows that the matrix-core form takes, a scale
+// that orders scores as the products are ordered, and enough to read if every row did so
+// for itself, to the tables' width, which the two launches here cost less than (counted
+// at two bytes a value; fp32 of D 128, whose waves are one to a SIMD, pays later).
 // us, every row for itself / shared, 28 query and 4 kv heads of 128 in bf16: 8 rows of
 // 4096 keys (68 MB) 17.6 / 24, of 8192 (135 MB) 28.8 / 25, 64 rows of 1024 keys (143 MB)
 // 23.6 / 33, of 2048 (277 MB) 37.8 / 34; 16 and 16 heads of 64: 8 rows of 2048 keys (69 MB)
-// 18.7 / 17.6, of 4096 25.0 / 17.6.
+// 18.7 / 17.6, of 4096 25.0 / 17.6.  In fp32, the first: 4 rows of 16384 keys (135 MB) 53 /
+// 62, 8 of 16384 (269) 91 / 69, 16 of 16384 (539) 165 / 98, 64 of 8192 (1082) 307 / 135; the
+// second: 4 rows of 4096 keys (68) 30 / 28, of 8192 (135) 49 / 33, 64 of 8192 (2164) 512 / 67.
 bool shares_prefix(int dtype, const PagedArgs& a) {
   const double bytes = 4.0 * double(a.N * a.Hk * a.D) * double(a.M * a.page);
-  return dtype != kF32 && a.N > 1 && bytes > double(128 << 20) && a.M * a.page >= kPrefixTile &&
+  const double least = (dtype == kF32 && a.D == 128 ? 2.0 : 1.0) * (128 << 20);
+  return a.N > 1 && bytes > least && a.M * a.page >= kPrefixTile &&
          a.scale_log2 >= 0.f && a.kn < (int64_t(1) << 26) && a.vn < (int64_t(1) << 26) &&
          paged_tile_form(dtype, a);
 }
@@ -913,7 +1112,7 @@ int64_t lay_out(PagedArgs& a, SharedArgs* x, char* work, int64_t own) {
 
 int64_t prefix_attn_workspace(int dtype, PagedArgs a) {
   const int64_t plain = paged_attn_workspace(dtype, a);
-  if (plain < 0 || dtype == kF32 || (a.D != 64 && a.D != 128)) return plain;
+  if (plain < 0 || (a.D != 64 && a.D != 128)) return plain;
   const int64_t own = paged_states_workspace(dtype, a);
   if (own < 0) return -1;
   const int64_t all = lay_out(a, nullptr, nullptr, own);
@@ -929,14 +1128,8 @@ hipError_t launch_prefix_attn(int dtype, PagedArgs a, void* workspace, hipStream
   a.split = reinterpret_cast<int2*>(work + own - round256(8 * a.N * a.per_request));
   SharedArgs x{};
   lay_out(a, &x, work, own);
-  const bool wide = a.D == 128, bf = dtype == kBF16;
-  const hipError_t e = bf ? (wide ? launch_prefix<bf16_t, 128>(x, stream)
-                            : launch_prefix<bf16_t, 64>(x, stream))
-                    : (wide ? launch_prefix<f16_t, 128>(x, stream)
-                            : launch_prefix<f16_t, 64>(x, stream));
-  if (e != hipSuccess) return e;
-  return bf ? (wide ? launch_join<bf16_t, 128>(x, stream) : launch_join<bf16_t, 64>(x, stream))
-            : (wide ? launch_join<f16_t, 128>(x, stream) : launch_join<f16_t, 64>(x, stream));
+  if (dtype == kF32) return launch_both<float>(x, stream);
+  return dtype == kBF16 ? launch_both<bf16_t>(x, stream) : launch_both<f16_t>(x, stream);
 }
 
 }  // namespace va

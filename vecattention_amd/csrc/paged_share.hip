@@ -9,8 +9,8 @@
 // the fork finds it.
 //
 // What bounds them are launches, and reads that wait for one another, not bytes: in us,
-// a fork of 512 rows of up to 2092 pages 36 in four launches (7.6 MB, 2 at a copy's rate),
-// a compaction of 256 rows 35 in five, prefixes of 256 rows of 8200 pages 9.3 in two.
+// a fork of 512 rows of up to 2092 pages 33 in four launches (7.6 MB, 2 at a copy's rate),
+// a compaction of 256 rows 34 in five, prefixes of 256 rows of 8200 pages 9.3 in two.
 // Each launch ends where all of a sum has to be there before its first use.
 #include "common.h"
 #include "lanes.h"
