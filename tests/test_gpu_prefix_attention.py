@@ -321,6 +321,15 @@ def test_offsets_past_32_bits():
     assert torch.equal(out, near)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("more", [0, 30])
+def test_fp32_tiles_of_every_height(D, more):
+    """8, 48 and 160 rows a kv head: one, two and four waves take turns at a tile's keys; `more`
+    rows that share nothing take the batch past the 64 that a wave counts by itself."""
+    check(make([(700, [3, 1]), (1030, [5] * 12), (390, [2] * 40)] + [(0, [20])] * more, 8, 2, D, 16,
+               "NHD", F32, 11))
+
+
 def test_streams_and_two_graphs():
     """Two captured graphs and eager calls on another stream, each with a workspace of its own."""
     note("graphs")
