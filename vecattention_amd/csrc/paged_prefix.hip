@@ -438,7 +438,7 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
       mneg = __builtin_inff();  // -(running maximum), less kBias
-      bool far = false;         // for some row, 2^16 or more
+      bool far = false;         // for some row, 2^16 or more in size
       lsum = 0.f;
       fill_ids(t0);
       At now{};
@@ -527,12 +527,13 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
               o[i][e] *= alpha;
           lsum *= alpha;
           mneg = to;
-          far = __any(mneg < -0x1p16f);
+          far = __any(__builtin_fabsf(mneg) > 0x1p16f && mneg != __builtin_inff());
         }
         const float bias = mneg == __builtin_inff() ? 0.f : mneg;  // no score yet: weights of 0
         // Scores are scaled and rounded as the maximum is where its steps are large: a fused
         // multiplication's exact product would lie tens of powers of two beside it from 2^27
-        // on.  Below 2^16 the two are within 2^-8 of each other.
+        // on, or -2^27 down: weights of 0, or beyond the type.  Below 2^16 the two are within
+        // 2^-8 of each other.
         vec bfrag[4];
         auto weights = [&](auto exponent) {
 #pragma unroll
