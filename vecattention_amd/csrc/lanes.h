@@ -108,6 +108,12 @@ __device__ inline float max3_plain(float a, float b, float c) {
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
+// min(a, b, c), likewise.
+__device__ inline float min3_plain(float a, float b, float c) {
+  float r;
+  asm("v_min3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
 __device__ inline float sum_halves(float x) {
   const uint32_t u = __builtin_bit_cast(uint32_t, x);
   const auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);

@@ -15,7 +15,8 @@
 // registers, rounded once to 16 bits (each weight by half a step at most, the same in the
 // sum of the values and in the weights' own sum, which puts an output off by about as
 // much as its own rounding; two parts a weight, as for the own keys, would double the
-// products).  Only whole 64-key tiles of a prefix are walked here, without masks; what is
+// products; fp16's small weights go in apart, by products of their own in the steps that
+// have any).  Only whole 64-key tiles of a prefix are walked here, without masks; what is
 // left of it comes with the row's own keys.
 //
 // us, bf16, D 128: 64 rows of 28 query and 4 kv heads that share 131072 keys: 152 for
@@ -264,8 +265,8 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
   constexpr uint32_t TB = PrefixLds<T, D, kWhole>::kTileBytes;
   constexpr int RPC = 1024 / kRowBytes, H = kTileKeys * kRowBytes / 1024 / kWaves;
   constexpr int NQK = D / 16, NB = D / 32, NPV = 4 * NB;
-  // fp16 holds weights down to 2^-24: those of 2^7 more are held, at most 2^15 of them.
-  constexpr float kBias = kIsF16<T> ? 7.f : 0.f;
+  // fp16's normal numbers begin at 2^-14: weights 2^7 times larger are held, 2^15 at most.
+  constexpr float kBias = kIsF16<T> ? 7.f : 0.f, kSmallest = -14.f;
   unsigned char* smem = shared.tiles;
   PiecesLds& lds = shared.pieces;
   auto& sbad = shared.bad;
@@ -498,7 +499,8 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
         if constexpr (kWhole) next = find(t + 2);  // here by the next barrier
         // The maximum's instructions are inline assembly, before which the compiler leaves no
         // wait for the matrix instructions: 11 wait states after the last one.
-        float tmax = 0.f;
+        constexpr bool kApart = kIsF16<T>;
+        float tmax = 0.f, tmin = 0.f;
         static_for<2>([&](auto half) {
           constexpr int hf = decltype(half)::value;
           if constexpr (hf == 1) asm volatile("s_nop 10" : "+v"(sc[1]));
@@ -509,6 +511,15 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
             u1 = max3_plain(u1, sc[hf][e + 2], sc[hf][e + 3]);
           }
           tmax = hf == 0 ? max_plain(u0, u1) : max3_plain(tmax, u0, u1);
+          if constexpr (kApart) {
+            float u2 = min3_plain(sc[hf][0], sc[hf][1], sc[hf][2]), u3 = sc[hf][3];
+#pragma unroll
+            for (int e = 4; e < 16; e += 4) {
+              u2 = min3_plain(u2, sc[hf][e], sc[hf][e + 1]);
+              u3 = min3_plain(u3, sc[hf][e + 2], sc[hf][e + 3]);
+            }
+            tmin = hf == 0 ? min3_plain(u2, u3, u3) : min3_plain(tmin, u2, u3);
+          }
         });
         // The maximum moves when a score's weight would exceed 2 to the slack.
         const float lead = tmax * a.scale_log2 + mneg;
@@ -534,8 +545,12 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
         // multiplication's exact product would lie tens of powers of two beside it from 2^27
         // on, or -2^27 down: weights of 0, or beyond the type.  Below 2^16 the two are within
         // 2^-8 of each other.
-        vec bfrag[4];
+        // fp16 weights below its normal numbers go in apart, 2^24 times larger, where a step has
+        // any: they keep their bits down to 2^-45 of the maximum's.
+        vec bfrag[4], blow[kApart ? 4 : 1];
+        bool small = false;
         auto weights = [&](auto exponent) {
+          if constexpr (kApart) small = __any(exponent(tmin) < kSmallest);
 #pragma unroll
           for (int f = 0; f < 4; ++f) {
             __builtin_amdgcn_sched_barrier(0);
@@ -544,6 +559,26 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
             for (int e = 0; e < 8; ++e)
               pr[e] = __builtin_amdgcn_exp2f(exponent(sc[f / 2][8 * (f % 2) + e]));
             bfrag[f] = M::pack(pr);
+          }
+          if constexpr (kApart) {
+            if (!small) return;
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+              __builtin_amdgcn_sched_barrier(0);
+              float pr[8], low[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                float s = sc[f / 2][8 * (f % 2) + e];
+                asm volatile("" : "+v"(s));  // computed again, not kept
+                const float x = exponent(s);
+                const float w = __builtin_amdgcn_exp2f(x);
+                pr[e] = x < kSmallest ? 0.f : w;
+                low[e] = x < kSmallest ? w * 0x1p24f : 0.f;
+              }
+              bfrag[f] = M::pack(pr);
+              blow[f] = M::pack(low);
+              asm volatile("" : "+v"(bfrag[f]), "+v"(blow[f]));  // packed here
+            }
           }
         };
         if (far)
@@ -554,6 +589,26 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
         uint32_t va = v0[0], vb1 = v0[1];
         asm volatile("" : "+v"(va), "+v"(vb1));
         const unsigned char* vb = smem + v_this;
+        if constexpr (kApart) {
+          if (small) {
+            auto scale = [&](float by) {
+#pragma unroll
+              for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[i][e] *= by;
+              lsum *= by;
+            };
+            scale(0x1p24f);
+#pragma unroll
+            for (int f = 0; f < NPV; ++f) {
+              __builtin_amdgcn_sched_barrier(0);
+              o[f % NB] = M::run(vread(vb, va, vb1, f), blow[f / NB], o[f % NB]);
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) lsum = M::add_pair(blow[j / 4], j % 4, lsum);
+            scale(0x1p-24f);
+          }
+        }
         constexpr int kVAhead = 2;
         vec vf[NPV];
 #pragma unroll
