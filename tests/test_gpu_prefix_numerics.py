@@ -1,5 +1,8 @@
-"""Attention of rows that share the beginnings of their pages where its arithmetic is at its ends,
-on an MI355X."""
+"""Attention of rows that share the beginnings of their pages where its arithmetic is at its ends:
+scores whose steps are large, weights far below the greatest one, infinities and NaN, in every type
+and with one, two and four waves at a tile's rows, on an MI355X."""
+import math
+
 import pytest
 import torch
 
@@ -87,3 +90,104 @@ def test_small_weights_beside_a_sink(groups, Hq, Hk, D, page, dtype):
                 off = (out[n].double().cpu() - want).abs()
                 assert bool((off <= ref.rounded(want, slack, dtype)).all()), (
                     at, gap, n, float((off / want.abs().clamp_min(1e-30)).max()))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("groups,Hq,Hk,D,page", SHAPES)
+def test_finite_outputs_beside_others(groups, Hq, Hk, D, page, dtype):
+    """An infinite value or a NaN among the shared values, or in a query, reaches the outputs that
+    the formula has it in; all others stay as they are, bit for bit."""
+    note("beside others", groups[0][0], Hq, Hk, D, page, dtype)
+    q, kc, vc, table, lens = make(groups, Hq, Hk, D, page, "NHD", dtype, D)
+    G, shared = Hq // Hk, groups[0][0] // page * page
+    clean, _ = run(q, kc, vc, table, lens)
+    assert bool(torch.isfinite(clean).all())
+    v = vc.clone()
+    row_of(v, table, 0, shared // 2, page)[0, 3] = math.inf
+    row_of(v, table, 0, 1, page)[0, 9] = -math.inf
+    row_of(v, table, 0, shared // 3, page)[Hk - 1, 5] = math.nan
+    want = clean.clone()
+    want[:, :G, 3], want[:, :G, 9] = math.inf, -math.inf
+    out, _ = run(q, kc, v, table, lens)
+    assert bool(torch.isnan(out[:, Hq - G:, 5]).all())
+    out[:, Hq - G:, 5] = want[:, Hq - G:, 5]
+    assert torch.equal(out, want)
+    q[1, 1, 7] = math.nan
+    out, _ = run(q, kc, vc, table, lens)
+    assert bool(torch.isnan(out[1, 1]).all())
+    out[1, 1] = clean[1, 1]
+    assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("page", [16, 24])
+def test_finite_outputs_beside_others_of_many_rows(page, dtype):
+    """The same of more rows than a wave counts by itself, in groups of one row to four."""
+    note("beside others, many rows", page, dtype)
+    groups = [(100 + 64 * (i % 5), [i % 7] * (1 + i % 4)) for i in range(90)]
+    q, kc, vc, table, lens = make(groups, 4, 2, 64, page, "NHD", dtype, 1)
+    clean, _ = run(q, kc, vc, table, lens)
+    want, n = clean.clone(), 0
+    for i, (_, own) in enumerate(groups):
+        if i % 3 == 0:
+            row_of(vc, table, n, 7, page)[1, 11] = -math.inf
+            want[n:n + len(own), 2:, 11] = -math.inf
+        n += len(own)
+    out, _ = run(q, kc, vc, table, lens)
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("groups,Hq,Hk,D,page", SHAPES)
+def test_infinite_values_of_tiny_weights(groups, Hq, Hk, D, page, dtype):
+    """An infinite value whose weight is too small for fp32, before and behind the key that makes
+    it so, is infinite all the same; beside a score of -infinity it is a NaN (0 times infinity)."""
+    note("tiny weights", groups[0][0], Hq, Hk, D, page, dtype)
+    q, kc, vc, table, lens = make(groups, Hq, Hk, D, page, "NHD", dtype, D)
+    shared = groups[0][0] // page * page
+    q[:] = 0
+    q[:, :, 0] = 1.0
+    kc[..., 0] = 0
+    row_of(kc, table, 0, shared // 2, page)[:, 0] = 560.0
+    row_of(vc, table, 0, 2, page)[0, 3] = math.inf
+    row_of(vc, table, 0, shared - 80, page)[0, 5] = -math.inf
+    row_of(vc, table, 0, shared // 3, page)[0, 7] = math.inf
+    row_of(kc, table, 0, shared // 3, page)[:, 0] = -math.inf
+    out, _ = run(q, kc, vc, table, lens, scale=1.0)
+    out = out[:, :Hq // Hk].double().cpu()
+    assert bool((out[:, :, 3] == math.inf).all()) and bool((out[:, :, 5] == -math.inf).all())
+    assert bool(torch.isnan(out[:, :, 7]).all())
+    great = row_of(vc, table, 0, shared // 2, page)[0].double()
+    others = [i for i in range(D) if i not in (3, 5, 7)]
+    # The great key's weight is 1, the others' below 2^-800.
+    assert bool((out[:, :, others] == great[others]).all())
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("D", [64, 128])
+def test_same_bits_in_graphs_and_outside(D, dtype):
+    """Eager calls, replays and calls on a side stream, of values with an infinity among them."""
+    from test_gpu_prefix_attention import widened
+    from vecattention_amd import paged_kv_prefix, paged_prefix_decode_attention
+    note("graph", D, dtype)
+    q, kc, vc, table, lens = make([(5000, [60, 7, 300, 1]), (640, [3] * 12)], 8, 2, D, 16, "NHD",
+                                  dtype, 3)
+    row_of(vc, table, 0, 77, 16)[0, 3] = math.inf
+    q, kc, vc, table, lens = (t.to(DEV) for t in (q, kc, vc, widened(table, kc), lens))
+    want = paged_prefix_decode_attention(q, kc, vc, table, lens, paged_kv_prefix(lens, table, 16))
+    assert int(torch.isinf(want).sum()) == 4 * 4 and not bool(torch.isnan(want).any())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        prefix = paged_kv_prefix(lens, table, 16)
+        out = paged_prefix_decode_attention(q, kc, vc, table, lens, prefix)
+    side = torch.cuda.Stream()
+    for _ in range(4):
+        out.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graph.replay()
+        eager = paged_prefix_decode_attention(q, kc, vc, table, lens,
+                                              paged_kv_prefix(lens, table, 16))
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(eager, want)

@@ -226,6 +226,68 @@ __device__ inline Group find_piece(const PagedArgs& a, uint32_t piece, uint32_t 
                uniform(g.tiles), uniform(g.steps)};
 }
 
+// The same by a wave alone.
+__device__ inline Group find_in_wave(const PagedArgs& a, uint32_t piece, uint32_t length,
+                                     const PiecesLds& lds, Sum* before) {
+  int32_t at = 0;
+  for (int32_t i = threadIdx.x % 64; i < kThreads; i += 64) {
+    const Sum b = lds.before[i];
+    const uint64_t here =
+        __ballot(piece >= b.pieces && piece - b.pieces < lds.mine[i].pieces);
+    if (here) at = i / 64 * 64 + __builtin_ctzll(here);
+  }
+  const int32_t lo = __builtin_amdgcn_readfirstlane(at) * run_of(a);
+  Group g = group_at(a, lo);
+  *before = lds.before[__builtin_amdgcn_readfirstlane(at)];
+  for (int32_t i = lo;;) {
+    const Sum n = pieces_of(a, g, length);
+    if (piece - before->pieces < n.pieces || ++i >= lo + run_of(a)) return g;
+    *before = Sum{plus(before->pieces, n.pieces), plus(before->more, n.more)};
+    g = group_at(a, i);
+  }
+}
+
+// One of them: a range of the 64-key tiles [t0, t0 + count) of a tile of rows.
+struct Piece {
+  uint32_t hk, tile, range, ranges, t0, count;
+  uint32_t slots;  // the first of the segment's further pieces
+  uint32_t rows;   // from this tile on
+};
+__device__ __forceinline__ Piece piece_at(const PagedArgs& a, const Group& grp, const Sum& before,
+                                          uint32_t piece, uint32_t length) {
+  Piece p;
+  p.ranges = (grp.steps - 1) / length + 1;
+  const uint32_t at = piece - before.pieces;
+  p.hk = at / (p.ranges * grp.tiles);
+  const uint32_t in_head = at - p.hk * p.ranges * grp.tiles;
+  p.range = in_head / grp.tiles;
+  p.tile = in_head - p.range * grp.tiles;
+  p.t0 = p.range * length;
+  p.count = grp.steps - p.t0 < length ? grp.steps - p.t0 : length;
+  p.slots = before.more + (p.hk * grp.tiles + p.tile) * (p.ranges - 1);
+  p.rows = uint32_t(grp.rows) * uint32_t(a.G) - p.tile * kRows;
+  return p;
+}
+// The row of place `place` of the tile (those behind the last are the last): request and head.
+struct RowOf {
+  int64_t request, head;
+};
+__device__ __forceinline__ RowOf row_of(const SharedArgs& x, const Group& grp, const Piece& p,
+                                        uint32_t place) {
+  const uint32_t row = p.tile * kRows + (place < p.rows ? place : p.rows - 1);
+  const uint32_t in = x.by_g.div(row);
+  return RowOf{grp.first + int64_t(in), p.hk * x.a.G + int64_t(row - in * uint32_t(x.a.G))};
+}
+// Where the state of a row over a piece lies: the row's own place for its first piece, the
+// place in a slot for the others; -1 for neither.
+__device__ __forceinline__ int64_t state_at(const SharedArgs& x, const Piece& p, uint32_t place,
+                                            const RowOf& row) {
+  if (place >= p.rows) return -1;
+  if (p.range == 0) return row.request * x.a.Hk * x.a.G + row.head;
+  const uint32_t slot = p.slots + p.range - 1;
+  return slot < uint32_t(x.groups) ? int64_t(slot) * x.stride + place : -1;
+}
+
 // 16 bytes a lane from `base` (uniform) + `offset` into LDS from base + kOffset on, as
 // copy16_row_to_lds_at.
 template <uint32_t kOffset>
@@ -246,6 +308,114 @@ __device__ inline void copy16_from(uint32_t lds_base, uint64_t address) {
 
 template <typename T> constexpr bool kIsF16 = std::is_same_v<T, f16_t>;
 template <typename T> constexpr bool kIsF32 = std::is_same_v<T, float>;
+
+// Leaves the state of a row over a piece: o[i][e], feature 32 i + 8 (e / 4) + 4 hh + e % 4.
+// Whether one of its sums is a NaN that the sum of the weights is none of.
+template <int D, int NB>
+__device__ __forceinline__ bool leave_state(const SharedArgs& x, const Piece& p, bool active,
+                                            uint32_t place, const RowOf& row, float m, float l,
+                                            const f32x16_t (&o)[NB]) {
+  const int hh = threadIdx.x % 64 / 32;
+  const int64_t to = active ? state_at(x, p, place, row) : -1;
+  if (to < 0) return false;
+  float* out = (p.range == 0 ? x.first : x.more) + to * D;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float4 y = make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
+      *reinterpret_cast<float4*>(out + 32 * i + 8 * g + 4 * hh) = y;
+      sum += (y.x + y.y) + (y.z + y.w);
+    }
+  if (hh == 0) {
+    (p.range == 0 ? x.first_ml : x.more_ml)[to] = make_float2(m, l);
+    if (p.range == 0)
+      x.record[row.request * x.a.Hk * x.a.G + row.head] =
+          make_int4(int(p.ranges) - 1, int(p.slots), int(place), 0);
+  }
+  return sum != sum && l == l;
+}
+
+// Values that are not finite meet weights of 0 (or too small for their type) and make NaN
+// of a row's sum; with any weight, however small, they would make it what they are, whatever
+// the others are, and with none (a score of -infinity) NaN.  So the sums that are NaN, and no
+// others, are made anew from those values alone: behind the work-group's pieces, once more
+// through them, so that the walk over the keys has the registers.  A wave for 32 rows of a
+// piece looks the values of its keys through, 1 KB a load, and takes those with such a value
+// one by one.  us, 64 rows of 28 and 4 heads of 128, 131072 keys, one value a NaN: 560 (183
+// without; 22900 where each row and query head went through its keys in the merge).
+template <typename T, int D>
+__device__ __forceinline__ void repair_piece(const SharedArgs& x, const Group& grp,
+                                             const Piece& p) {
+  constexpr int kPart = 16 / int(sizeof(T)), kLanes = D / kPart, kKeys = 64 / kLanes, U = 4;
+  const PagedArgs& a = x.a;
+  int thread = threadIdx.x;
+  asm volatile("" : "+v"(thread));  // what follows from it is formed here, not kept
+  const int lane = thread % 64, hh = lane / 32;
+  const uint32_t place = thread / 64 * 32 + lane % 32;
+  const RowOf mine = row_of(x, grp, p, place);
+  const int64_t at = state_at(x, p, place, mine);
+  float* sums = (p.range == 0 ? x.first : x.more) + at * D;
+  const T* q = static_cast<const T*>(a.q) + mine.request * a.qn + mine.head * a.qh;
+  const T* kbase = static_cast<const T*>(a.k) + p.hk * a.kh;
+  const T* vbase = static_cast<const T*>(a.v) + p.hk * a.vh;
+  const int32_t* table = a.table + grp.first * a.table_stride;
+  auto finite = [](float v) { return __builtin_fabsf(v) < __builtin_inff(); };
+  auto key_row = [&](uint32_t key, const T* base, int64_t sp, int64_t sn) {
+    const uint32_t page = a.by_page.div(key);
+    const int32_t id = table[page];
+    return base + (is_page(id, a.num_pages) ? id : 0) * sp +
+           int64_t(key - page * uint32_t(a.page)) * sn;
+  };
+  // Bit 4 (f / 8) + f % 4 of `nan`: feature f of the lane's half (f % 8 / 4 == hh).
+  uint64_t nan = 0;
+  if (at >= 0) {
+    const float l = (p.range == 0 ? x.first_ml : x.more_ml)[at].y;
+#pragma unroll 1
+    for (int i = 0; i < D / 2 && l == l; ++i) {
+      float& sum = sums[8 * (i / 4) + 4 * hh + i % 4];
+      if (sum == sum) continue;
+      nan |= uint64_t(1) << i;
+      sum = 0.f;
+    }
+  }
+  if (!__any(nan != 0)) return;
+  struct alignas(16) Part { T x[kPart]; };
+  const uint32_t end = (p.t0 + p.count) * kPrefixTile;
+  for (uint32_t k0 = p.t0 * kPrefixTile; k0 < end; k0 += U * kKeys) {
+    Part v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t key = k0 + u * kKeys + lane / kLanes;
+      v[u] = reinterpret_cast<const Part*>(
+          key_row(key < end ? key : end - 1, vbase, a.vp, a.vn))[lane % kLanes];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      bool odd = false;
+#pragma unroll
+      for (int e = 0; e < kPart; ++e) odd |= !finite(to_f32(v[u].x[e]));
+      uint64_t found = __ballot(odd && k0 + u * kKeys + lane / kLanes < end);
+      while (found) {
+        const int in = __builtin_ctzll(found) / kLanes;  // of the load's keys
+        found &= ~(((uint64_t(1) << kLanes) - 1) << (in * kLanes));
+        const uint32_t key = k0 + u * kKeys + in;
+        const T *k = key_row(key, kbase, a.kp, a.kn), *value = key_row(key, vbase, a.vp, a.vn);
+        float s = 0.f;
+#pragma unroll 4
+        for (int d = hh * (D / 2); d < (hh + 1) * (D / 2); ++d) s += to_f32(q[d]) * to_f32(k[d]);
+        const bool none = sum_halves(s) * a.scale_log2 == -__builtin_inff();
+#pragma unroll 1
+        for (int i = 0; i < D / 2; ++i) {
+          const int f = 8 * (i / 4) + 4 * hh + i % 4;
+          const float y = to_f32(value[f]);
+          if (!finite(y) && (nan >> i & 1)) sums[f] += none ? __builtin_nanf("") : y;
+        }
+      }
+    }
+  }
+}
 
 // kWhole: pages of a multiple of 16 tokens, so that the 16 keys that a wave copies of
 // a tile lie in one.
@@ -308,29 +478,19 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
     }
   }
 
+  bool nan = false;
   for (uint32_t piece = number; piece < all.count; piece += uint32_t(x.groups)) {
     Sum before;
     if (few && piece != number) __syncthreads();  // the piece before is done with its flags
     const Group grp = few ? find_in_lanes(lanes, piece, &before)
                           : find_piece(a, piece, all.length, lds, &before);
-    const uint32_t ranges = (grp.steps - 1) / all.length + 1;
-    const uint32_t at = piece - before.pieces, hk = at / (ranges * grp.tiles);
-    const uint32_t in_head = at - hk * ranges * grp.tiles, range = in_head / grp.tiles;
-    const uint32_t tile = in_head - range * grp.tiles, t0 = range * all.length;
-    const uint32_t count = grp.steps - t0 < all.length ? grp.steps - t0 : all.length;
-    // The slots of the segment's further pieces.
-    const uint32_t slots = before.more + (hk * grp.tiles + tile) * (ranges - 1);
-    const uint32_t rows = uint32_t(grp.rows) * uint32_t(a.G) - tile * kRows;  // from this tile on
+    const Piece pc = piece_at(a, grp, before, piece, all.length);
+    const uint32_t hk = pc.hk, t0 = pc.t0, count = pc.count, rows = pc.rows;
     const bool active = uint32_t(32 * wave) < rows;  // uniform
-    // The lane's row: request first + row / G, head row % G of the kv head.
-    auto place_of = [&](uint32_t& place, int64_t& request, int64_t& head) {
+    auto place_of = [&]() {  // of the lane
       uint32_t l = uint32_t(l32);
       asm volatile("" : "+v"(l));  // formed where it is used
-      place = uint32_t(32 * wave) + l;
-      const uint32_t row = tile * kRows + (place < rows ? place : rows - 1);
-      const uint32_t in = x.by_g.div(row);
-      request = grp.first + in;
-      head = hk * a.G + (row - in * uint32_t(a.G));
+      return uint32_t(32 * wave) + l;
     };
     const int32_t* table = a.table + int64_t(grp.first) * a.table_stride;
     const T* kbase = static_cast<const T*>(a.k) + int64_t(hk) * a.kh;
@@ -339,10 +499,8 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
 
     vec qreg[NQK];
     {
-      uint32_t place;
-      int64_t request, head;
-      place_of(place, request, head);
-      const T* qp = static_cast<const T*>(a.q) + request * a.qn + head * a.qh;
+      const RowOf row = row_of(x, grp, pc, place_of());
+      const T* qp = static_cast<const T*>(a.q) + row.request * a.qn + row.head * a.qh;
 #pragma unroll
       for (int s = 0; s < NQK; ++s)
         qreg[s] = __builtin_bit_cast(vec, *reinterpret_cast<const uint4*>(qp + 16 * s + 8 * hh));
@@ -564,20 +722,18 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
             if (!small) return;
 #pragma unroll
             for (int f = 0; f < 4; ++f) {
-              __builtin_amdgcn_sched_barrier(0);
-              float pr[8], low[8];
+              float high[8], low[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
                 float s = sc[f / 2][8 * (f % 2) + e];
                 asm volatile("" : "+v"(s));  // computed again, not kept
-                const float x = exponent(s);
-                const float w = __builtin_amdgcn_exp2f(x);
-                pr[e] = x < kSmallest ? 0.f : w;
+                const float x = exponent(s), w = __builtin_amdgcn_exp2f(x);
+                high[e] = x < kSmallest ? 0.f : w;
                 low[e] = x < kSmallest ? w * 0x1p24f : 0.f;
               }
-              bfrag[f] = M::pack(pr);
+              bfrag[f] = M::pack(high);
               blow[f] = M::pack(low);
-              asm volatile("" : "+v"(bfrag[f]), "+v"(blow[f]));  // packed here
+              asm volatile("" : "+v"(bfrag[f]), "+v"(blow[f]));  // rounded here, not later
             }
           }
         };
@@ -649,25 +805,16 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
     lds_barrier();
     float l = sum_halves(lsum);
     if (sbad[0] | sbad[1] | sbad[2] | sbad[3]) l = __builtin_nanf("");
-    uint32_t place;
-    int64_t request, head;
-    place_of(place, request, head);
-    const uint32_t slot = slots + range - 1;
-    if (active && place < rows && (range == 0 || slot < uint32_t(x.groups))) {
-      const int64_t q_row = request * a.Hk * a.G + head;
-      const int64_t to = range == 0 ? q_row : int64_t(slot) * x.stride + place;
-      float* out = (range == 0 ? x.first : x.more) + to * D;
-#pragma unroll
-      for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<float4*>(out + 32 * i + 8 * g + 4 * hh) =
-              make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
-      if (hh == 0) {
-        (range == 0 ? x.first_ml : x.more_ml)[to] = make_float2(-mneg, l);
-        if (range == 0) x.record[q_row] = make_int4(int(ranges) - 1, int(slots), int(place), 0);
-      }
-    }
+    const uint32_t place = place_of();
+    nan |= leave_state<D>(x, pc, active, place, row_of(x, grp, pc, place), -mneg, l, o);
+  }
+  if (!__any(nan)) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");  // what other lanes have left is read
+  for (uint32_t piece = number; piece < all.count; piece += uint32_t(x.groups)) {
+    Sum before;
+    const Group grp = few ? find_in_lanes(lanes, piece, &before)
+                          : find_in_wave(a, piece, all.length, lds, &before);
+    repair_piece<T, D>(x, grp, piece_at(a, grp, before, piece, all.length));
   }
 }
 
@@ -699,26 +846,22 @@ __device__ __forceinline__ void prefix_tile_f32(const SharedArgs& x, PrefixLdsF3
   // Neighbouring pieces to one XCD.
   const uint32_t eighth = uint32_t(x.groups) / 8;
   const uint32_t number = block < 8 * eighth ? block % 8 * eighth + block / 8 : block;
+  bool nan = false;
   for (uint32_t piece = number; piece < all.count; piece += uint32_t(x.groups)) {
     Sum before;
     if (few && piece != number) __syncthreads();  // the piece before is done with the LDS
     const Group grp = few ? find_in_lanes(lanes, piece, &before)
                           : find_piece(a, piece, all.length, lds, &before);
-    const uint32_t ranges = (grp.steps - 1) / all.length + 1;
-    const uint32_t at = piece - before.pieces, hk = at / (ranges * grp.tiles);
-    const uint32_t in_head = at - hk * ranges * grp.tiles, range = in_head / grp.tiles;
-    const uint32_t tile = in_head - range * grp.tiles, t0 = range * all.length;
-    const uint32_t count = grp.steps - t0 < all.length ? grp.steps - t0 : all.length;
-    const uint32_t slots = before.more + (hk * grp.tiles + tile) * (ranges - 1);
-    const uint32_t rows = uint32_t(grp.rows) * uint32_t(a.G) - tile * kRows;
+    const Piece pc = piece_at(a, grp, before, piece, all.length);
+    const uint32_t hk = pc.hk, t0 = pc.t0, count = pc.count, rows = pc.rows;
     const int blocks = rows > 64 ? 4 : rows > 32 ? 2 : 1, parts = kWaves / blocks;
     const int block_of = wave % blocks, part = wave / blocks;
     const bool active = uint32_t(32 * block_of) < rows;  // uniform
-    const uint32_t place = uint32_t(32 * block_of + l32);
-    const uint32_t row = tile * kRows + (place < rows ? place : rows - 1);
-    const uint32_t in = x.by_g.div(row);
-    const int64_t request = grp.first + in;
-    const int64_t head = hk * a.G + (row - in * uint32_t(a.G));
+    auto place_of = [&]() {  // of the lane
+      uint32_t l = uint32_t(l32);
+      asm volatile("" : "+v"(l));  // formed where it is used
+      return uint32_t(32 * block_of) + l;
+    };
     const int32_t* table = a.table + int64_t(grp.first) * a.table_stride;
     const float* kbase = static_cast<const float*>(a.k) + int64_t(hk) * a.kh + hh * (D / 2);
     const float* vbase = static_cast<const float*>(a.v) + int64_t(hk) * a.vh + l32;
@@ -730,7 +873,9 @@ __device__ __forceinline__ void prefix_tile_f32(const SharedArgs& x, PrefixLdsF3
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
     if (active) {
-      const float* qp = static_cast<const float*>(a.q) + request * a.qn + head * a.qh + hh * (D / 2);
+      const RowOf row = row_of(x, grp, pc, place_of());
+      const float* qp =
+          static_cast<const float*>(a.q) + row.request * a.qn + row.head * a.qh + hh * (D / 2);
       float4 q[NQ];
 #pragma unroll
       for (int c = 0; c < NQ; ++c) q[c] = reinterpret_cast<const float4*>(qp)[c];
@@ -741,7 +886,7 @@ __device__ __forceinline__ void prefix_tile_f32(const SharedArgs& x, PrefixLdsF3
       auto key_of = [&](uint32_t t) { return (t < end ? t : end - 1) * kStep + uint32_t(l32); };
       auto entry = [&](uint32_t t) { return table[a.by_page.div(key_of(t))]; };
       struct Key { int32_t id; uint32_t in; };
-      auto place_of = [&](uint32_t t, int32_t id) {
+      auto key_at = [&](uint32_t t, int32_t id) {
         if (!is_page(id, a.num_pages)) {
           bad = true;
           id = 0;
@@ -755,7 +900,7 @@ __device__ __forceinline__ void prefix_tile_f32(const SharedArgs& x, PrefixLdsF3
 #pragma unroll
         for (int c = 0; c < NQ; ++c) k[c] = reinterpret_cast<const float4*>(p)[c];
       };
-      Key now = place_of(from, entry(from));
+      Key now = key_at(from, entry(from));
       load_k(now);
       int32_t next_id = entry(from + parts);
       for (uint32_t t = from; t < end; t += parts) {
@@ -779,7 +924,7 @@ __device__ __forceinline__ void prefix_tile_f32(const SharedArgs& x, PrefixLdsF3
           sc = __builtin_amdgcn_mfma_f32_32x32x2f32(k[c].z, q[c].z, sc, 0, 0, 0);
           sc = __builtin_amdgcn_mfma_f32_32x32x2f32(k[c].w, q[c].w, sc, 0, 0, 0);
         }
-        now = place_of(t + parts, next_id);
+        now = key_at(t + parts, next_id);
         load_k(now);
         next_id = entry(t + 2 * parts);
         float top = m;
@@ -836,22 +981,16 @@ __device__ __forceinline__ void prefix_tile_f32(const SharedArgs& x, PrefixLdsF3
         m = top;
       }
     }
-    const uint32_t slot = slots + range - 1;
-    if (active && place < rows && (range == 0 || slot < uint32_t(x.groups))) {
-      const int64_t q_row = request * a.Hk * a.G + head;
-      const int64_t to = range == 0 ? q_row : int64_t(slot) * x.stride + place;
-      float* out = (range == 0 ? x.first : x.more) + to * D;
-#pragma unroll
-      for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<float4*>(out + 32 * i + 8 * g + 4 * hh) =
-              make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
-      if (hh == 0) {
-        (range == 0 ? x.first_ml : x.more_ml)[to] = make_float2(m, l);
-        if (range == 0) x.record[q_row] = make_int4(int(ranges) - 1, int(slots), int(place), 0);
-      }
-    }
+    const uint32_t place = place_of();
+    nan |= leave_state<D>(x, pc, active, place, row_of(x, grp, pc, place), m, l, o);
+  }
+  if (!__any(nan)) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");  // what other lanes have left is read
+  for (uint32_t piece = number; piece < all.count; piece += uint32_t(x.groups)) {
+    Sum before;
+    const Group grp = few ? find_in_lanes(lanes, piece, &before)
+                          : find_in_wave(a, piece, all.length, lds, &before);
+    repair_piece<float, D>(x, grp, piece_at(a, grp, before, piece, all.length));
   }
 }
 
@@ -876,59 +1015,6 @@ __global__ __launch_bounds__(kThreads, kIsF32<T> ? 1 : D == 128 ? 2 : 3) void pr
     prefix_tile<T, D, kWhole>(x, lds.prefix, blockIdx.x - own);
 }
 
-// One row's state over its first `keys` keys in fp32, a wave a key: for rows whose
-// values are not finite, which the matrix products' rounded weights (0 for a key far
-// below the others) would make NaN of.  To sm, sl and so of each wave.
-template <typename T, int D, int kW>
-__device__ void row_state(const PagedArgs& a, int64_t n, uint32_t head, uint32_t hk, int32_t keys,
-                          float (&sm)[kW], float (&sl)[kW], float (*so)[D]) {
-  constexpr int NF = D / 64, U = 4;
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const T* qp = static_cast<const T*>(a.q) + n * a.qn + int64_t(head) * a.qh;
-  const int32_t* table = a.table + n * a.table_stride;
-  float q[NF], acc[NF], m = -__builtin_inff(), l = 0.f;
-#pragma unroll
-  for (int j = 0; j < NF; ++j) q[j] = to_f32(qp[lane + 64 * j]), acc[j] = 0.f;
-  for (int32_t k0 = U * wave; k0 < keys; k0 += U * kW) {
-    float kf[U][NF], vf[U][NF];
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const uint32_t key = uint32_t(k0 + i), p = a.by_page.div(key);  // keys: whole tiles
-      int64_t id = table[p];
-      if (!is_page(int32_t(id), a.num_pages)) id = 0, bad = true;
-      const uint32_t in = key - p * uint32_t(a.page);
-      const T* kr = static_cast<const T*>(a.k) + id * a.kp + in * a.kn + int64_t(hk) * a.kh;
-      const T* vr = static_cast<const T*>(a.v) + id * a.vp + in * a.vn + int64_t(hk) * a.vh;
-#pragma unroll
-      for (int j = 0; j < NF; ++j) {
-        kf[i][j] = to_f32(kr[lane + 64 * j]);
-        vf[i][j] = to_f32(vr[lane + 64 * j]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      float s = 0.f;
-#pragma unroll
-      for (int j = 0; j < NF; ++j) s += q[j] * kf[i][j];
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
-      s = bad ? __builtin_nanf("") : s * a.scale_log2;
-      const float top = __builtin_fmaxf(m, s), ms = top == -__builtin_inff() ? 0.f : top;
-      const float f = __builtin_amdgcn_exp2f(m - ms), w = __builtin_amdgcn_exp2f(s - ms);
-      l = l * f + w;
-#pragma unroll
-      for (int j = 0; j < NF; ++j)
-        acc[j] = weighed(f, acc[j]) +
-                 (s != -__builtin_inff() ? weighed(w, vf[i][j]) : w * vf[i][j]);
-      m = top;
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < NF; ++j) so[wave][lane + 64 * j] = acc[j];
-  if (lane == 0) sm[wave] = m, sl[wave] = l;
-}
-
 // Joins the states of a (request, query head): those of the prefix's shares, then
 // those of its own keys, always in this order.
 constexpr int kJoinThreads = 128;
@@ -936,11 +1022,11 @@ template <typename T, int D>
 __global__ __launch_bounds__(kJoinThreads) void prefix_merge_kernel(SharedArgs x) {
   constexpr int kW = kJoinThreads / 64;
   constexpr int kLanes = D / 4, kSide = kJoinThreads / kLanes, U = 8;
-  constexpr int kMost = 2 * 512 + 2 + kW;
+  constexpr int kMost = 2 * 512 + 2;
   typedef float vec4 __attribute__((ext_vector_type(4)));
   __shared__ float weight[kMost];
   __shared__ vec4 sacc[kJoinThreads];
-  __shared__ float top[kW], den[kW], sm[kW], sl[kW];
+  __shared__ float top[kW], den[kW];
   const PagedArgs& a = x.a;
   const int64_t row = blockIdx.x;
   const uint32_t Hq = uint32_t(a.Hk * a.G), n = uint32_t(row) / Hq, head = uint32_t(row) - n * Hq;
@@ -970,16 +1056,13 @@ __global__ __launch_bounds__(kJoinThreads) void prefix_merge_kernel(SharedArgs x
   const int own_from = split.x < 0 ? 0 : split.x / 2;
   const int own = 1 + (split.x < 0 ? 0 : split.y - own_from);
   const int64_t slots = 2 * int64_t(a.groups);
-  // Part i: `own` of them from i = 0 on, those of the prefix behind; with `exact` these are
-  // the waves' states of row_state, in place of weights not used yet.
-  bool exact = false;
-  auto so = [&]() { return reinterpret_cast<float(*)[D]>(&sacc[0]); };
+  // Part i: `own` of them from i = 0 on, those of the prefix behind.
+  const int parts = own + pre;
   auto ml = [&](int i) {
     if (i < own)
       return i == 0 ? a.state_ml[row]
                     : reinterpret_cast<const float2*>(a.part)[2 * (own_from + i) * a.rows + r];
     i -= own;
-    if (exact) return make_float2(sm[i], sl[i]);
     return i == 0 ? x.first_ml[row] : x.more_ml[int64_t(pre_from + i - 1) * x.stride + place];
   };
   auto state = [&](int i) {
@@ -993,86 +1076,58 @@ __global__ __launch_bounds__(kJoinThreads) void prefix_merge_kernel(SharedArgs x
     }
     return reinterpret_cast<const vec4*>(p)[c];
   };
-  float l;
-  auto weights = [&](int parts) {
-    float m = -__builtin_inff();
-    for (int i = me; i < parts; i += kJoinThreads) {
-      const float2 y = ml(i);
-      if (!(y.y == 0.f)) m = __builtin_fmaxf(m, y.x);
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) m = __builtin_fmaxf(m, __shfl_xor(m, d));
-    if (me % 64 == 0) top[me / 64] = m;
-    lds_barrier();
-#pragma unroll
-    for (int w = 0; w < kW; ++w) m = __builtin_fmaxf(m, top[w]);
-    l = 0.f;
-    for (int i = me; i < parts; i += kJoinThreads) {
-      const float2 y = ml(i);
-      const float f = __builtin_amdgcn_exp2f(y.x - m);
-      weight[i] = y.y == 0.f ? -1.f : f;  // -1: no weight at all
-      l += y.y == 0.f ? 0.f : f * y.y;
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
-    if (me % 64 == 0) den[me / 64] = l;
-    lds_barrier();
-    l = 0.f;
-#pragma unroll
-    for (int w = 0; w < kW; ++w) l += den[w];
-  };
-  auto add = [&](vec4& acc, float f, vec4 y) {
-    if (f > 0.f) acc += f * y;
-    if (f == 0.f || f != f)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] += f != f ? f : weighed(f, y[e]);
-  };
   vec4 y[U];
-  auto load = [&](int from, int parts) {
+  auto load = [&](int from) {
 #pragma unroll
     for (int i = 0; i < U; ++i)
       y[i] = state(from + i * kSide < parts ? from + i * kSide : parts - 1);
   };
-  auto gather = [&](int parts) {  // the first ones are loaded
-    vec4 acc = vec4(0.f);
-    for (int from = side; from < parts; from += U * kSide) {
-      vec4 z[U];
-#pragma unroll
-      for (int i = 0; i < U; ++i) z[i] = y[i];
-      if (from + U * kSide < parts) load(from + U * kSide, parts);
-#pragma unroll
-      for (int i = 0; i < U; ++i)
-        add(acc, from + i * kSide < parts ? weight[from + i * kSide] : -1.f, z[i]);
-    }
-    sacc[me] = acc;
-    lds_barrier();
-    acc = sacc[c];
-#pragma unroll
-    for (int i = 1; i < kSide; ++i) acc += sacc[i * kLanes + c];
-    return acc;
-  };
-  load(side, own + pre);
-  weights(own + pre);
-  vec4 acc = gather(own + pre);
-  bool nan = false;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) nan |= acc[e] != acc[e];
-  if (pre > 0 && l == l && __syncthreads_or(nan)) {
-    // (The row's own table lists the same pages.)
-    row_state<T, D, kW>(a, n, head, hk, shared, sm, sl, so());
-    exact = true;
-    __syncthreads();
-    vec4 rest[kW];
-#pragma unroll
-    for (int w = 0; w < kW; ++w) rest[w] = *reinterpret_cast<const vec4*>(&so()[w][4 * c]);
-    __syncthreads();
-    load(side, own);
-    weights(own + kW);
-    acc = gather(own);
-#pragma unroll
-    for (int w = 0; w < kW; ++w) add(acc, weight[own + w], rest[w]);
+  load(side);
+  float m = -__builtin_inff();
+  for (int i = me; i < parts; i += kJoinThreads) {
+    const float2 s = ml(i);
+    if (!(s.y == 0.f)) m = __builtin_fmaxf(m, s.x);
   }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) m = __builtin_fmaxf(m, __shfl_xor(m, d));
+  if (me % 64 == 0) top[me / 64] = m;
+  lds_barrier();
+#pragma unroll
+  for (int w = 0; w < kW; ++w) m = __builtin_fmaxf(m, top[w]);
+  float l = 0.f;
+  for (int i = me; i < parts; i += kJoinThreads) {
+    const float2 s = ml(i);
+    const float f = __builtin_amdgcn_exp2f(s.x - m);
+    weight[i] = s.y == 0.f ? -1.f : f;  // -1: no weight at all
+    l += s.y == 0.f ? 0.f : f * s.y;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
+  if (me % 64 == 0) den[me / 64] = l;
+  lds_barrier();
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kW; ++w) l += den[w];
+  vec4 acc = vec4(0.f);
+  for (int from = side; from < parts; from += U * kSide) {
+    vec4 z[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) z[i] = y[i];
+    if (from + U * kSide < parts) load(from + U * kSide);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const float f = from + i * kSide < parts ? weight[from + i * kSide] : -1.f;
+      if (f > 0.f) acc += f * z[i];
+      if (f == 0.f || f != f)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += f != f ? f : weighed(f, z[i][e]);
+    }
+  }
+  sacc[me] = acc;
+  lds_barrier();
   if (side != 0) return;
+#pragma unroll
+  for (int i = 1; i < kSide; ++i) acc += sacc[i * kLanes + c];
   struct alignas(sizeof(T) * 4) Out { T v[4]; } z;
 #pragma unroll
   for (int e = 0; e < 4; ++e) z.v[e] = Round<T>::store(acc[e] / l);
