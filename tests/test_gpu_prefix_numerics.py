@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import paged_reference as ref
-from test_gpu_prefix_attention import make, note, run
+from test_gpu_prefix_attention import check, make, note, room, run
 
 pytestmark = pytest.mark.gpu
 
@@ -161,6 +161,54 @@ def test_infinite_values_of_tiny_weights(groups, Hq, Hk, D, page, dtype):
     others = [i for i in range(D) if i not in (3, 5, 7)]
     # The great key's weight is 1, the others' below 2^-800.
     assert bool((out[:, :, others] == great[others]).all())
+
+
+@pytest.mark.parametrize("groups,Hq,Hk,D,page", SHAPES)
+def test_keys_that_are_not_finite_in_fp32(groups, Hq, Hk, D, page):
+    for value in (math.inf, math.nan):
+        note("keys", groups[0][0], Hq, Hk, D, page, value)
+        q, kc, vc, table, lens = make(groups + [(320, [4, 4])], Hq, Hk, D, page, "NHD", F32)
+        rows, G = len(groups[0][1]), Hq // Hk
+        q[:, :, 5] = q[:, :, 5].abs() + 1
+        kc[int(table[0, 3]), 2, Hk - 1, 5] = value
+        out, _ = run(q, kc, vc, table, lens)
+        assert bool(torch.isnan(out[:rows, Hq - G:]).all())
+        want, slack = room(q, torch.where(torch.isfinite(kc), kc, 0), vc, table, lens, "NHD")
+        fine = (out.double().cpu() - want).abs() <= ref.rounded(want, slack, F32)
+        assert bool(fine[rows:].all()) and bool(fine[:rows, :Hq - G].all())
+        # Scores of -infinity: a weight of 0, and rows of such keys alone 0 / 0.
+        q, kc, vc, table, lens = make([(groups[0][0], groups[0][1]), (320, [0, 0])], Hq, Hk, D, page,
+                                      "NHD", F32)
+        q[:, :, 5] = 1
+        kc[int(table[0, 3]), 2, :, 5] = -math.inf
+        whole = 320 // page * page
+        for n in (rows, rows + 1):
+            for t in range(int(lens[n])):
+                row_of(kc, table, n, t, page)[:, 5] = -math.inf
+        assert whole >= 64
+        out, _ = run(q, kc, vc, table, lens)
+        assert bool(torch.isnan(out[rows:]).all())
+        kc[int(table[0, 3]), 2] = 0
+        kc[int(table[0, 3]), 2, :, 5] = -30000.0  # a weight of 0 in any type
+        want, slack = room(q[:rows], kc, vc, table[:rows], lens[:rows], "NHD")
+        assert bool(((out[:rows].double().cpu() - want).abs()
+                     <= ref.rounded(want, slack, F32)).all())
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 3.0, 1e-4])
+@pytest.mark.parametrize("groups,Hq,Hk,D,page", SHAPES[1:])
+def test_scales_in_fp32(groups, Hq, Hk, D, page, scale):
+    check(make(groups, Hq, Hk, D, page, "NHD", F32, 6), scale=scale)
+
+
+@pytest.mark.parametrize("D,page", [(128, 16), (64, 24)])
+def test_long_prefixes_in_many_shares_in_fp32(D, page):
+    check(make([(20011, [33, 5, 1, 800]), (6000, [1, 2])], 8, 2, D, page, "NHD", F32, D + page))
+
+
+def test_prefix_of_30000_keys():
+    for dtype in (BF16, F16, F32):
+        check(make([(30001, [12, 5])], 4, 2, 64, 16, "HND", dtype, 30), layout="HND")
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
