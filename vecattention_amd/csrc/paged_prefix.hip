@@ -1154,6 +1154,7 @@ hipError_t launch_prefix(const SharedArgs& x, hipStream_t stream) {
 }
 template <typename T, int D>
 hipError_t launch_join(const SharedArgs& x, hipStream_t stream) {
+  // (At most 2^23 rows: fewer than 2^32 threads.)
   hipLaunchKernelGGL((prefix_merge_kernel<T, D>), dim3(unsigned(x.a.N * x.a.Hk * x.a.G)),
                      dim3(kJoinThreads), 0, stream, x);
   return hipGetLastError();
@@ -1179,9 +1180,7 @@ hipError_t launch_both(const SharedArgs& x, hipStream_t stream) {
 bool shares_prefix(int dtype, const PagedArgs& a) {
   const double bytes = 4.0 * double(a.N * a.Hk * a.D) * double(a.M * a.page);
   const double least = (dtype == kF32 && a.D == 128 ? 2.0 : 1.0) * (128 << 20);
-  // The merge takes a work-group a row, and a launch fewer than 2^32 threads.
-  const bool fits = a.N * a.Hk * a.G < (int64_t(1) << 32) / kJoinThreads;
-  return fits && a.N > 1 && bytes > least && a.M * a.page >= kPrefixTile &&
+  return a.N > 1 && bytes > least && a.M * a.page >= kPrefixTile &&
          a.scale_log2 >= 0.f && a.kn < (int64_t(1) << 26) && a.vn < (int64_t(1) << 26) &&
          paged_tile_form(dtype, a);
 }
