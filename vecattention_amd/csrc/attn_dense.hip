@@ -30,22 +30,12 @@
 // issue priorities measured within 1%.  The statistics form (no V) is bound
 // by its VALU work, so five work-groups per CU on two K tiles each: the dense
 // pass of 32760 keys of 12 heads takes 3.3 ms, 3.8 in the 64-row form.
-#include "attn_common.h"
+#include "dense_tile.h"
 #include "lanes.h"
-#include "mfma.h"
 
 namespace va {
 
 constexpr int kDenseRows = 128;  // query rows per work-group
-
-template <int D>
-struct DenseShape {
-  static constexpr int kRowBytes = 2 * D;
-  static constexpr int kTileBytes = kTileKeys * kRowBytes;    // one K (or V) tile
-  static constexpr int kChunks = D / 8;                       // 16-byte chunks per row
-  static constexpr int kRowsPerCopy = 1024 / kRowBytes;       // rows per 1 KB copy
-  static constexpr int kCopies = kTileBytes / 1024 / 4;       // per wave and tile
-};
 
 // stats: row i of head bh gets stats[(bh * Sq + i) * 2 + {0, 1}] = (m, l), l =
 // sum over its keys of 2^(s * scale_log2 - m) in fp32.  Row i sees keys up to
@@ -57,14 +47,12 @@ __global__ __launch_bounds__(256, kStats ? (D == 128 ? 5 : 6) : (D == 128 ? 3 : 
     int64_t svs, T* __restrict__ out, int64_t sob, int64_t soh, int64_t sos, int64_t B,
     int64_t Hq, int64_t Hk, int64_t Sq, int64_t Sk, int causal, float scale_log2, int64_t nblk,
     int64_t qoff, float* __restrict__ stats) {
-  using S = DenseShape<D>;
-  using M = Mfma<T>;
-  using vec = typename M::vec;
+  using S = DenseTile<T, D>;
+  using M = typename S::M;
+  using vec = typename S::vec;
   constexpr int H = S::kCopies, NCH = S::kChunks, RPC = S::kRowsPerCopy;
   constexpr uint32_t TB = uint32_t(S::kTileBytes);
-  constexpr int NQK = D / 16;   // QK MFMAs per 32 keys
-  constexpr int NB = D / 32;    // output blocks of 32 features
-  constexpr int NPV = 4 * NB;   // PV MFMAs per tile (16 keys each)
+  constexpr int NQK = S::NQK, NB = S::NB, NPV = S::NPV;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[(kStats ? 2 : 3) * S::kTileBytes];
 
   const int tid = threadIdx.x;
@@ -136,19 +124,7 @@ __global__ __launch_bounds__(256, kStats ? (D == 128 ? 5 : 6) : (D == 128 ? 3 : 
         rs, lds_copy_base, uint64_t(key) | (uint64_t(ch ^ (x * kXorStep)) << 32));
   };
 
-  // ---- LDS read offsets (see attn_mfma.hip): K row l32 (+ 32 for the second
-  // half of the tile), chunk 2s + hh = k0 ^ 32s; V^T rows 8r + 4hh + j (+ 16
-  // per MFMA step), features 32i + ...: v0r ^ 64i.
-  const uint32_t k0 = uint32_t(l32 * S::kRowBytes + 16 * (hh ^ chunk_swizzle<D>(l32)));
-  uint32_t v0[2];
-  {
-    const int j = (lane % 16) / 4, g2 = 2 * ((lane / 16) % 2) + (lane % 4) / 2;
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int R = 8 * r + 4 * hh + j;
-      v0[r] = uint32_t(R * S::kRowBytes + 16 * (g2 ^ chunk_swizzle<D>(R)) + 8 * (lane % 2));
-    }
-  }
+  const typename S::Offsets at(lane);
 
   f32x16_t o[NB];
 #pragma unroll
@@ -179,38 +155,11 @@ __global__ __launch_bounds__(256, kStats ? (D == 128 ? 5 : 6) : (D == 128 ? 3 : 
     }
   };
   auto prob = [&](float s) { return __builtin_amdgcn_exp2f(__builtin_fmaf(s, scale_log2, mneg)); };
-  auto kread = [&](const unsigned char* kb, uint32_t kx, int i) {  // operand of QK MFMA i
-    return __builtin_bit_cast(vec, *reinterpret_cast<const uint4*>(
-                                       kb + (kx ^ uint32_t(32 * (i % NQK))) +
-                                       i / NQK * 32 * S::kRowBytes));
-  };
-  // S^T of a tile's two 32-key halves; the copies go out between the MFMAs.
-  constexpr int kAhead = 2;
   auto qk = [&](const unsigned char* kb, f32x16_t (&sc)[2], auto&& copies) {
-    uint32_t kx = k0;
-    asm volatile("" : "+v"(kx));  // the offsets are rebuilt, not kept
-    vec a[2 * NQK];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) a[i] = kread(kb, kx, i);
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) sc[hf][e] = 0.f;
-    __builtin_amdgcn_s_setprio(2);
-#pragma unroll
-    for (int i = 0; i < 2 * NQK; ++i) {
-      __builtin_amdgcn_sched_barrier(0);
-      if (i + kAhead < 2 * NQK) a[i + kAhead] = kread(kb, kx, i + kAhead);
-      sc[i / NQK] = M::run(a[i], qreg[i % NQK], sc[i / NQK]);
-      static_for<H>([&](auto c) {
-        if (c * 2 * NQK / H == i) copies(c);
-      });
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_setprio(0);
+    S::scores(kb, at.k, qreg, sc, copies);
   };
   // Scores of keys this lane's row does not see become -inf (tiles from
-  // m_tile on).  Slot of sc[hf][e]: 32hf + 8(e/4) + 4hh + e%4.
+  // m_tile on).
   auto mask = [&](int t, f32x16_t (&sc)[2]) {
     if (t < m_tile) return;
     const int lim = last_key - t * kTileKeys - 4 * hh;
@@ -268,17 +217,6 @@ __global__ __launch_bounds__(256, kStats ? (D == 128 ? 5 : 6) : (D == 128 ? 3 : 
     // ...: as the sparse kernel's ring form.
     static_for<H>([&](auto x) { copy(krs, lds_off<0>{}, x, 0); });
     static_for<H>([&](auto x) { copy(vrs, lds_off<TB>{}, x, 0); });
-    auto vread = [&](const unsigned char* vb, uint32_t va, uint32_t vb1, int f) {
-      const int sub = f / NB, i = f % NB;  // 16 keys of step sub, features [32i, +32)
-      const unsigned char* p0 = vb + (va ^ uint32_t(64 * i)) + sub * 16 * S::kRowBytes;
-      const unsigned char* p1 = vb + (vb1 ^ uint32_t(64 * i)) + sub * 16 * S::kRowBytes;
-      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) s16x4_t*)(p0));
-      const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) s16x4_t*)(p1));
-      const s16x4_t both[2] = {lo, hi};
-      return __builtin_bit_cast(vec, both);
-    };
     // first: the step of tile 0, whose probabilities go in as two 16-bit parts.
     auto step = [&](int t, auto r_tag, auto first_tag) {
       constexpr int r = decltype(r_tag)::value;
@@ -317,33 +255,24 @@ __global__ __launch_bounds__(256, kStats ? (D == 128 ? 5 : 6) : (D == 128 ? 3 : 
       }
       // ---- V(t) landed; every wave is done with K(t)
       vm_lds_barrier_keep<H>();
-      uint32_t va = v0[0], vb1 = v0[1];
-      asm volatile("" : "+v"(va), "+v"(vb1));
-      const unsigned char* vb = smem + v_this;
-      constexpr int kVAhead = 2;
-      vec vf[NPV];
+      uint32_t v0 = at.v[0], v1 = at.v[1];
+      asm volatile("" : "+v"(v0), "+v"(v1));
+      S::values(
+          smem + v_this, v0, v1,
+          [&](int f, vec v) {
+            o[f % NB] = M::run(v, bfrag[f / NB], o[f % NB]);
+            if constexpr (first) o[f % NB] = M::run(v, brest[f / NB], o[f % NB]);
+          },
+          vcopies,
+          [&](int f) {
 #pragma unroll
-      for (int f = 0; f < kVAhead; ++f) vf[f] = vread(vb, va, vb1, f);
-      __builtin_amdgcn_s_setprio(1);
+            for (int j = f * 16 / NPV; j < (f + 1) * 16 / NPV; ++j)
+              lsum = M::add_pair(bfrag[j / 4], j % 4, lsum);
+            if constexpr (first)
 #pragma unroll
-      for (int f = 0; f < NPV; ++f) {
-        __builtin_amdgcn_sched_barrier(0);
-        if (f + kVAhead < NPV) vf[f + kVAhead] = vread(vb, va, vb1, f + kVAhead);
-        o[f % NB] = M::run(vf[f], bfrag[f / NB], o[f % NB]);
-        if constexpr (first) o[f % NB] = M::run(vf[f], brest[f / NB], o[f % NB]);
-        static_for<H>([&](auto c) {
-          if (c * NPV / H == f) vcopies(c);
-        });
-#pragma unroll
-        for (int j = f * 16 / NPV; j < (f + 1) * 16 / NPV; ++j)
-          lsum = M::add_pair(bfrag[j / 4], j % 4, lsum);
-        if constexpr (first)
-#pragma unroll
-          for (int j = f * 16 / NPV; j < (f + 1) * 16 / NPV; ++j)
-            lsum = M::add_pair(brest[j / 4], j % 4, lsum);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      __builtin_amdgcn_s_setprio(0);
+              for (int j = f * 16 / NPV; j < (f + 1) * 16 / NPV; ++j)
+                lsum = M::add_pair(brest[j / 4], j % 4, lsum);
+          });
     };
     if (ntiles > 0) step(0, std::integral_constant<int, 0>{}, std::true_type{});
     for (int t = 1; t < ntiles; t += 3) {

@@ -29,9 +29,8 @@
 // ahead; three work-groups a CU; the keys of a step between two waves where a tile has 64
 // rows at most (a half step takes 0.8 of a whole one: 162 -> 184 with twice the steps a
 // piece); ranges that begin their walks at different steps.
-#include "attn_common.h"
+#include "dense_tile.h"
 #include "lanes.h"
-#include "mfma.h"
 #include "paged_ops.h"
 #include "paged_tile.h"
 
@@ -420,8 +419,7 @@ __device__ __forceinline__ void repair_piece(const SharedArgs& x, const Group& g
 // kWhole: pages of a multiple of 16 tokens, so that the 16 keys that a wave copies of
 // a tile lie in one.
 template <typename T, int D, bool kWhole> struct PrefixLds {
-  static constexpr uint32_t kTileBytes = uint32_t(kTileKeys * 2 * D);
-  __attribute__((aligned(1024))) unsigned char tiles[3 * kTileBytes];
+  __attribute__((aligned(1024))) unsigned char tiles[3 * DenseTile<T, D>::kTileBytes];
   PiecesLds pieces;
   int bad[kWaves];
   int32_t ids[kWhole ? 1 : kIdKeys + 2];
@@ -429,12 +427,12 @@ template <typename T, int D, bool kWhole> struct PrefixLds {
 template <typename T, int D, bool kWhole>
 __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D, kWhole>& shared,
                                             uint32_t block) {
-  using M = Mfma<T>;
-  using vec = typename M::vec;
-  constexpr int kRowBytes = 2 * D, NCH = D / 8;
-  constexpr uint32_t TB = PrefixLds<T, D, kWhole>::kTileBytes;
-  constexpr int RPC = 1024 / kRowBytes, H = kTileKeys * kRowBytes / 1024 / kWaves;
-  constexpr int NQK = D / 16, NB = D / 32, NPV = 4 * NB;
+  using S = DenseTile<T, D>;
+  using M = typename S::M;
+  using vec = typename S::vec;
+  constexpr int H = S::kCopies, NCH = S::kChunks, RPC = S::kRowsPerCopy;
+  constexpr uint32_t TB = uint32_t(S::kTileBytes);
+  constexpr int NQK = S::NQK, NB = S::NB, NPV = S::NPV;
   // fp16's normal numbers begin at 2^-14: weights 2^7 times larger are held, 2^15 at most.
   constexpr float kBias = kIsF16<T> ? 7.f : 0.f, kSmallest = -14.f;
   unsigned char* smem = shared.tiles;
@@ -466,17 +464,7 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
   const uint32_t kn2 = uint32_t(a.kn) * 2, vn2 = uint32_t(a.vn) * 2;
   const uint32_t krow = uint32_t(lane / NCH) * kn2, vrow = uint32_t(lane / NCH) * vn2;
 
-  // ---- LDS read offsets, as in dense attention.
-  const uint32_t k0 = uint32_t(l32 * kRowBytes + 16 * (hh ^ chunk_swizzle<D>(l32)));
-  uint32_t v0[2];
-  {
-    const int j = (lane % 16) / 4, g2 = 2 * ((lane / 16) % 2) + (lane % 4) / 2;
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int R = 8 * r + 4 * hh + j;
-      v0[r] = uint32_t(R * kRowBytes + 16 * (g2 ^ chunk_swizzle<D>(R)) + 8 * (lane % 2));
-    }
-  }
+  const typename S::Offsets offset(lane);
 
   bool nan = false;
   for (uint32_t piece = number; piece < all.count; piece += uint32_t(x.groups)) {
@@ -574,23 +562,6 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
 
     f32x16_t o[NB];
     float mneg, lsum;
-    auto kread = [&](const unsigned char* kb, uint32_t kx, int i) {
-      return __builtin_bit_cast(vec, *reinterpret_cast<const uint4*>(
-                                         kb + (kx ^ uint32_t(32 * (i % NQK))) +
-                                         i / NQK * 32 * kRowBytes));
-    };
-    auto vread = [&](const unsigned char* vb, uint32_t va, uint32_t vb1, int f) {
-      const int sub = f / NB, i = f % NB;
-      const unsigned char* p0 = vb + (va ^ uint32_t(64 * i)) + sub * 16 * kRowBytes;
-      const unsigned char* p1 = vb + (vb1 ^ uint32_t(64 * i)) + sub * 16 * kRowBytes;
-      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) s16x4_t*)(p0));
-      const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) s16x4_t*)(p1));
-      const s16x4_t both[2] = {lo, hi};
-      return __builtin_bit_cast(vec, both);
-    };
-
     {
 #pragma unroll
       for (int i = 0; i < NB; ++i)
@@ -629,31 +600,7 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
           return;
         } else {
         f32x16_t sc[2];
-        {
-          const unsigned char* kb = smem + k_this;
-          uint32_t kx = k0;
-          asm volatile("" : "+v"(kx));
-          constexpr int kAhead = 2;
-          vec kf[2 * NQK];
-#pragma unroll
-          for (int i = 0; i < kAhead; ++i) kf[i] = kread(kb, kx, i);
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) sc[hf][e] = 0.f;
-          __builtin_amdgcn_s_setprio(2);
-#pragma unroll
-          for (int i = 0; i < 2 * NQK; ++i) {
-            __builtin_amdgcn_sched_barrier(0);
-            if (i + kAhead < 2 * NQK) kf[i + kAhead] = kread(kb, kx, i + kAhead);
-            sc[i / NQK] = M::run(kf[i], qreg[i % NQK], sc[i / NQK]);
-            static_for<H>([&](auto c) {
-              if (c * 2 * NQK / H == i) kcopies(c);
-            });
-          }
-          __builtin_amdgcn_sched_barrier(0);
-          __builtin_amdgcn_s_setprio(0);
-        }
+        S::scores(smem + k_this, offset.k, qreg, sc, kcopies);
         if constexpr (kWhole) next = find(t + 2);  // here by the next barrier
         // The maximum's instructions are inline assembly, before which the compiler leaves no
         // wait for the matrix instructions: 11 wait states after the last one.
@@ -742,8 +689,8 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
         else
           weights([&](float s) { return __builtin_fmaf(s, a.scale_log2, bias); });
         vm_lds_barrier_keep<H>();  // V(t) landed; every wave is done with K(t)
-        uint32_t va = v0[0], vb1 = v0[1];
-        asm volatile("" : "+v"(va), "+v"(vb1));
+        uint32_t v0 = offset.v[0], v1 = offset.v[1];
+        asm volatile("" : "+v"(v0), "+v"(v1));
         const unsigned char* vb = smem + v_this;
         if constexpr (kApart) {
           if (small) {
@@ -758,32 +705,21 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
 #pragma unroll
             for (int f = 0; f < NPV; ++f) {
               __builtin_amdgcn_sched_barrier(0);
-              o[f % NB] = M::run(vread(vb, va, vb1, f), blow[f / NB], o[f % NB]);
+              o[f % NB] = M::run(S::vread(vb, v0, v1, f), blow[f / NB], o[f % NB]);
             }
 #pragma unroll
             for (int j = 0; j < 16; ++j) lsum = M::add_pair(blow[j / 4], j % 4, lsum);
             scale(0x1p-24f);
           }
         }
-        constexpr int kVAhead = 2;
-        vec vf[NPV];
+        S::values(
+            vb, v0, v1, [&](int f, vec v) { o[f % NB] = M::run(v, bfrag[f / NB], o[f % NB]); },
+            vcopies,
+            [&](int f) {
 #pragma unroll
-        for (int f = 0; f < kVAhead; ++f) vf[f] = vread(vb, va, vb1, f);
-        __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int f = 0; f < NPV; ++f) {
-          __builtin_amdgcn_sched_barrier(0);
-          if (f + kVAhead < NPV) vf[f + kVAhead] = vread(vb, va, vb1, f + kVAhead);
-          o[f % NB] = M::run(vf[f], bfrag[f / NB], o[f % NB]);
-          static_for<H>([&](auto c) {
-            if (c * NPV / H == f) vcopies(c);
-          });
-#pragma unroll
-          for (int j = f * 16 / NPV; j < (f + 1) * 16 / NPV; ++j)
-            lsum = M::add_pair(bfrag[j / 4], j % 4, lsum);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_setprio(0);
+              for (int j = f * 16 / NPV; j < (f + 1) * 16 / NPV; ++j)
+                lsum = M::add_pair(bfrag[j / 4], j % 4, lsum);
+            });
         }
       };
       auto steps = [&](auto active_tag) {
