@@ -621,6 +621,7 @@ __global__ __launch_bounds__(QPS * 4, (kRing3 || D == 64) ? 3 : 2) void attn_mfm
       __builtin_amdgcn_s_setprio(0);
       mask(t, sc);
       float tmax = -__builtin_inff();
+      settle(sc);
 #pragma unroll
       for (int e = 0; e < 16; e += 2) tmax = max3_plain(tmax, sc[e], sc[e + 1]);
       rescale(tmax);
@@ -683,6 +684,7 @@ __global__ __launch_bounds__(QPS * 4, (kRing3 || D == 64) ? 3 : 2) void attn_mfm
       s_cur = qk(smem);
       mask(0, s_cur);
       float tmax = -__builtin_inff();
+      settle(s_cur);
 #pragma unroll
       for (int e = 0; e < 16; e += 2) tmax = max3_plain(tmax, s_cur[e], s_cur[e + 1]);
       rescale(tmax);
@@ -748,6 +750,7 @@ __global__ __launch_bounds__(QPS * 4, (kRing3 || D == 64) ? 3 : 2) void attn_mfm
         for (int e = 0; e < 4; ++e) ps[e] += ps[e + 4];
         lsum += (ps[0] + ps[2]) + (ps[1] + ps[3]);
         float tmax = -__builtin_inff();
+        settle(s_next);
 #pragma unroll
         for (int e = 0; e < 16; e += 2) tmax = max3_plain(tmax, s_next[e], s_next[e + 1]);
         rescale(tmax);

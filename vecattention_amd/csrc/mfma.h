@@ -46,4 +46,8 @@ template <> struct Mfma<f16_t> {
   }
 };
 
+// Before inline assembly (max3_plain) reads a 32x32x16 product: 11 wait states behind its last
+// instruction, which the compiler leaves before instructions that it knows, no others.
+__device__ inline void settle(f32x16_t& x) { asm volatile("s_nop 10" : "+v"(x)); }
+
 }  // namespace va

@@ -602,13 +602,11 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
         f32x16_t sc[2];
         S::scores(smem + k_this, offset.k, qreg, sc, kcopies);
         if constexpr (kWhole) next = find(t + 2);  // here by the next barrier
-        // The maximum's instructions are inline assembly, before which the compiler leaves no
-        // wait for the matrix instructions: 11 wait states after the last one.
         constexpr bool kApart = kIsF16<T>;
         float tmax = 0.f, tmin = 0.f;
         static_for<2>([&](auto half) {
           constexpr int hf = decltype(half)::value;
-          if constexpr (hf == 1) asm volatile("s_nop 10" : "+v"(sc[1]));
+          if constexpr (hf == 1) settle(sc[1]);
           float u0 = max3_plain(sc[hf][0], sc[hf][1], sc[hf][2]), u1 = sc[hf][3];
 #pragma unroll
           for (int e = 4; e < 16; e += 4) {
