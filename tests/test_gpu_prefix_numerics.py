@@ -7,7 +7,9 @@ import pytest
 import torch
 
 import paged_reference as ref
-from test_gpu_prefix_attention import check, make, note, room, run
+from test_gpu_prefix_attention import check, make, note, room, run, widened
+from vecattention_amd import (paged_decode_attention, paged_kv_prefix,
+                              paged_prefix_decode_attention)
 
 pytestmark = pytest.mark.gpu
 
@@ -177,8 +179,7 @@ def test_keys_that_are_not_finite_in_fp32(groups, Hq, Hk, D, page):
         fine = (out.double().cpu() - want).abs() <= ref.rounded(want, slack, F32)
         assert bool(fine[rows:].all()) and bool(fine[:rows, :Hq - G].all())
         # Scores of -infinity: a weight of 0, and rows of such keys alone 0 / 0.
-        q, kc, vc, table, lens = make([(groups[0][0], groups[0][1]), (320, [0, 0])], Hq, Hk, D, page,
-                                      "NHD", F32)
+        q, kc, vc, table, lens = make(groups + [(320, [0, 0])], Hq, Hk, D, page, "NHD", F32)
         q[:, :, 5] = 1
         kc[int(table[0, 3]), 2, :, 5] = -math.inf
         whole = 320 // page * page
@@ -215,8 +216,6 @@ def test_prefix_of_30000_keys():
 @pytest.mark.parametrize("D", [64, 128])
 def test_same_bits_in_graphs_and_outside(D, dtype):
     """Eager calls, replays and calls on a side stream, of values with an infinity among them."""
-    from test_gpu_prefix_attention import widened
-    from vecattention_amd import paged_kv_prefix, paged_prefix_decode_attention
     note("graph", D, dtype)
     q, kc, vc, table, lens = make([(5000, [60, 7, 300, 1]), (640, [3] * 12)], 8, 2, D, 16, "NHD",
                                   dtype, 3)
@@ -239,3 +238,41 @@ def test_same_bits_in_graphs_and_outside(D, dtype):
                                               paged_kv_prefix(lens, table, 16))
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(eager, want)
+
+
+def both(N, shared, Hq, Hk, D, dtype, more=0):
+    """(shared form or not, every row for itself) of N rows over the same whole pages of 16, in
+    tables with room for `more` keys."""
+    g = torch.Generator(device=DEV).manual_seed(N + shared)
+    shape = (shared // 16 + 1, 16, Hk, D)
+    kc, vc = (torch.randn(shape, generator=g, device=DEV).to(dtype) for _ in range(2))
+    q = torch.randn(N, Hq, D, generator=g, device=DEV).to(dtype)
+    table = torch.full((N, (shared + more) // 16), -1, dtype=torch.int32, device=DEV)
+    table[:, :shared // 16] = torch.arange(shared // 16, device=DEV)
+    lens = torch.full((N,), shared, dtype=torch.int32, device=DEV)
+    prefix = paged_kv_prefix(lens, table, 16)
+    assert prefix.prefix_lens.tolist() == [shared] * N
+    return (paged_prefix_decode_attention(q, kc, vc, table, lens, prefix),
+            paged_decode_attention(q, kc, vc, table, lens))
+
+
+def test_batches_that_are_faster_row_by_row():
+    """Many rows of short tables, and few rows of few keys, take the form of one row, bit for bit;
+    batches past the border the shared one, with the same result to the types' roundings."""
+    for N, keys, Hq, Hk, D, dtype in ((200, 256, 16, 16, 64, BF16), (200, 256, 32, 8, 128, BF16),
+                                      (64, 512, 32, 8, 128, F16), (64, 1024, 28, 4, 128, BF16),
+                                      (8, 4096, 28, 4, 128, F16), (8, 8192, 28, 4, 128, F32),
+                                      (2, 2048, 16, 16, 64, F32)):
+        note("by rows", N, keys, Hq, Hk, D, dtype)
+        assert torch.equal(*both(N, keys, Hq, Hk, D, dtype)), (N, keys)
+    for N, keys, Hq, Hk, D, dtype, more in (
+            (200, 512, 16, 16, 64, BF16, 0), (64, 1536, 28, 4, 128, BF16, 0),
+            (8, 2048, 16, 16, 64, F16, 0), (8, 2048, 16, 16, 64, F32, 0),
+            (300, 640, 4, 1, 128, F16, 2000), (8, 6144, 28, 4, 128, BF16, 0)):
+        note("shared", N, keys, Hq, Hk, D, dtype)
+        out, want = both(N, keys, Hq, Hk, D, dtype, more)
+        assert not torch.equal(out, want), (N, keys)
+        # Weights rounded by half a step each in both sums, against values of size 1 whose mean
+        # over `keys` equal-like weights is about keys^-1/2: in the norm, one step of the type.
+        off = float((out.double() - want.double()).norm() / want.double().norm())
+        assert off < 2 * ref.HALF_STEP[dtype] if dtype != F32 else off < 2.0 ** -18, (N, off)

@@ -1101,22 +1101,35 @@ hipError_t launch_both(const SharedArgs& x, hipStream_t stream) {
   return wide ? launch_join<T, 128>(x, stream) : launch_join<T, 64>(x, stream);
 }
 
-// Whether the prefix is computed once: rows that the matrix-core form takes, a scale
-// that orders scores as the products are ordered, and enough to read if every row did so
-// for itself, to the tables' width, which the two launches here cost less than (counted
-// at two bytes a value; fp32 of D 128, whose waves are one to a SIMD, pays later).
-// us, every row for itself / shared, 28 query and 4 kv heads of 128 in bf16: 8 rows of
-// 4096 keys (68 MB) 17.6 / 24, of 8192 (135 MB) 28.8 / 25, 64 rows of 1024 keys (143 MB)
-// 23.6 / 33, of 2048 (277 MB) 37.8 / 34; 16 and 16 heads of 64: 8 rows of 2048 keys (69 MB)
-// 18.7 / 17.6, of 4096 25.0 / 17.6.  In fp32, the first: 4 rows of 16384 keys (135 MB) 53 /
-// 62, 8 of 16384 (269) 91 / 69, 16 of 16384 (539) 165 / 98, 64 of 8192 (1082) 307 / 135; the
-// second: 4 rows of 4096 keys (68) 30 / 28, of 8192 (135) 49 / 33, 64 of 8192 (2164) 512 / 67.
+// Whether the prefix is computed once: rows that the matrix-core form takes, a scale that
+// orders scores as the products are ordered, and enough to read if every row did so for
+// itself, to the tables' width (the lengths are known to the GPU only).  What the two launches
+// here cost at any length grows with the rows (states written and merged), and tables of few
+// keys have a form of one launch otherwise.  us, every row for itself / shared, bf16, N rows
+// that share all of `keys` (room in MB at two bytes a value):
+//   28 + 4 heads of 128     8 x 4096 (67) 18.5 / 23.0, 8 x 6144 (101) 23.8 / 22.8,
+//     8 x 8192 (135) 28.9 / 24.2, 2 x 32768 (134) 28.0 / 31.2, 3 x 32768 (201) 38.0 / 31.2,
+//     64 x 1024 (136) 24.5 / 27.3, 64 x 1536 (203) 29.6 / 27.6, 200 x 512 (216) 35.7 / 42.1,
+//     200 x 1024 (426) 54.2 / 43.3
+//   32 + 8 heads of 128     64 x 512 (138) 19.7 / 28.9, 64 x 1024 (273) 33.1 / 29.7,
+//     200 x 256 (223) 22.7 / 45.5, 200 x 512 (433) 59.3 / 45.9
+//   16 + 16 heads of 64     8 x 1024 (34) 14.2 / 14.7, 8 x 2048 (68) 19.2 / 14.6,
+//     64 x 512 (138) 20.3 / 20.7, 64 x 1024 (273) 30.9 / 21.1, 200 x 256 (223) 26.4 / 49.9,
+//     200 x 512 (433) 76.9 / 49.7
+// fp32, 28 + 4 heads of 128: 8 x 8192 (135) 52 / 56, 4 x 16384 (134) 51 / 62, 8 x 16384 (269)
+// 89 / 70, 64 x 2048 (271) 86 / 76; 16 + 16 of 64: 4 x 4096 (67) 28.4 / 27.2, 8 x 2048 (68)
+// 28.1 / 23.0.  Of 138 such points the rule is 11% above the better side at one, and below 10
+// at the others.
+constexpr int64_t kLeastKeys = 512;
 bool shares_prefix(int dtype, const PagedArgs& a) {
+  const double mib = 1 << 20, rows = double(a.N * a.Hk * a.G);
   const double bytes = 4.0 * double(a.N * a.Hk * a.D) * double(a.M * a.page);
-  const double least = (dtype == kF32 && a.D == 128 ? 2.0 : 1.0) * (128 << 20);
-  return a.N > 1 && bytes > least && a.M * a.page >= kPrefixTile &&
-         a.scale_log2 >= 0.f && a.kn < (int64_t(1) << 26) && a.vn < (int64_t(1) << 26) &&
-         paged_tile_form(dtype, a);
+  const bool wide = a.D == 128;
+  const double least = dtype == kF32 ? (wide ? 256 : 64) * mib
+                       : wide        ? 80 * mib + 48 * 1024 * rows
+                                     : 48 * mib + 24 * 1024 * rows;
+  return a.N > 1 && bytes >= least && a.M * a.page >= kLeastKeys && a.scale_log2 >= 0.f &&
+         a.kn < (int64_t(1) << 26) && a.vn < (int64_t(1) << 26) && paged_tile_form(dtype, a);
 }
 
 // The regions of the workspace, behind those of the rows' own keys (`own` bytes).
