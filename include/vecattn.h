@@ -601,8 +601,9 @@ int va_paged_prefix(const int32_t* kv_lens, int64_t N, const int32_t* block_tabl
 /*
  * va_paged_decode_attn for rows in groups that share their first pages
  * (prefix_lens and group_rows as va_paged_prefix makes them, from these tables):
- * the same results, but the keys of a group's prefix are read once for all of its
- * rows, through the table of the group's first row.  Rows of a group have to hold
+ * the same results up to rounding, but the keys of a group's prefix are read once for
+ * all of its rows, through the table of the group's first row; 16-bit types round the
+ * weights of these keys to their bits once (va_paged_decode_attn keeps two parts).  Rows of a group have to hold
  * prefix_lens tokens at least and list the same pages for them.  workspace: of
  * va_paged_prefix_decode_workspace_size() bytes (-1: sizes that are not
  * supported), 16-byte aligned; calls that may overlap need one each.

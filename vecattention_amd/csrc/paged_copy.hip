@@ -1,4 +1,4 @@
-// Pages of a key-value cache to other pages of it, in all layers with one launch:
+// Pages of a key-value cache to other pages of it, in up to 32 layers with one launch:
 // the tails of forked rows and the moves of a compaction.  A copy of whole rows:
 // HBM for many pages, latency for a few.  A page is cut into pieces of 16 bytes
 // (of one element where strides or addresses allow no more), numbered along the
@@ -8,7 +8,8 @@
 // us, 1500 pages of 32 KB in eight caches (786 MB read and written): 233 with every
 // piece's place found by two divisions, which made it 70 us of arithmetic; 158 (5.0 TB/s,
 // a large copy's rate) where pages are blocks without gaps, whose pieces need none.  Last
-// pages of eight rows in 4 layers: 5.1, the launch.
+// pages of eight rows in 4 layers: 5.1, the launch.  An empty entry costs a work-group an
+// iteration in every cache: 50000 of them 43 in 4 layers, 279 in 28.
 #include "common.h"
 #include "paged_ops.h"
 

@@ -14,17 +14,19 @@
 // K Q^T and O^T += V^T P^T on 32x32x16 matrix instructions, weights from the scores'
 // registers, rounded once to 16 bits (each weight by half a step at most, the same in the
 // sum of the values and in the weights' own sum, which puts an output off by about as
-// much as its own rounding; two parts a weight, as for the own keys, would double the
-// products; fp16's small weights go in apart, by products of their own in the steps that
-// have any).  Only whole 64-key tiles of a prefix are walked here, without masks; what is
+// much as its own rounding: in bf16 2.3e-3 of the outputs' norm, against 1.7e-3 with two
+// parts a weight as for the own keys, which take 198 us where one takes 156, 33 for 31 in
+// the cases below).  fp16's small weights go in apart, by products of their own in the steps
+// that have any (131072 keys behind a sink 20 nats above them: 250 us for 185).  Only whole 64-key tiles of a prefix are walked here, without masks; what is
 // left of it comes with the row's own keys.
 //
-// us, bf16, D 128: 64 rows of 28 query and 4 kv heads that share 131072 keys: 152 for
-// 120 GFLOP (790 TFLOP/s; the rows' tiles hold 8/7 of that): 30 at any length (launches,
+// us, bf16, D 128: 64 rows of 28 query and 4 kv heads that share 131072 keys: 156 for
+// 120 GFLOP (770 TFLOP/s; the rows' tiles hold 8/7 of that): 30 at any length (launches,
 // counting, 33 MB of states written and read again), then steps at 1000 TFLOP/s and more,
 // where the matrix cores' power is the bound, as in dense attention.  Every row for
-// itself: 2466.  40 rows of 32 query and 8 kv heads in six groups of 8192 keys: 34 for
-// 96 MB (19 at a copy's rate), where every row for itself takes 67.
+// itself: 2466.  40 rows of 32 query and 8 kv heads in six groups of 8192 keys: 31 for
+// 96 MB (15 at a large read's 6.3 TB/s), where every row for itself takes 67: at 27 rows a kv
+// head one wave of four computes.
 // Tried, and no faster: rings of four and six slots; two to eight K and V fragments read
 // ahead; three work-groups a CU; the keys of a step between two waves where a tile has 64
 // rows at most (a half step takes 0.8 of a whole one: 162 -> 184 with twice the steps a
@@ -758,7 +760,7 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
 // on), O^T += V^T P^T in D/2 more, weights from the scores' registers.  Where a tile has 64
 // (32) rows at most, two (four) waves take turns at the same rows' keys.  Bound by the fp32
 // matrix cores: 8192 cycles for 32 keys of D 128, beside which loads and exponentials are
-// little (64 rows of 28 and 4 heads of 128 over 8192 keys: 135 us for 7.5 GFLOP, of which 45
+// little (64 rows of 28 and 4 heads of 128 over 8192 keys: 137 us for 7.5 GFLOP, of which 45
 // at any length; every row for itself 307).
 template <int D> struct PrefixLdsF32 {
   PiecesLds pieces;

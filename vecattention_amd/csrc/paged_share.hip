@@ -11,7 +11,11 @@
 // What bounds them are launches, and reads that wait for one another, not bytes: in us,
 // a fork of 512 rows of up to 2092 pages 33 in four launches (7.6 MB, 2 at a copy's rate),
 // a compaction of 256 rows 34 in five, prefixes of 256 rows of 8200 pages 9.3 in two.
-// Each launch ends where all of a sum has to be there before its first use.
+// Each launch ends where all of a sum has to be there before its first use; those over
+// pages have a work-group for 4096 of them, too few to fill the GPU below a million pages
+// (scan, count and place take 7 to 9 us for 140,000 to 400,000).  Rows look for their parent,
+// or their group, among all rows before them: a fork of 8192 rows of 8 pages 92, of 65536
+// 2014; prefixes 141 to 192 and 7629 to 10372.
 #include "common.h"
 #include "lanes.h"
 #include "paged_ops.h"

@@ -148,7 +148,9 @@ def paged_kv_fork(kv_lens, parents, block_tables, page_shares, free_pages, page_
     front of ``free_head`` and in ascending order, and the copies take theirs from
     there.  Where the list ends they get -1 (``paged_decode_attention`` answers NaN
     for such a row) and the new ``free_head`` exceeds the list; a list with an entry
-    for every page of the cache has room for all that return.  At most 65536 rows.
+    for every page of the cache has room for all that return.  At most 65536 rows, each
+    of which looks at all before it: 33 us for 512 of long prompts, 0.1 ms for 8192 short
+    ones, 2 ms for 65536.
     """
     return PagedFork._make(nat.host_call("fork", block_tables, kv_lens, parents, block_tables,
                                          page_shares, free_pages, page_size, free_head,
@@ -179,13 +181,17 @@ def paged_kv_compact(kv_lens, block_tables, page_shares, free_pages, page_size, 
 
 
 def copy_paged_kv(k_caches, v_caches, src_pages, dst_pages, rows=None, kv_layout="NHD"):
-    """Pages to other pages of the same caches, in place, all layers in one launch.
+    """Pages to other pages of the same caches, in place, up to 32 layers a launch.
 
     k_caches, v_caches: the cache of one layer, or lists of those of all layers (one
     shape, type and strides).  src_pages, dst_pages: (C,) int32; an entry with a page
     outside the cache (-1) copies nothing.  The pages copied to must be distinct, and
     none of them copied from.  rows: (C,) int32, the tokens at the beginning of each
     page that are copied (None: all); the rows behind them stay.
+
+    An empty entry takes time, a little of it: a list of 50000 that are all -1 takes
+    44 us for 4 layers, 280 for 28.  A program that knows how many moves a compaction
+    can have at most (its requests' pages) passes that much of the lists.
     """
     one = k_caches[0] if isinstance(k_caches, (list, tuple)) and k_caches else k_caches
     nat.host_call("copy", one, k_caches, v_caches, src_pages, dst_pages, rows, kv_layout)
@@ -205,7 +211,9 @@ def paged_kv_prefix(kv_lens, block_tables, page_size, group_ids=None):
     prompt that all requests begin with makes one group of them: ids say which larger
     parts to share instead).  ``prefix_lens`` are the tokens of the whole pages that
     all rows of a group begin with, 0 where a row is alone.  What it finds stays true
-    while rows grow; after a fork or a compaction it has to be found anew.
+    while rows grow; after a fork or a compaction it has to be found anew.  At most 65536
+    rows, each of which looks at all before it: 10 us for 256, 0.2 ms for 8192, 10 ms
+    for 65536.
     """
     return SharedPrefix._make(nat.host_call("prefix", block_tables, kv_lens, block_tables,
                                             page_size, group_ids))
@@ -218,8 +226,16 @@ def paged_prefix_decode_attention(q, k_cache, v_cache, block_tables, kv_lens, pr
     prefix: ``paged_kv_prefix`` of these rows (a pair of prefix_lens and group_rows).
     The keys and values of a group's prefix are read once, for the query heads of all
     of its rows together, and every row's own keys after them; otherwise arguments and
-    result are those of ``paged_decode_attention``.  Rows of a group hold at least
+    result are those of ``paged_decode_attention``, up to rounding: in 16-bit types a
+    shared key's weight is rounded to the type's bits once, where the other keeps two
+    parts, so an output is off by about its own rounding more (in bf16 2.3e-3 in the
+    norm against 1.7e-3, in fp16 2.9e-4 against 2.1e-4).  Rows of a group hold at least
     prefix_lens tokens, and list the same pages for them.
+
+    Batches too small to gain, by the tables' width, take ``paged_decode_attention``'s
+    own path.  Past that, a batch that shares little takes longer here than there: by up
+    to 12% with 28 + 4 heads of 128 and 30% with 16 + 16 of 64 where at most 64 tokens are
+    shared, and by 3 to 9 us where tables have room for far more than the rows hold.
     """
     prefix_lens, group_rows = prefix
     return nat.host_call("prefix_decode", q, q, k_cache, v_cache, block_tables, kv_lens,
