@@ -276,3 +276,25 @@ def test_batches_that_are_faster_row_by_row():
         # over `keys` equal-like weights is about keys^-1/2: in the norm, one step of the type.
         off = float((out.double() - want.double()).norm() / want.double().norm())
         assert off < 2 * ref.HALF_STEP[dtype] if dtype != F32 else off < 2.0 ** -18, (N, off)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("count,Hq,Hk,D,page", [(32, 32, 32, 64, 16), (40, 32, 16, 64, 24)])
+def test_more_pieces_than_work_groups(count, Hq, Hk, D, page, dtype):
+    """1024 and 640 pieces of work, for 512 work-groups: of up to 64 rows, which a wave counts by
+    itself, and of more; with infinite values in some groups, all other outputs bit for bit."""
+    note("pieces", count, Hq, Hk, D, page, dtype)
+    groups = [(100 + 64 * (i % 4), [i % 5, 3]) for i in range(count)]
+    case = make(groups, Hq, Hk, D, page, "NHD", dtype, 7)
+    clean, _ = check(case)
+    q, kc, vc, table, lens = case
+    want = clean.clone()
+    for i in range(0, count, 3):
+        row_of(vc, table, 2 * i, 5, page)[Hk - 1, 11] = math.inf
+        row_of(vc, table, 2 * i, 40, page)[0, 2] = math.nan
+        want[2 * i:2 * i + 2, -(Hq // Hk):, 11] = math.inf
+    out, _ = run(q, kc, vc, table, lens)
+    for i in range(0, count, 3):
+        assert bool(torch.isnan(out[2 * i:2 * i + 2, :Hq // Hk, 2]).all())
+        out[2 * i:2 * i + 2, :Hq // Hk, 2] = want[2 * i:2 * i + 2, :Hq // Hk, 2]
+    assert torch.equal(out, want)
