@@ -1128,8 +1128,8 @@ bool shares_prefix(int dtype, const PagedArgs& a) {
   const double bytes = 4.0 * double(a.N * a.Hk * a.D) * double(a.M * a.page);
   const bool wide = a.D == 128;
   const double least = dtype == kF32 ? (wide ? 256 : 64) * mib
-                       : wide        ? 80 * mib + 48 * 1024 * rows
-                                     : 48 * mib + 24 * 1024 * rows;
+                       : wide        ? 80 * mib + 40 * 1024 * rows
+                                     : 48 * mib + 20 * 1024 * rows;
   return a.N > 1 && bytes >= least && a.M * a.page >= kLeastKeys && a.scale_log2 >= 0.f &&
          a.kn < (int64_t(1) << 26) && a.vn < (int64_t(1) << 26) && paged_tile_form(dtype, a);
 }
