@@ -17,8 +17,9 @@
 // much as its own rounding: in bf16 2.3e-3 of the outputs' norm, against 1.7e-3 with two
 // parts a weight as for the own keys, which take 198 us where one takes 156, 33 for 31 in
 // the cases below).  fp16's small weights go in apart, by products of their own in the steps
-// that have any (131072 keys behind a sink 20 nats above them: 250 us for 185).  Only whole 64-key tiles of a prefix are walked here, without masks; what is
-// left of it comes with the row's own keys.
+// that have any (131072 keys behind a sink 20 nats above them: 250 us for 185).  Only whole
+// 64-key tiles of a prefix are walked here, without masks; what is left of it comes with the
+// row's own keys.
 //
 // us, bf16, D 128: 64 rows of 28 query and 4 kv heads that share 131072 keys: 156 for
 // 120 GFLOP (770 TFLOP/s; the rows' tiles hold 8/7 of that): 30 at any length (launches,
@@ -650,6 +651,7 @@ __device__ __forceinline__ void prefix_tile(const SharedArgs& x, PrefixLds<T, D,
         // multiplication's exact product would lie tens of powers of two beside it from 2^27
         // on, or -2^27 down: weights of 0, or beyond the type.  Below 2^16 the two are within
         // 2^-8 of each other.
+        //
         // fp16 weights below its normal numbers go in apart, 2^24 times larger, where a step has
         // any: they keep their bits down to 2^-45 of the maximum's.
         vec bfrag[4], blow[kApart ? 4 : 1];
